@@ -125,7 +125,7 @@ def _values(g, dtype, *shape):
 class _Cache:
     """What the caches below have in common with the framework's: tensors and sizes."""
 
-    def __init__(self, B, H, max_len, D, fp8):
+    def __init__(self, B, H, max_len, D, fp8, weights):
         self.B, self.H, self.max_len, self.D = B, H, max_len, D
         kind = torch.float8_e4m3fn if fp8 else torch.bfloat16
         self.k = torch.zeros(B, H, max_len, D, device="cuda").to(kind)
@@ -135,14 +135,15 @@ class _Cache:
             self.v_scale = torch.ones_like(self.k_scale)
             self.k_tail = torch.zeros(B, H, BLOCK, D, dtype=torch.bfloat16, device="cuda")
             self.v_tail = torch.zeros_like(self.k_tail)
+        self.weights = torch.zeros(B, H, max_len, device="cuda") if weights else None
         self.lengths = torch.zeros(B, dtype=torch.int32, device="cuda")
 
 
-def _cache(B, H, max_len, D, fp8):
+def _cache(B, H, max_len, D, fp8=False, weights=False):
     if own:   # the framework's cache has a workspace of its own beside the same tensors
         import dadgpt_b200 as dad
-        return (dad.KVCacheFP8 if fp8 else dad.KVCacheBF16)(B, H, max_len, D)
-    return _Cache(B, H, max_len, D, fp8)
+        return dad.KVCacheFP8(B, H, max_len, D) if fp8 else dad.KVCacheBF16(B, H, max_len, D, weights=weights)
+    return _Cache(B, H, max_len, D, fp8, weights)
 
 
 def prepare(case, seed):
@@ -163,7 +164,7 @@ def prepare(case, seed):
         return s
     B, H, L = case["B"], case["H"], case["max_len"]
     if kind == "fill_fp8":
-        s.cache = _cache(B, H, L, D, True)
+        s.cache = _cache(B, H, L, D, fp8=True)
         dtype = torch.float32 if case["dtype"] == "f32" else torch.bfloat16
         s.k_heads, s.v_heads = (_values(g, dtype, B, H, case["S"], D) for _ in range(2))
         s.counts = _lengths(g, B, case["S"]) if case["ragged"] else torch.full((B,), case["S"], dtype=torch.int32, device="cuda")
@@ -171,16 +172,15 @@ def prepare(case, seed):
     s.start = _lengths(g, B, case["longest"])
     k, v = (_values(g, torch.bfloat16, B, H, L, D) for _ in range(2))
     if kind == "evict":
-        s.src, s.dst = _cache(B, H, L, D, False), _cache(B, H, L, D, False)
+        s.src, s.dst = _cache(B, H, L, D, weights=True), _cache(B, H, L, D, weights=True)
         s.src.k.copy_(k)
         s.src.v.copy_(v)
         s.src.lengths.copy_(s.start)
         # a few rows gather most of the weight
-        s.weights = torch.empty(B, H, L, device="cuda").exponential_(generator=g).pow_(3.0)
-        s.weights_kept = torch.zeros_like(s.weights)
+        s.src.weights.exponential_(generator=g).pow_(3.0)
         return s
     fp8 = kind == "decode_fp8"
-    s.cache = _cache(B, H, L, D, fp8)
+    s.cache = _cache(B, H, L, D, fp8, case.get("weights", False))
     if fp8:
         _fill_plain(s.cache, k, v, s.start)
     else:
@@ -188,10 +188,8 @@ def prepare(case, seed):
         s.cache.v.copy_(v)
     s.q, s.k_new, s.v_new = (_values(g, torch.bfloat16, B, H, D) for _ in range(3))
     s.out = torch.empty_like(s.q)
-    s.weights = s.weights_start = None
     if case.get("weights"):
         s.weights_start = torch.empty(B, H, L, device="cuda").exponential_(generator=g)
-        s.weights = s.weights_start.clone()
     return s
 
 
@@ -285,9 +283,9 @@ def _decode_window_plain(s):
     seen = _visible(n[:, None], rows[None], case["window"], case["sinks"])
     out, p = _attend(s.q, c.k.float(), c.v.float(), seen, s.scale)
     s.out.copy_(out)
-    if s.weights is not None:
+    if case["weights"]:
         new = rows[None] == n[:, None]
-        s.weights.copy_(torch.where(new[:, None], p, s.weights + p))
+        c.weights.copy_(torch.where(new[:, None], p, c.weights + p))
     c.lengths.copy_(c.lengths + 1)
 
 
@@ -296,7 +294,7 @@ def _evict_plain(s):
     budget, recent, L = case["budget"], case["recent"], case["max_len"]
     n = src.lengths.long()[:, None, None]
     rows = torch.arange(L, device="cuda")
-    key = torch.where(rows < n - recent, s.weights, -1.0)                         # weights are not negative
+    key = torch.where(rows < n - recent, src.weights, -1.0)                         # weights are not negative
     key = torch.where((rows >= n - recent) & (rows < n), float("inf"), key)
     order = torch.sort(key, dim=-1, descending=True, stable=True).indices          # equal ones: lowest index first
     rank = torch.empty_like(order).scatter_(-1, order, rows.expand_as(order))
@@ -308,7 +306,7 @@ def _evict_plain(s):
     for to, rows_of in ((dst.k, src.k), (dst.v, src.v)):
         got = rows_of.gather(2, place[..., None].expand(-1, -1, -1, case["D"]))
         to[:, :, :budget] = torch.where(good[..., None], got, to[:, :, :budget])
-    s.weights_kept[..., :budget] = torch.where(good, s.weights.gather(2, place), s.weights_kept[..., :budget])
+    dst.weights[..., :budget] = torch.where(good, src.weights.gather(2, place), dst.weights[..., :budget])
     dst.lengths.copy_(src.lengths.clamp(max=budget))
 
 
@@ -355,10 +353,10 @@ def run(s):
         return s.out, s.lse, s.dq, s.dk, s.dv
     if kind == "evict":
         if own:
-            dad.kv_cache_evict_bf16(s.dst, s.src, s.weights_kept, s.weights, case["budget"], case["recent"])
+            dad.kv_cache_evict_bf16(s.dst, s.src, case["budget"], case["recent"])
         else:
             _evict_plain(s)
-        return s.dst.k, s.dst.v, s.weights_kept, s.dst.lengths
+        return s.dst.k, s.dst.v, s.dst.weights, s.dst.lengths
     c = s.cache
     c.lengths.copy_(s.start)   # the same token again
     if kind == "decode_fp8":
@@ -367,14 +365,14 @@ def run(s):
         else:
             _decode_fp8_plain(s)
         return s.out, c.k, c.v, c.k_scale, c.v_scale, c.k_tail, c.v_tail, c.lengths
-    if s.weights is not None:
-        s.weights.copy_(s.weights_start)
+    if case["weights"]:
+        c.weights.copy_(s.weights_start)
     if own:
         dad.decode_attention_bf16_window(s.out, s.q, s.k_new, s.v_new, c, s.scale, window=case["window"],
-                                         sinks=case["sinks"], weights=s.weights)
+                                         sinks=case["sinks"], weights=case["weights"])
     else:
         _decode_window_plain(s)
-    return s.out, c.k, c.v, c.lengths, s.weights
+    return s.out, c.k, c.v, c.lengths, c.weights
 
 
 def _mean_rows(case):
@@ -452,7 +450,7 @@ def _exact_decode(s, case):
     B, H, D = case["B"], case["H"], case["D"]
     fp8 = case["kind"] == "decode_fp8"
     out = torch.empty(B, H, D, dtype=torch.float64, device="cuda")
-    weights = None if s.weights is None else s.weights_start.double()
+    weights = s.weights_start.double() if case.get("weights") else None
     for b, n in enumerate(s.start.tolist()):
         sides = []
         for data, new in ((s.cache.k, s.k_new), (s.cache.v, s.v_new)):
