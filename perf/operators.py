@@ -199,8 +199,9 @@ def _quantised(x):
     """[..., tokens, D] in whole blocks -> e4m3 values of the same shape, a power of two for each block: the least that
     keeps the block's largest value within 448 = 0.875 * 2^9."""
     blocks = x.float().unflatten(-2, (-1, BLOCK))
-    mantissa, exponent = torch.frexp(blocks.abs().amax((-1, -2)))
-    exponent = (exponent - 9 + (mantissa > 0.875)).clamp(min=-126)
+    most = blocks.abs().amax((-1, -2))
+    mantissa, exponent = torch.frexp(most)
+    exponent = torch.where(most > 0, exponent - 9 + (mantissa > 0.875), -126).clamp(min=-126)
     scale = torch.ldexp(torch.ones_like(mantissa), exponent)
     return (blocks / scale[..., None, None]).to(torch.float8_e4m3fn).flatten(-3, -2), scale
 
