@@ -36,6 +36,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "decode_common.cuh"
 #include "sm100_ptx.cuh"
 
 namespace dadattn {
@@ -49,40 +50,9 @@ constexpr int kFewStages = 4, kFewPerSm = 3;
 constexpr int kManyStages = 3, kManyPerSm = 4;
 constexpr int kMaxStages = 4;
 constexpr int kItemRing = 2;        // items a CTA's producer may be ahead
-constexpr unsigned kTicketGroups = 32;  // first-level counters of the "all lengths read" tickets
-constexpr int kMaxRanked = 256;     // sequences whose lengths a CTA copies and can rank
 constexpr int kMaxCluster = 8;      // CTAs that share a head of one sequence or two (portable cluster size)
 constexpr int kMaxPaired = 64;      // sequences of a call up to which clusters share two
 constexpr long long kBytesPerRank = 65536;    // and the K + V bytes that are worth one of them
-
-// A 16-byte piece of a row as float pairs, and the softmax's exponential. Scores are kept in units
-// that exp_of() takes: natural units and expf for fp32 caches, log2 units and ex2 for bf16 ones
-// (whose 2^-9 rounding of the inputs is far above the difference).
-template <typename T>
-struct Elem;
-template <>
-struct Elem<float> {
-  static constexpr int kPerLane = 4;
-  static constexpr float kUnit = 1.0f;
-  __device__ static void unpack(float2 (&f)[2], const uint4& raw) {
-    f[0] = make_float2(__uint_as_float(raw.x), __uint_as_float(raw.y));
-    f[1] = make_float2(__uint_as_float(raw.z), __uint_as_float(raw.w));
-  }
-  __device__ static float exp_of(float x) { return expf(x); }
-  __device__ static float from_float(float x) { return x; }
-};
-template <>
-struct Elem<__nv_bfloat16> {
-  static constexpr int kPerLane = 8;
-  static constexpr float kUnit = 1.4426950408889634f;
-  __device__ static void unpack(float2 (&f)[4], const uint4& raw) {
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
-  }
-  __device__ static float exp_of(float x) { return ptx::ex2(x); }
-  __device__ static __nv_bfloat16 from_float(float x) { return __float2bfloat16_rn(x); }
-};
 
 // Workspace: B*H words, of which the first is the item counter, then the 1 + kTicketGroups counters
 // of the "all lengths read" tickets (uint32, all zero between calls), padded to 256 bytes. No more is
@@ -147,23 +117,6 @@ struct DecodeShared {
   };
 };
 
-__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   ptx::smem_u32(smem_dst)),
-               "l"(src), "r"(bytes), "r"(ptx::smem_u32(bar))
-               : "memory");
-}
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-// stores to the same shared-memory variable of another CTA of the cluster
-__device__ __forceinline__ uint32_t cluster_address(const void* own, int cta) {
-  uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(ptx::smem_u32(own)), "r"(cta));
-  return a;
-}
-__device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
-}
 __device__ __forceinline__ void consumers_sync() {
   asm volatile("bar.sync 1, %0;" ::"n"(kDecodeWarps * 32) : "memory");
 }
@@ -236,32 +189,7 @@ decode_kernel(T* __restrict__ out, unsigned* __restrict__ item_counter, unsigned
   if (kPairs && threadIdx.x < 2) sh.member[threadIdx.x] = make_int2(-1, -1);
   __syncthreads();
   if (kPersistent && reorder) {
-    // rank(s) = number of sequences that come before s (longer, or as long with a smaller index);
-    // with the count padded to a power of two n_pad (32..256; padding is INT_MIN and comes last),
-    // 128 threads share out the n_pad^2 comparisons.
-    const int t = threadIdx.x;
-    if (t < 128) {
-      const int lg = 32 - __clz(B - 1);   // n_pad = 1 << lg, 5 <= lg <= 8
-      const int n_pad = 1 << lg;
-      const int groups = lg < 7 ? 128 >> lg : 1;
-      const int per = n_pad / groups, g = (t >> lg) & (groups - 1);
-      for (int si = t & (n_pad - 1); si < n_pad; si += 128) {
-        const int mine = sh.lens[si];
-        int count = 0;
-#pragma unroll 4
-        for (int j = g * per; j < (g + 1) * per; j += 4) {
-          const int4 o = *reinterpret_cast<const int4*>(sh.lens + j);   // broadcast reads
-          count += static_cast<int>(o.x > mine) | (static_cast<int>(o.x == mine) & static_cast<int>(j + 0 < si));
-          count += static_cast<int>(o.y > mine) | (static_cast<int>(o.y == mine) & static_cast<int>(j + 1 < si));
-          count += static_cast<int>(o.z > mine) | (static_cast<int>(o.z == mine) & static_cast<int>(j + 2 < si));
-          count += static_cast<int>(o.w > mine) | (static_cast<int>(o.w == mine) & static_cast<int>(j + 3 < si));
-        }
-        if (count) atomicAdd(&sh.place[si], count);
-      }
-    }
-    __syncthreads();
-    for (int i = t; i < B; i += kDecodeThreads) sh.order[sh.place[i]] = i;
-    __syncthreads();
+    rank_by_length(sh.lens, sh.place, sh.order, B, kDecodeThreads);
   }
 
   // Item e of the call. A sequence whose length is outside [0, max_len) is skipped (rows = 0) and
@@ -321,21 +249,7 @@ decode_kernel(T* __restrict__ out, unsigned* __restrict__ item_counter, unsigned
   // for before the first remote store
   if (!kPersistent) cluster_arrive();
 
-  // Every CTA of the call draws a ticket once it has read the lengths; whoever holds the last one
-  // knows that nobody will read them again and advances them. Two levels keep the atomics off one
-  // address: the CTAs are dealt into kTicketGroups groups; the last of each group draws from a
-  // second counter, and the last of those advances.
-  const unsigned group = blockIdx.x % kTicketGroups;
-  auto draw_ticket = [&]() { return atomicAdd(&seq_tickets[1 + group], 1u); };
-  auto is_last = [&](unsigned ticket) -> bool {
-    const unsigned all_ctas = gridDim.x;
-    if (ticket != (all_ctas - group + kTicketGroups - 1) / kTicketGroups - 1) return false;
-    seq_tickets[1 + group] = 0;   // ready for the next call
-    const unsigned groups = all_ctas < kTicketGroups ? all_ctas : kTicketGroups;
-    if (atomicAdd(&seq_tickets[0], 1u) != groups - 1) return false;
-    seq_tickets[0] = 0;
-    return true;
-  };
+  const LengthTickets tickets{seq_tickets};
 
   volatile int* abort_flag = &sh.abort_flag;
   if (warp == kDecodeWarps) {
@@ -344,9 +258,9 @@ decode_kernel(T* __restrict__ out, unsigned* __restrict__ item_counter, unsigned
       // The ticket is drawn now and looked at once the ring is full: its round trip and the advance
       // of the lengths stay off the path to the kernel's end.
       bool ticket_due = lengths != nullptr && snapshot;
-      const unsigned ticket = ticket_due ? draw_ticket() : 0;
+      const unsigned ticket = ticket_due ? tickets.draw() : 0;
       auto settle_ticket = [&]() {
-        if (ticket_due && is_last(ticket)) {
+        if (ticket_due && tickets.is_last(ticket)) {
           if (early) pdl_wait();   // the kernel ahead may still read the lengths
           for (int j = 0; j < B; ++j) {
             const int len = sh.lens[j];
@@ -618,7 +532,7 @@ decode_kernel(T* __restrict__ out, unsigned* __restrict__ item_counter, unsigned
   if (lengths != nullptr && !snapshot) {   // the lengths were read all along: tickets only now
     __shared__ int sh_advance;
     __syncthreads();
-    if (threadIdx.x == 0) sh_advance = is_last(draw_ticket());
+    if (threadIdx.x == 0) sh_advance = tickets.is_last(tickets.draw());
     __syncthreads();
     if (sh_advance)
       for (int i = threadIdx.x; i < B; i += kDecodeThreads) {
