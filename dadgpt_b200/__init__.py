@@ -7,8 +7,11 @@ the reference's cuda/gpu_ops.cuh, taking torch CUDA tensors for device memory an
 """
 from .attention import (  # noqa: F401
     KVCacheBF16,
+    KVCacheFP8,
     decode_attention_bf16,
+    decode_attention_bf16_window,
     decode_attention_f32,
+    decode_attention_fp8,
     dropout_mask,
     dropout_mask_bits,
     gpu_flash_attention_backward,
@@ -20,6 +23,8 @@ from .attention import (  # noqa: F401
     gpu_flash_attention_forward_bf16_interleaved,
     gpu_flash_attention_forward_via_bf16,
     gpu_flash_attention_supported,
+    kv_cache_evict_bf16,
+    kv_cache_fill_fp8,
     set_decode_early_start,
 )
 

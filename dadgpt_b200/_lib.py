@@ -47,6 +47,12 @@ SIGNATURES = {
     "dadattn_set_decode_early_start": (I, [I]),
     "dadattn_decode_bf16_noalloc": (I, [P] * 7 + [I, I, I, I, F, P]),
     "dadattn_decode_noalloc_status": (I, [P]),
+    "dadattn_decode_window_workspace_bytes": (SZ, [I, I, I, I, I]),
+    "dadattn_decode_bf16_window": (I, [P] * 8 + [I, I, I, I, F, I, I, P, SZ, P]),
+    "dadattn_kv_cache_evict_bf16": (I, [P] * 8 + [I] * 7 + [P]),
+    "dadattn_fp8_scale_blocks": (I, [I]),
+    "dadattn_kv_cache_fill_fp8": (I, [P] * 10 + [I] * 6 + [P]),
+    "dadattn_decode_fp8": (I, [P] * 11 + [I, I, I, I, F, I, I, P, SZ, P]),
     "dadattn_device_status": (I, [P]),
 }
 

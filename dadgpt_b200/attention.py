@@ -137,16 +137,21 @@ def decode_attention_f32(out, q, k_new, v_new, k_cache, v_cache, pos, scale):
 
 class KVCacheBF16:
     """Batched counterpart of the reference's ``struct KVCache`` (src/model.hpp:140-152) for one
-    layer: k, v [B,H,max_len,D] bf16, per-sequence lengths on the device, the decode kernel's workspace."""
+    layer: k, v [B,H,max_len,D] bf16, per-sequence lengths on the device, the decode kernel's workspace.
+    With ``weights``, also the rows' accumulated attention weights [B,H,max_len] fp32, which
+    :func:`decode_attention_bf16_window` adds up and :func:`kv_cache_evict_bf16` goes by."""
 
-    def __init__(self, B, H, max_len, D, device="cuda"):
+    def __init__(self, B, H, max_len, D, device="cuda", weights=False):
         self.B, self.H, self.max_len, self.D = B, H, max_len, D
         self.k = torch.zeros(B, H, max_len, D, dtype=torch.bfloat16, device=device)
         self.v = torch.zeros_like(self.k)
         self.lengths = torch.zeros(B, dtype=torch.int32, device=device)
-        nbytes = int(_lib.load().dadattn_decode_workspace_bytes(B, H, D, max_len))
+        self.weights = torch.zeros(B, H, max_len, dtype=torch.float32, device=device) if weights else None
+        lib = _lib.load()
+        nbytes = max(lib.dadattn_decode_workspace_bytes(B, H, D, max_len),
+                     lib.dadattn_decode_window_workspace_bytes(B, H, D, max_len, 1 if weights else 0))
         # zero-filled once: the counters must start at zero (include/dadattn.h)
-        self.workspace = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        self.workspace = torch.zeros(int(nbytes), dtype=torch.uint8, device=device)
 
 
 def decode_attention_bf16(out, q, k_new, v_new, cache: KVCacheBF16, scale):
@@ -154,6 +159,65 @@ def decode_attention_bf16(out, q, k_new, v_new, cache: KVCacheBF16, scale):
     sequence's length, attend, write out [B,H,D], lengths += 1."""
     _native().decode_bf16(out, q, k_new, v_new, cache.k, cache.v, cache.lengths, cache.B, cache.H, cache.D,
                           cache.max_len, scale, cache.workspace)
+
+
+def decode_attention_bf16_window(out, q, k_new, v_new, cache: KVCacheBF16, scale, *, window=0, sinks=0, weights=False):
+    """:func:`decode_attention_bf16` over a sliding window: the token at row L of its sequence sees row j <= L iff
+    L - j < window or j < sinks (window = 0: every row). With ``weights``, each visible row's probability is added to
+    ``cache.weights`` (and the appended row's weight set to its own); the cache was made with ``weights=True``."""
+    if weights and cache.weights is None:
+        raise ValueError("the cache has no weights: make it with weights=True")
+    _native().decode_bf16_window(cache.B, cache.H, cache.D, cache.max_len, scale, window, sinks, out, q, k_new, v_new,
+                                 cache.k, cache.v, cache.lengths, cache.weights if weights else None, cache.workspace)
+
+
+def kv_cache_evict_bf16(dst: KVCacheBF16, src: KVCacheBF16, budget, recent=0):
+    """Keeps ``budget`` rows of every sequence and head of ``src`` that has more: the last ``recent`` ones and the
+    heaviest of the others by ``src.weights`` (equal ones: the lower index). K, V and weights of the rows that stay go,
+    in order, to rows 0.. of ``dst``, another cache or ``src`` itself, and ``dst.lengths`` becomes min(length, budget)."""
+    if dst.weights is None or src.weights is None:
+        raise ValueError("eviction goes by the weights: make the caches with weights=True")
+    _native().evict_bf16(src.B, src.H, src.D, dst.max_len, src.max_len, budget, recent, dst.k, dst.v, dst.weights,
+                         dst.lengths, src.k, src.v, src.weights, src.lengths)
+
+
+FP8_BLOCK = 64   # tokens that share a scale (DADATTN_FP8_BLOCK)
+
+
+class KVCacheFP8:
+    """A cache of one layer in 8 bits: k, v [B,H,max_len,D] e4m3 codes in blocks of 64 tokens, k_scale, v_scale
+    [B,H,max_len // 64] powers of two, the rows behind the last whole block in k_tail, v_tail [B,H,64,D] bf16,
+    per-sequence lengths on the device, the decode kernel's workspace. Row j of a whole block stands for
+    ``k[b,h,j] * k_scale[b,h,j // 64]``, a later one is ``k_tail[b,h,j % 64]``."""
+
+    def __init__(self, B, H, max_len, D, device="cuda"):
+        self.B, self.H, self.max_len, self.D = B, H, max_len, D
+        lib = _lib.load()
+        self.k = torch.zeros(B, H, max_len, D, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+        self.v = torch.zeros_like(self.k)
+        self.k_scale = torch.ones(B, H, lib.dadattn_fp8_scale_blocks(max_len), dtype=torch.float32, device=device)
+        self.v_scale = torch.ones_like(self.k_scale)
+        self.k_tail = torch.zeros(B, H, FP8_BLOCK, D, dtype=torch.bfloat16, device=device)
+        self.v_tail = torch.zeros_like(self.k_tail)
+        self.lengths = torch.zeros(B, dtype=torch.int32, device=device)
+        nbytes = int(lib.dadattn_decode_window_workspace_bytes(B, H, D, max_len, 0))
+        self.workspace = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+
+
+def kv_cache_fill_fp8(cache: KVCacheFP8, k_heads, v_heads, counts=None):
+    """A prefill's heads [B,H,S,D] (fp32 or bf16) into ``cache``: the first counts[b] rows (int32 [B] on the device;
+    None: all S) of every sequence, which becomes that long."""
+    S = k_heads.shape[2] if k_heads.dim() == 4 else 0   # (other shapes are refused by name)
+    _native().fill_fp8(cache.B, cache.H, S, cache.max_len, cache.D, cache.k, cache.v, cache.k_scale, cache.v_scale,
+                       cache.k_tail, cache.v_tail, cache.lengths, k_heads, v_heads, counts)
+
+
+def decode_attention_fp8(out, q, k_new, v_new, cache: KVCacheFP8, scale, *, window=0, sinks=0):
+    """One decode step for every sequence of an 8-bit ``cache``: append k_new / v_new [B,H,D] bf16, attend over the
+    rows that :func:`decode_attention_bf16_window` would, write out [B,H,D], lengths += 1."""
+    _native().decode_fp8(cache.B, cache.H, cache.D, cache.max_len, scale, window, sinks, out, q, k_new, v_new, cache.k,
+                         cache.v, cache.k_scale, cache.v_scale, cache.k_tail, cache.v_tail, cache.lengths,
+                         cache.workspace)
 
 
 def set_decode_early_start(on: bool) -> None:

@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -30,6 +31,7 @@ const char* type_name(at::ScalarType t) {
     case at::kBFloat16: return "torch.bfloat16";
     case at::kByte: return "torch.uint8";
     case at::kInt: return "torch.int32";
+    case at::kFloat8_e4m3fn: return "torch.float8_e4m3fn";
     default: return c10::toString(t);
   }
 }
@@ -66,6 +68,29 @@ class Args {
       throw Bad{};
     }
     return t;
+  }
+  // the same, on the current device and of the given shape
+  const at::Tensor& here(const char* name, at::ScalarType type, std::initializer_list<int64_t> shape);
+  const at::Tensor& workspace() {
+    const at::Tensor& t = tensor("workspace");
+    if (!t.is_cuda() || !t.is_contiguous()) {
+      PyErr_SetString(PyExc_ValueError, "workspace must be a contiguous CUDA tensor");
+      throw Bad{};
+    }
+    need_current("workspace", t);
+    return t;
+  }
+  static void need_current(const char* name, const at::Tensor& t) {
+    const int current = c10::cuda::current_device();
+    if (t.get_device() == current) return;
+    PyErr_Format(PyExc_ValueError, "%s is on cuda:%d, the current device is cuda:%d", name, static_cast<int>(t.get_device()), current);
+    throw Bad{};
+  }
+  // the type of the next argument, a tensor
+  at::ScalarType peek_type(const char* name) {
+    const at::ScalarType type = tensor(name).scalar_type();
+    --i_;
+    return type;
   }
   bool none() {
     if (a_[i_] != Py_None) return false;
@@ -113,6 +138,13 @@ void need_shape(const char* name, const at::Tensor& t, std::initializer_list<int
   throw Bad{};
 }
 
+const at::Tensor& Args::here(const char* name, at::ScalarType type, std::initializer_list<int64_t> shape) {
+  const at::Tensor& t = need(name, type);
+  need_current(name, t);
+  need_shape(name, t, shape);
+  return t;
+}
+
 void need_shapes(std::initializer_list<std::pair<const char*, std::reference_wrapper<const at::Tensor>>> tensors,
                  std::initializer_list<int64_t> shape) {
   for (const auto& [name, t] : tensors) need_shape(name, t.get(), shape);
@@ -120,6 +152,7 @@ void need_shapes(std::initializer_list<std::pair<const char*, std::reference_wra
 
 void* ptr(const at::Tensor& t) { return t.data_ptr(); }
 float* f32(const at::Tensor& t) { return static_cast<float*>(t.data_ptr()); }
+uint8_t* b8(const at::Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
 uint16_t* b16(const at::Tensor& t) { return static_cast<uint16_t*>(t.data_ptr()); }
 dadattn_stream_t stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 
@@ -156,7 +189,7 @@ PyObject* guarded(F&& f) {
   }
 }
 
-constexpr at::ScalarType kF = at::kFloat, kB = at::kBFloat16;
+constexpr at::ScalarType kF = at::kFloat, kB = at::kBFloat16, k8 = at::kFloat8_e4m3fn;
 
 // out, lse, q, k, v, BH, S, D, scale, rate, seed, offset, unit0
 PyObject* fwd_f32(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -408,6 +441,99 @@ PyObject* decode_bf16(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// B, H, D, max_len, scale, window, sinks, out, q, k_new, v_new, k_cache, v_cache, lengths, weights or None, workspace
+PyObject* decode_bf16_window(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args p(a, n, 16, "decode_bf16_window");
+    const int B = p.integer(), H = p.integer(), D = p.integer(), L = p.integer();
+    const float scale = p.real();
+    const int window = p.integer(), sinks = p.integer();
+    const at::Tensor &out = p.here("out", kB, {B, H, D}), &q = p.here("q", kB, {B, H, D}),
+                     &kn = p.here("k_new", kB, {B, H, D}), &vn = p.here("v_new", kB, {B, H, D}),
+                     &k = p.here("k_cache", kB, {B, H, L, D}), &v = p.here("v_cache", kB, {B, H, L, D}),
+                     &len = p.here("lengths", at::kInt, {B});
+    float* const weights = p.none() ? nullptr : f32(p.here("weights", kF, {B, H, L}));
+    const at::Tensor& ws = p.workspace();
+    int32_t* const lengths = static_cast<int32_t*>(ptr(len));
+    void* const w = ptr(ws);
+    const size_t bytes = ws.nbytes();
+    const dadattn_stream_t st = stream();
+    return done(without_gil([&] {
+      return dadattn_decode_bf16_window(b16(out), b16(q), b16(kn), b16(vn), b16(k), b16(v), lengths, weights, B, H, D, L,
+                                        scale, window, sinks, w, bytes, st);
+    }));
+  });
+}
+
+// B, H, D, max_len, scale, window, sinks, out, q, k_new, v_new, k_cache, v_cache, k_scale, v_scale, k_tail, v_tail,
+// lengths, workspace
+PyObject* decode_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args p(a, n, 19, "decode_fp8");
+    const int B = p.integer(), H = p.integer(), D = p.integer(), L = p.integer();
+    const float scale = p.real();
+    const int window = p.integer(), sinks = p.integer(), blocks = dadattn_fp8_scale_blocks(L);
+    const at::Tensor &out = p.here("out", kB, {B, H, D}), &q = p.here("q", kB, {B, H, D}),
+                     &kn = p.here("k_new", kB, {B, H, D}), &vn = p.here("v_new", kB, {B, H, D}),
+                     &k = p.here("k_cache", k8, {B, H, L, D}), &v = p.here("v_cache", k8, {B, H, L, D}),
+                     &ks = p.here("k_scale", kF, {B, H, blocks}), &vs = p.here("v_scale", kF, {B, H, blocks}),
+                     &kt = p.here("k_tail", kB, {B, H, DADATTN_FP8_BLOCK, D}),
+                     &vt = p.here("v_tail", kB, {B, H, DADATTN_FP8_BLOCK, D}), &len = p.here("lengths", at::kInt, {B});
+    const at::Tensor& ws = p.workspace();
+    int32_t* const lengths = static_cast<int32_t*>(ptr(len));
+    void* const w = ptr(ws);
+    const size_t bytes = ws.nbytes();
+    const dadattn_stream_t st = stream();
+    return done(without_gil([&] {
+      return dadattn_decode_fp8(b16(out), b16(q), b16(kn), b16(vn), b8(k), b8(v), f32(ks), f32(vs), b16(kt), b16(vt),
+                                lengths, B, H, D, L, scale, window, sinks, w, bytes, st);
+    }));
+  });
+}
+
+// B, H, S, max_len, D, k_cache, v_cache, k_scale, v_scale, k_tail, v_tail, lengths, k_heads, v_heads, counts or None
+PyObject* fill_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args p(a, n, 15, "fill_fp8");
+    const int B = p.integer(), H = p.integer(), S = p.integer(), L = p.integer(), D = p.integer();
+    const int blocks = dadattn_fp8_scale_blocks(L);
+    const at::Tensor &k = p.here("k_cache", k8, {B, H, L, D}), &v = p.here("v_cache", k8, {B, H, L, D}),
+                     &ks = p.here("k_scale", kF, {B, H, blocks}), &vs = p.here("v_scale", kF, {B, H, blocks}),
+                     &kt = p.here("k_tail", kB, {B, H, DADATTN_FP8_BLOCK, D}),
+                     &vt = p.here("v_tail", kB, {B, H, DADATTN_FP8_BLOCK, D}), &len = p.here("lengths", at::kInt, {B});
+    const at::ScalarType type = p.peek_type("k_heads") == kB ? kB : kF;
+    const at::Tensor &kh = p.here("k_heads", type, {B, H, S, D}), &vh = p.here("v_heads", type, {B, H, S, D});
+    const int32_t* const counts = p.none() ? nullptr : static_cast<const int32_t*>(ptr(p.here("counts", at::kInt, {B})));
+    int32_t* const lengths = static_cast<int32_t*>(ptr(len));
+    const void *const kp = ptr(kh), *const vp = ptr(vh);
+    const dadattn_stream_t st = stream();
+    return done(without_gil([&] {
+      return dadattn_kv_cache_fill_fp8(b8(k), b8(v), f32(ks), f32(vs), b16(kt), b16(vt), lengths, kp, vp, counts, B, H, S, L,
+                                       D, type == kB, st);
+    }));
+  });
+}
+
+// B, H, D, max_len of the destination and of the source, budget, recent, (k, v, weights, lengths) of both
+PyObject* evict_bf16(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args p(a, n, 15, "evict_bf16");
+    const int B = p.integer(), H = p.integer(), D = p.integer(), Ld = p.integer(), Ls = p.integer(), budget = p.integer(),
+              recent = p.integer();
+    const at::Tensor &kd = p.here("k of the destination", kB, {B, H, Ld, D}), &vd = p.here("v of the destination", kB, {B, H, Ld, D}),
+                     &wd = p.here("weights of the destination", kF, {B, H, Ld}),
+                     &ld = p.here("lengths of the destination", at::kInt, {B}),
+                     &ks = p.here("k of the source", kB, {B, H, Ls, D}), &vs = p.here("v of the source", kB, {B, H, Ls, D}),
+                     &ws = p.here("weights of the source", kF, {B, H, Ls}), &ls = p.here("lengths of the source", at::kInt, {B});
+    int32_t *const to = static_cast<int32_t*>(ptr(ld)), *const from = static_cast<int32_t*>(ptr(ls));
+    const dadattn_stream_t st = stream();
+    return done(without_gil([&] {
+      return dadattn_kv_cache_evict_bf16(b16(kd), b16(vd), f32(wd), to, b16(ks), b16(vs), f32(ws), from, B, H, D, Ld, Ls,
+                                         budget, recent, st);
+    }));
+  });
+}
+
 PyObject* set_error_class(PyObject*, PyObject* cls) {
   Py_XINCREF(cls);
   Py_XDECREF(g_error_class);
@@ -418,7 +544,8 @@ PyObject* set_error_class(PyObject*, PyObject* cls) {
 #define FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {FAST(fwd_f32), FAST(bwd_f32), FAST(fwd_bf16), FAST(bwd_bf16), FAST(fwd_bf16_strided),
                            FAST(bwd_bf16_strided), FAST(fwd_via_bf16), FAST(bwd_via_bf16), FAST(mask_bits),
-                           FAST(decode_f32), FAST(decode_bf16),
+                           FAST(decode_f32), FAST(decode_bf16), FAST(decode_bf16_window), FAST(decode_fp8), FAST(fill_fp8),
+                           FAST(evict_bf16),
                            {"set_error_class", set_error_class, METH_O, nullptr},
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

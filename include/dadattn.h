@@ -317,6 +317,73 @@ int dadattn_decode_bf16_noalloc(uint16_t* out, const uint16_t* q, const uint16_t
  * stays usable). No counterpart in the reference. */
 int dadattn_decode_noalloc_status(dadattn_stream_t stream);
 
+/* ---- decode over part of a cache, with the attention weights added up ---------------------------- */
+
+/* Largest max_len of the calls below. */
+#define DADATTN_MAX_CACHE_LEN (1 << 30)
+
+/* dadattn_decode_bf16 over the rows that a sliding window leaves visible (no counterpart in the reference, which attends
+ * over everything): the token at row L = lengths[b] sees row j <= L iff L - j < window or j < sinks; window = 0: all rows.
+ * Rows that are not seen are not read. The token is appended and lengths[b] advanced as in dadattn_decode_bf16, a sequence
+ * with L outside [0, max_len) is left untouched and reported the same way.
+ * weights (may be NULL): [B,H,max_len] fp32. Each visible row's softmax probability is added to its weight, and the
+ * appended row's weight is set to its probability, so that nothing has to be cleared when a sequence starts.
+ * workspace: at least dadattn_decode_window_workspace_bytes(B, H, D, max_len, weights != NULL) bytes, 16-byte aligned, with
+ * the rules of dadattn_decode_bf16's: zero-filled once, to be zero-filled again when B, H or max_len change, not shared by
+ * calls that overlap on the GPU (two replays of captured graphs among them). Calls of dadattn_decode_bf16 on the same B, H
+ * and max_len may use the same workspace in turn, where it is as large as both ask for. These calls never start early. */
+size_t dadattn_decode_window_workspace_bytes(int B, int H, int D, int max_len, int with_weights);
+int dadattn_decode_bf16_window(uint16_t* out, const uint16_t* q, const uint16_t* k_new, const uint16_t* v_new,
+                               uint16_t* k_cache, uint16_t* v_cache, int32_t* lengths, float* weights, int B, int H, int D,
+                               int max_len, float scale, int window, int sinks, void* workspace, size_t workspace_bytes,
+                               dadattn_stream_t stream);
+
+/* Eviction by accumulated weight. Per (sequence, head), of n = lengths_src[b] rows: all stay where n <= budget; else the
+ * last `recent` rows and, of the others, the budget - recent with the largest weights (equal ones: the lower index; NaN
+ * counts as the least). What stays is moved to rows 0.. of the destination, in order, K, V and weight alike, and
+ * lengths_dst[b] becomes min(n, budget). Other rows of the destination are left as they were.
+ * k, v [B,H,max_len,D] bf16, weights [B,H,max_len] fp32, 1 <= budget <= max_len_dst, 0 <= recent <= budget. The destination
+ * is another cache, or the source itself (all four arrays the same; the arrays do not overlap otherwise). A sequence whose
+ * length is outside [0, max_len_src] is left untouched and reported through DADATTN_E_ARG at the next
+ * dadattn_device_status(). Every head keeps rows of its own choice: only for models whose keys do not depend on the row they
+ * lie in (positions added to the embeddings, as in GPT-2, or rotated into the keys before they are cached), and without
+ * dadattn_decode_bf16_window's window, which counts rows. No counterpart in the reference. */
+int dadattn_kv_cache_evict_bf16(uint16_t* k_dst, uint16_t* v_dst, float* weights_dst, int32_t* lengths_dst,
+                                const uint16_t* k_src, const uint16_t* v_src, const float* weights_src,
+                                const int32_t* lengths_src, int B, int H, int D, int max_len_dst, int max_len_src, int budget,
+                                int recent, dadattn_stream_t stream);
+
+/* ---- 8-bit KV cache ------------------------------------------------------------------------------ */
+
+/* A cache in 8 bits with a scale for each block of DADATTN_FP8_BLOCK tokens and head (no counterpart in the reference):
+ *   k_cache, v_cache [B,H,max_len,D] e4m3 codes; rows of whole blocks. Row j stands for code * scale[b,h,j / 64].
+ *   k_scale, v_scale [B,H,dadattn_fp8_scale_blocks(max_len)] fp32 powers of two: the least 2^e, e >= -126, with which the
+ *     block's largest finite element is at most 448 * 2^e. Infinities and NaN are kept as NaN.
+ *   k_tail, v_tail [B,H,64,D] bf16: the rows behind the last whole block, row j at j % 64.
+ *   lengths [B] int32.
+ * An element is rounded to bf16 (where it is not already) and then, when its block is complete, once to e4m3: by at most
+ * 2^-4 of itself, or 2^-10 of the scale where that is more. A cache holds the same bytes whether a prompt filled it or
+ * single tokens did. */
+#define DADATTN_FP8_BLOCK 64
+int dadattn_fp8_scale_blocks(int max_len);   /* max_len / 64, one at least */
+
+/* Fills the first counts[b] rows of every sequence from a prefill's heads k_heads, v_heads [B,H,S,D] (fp32, or bf16 when
+ * heads_are_bf16; rows behind counts[b] are padding and not read) and sets lengths[b] = counts[b]. counts NULL: S rows of
+ * every sequence (S <= max_len). A sequence with counts[b] outside [0, min(S, max_len)] is left untouched and reported
+ * through DADATTN_E_ARG at the next dadattn_device_status(). D 64 or 128; one sequence of a larger cache: pointers to its
+ * part and B = 1. */
+int dadattn_kv_cache_fill_fp8(uint8_t* k_cache, uint8_t* v_cache, float* k_scale, float* v_scale, uint16_t* k_tail,
+                              uint16_t* v_tail, int32_t* lengths, const void* k_heads, const void* v_heads,
+                              const int32_t* counts, int B, int H, int S, int max_len, int D, int heads_are_bf16,
+                              dadattn_stream_t stream);
+
+/* dadattn_decode_bf16_window on an 8-bit cache (without weights): the token goes to the tail, the visible rows are attended
+ * to in fp32 arithmetic, and a tail that is then full becomes a block. workspace as there, with_weights = 0. */
+int dadattn_decode_fp8(uint16_t* out, const uint16_t* q, const uint16_t* k_new, const uint16_t* v_new, uint8_t* k_cache,
+                       uint8_t* v_cache, float* k_scale, float* v_scale, uint16_t* k_tail, uint16_t* v_tail,
+                       int32_t* lengths, int B, int H, int D, int max_len, float scale, int window, int sinks,
+                       void* workspace, size_t workspace_bytes, dadattn_stream_t stream);
+
 /* Synchronises the stream and returns the sticky device-side status word of this device
  * (0, or a DADATTN_E_* code recorded by a kernel: a bounded wait that ran out, a sequence at
  * max_len). Clears the word. For a wait that ran out dadattn_last_error() names the source line
