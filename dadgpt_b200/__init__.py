@@ -17,10 +17,12 @@ from .attention import (  # noqa: F401
     gpu_flash_attention_backward,
     gpu_flash_attention_backward_bf16,
     gpu_flash_attention_backward_bf16_interleaved,
+    gpu_flash_attention_backward_bf16_window,
     gpu_flash_attention_backward_via_bf16,
     gpu_flash_attention_forward,
     gpu_flash_attention_forward_bf16,
     gpu_flash_attention_forward_bf16_interleaved,
+    gpu_flash_attention_forward_bf16_window,
     gpu_flash_attention_forward_via_bf16,
     gpu_flash_attention_supported,
     kv_cache_evict_bf16,

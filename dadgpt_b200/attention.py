@@ -96,6 +96,22 @@ def gpu_flash_attention_backward_bf16_interleaved(dq, dk, dv, workspace, dout, o
                                offset, unit0)
 
 
+def gpu_flash_attention_forward_bf16_window(out, lse, q, k, v, BH, S, d_head, scale, window, sinks=0):
+    """bf16 forward with a sliding window: query i sees key j <= i iff i - j < window or j < sinks (window = 0: every
+    j <= i). Arguments as in :func:`gpu_flash_attention_forward_bf16`; head sizes 64 and 128."""
+    _native().fwd_bf16_window(BH, S, d_head, scale, window, sinks, out, lse, q, k, v)
+
+
+def flash_backward_bf16_window_workspace_bytes(BH, S, d_head) -> int:
+    return int(_lib.load().dadattn_flash_bwd_bf16_window_workspace_bytes(BH, S, d_head))
+
+
+def gpu_flash_attention_backward_bf16_window(dq, dk, dv, workspace, dout, out, lse, q, k, v, BH, S, d_head, scale,
+                                             window, sinks=0):
+    """Backward of the call above, with its ``window`` and ``sinks``."""
+    _native().bwd_bf16_window(BH, S, d_head, scale, window, sinks, dq, dk, dv, workspace, dout, out, lse, q, k, v)
+
+
 def flash_f32_via_bf16_workspace_bytes(BH, S, d_head) -> int:
     return int(_lib.load().dadattn_flash_f32_via_bf16_workspace_bytes(BH, S, d_head))
 

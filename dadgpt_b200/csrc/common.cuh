@@ -204,6 +204,14 @@ int launch_fwd_bf16_d64(uint16_t* out, float* lse, const uint16_t* q, const uint
 // Whether the calling thread's backward is the single-pass one (dadattn_set_bwd_deterministic).
 bool bwd_single_pass();
 
+// Single-pass backward with a sliding window (flash_window_fwd_sm100.cu): 1 <= window <= S, 0 <= sinks <= S.
+int launch_bwd_window_d64(uint16_t* dq, uint16_t* dk, uint16_t* dv, void* workspace, const uint16_t* dout, const uint16_t* out,
+                          const float* lse, const uint16_t* q, const uint16_t* k, const uint16_t* v, int BH, int S,
+                          float scale, int window, int sinks, cudaStream_t st);
+int launch_bwd_window_d128(uint16_t* dq, uint16_t* dk, uint16_t* dv, void* workspace, const uint16_t* dout, const uint16_t* out,
+                           const float* lse, const uint16_t* q, const uint16_t* k, const uint16_t* v, int BH, int S,
+                           float scale, int window, int sinks, cudaStream_t st);
+
 // bf16 operands, fp32 results (flash_f32_via_bf16.cu), head size 64.
 int launch_fwd_bf16_d64_f32(float* out, float* lse, const uint16_t* q, const uint16_t* k, const uint16_t* v, int BH,
                             int S, float scale, cudaStream_t st);

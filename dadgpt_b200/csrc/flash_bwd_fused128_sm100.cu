@@ -99,7 +99,9 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
                : "memory");
 }
 
-template <bool DROP>
+// WINDOW: query q sees key k iff k <= q and (q - k < window or k < sinks). A key tile without first tokens then ends with
+// the last query whose window reaches it; 1 <= window <= S.
+template <bool DROP, bool WINDOW>
 __global__ void __launch_bounds__(kGThreads, 1)
 flash_bwd_fused128_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                           const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
@@ -107,7 +109,7 @@ flash_bwd_fused128_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
                           float* __restrict__ dq_ws, const float* __restrict__ lse,
                           const float* __restrict__ delta, int S, float scale, float rate,
                           const __grid_constant__ PhiloxRounds rng, int64_t unit0, LeveledGrid order,
-                          int* __restrict__ status) {
+                          int* __restrict__ status, int window, int sinks) {
   using L = G128Smem;
   constexpr int D = kGD;
   constexpr uint32_t kTmemCols = 512;
@@ -126,8 +128,8 @@ flash_bwd_fused128_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
   int own, bh;
   if (!leveled_block(order, own, bh)) return;
   const int first = 2 * own;
-  const int n_it = n_sub - first;
   const int k0 = own * kGKeys;
+  const int n_it = (WINDOW && k0 >= sinks ? min((k0 + kGKeys - 1 + window - 1) / kGSub + 1, n_sub) : n_sub) - first;
 
   if ((smem_u32(smem) & 1023u) != 0) {
     if (threadIdx.x == 0) atomicExch(status, DADATTN_E_CUDA);
@@ -363,6 +365,11 @@ flash_bwd_fused128_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
         for (int c = 0; c < 16; ++c)
           if (key > q0 + c) x1[c] = 0u;
       }
+      if (WINDOW && (first + i) * kGSub + kGSub - 1 - k0 >= window && key >= sinks) {   // and across the window's beginning
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+          if (q0 + c - key >= window) x1[c] = 0u;
+      }
       uint32_t keep = 0xffffu;
       if (DROP) {
         // where the warp's 32 x 16 block has visible pairs (the same number of draws in every lane: a warp's loop
@@ -526,10 +533,11 @@ size_t fused128_bwd_workspace_bytes(int BH, int S) {
   return delta_bytes + static_cast<size_t>(BH) * n_sub * kGDqTileBytes;
 }
 
-int launch_bwd_fused_d128(uint16_t* dq, uint16_t* dk, uint16_t* dv, void* workspace, const uint16_t* dout,
-                          const uint16_t* out, const float* lse, const uint16_t* q, const uint16_t* k,
-                          const uint16_t* v, int BH, int S, float scale, float rate, uint64_t seed,
-                          uint64_t offset, int64_t unit0, cudaStream_t st) {
+// window = 0: none
+static int launch_bwd_d128(uint16_t* dq, uint16_t* dk, uint16_t* dv, void* workspace, const uint16_t* dout,
+                           const uint16_t* out, const float* lse, const uint16_t* q, const uint16_t* k,
+                           const uint16_t* v, int BH, int S, float scale, float rate, uint64_t seed,
+                           uint64_t offset, int64_t unit0, int window, int sinks, cudaStream_t st) {
   using BF = __nv_bfloat16;
   const size_t delta_bytes = (static_cast<size_t>(BH) * S * sizeof(float) + 255) / 256 * 256;
   const int n_sub = (S + kGSub - 1) / kGSub;
@@ -560,19 +568,36 @@ int launch_bwd_fused_d128(uint16_t* dq, uint16_t* dk, uint16_t* dv, void* worksp
   //    1536      192 x 1024    278 / 290     3072  192 x 2048  808 / 827      12288  192 x 8192  9441-9477 / 9500-9624
   // (6 x 65536, units one by one: 16.7-17.0 ms / 16.7.) Before the products were issued by a whole warp and dQ
   // left its staging buffer, unit by unit had been the better one beyond 2048 CTAs.
-  const LeveledGrid order = leveled_grid(32768, S, BH);
-  const bool drop = rate > 0.f;
-  auto kern = drop ? flash_bwd_fused128_kernel<true> : flash_bwd_fused128_kernel<false>;
+  // With a window all units are one group: the tiles of the first tokens, which every query sees, are the only long ones
+  // and start ahead of all others. (As long as the grid's second dimension holds the levels.)
+  const bool one_group = window > 0 && (S + kGKeys - 1) / kGKeys <= 65535;
+  const LeveledGrid order = one_group ? LeveledGrid{BH, BH} : leveled_grid(32768, S, BH);
+  const int variant = window > 0 ? 2 : rate > 0.f ? 1 : 0;
+  auto kern = variant == 2 ? flash_bwd_fused128_kernel<false, true>
+              : variant == 1 ? flash_bwd_fused128_kernel<true, false> : flash_bwd_fused128_kernel<false, false>;
   DAD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G128Smem::kBytes));
-  static std::atomic<int> regs_seen[2];
-  if (int rc = check_launch_registers(reinterpret_cast<const void*>(kern), kGRegsLaunch, regs_seen[drop])) return rc;
+  static std::atomic<int> regs_seen[3];
+  if (int rc = check_launch_registers(reinterpret_cast<const void*>(kern), kGRegsLaunch, regs_seen[variant])) return rc;
   DAD_CUDA(launch_pdl(kern, leveled_blocks(order, (S + kGKeys - 1) / kGKeys), dim3(kGThreads),
-                      G128Smem::kBytes, st, mk, mv, mq, mdo, mdk, mdv, dq_ws, lse, static_cast<const float*>(delta), S, scale, rate, rng, unit0, order, status));
+                      G128Smem::kBytes, st, mk, mv, mq, mdo, mdk, mdv, dq_ws, lse, static_cast<const float*>(delta), S, scale, rate, rng, unit0, order, status, window, sinks));
   stage_event(2, st);
   DAD_CUDA(launch_pdl(fused128_convert_kernel, dim3(n_sub, BH), dim3(256), 0, st,
                       reinterpret_cast<BF*>(dq), dq_ws, S, n_sub));
   stage_event(3, st);
   return DADATTN_OK;
+}
+
+int launch_bwd_fused_d128(uint16_t* dq, uint16_t* dk, uint16_t* dv, void* workspace, const uint16_t* dout,
+                          const uint16_t* out, const float* lse, const uint16_t* q, const uint16_t* k,
+                          const uint16_t* v, int BH, int S, float scale, float rate, uint64_t seed,
+                          uint64_t offset, int64_t unit0, cudaStream_t st) {
+  return launch_bwd_d128(dq, dk, dv, workspace, dout, out, lse, q, k, v, BH, S, scale, rate, seed, offset, unit0, 0, 0, st);
+}
+
+int launch_bwd_window_d128(uint16_t* dq, uint16_t* dk, uint16_t* dv, void* workspace, const uint16_t* dout, const uint16_t* out,
+                           const float* lse, const uint16_t* q, const uint16_t* k, const uint16_t* v, int BH, int S,
+                           float scale, int window, int sinks, cudaStream_t st) {
+  return launch_bwd_d128(dq, dk, dv, workspace, dout, out, lse, q, k, v, BH, S, scale, 0.f, 0, 0, 0, window, sinks, st);
 }
 
 }  // namespace dadattn

@@ -125,7 +125,20 @@ __device__ __forceinline__ uint32_t byte_signs(uint32_t w) {
 struct Item {
   int kt, bh, n_it;
 };
-__device__ __forceinline__ Item decode_item(int item, int BH, int n_tiles, int group_bh) {
+// The query tiles that can see key tile kt: all from the diagonal on, or with a window (query q sees key k iff k <= q and
+// (q - k < window or k < sinks); 1 <= window <= S) only those that it reaches from, unless the tile has first tokens.
+// 0 for the end mark, kt = n_tiles.
+template <bool WINDOW>
+struct Reach {
+  int n_tiles, window, sinks;
+  __device__ __forceinline__ int operator()(int kt) const {
+    if (!WINDOW || kt * kFT < sinks) return n_tiles - kt;
+    return min((kt * kFT + kFT - 1 + window - 1) / kFT + 1, n_tiles) - kt;
+  }
+};
+template <bool WINDOW>
+__device__ __forceinline__ Item decode_item(int item, int BH, const Reach<WINDOW>& reach, int group_bh) {
+  const int n_tiles = reach.n_tiles;
   const int per_group = group_bh * n_tiles;
   const int grp = item / per_group;
   const int r = item - grp * per_group;
@@ -134,33 +147,35 @@ __device__ __forceinline__ Item decode_item(int item, int BH, int n_tiles, int g
   Item t;
   t.kt = r / gb;
   t.bh = bh0 + r - t.kt * gb;
-  t.n_it = n_tiles - t.kt;
+  t.n_it = reach(t.kt);
   return t;
 }
 
 // Items are handed out by a global counter; the producer thread takes them and publishes each, decoded
 // (the divisions would sit in every role's chain), through a four-entry ring in shared memory, which the
 // other roles read in the same order. An entry beyond the last item has n_it = 0.
+template <bool WINDOW>
 struct ItemFeed {
   FusedBars* bars;
   volatile int* abort_flag;
-  int n_tiles, n_read;
+  Reach<WINDOW> reach;
+  int n_read;
   // the next item of this CTA; n_it = 0 when there is none (or the kernel is aborting)
   __device__ __forceinline__ Item fetch() {
     const int slot = n_read & (kFRing - 1);
-    if (!mbar_wait(&bars->item_ready[slot], (n_read / kFRing) & 1, abort_flag)) return Item{n_tiles, 0, 0};
+    if (!mbar_wait(&bars->item_ready[slot], (n_read / kFRing) & 1, abort_flag)) return Item{reach.n_tiles, 0, 0};
     const volatile int2& e = bars->ring[slot];
     const int kt = e.x, bh = e.y;
     mbar_arrive(&bars->item_free[slot]);
     ++n_read;
-    return Item{kt, bh, n_tiles - kt};
+    return Item{kt, bh, reach(kt)};
   }
 };
 
 // DROP: 0 = no dropout, 1 = Philox drawn in the kernel, 2 = keep bits read from `mask_bits`
 // (dadattn_dropout_mask_bits; layout in common.cuh). F32: dK and dV leave as fp32, through maps like
 // map_dqw, whose tensor is then the caller's own zero-filled fp32 dQ (nothing rounds it afterwards).
-template <int DROP, bool F32>
+template <int DROP, bool F32, bool WINDOW>
 __global__ void __launch_bounds__(kFThreads, 1)
 flash_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
@@ -168,7 +183,7 @@ flash_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                        const __grid_constant__ CUtensorMap map_dv, const float* __restrict__ lse,
                        const float* __restrict__ delta, int* __restrict__ item_counter, int BH, int S,
                        int heads, int group_bh, float scale, float rate, PhiloxKey rng, int64_t unit0,
-                       const uint32_t* __restrict__ mask_bits, int* __restrict__ status) {
+                       const uint32_t* __restrict__ mask_bits, int* __restrict__ status, int window, int sinks) {
   using L = FusedSmem;
   constexpr int D = kFD;
   constexpr uint32_t kTmemCols = 512;
@@ -183,6 +198,7 @@ flash_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int n_tiles = (S + kFT - 1) / kFT;
   const int n_items = n_tiles * BH;
+  const Reach<WINDOW> reach{n_tiles, window, sinks};
 
   if ((smem_u32(smem) & 1023u) != 0) {
     if (threadIdx.x == 0) atomicExch(status, DADATTN_E_CUDA);
@@ -251,7 +267,7 @@ flash_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       };
       // the first item is the CTA's own index; the counter hands out the rest
       auto decode = [&](int item) -> Item {
-        return item < n_items ? decode_item(item, BH, n_tiles, group_bh) : Item{n_tiles, 0, 0};
+        return item < n_items ? decode_item(item, BH, reach, group_bh) : Item{n_tiles, 0, 0};
       };
       Item t = decode(static_cast<int>(blockIdx.x));
       bool ok = publish(t);
@@ -315,7 +331,7 @@ flash_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         mma_commit(&bars->dp_full);
       };
 
-      ItemFeed feed{bars, abort_flag, n_tiles, 0};
+      ItemFeed<WINDOW> feed{bars, abort_flag, reach, 0};
       int n_it = feed.fetch().n_it, n_nxt = 0;
       bool ok = n_it > 0 && mbar_wait(&bars->kv_full[0], 0, abort_flag) && mbar_wait(&bars->qdo_full[0], 0, abort_flag);
       if (ok) {
@@ -387,7 +403,7 @@ flash_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       const uint64_t keep = l2_policy_evict_last();
       prefetch_tensormap(&map_dk);
       prefetch_tensormap(&map_dv);
-      ItemFeed feed{bars, abort_flag, n_tiles, 0};
+      ItemFeed<WINDOW> feed{bars, abort_flag, reach, 0};
       uint32_t turn = 0;   // parity of the staging panels' use
       auto hand_back = [&]() {
         bulk_wait_read<1>();
@@ -432,7 +448,7 @@ flash_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     // follow the arithmetic that read it, have given their stage back; that barrier's next phase needs
     // this warp's scalars of tile g + 1.
     float* vec = reinterpret_cast<float*>(smem + L::kVec);
-    ItemFeed feed{bars, abort_flag, n_tiles, 0};
+    ItemFeed<WINDOW> feed{bars, abort_flag, reach, 0};
     Item t = feed.fetch();
     Item nxt = t.n_it > 0 ? feed.fetch() : t;
     float rl[4], rd[4];
@@ -477,7 +493,7 @@ flash_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const int quad = warp % 4;
     const int row = quad * 32 + lane;     // TMEM lane = query row (dQ) or key row (dK / dV)
     const uint32_t tlane = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    ItemFeed feed{bars, abort_flag, n_tiles, 0};
+    ItemFeed<WINDOW> feed{bars, abort_flag, reach, 0};
     bool ok = true;
     int g = 0;
     uint32_t back = 1;   // parity of the staging panels' return from their last use (none yet: passes)
@@ -580,7 +596,7 @@ flash_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       return w;
     };
 
-    ItemFeed feed{bars, abort_flag, n_tiles, 0};
+    ItemFeed<WINDOW> feed{bars, abort_flag, reach, 0};
     int g = 0;
 
     for (Item t = feed.fetch(); ok && t.n_it > 0; t = feed.fetch()) {
@@ -615,6 +631,12 @@ flash_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 #pragma unroll
           for (int c = 0; c < 32; ++c)
             if (row > cg * 32 + c) x[c] = 0u;
+        }
+        if (WINDOW && i * kFT + kFT - 1 >= window && t.kt * kFT + row >= sinks) {   // across the window's beginning
+          const int hidden = window + row - (i * kFT + cg * 32);   // columns from here on
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (c >= hidden) x[c] = 0u;
         }
 
         if (DROP == 1 && (!diagonal || quad <= cg)) {   // (beyond the diagonal there is nothing to drop)
@@ -823,8 +845,8 @@ size_t fused_bwd_workspace_bytes(int BH, int S) {
 static int launch_fused_kernel(float* dq_ws, uint16_t* dk, uint16_t* dv, float* f32_dk, float* f32_dv, const float* delta,
                                int* item_counter, const uint16_t* dout, const float* lse, const uint16_t* q,
                                const uint16_t* k, const uint16_t* v, int BH, int S, const UnitLayout& lay, float scale,
-                               float rate, const PhiloxKey& rng, int64_t unit0, const uint32_t* mask_bits,
-                               cudaStream_t st) {
+                               float rate, const PhiloxKey& rng, int64_t unit0, const uint32_t* mask_bits, int window,
+                               int sinks, cudaStream_t st) {
   CUtensorMap mq, mk, mv, mdo, mws, mdk, mdv;
   if (int rc = make_tensor_map_bf16_units(&mq, q, BH, S, kFD, kFT, lay)) return rc;
   if (int rc = make_tensor_map_bf16_units(&mk, k, BH, S, kFD, kFT, lay)) return rc;
@@ -852,16 +874,18 @@ static int launch_fused_kernel(float* dq_ws, uint16_t* dk, uint16_t* dv, float* 
   DAD_CUDA(cudaGetDevice(&dev));
   DAD_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
   dim3 grid(static_cast<unsigned>(n_items < sms ? n_items : sms));
-  const int group_bh = static_cast<int64_t>(BH) * S <= kFAllInL2 ? BH : leveled_grid(65536, S, BH).group;
-  const int variant = f32_dk ? 3 : rate > 0.f ? (mask_bits ? 2 : 1) : 0;
-  auto kern = variant == 3 ? flash_bwd_fused_kernel<0, true> : variant == 2 ? flash_bwd_fused_kernel<2, false>
-              : variant == 1 ? flash_bwd_fused_kernel<1, false> : flash_bwd_fused_kernel<0, false>;
+  // (With a window the tiles of the first tokens, which every query sees, are the only long ones: all units in one group.)
+  const int group_bh = window > 0 || static_cast<int64_t>(BH) * S <= kFAllInL2 ? BH : leveled_grid(65536, S, BH).group;
+  const int variant = window > 0 ? 4 : f32_dk ? 3 : rate > 0.f ? (mask_bits ? 2 : 1) : 0;
+  auto kern = variant == 4 ? flash_bwd_fused_kernel<0, false, true>
+              : variant == 3 ? flash_bwd_fused_kernel<0, true, false> : variant == 2 ? flash_bwd_fused_kernel<2, false, false>
+              : variant == 1 ? flash_bwd_fused_kernel<1, false, false> : flash_bwd_fused_kernel<0, false, false>;
   DAD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FusedSmem::kBytes));
-  static std::atomic<int> regs_seen[4];
+  static std::atomic<int> regs_seen[5];
   if (int rc = check_launch_registers(reinterpret_cast<const void*>(kern), kRegsLaunch, regs_seen[variant])) return rc;
   DAD_CUDA(launch_pdl(kern, grid, dim3(kFThreads), FusedSmem::kBytes, st, mq, mk, mv, mdo, mws, mdk, mdv,
                       lse, delta, item_counter, BH, S, lay.heads, group_bh, scale, rate,
-                      rng, unit0, mask_bits, status));
+                      rng, unit0, mask_bits, status, window, sinks));
   return DADATTN_OK;
 }
 
@@ -871,14 +895,15 @@ int launch_bwd_fused_d64_f32(float* dq32, float* dk32, float* dv32, const float*
                              const uint16_t* dout, const float* lse, const uint16_t* q, const uint16_t* k,
                              const uint16_t* v, int BH, int S, float scale, cudaStream_t st) {
   return launch_fused_kernel(dq32, nullptr, nullptr, dk32, dv32, delta, item_counter, dout, lse, q, k, v, BH, S,
-                             unit_layout(BH, 1, S, kFD, false), scale, 0.f, PhiloxKey{}, 0, nullptr, st);
+                             unit_layout(BH, 1, S, kFD, false), scale, 0.f, PhiloxKey{}, 0, nullptr, 0, 0, st);
 }
 
-int launch_bwd_fused_d64(uint16_t* dq, uint16_t* dk, uint16_t* dv, void* workspace, const uint16_t* dout,
-                         const uint16_t* out, const float* lse, const uint16_t* q, const uint16_t* k,
-                         const uint16_t* v, int BH, int S, float scale, float rate, uint64_t seed,
-                         uint64_t offset, int64_t unit0, const uint32_t* mask_bits, int heads,
-                         cudaStream_t st) {
+// window = 0: none
+static int launch_bwd_d64(uint16_t* dq, uint16_t* dk, uint16_t* dv, void* workspace, const uint16_t* dout,
+                          const uint16_t* out, const float* lse, const uint16_t* q, const uint16_t* k,
+                          const uint16_t* v, int BH, int S, float scale, float rate, uint64_t seed,
+                          uint64_t offset, int64_t unit0, const uint32_t* mask_bits, int heads, int window, int sinks,
+                          cudaStream_t st) {
   using BF = __nv_bfloat16;
   // heads > 0: every bf16 tensor is the interleaved [B*S, heads*64] activation (BH = B * heads)
   const UnitLayout lay = heads > 0 ? unit_layout(BH / heads, heads, S, kFD, true) : unit_layout(BH, 1, S, kFD, false);
@@ -896,7 +921,7 @@ int launch_bwd_fused_d64(uint16_t* dq, uint16_t* dk, uint16_t* dv, void* workspa
                       reinterpret_cast<const BF*>(out), rows, S, lay));
   stage_event(1, st);
   if (int rc = launch_fused_kernel(dq_ws, dk, dv, nullptr, nullptr, delta, item_counter, dout, lse, q, k, v, BH, S, lay,
-                                   scale, rate, make_philox(seed, offset), unit0, mask_bits, st))
+                                   scale, rate, make_philox(seed, offset), unit0, mask_bits, window, sinks, st))
     return rc;
   stage_event(2, st);
   const int64_t n8 = rows * kFD / 8;
@@ -905,6 +930,22 @@ int launch_bwd_fused_d64(uint16_t* dq, uint16_t* dk, uint16_t* dv, void* workspa
                       st, reinterpret_cast<BF*>(dq), dq_ws, n8, S, lay));
   stage_event(3, st);
   return DADATTN_OK;
+}
+
+int launch_bwd_fused_d64(uint16_t* dq, uint16_t* dk, uint16_t* dv, void* workspace, const uint16_t* dout,
+                         const uint16_t* out, const float* lse, const uint16_t* q, const uint16_t* k,
+                         const uint16_t* v, int BH, int S, float scale, float rate, uint64_t seed,
+                         uint64_t offset, int64_t unit0, const uint32_t* mask_bits, int heads,
+                         cudaStream_t st) {
+  return launch_bwd_d64(dq, dk, dv, workspace, dout, out, lse, q, k, v, BH, S, scale, rate, seed, offset, unit0, mask_bits,
+                        heads, 0, 0, st);
+}
+
+int launch_bwd_window_d64(uint16_t* dq, uint16_t* dk, uint16_t* dv, void* workspace, const uint16_t* dout, const uint16_t* out,
+                          const float* lse, const uint16_t* q, const uint16_t* k, const uint16_t* v, int BH, int S,
+                          float scale, int window, int sinks, cudaStream_t st) {
+  return launch_bwd_d64(dq, dk, dv, workspace, dout, out, lse, q, k, v, BH, S, scale, 0.f, 0, 0, 0, nullptr, 0, window,
+                        sinks, st);
 }
 
 }  // namespace dadattn

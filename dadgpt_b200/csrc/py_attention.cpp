@@ -333,6 +333,43 @@ PyObject* bwd_bf16_strided(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// BH, S, D, scale, window, sinks, out, lse, q, k, v
+PyObject* fwd_bf16_window(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args p(a, n, 11, "fwd_bf16_window");
+    const int BH = p.integer(), S = p.integer(), D = p.integer();
+    const float scale = p.real();
+    const int window = p.integer(), sinks = p.integer();
+    const at::Tensor &out = p.here("out", kB, {BH, S, D}), &lse = p.here("lse", kF, {BH, S}), &q = p.here("q", kB, {BH, S, D}),
+                     &k = p.here("k", kB, {BH, S, D}), &v = p.here("v", kB, {BH, S, D});
+    const dadattn_stream_t st = stream();
+    return done(without_gil([&] {
+      return dadattn_flash_fwd_bf16_window(b16(out), f32(lse), b16(q), b16(k), b16(v), BH, S, D, scale, window, sinks, st);
+    }));
+  });
+}
+
+// BH, S, D, scale, window, sinks, dq, dk, dv, workspace, dout, out, lse, q, k, v
+PyObject* bwd_bf16_window(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args p(a, n, 16, "bwd_bf16_window");
+    const int BH = p.integer(), S = p.integer(), D = p.integer();
+    const float scale = p.real();
+    const int window = p.integer(), sinks = p.integer();
+    const at::Tensor &dq = p.here("dq", kB, {BH, S, D}), &dk = p.here("dk", kB, {BH, S, D}), &dv = p.here("dv", kB, {BH, S, D}),
+                     &ws = p.workspace(), &dout = p.here("dout", kB, {BH, S, D}), &out = p.here("out", kB, {BH, S, D}),
+                     &lse = p.here("lse", kF, {BH, S}), &q = p.here("q", kB, {BH, S, D}), &k = p.here("k", kB, {BH, S, D}),
+                     &v = p.here("v", kB, {BH, S, D});
+    void* const w = ptr(ws);
+    const size_t bytes = ws.nbytes();
+    const dadattn_stream_t st = stream();
+    return done(without_gil([&] {
+      return dadattn_flash_bwd_bf16_window(b16(dq), b16(dk), b16(dv), w, bytes, b16(dout), b16(out), f32(lse), b16(q), b16(k),
+                                           b16(v), BH, S, D, scale, window, sinks, st);
+    }));
+  });
+}
+
 // out, lse, q, k, v, BH, S, D, scale, workspace
 PyObject* fwd_via_bf16(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -543,7 +580,7 @@ PyObject* set_error_class(PyObject*, PyObject* cls) {
 
 #define FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {FAST(fwd_f32), FAST(bwd_f32), FAST(fwd_bf16), FAST(bwd_bf16), FAST(fwd_bf16_strided),
-                           FAST(bwd_bf16_strided), FAST(fwd_via_bf16), FAST(bwd_via_bf16), FAST(mask_bits),
+                           FAST(bwd_bf16_strided), FAST(fwd_bf16_window), FAST(bwd_bf16_window), FAST(fwd_via_bf16), FAST(bwd_via_bf16), FAST(mask_bits),
                            FAST(decode_f32), FAST(decode_bf16), FAST(decode_bf16_window), FAST(decode_fp8), FAST(fill_fp8),
                            FAST(evict_bf16),
                            {"set_error_class", set_error_class, METH_O, nullptr},

@@ -36,6 +36,9 @@ extern "C" {
 #define DADATTN_E_TIMEOUT (-4)     /* a bounded device-side wait ran out (see dadattn_device_status) */
 #define DADATTN_E_WORKSPACE (-5)   /* workspace too small */
 
+/* Largest S and max_len of the calls that say so. */
+#define DADATTN_MAX_CACHE_LEN (1 << 30)
+
 typedef void* dadattn_stream_t; /* cudaStream_t */
 
 const char* dadattn_last_error(void);
@@ -169,6 +172,21 @@ int dadattn_flash_bwd_bf16_strided(uint16_t* dq, uint16_t* dk, uint16_t* dv, voi
                                    const uint16_t* v, int B, int H, int S, int D, float scale,
                                    float rate, uint64_t seed, uint64_t offset, int64_t unit0,
                                    dadattn_stream_t stream);
+
+/* dadattn_flash_fwd_bf16 / dadattn_flash_bwd_bf16 with a sliding window (no counterpart in the reference): query i sees
+ * key j iff j <= i and (i - j < window or j < sinks), the first `sinks` tokens staying visible; window = 0: every j <= i.
+ * Head sizes 64 and 128, no dropout. lse is that of the visible scores, and the backward takes the forward's window and
+ * sinks. Keys outside every query's reach cost nothing: work goes by the 64-key tiles (backward: 128-key tiles and the
+ * queries that reach them) with a visible pair in them. As in the calls above, a row that is infinite or NaN makes NaN
+ * of the rows that share a tile with one that sees it. The backward must be the single-pass one (the default), its
+ * workspace is 256-byte aligned. */
+int dadattn_flash_fwd_bf16_window(uint16_t* out, float* lse, const uint16_t* q, const uint16_t* k, const uint16_t* v, int BH,
+                                  int S, int D, float scale, int window, int sinks, dadattn_stream_t stream);
+size_t dadattn_flash_bwd_bf16_window_workspace_bytes(int BH, int S, int D);
+int dadattn_flash_bwd_bf16_window(uint16_t* dq, uint16_t* dk, uint16_t* dv, void* workspace, size_t workspace_bytes,
+                                  const uint16_t* dout, const uint16_t* out, const float* lse, const uint16_t* q,
+                                  const uint16_t* k, const uint16_t* v, int BH, int S, int D, float scale, int window,
+                                  int sinks, dadattn_stream_t stream);
 
 /* By default the backward is a single-pass kernel (one per head size) that forms the
  * probabilities once and adds each key tile's dQ contribution into an fp32 accumulator in the
@@ -319,15 +337,13 @@ int dadattn_decode_noalloc_status(dadattn_stream_t stream);
 
 /* ---- decode over part of a cache, with the attention weights added up ---------------------------- */
 
-/* Largest max_len of the calls below. */
-#define DADATTN_MAX_CACHE_LEN (1 << 30)
-
 /* dadattn_decode_bf16 over the rows that a sliding window leaves visible (no counterpart in the reference, which attends
  * over everything): the token at row L = lengths[b] sees row j <= L iff L - j < window or j < sinks; window = 0: all rows.
  * Rows that are not seen are not read. The token is appended and lengths[b] advanced as in dadattn_decode_bf16, a sequence
  * with L outside [0, max_len) is left untouched and reported the same way.
  * weights (may be NULL): [B,H,max_len] fp32. Each visible row's softmax probability is added to its weight, and the
  * appended row's weight is set to its probability, so that nothing has to be cleared when a sequence starts.
+ * max_len is at most DADATTN_MAX_CACHE_LEN, here and in the calls below.
  * workspace: at least dadattn_decode_window_workspace_bytes(B, H, D, max_len, weights != NULL) bytes, 16-byte aligned, with
  * the rules of dadattn_decode_bf16's: zero-filled once, to be zero-filled again when B, H or max_len change, not shared by
  * calls that overlap on the GPU (two replays of captured graphs among them). Calls of dadattn_decode_bf16 on the same B, H

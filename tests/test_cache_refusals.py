@@ -92,3 +92,36 @@ def test_tensors_are_checked_in_python(lib):
     with pytest.raises(ValueError, match="CUDA tensor"):
         dad.kv_cache_evict_bf16(weighted, weighted, 10)
     assert issubclass(_lib.DadAttnError, RuntimeError)
+
+
+def _forward(lib, **change):
+    a = dict(out=P, lse=P, q=P, k=P, v=P, BH=4, S=100, D=64, scale=0.125, window=8, sinks=2, stream=None)
+    a.update(change)
+    return lib.dadattn_flash_fwd_bf16_window(*a.values())
+
+
+def _backward(lib, **change):
+    a = dict(dq=P, dk=P, dv=P, workspace=P, bytes=1 << 30, dout=P, out=P, lse=P, q=P, k=P, v=P, BH=4, S=100, D=64, scale=0.125,
+             window=8, sinks=2, stream=None)
+    a.update(change)
+    return lib.dadattn_flash_bwd_bf16_window(*a.values())
+
+
+COMMON = [(dict(q=None), -1), (dict(lse=None), -1), (dict(lse=P + 2), -1), (dict(v=P + 8), -1), (dict(BH=0), -1), (dict(S=-1), -1),
+          (dict(BH=65536), -2), (dict(S=(1 << 30) + 1), -2), (dict(D=32), -2), (dict(scale=0.0), -1), (dict(scale=-1.0), -1),
+          (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1), (dict(window=-1), -1), (dict(sinks=-2), -1)]
+
+
+@pytest.mark.parametrize("call,change,code", [(_forward, *c) for c in COMMON] + [(_backward, *c) for c in COMMON] +
+                         [(_backward, dict(workspace=P + 16), -1), (_backward, dict(bytes=100), -5), (_backward, dict(dout=None), -1)],
+                         ids=lambda x: x.__name__ if callable(x) else str(x))
+def test_windowed_attention_refuses(lib, call, change, code):
+    assert call(lib, **change) == code and lib.dadattn_last_error()
+
+
+def test_windowed_attention_checks_tensors(lib):
+    x, lse = torch.zeros(2, 8, 64, dtype=torch.bfloat16), torch.zeros(2, 8)
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        dad.gpu_flash_attention_forward_bf16_window(x, lse, x, x, x, 2, 8, 64, 0.125, 4)
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        dad.gpu_flash_attention_backward_bf16_window(x, x, x, x, x, x, lse, x, x, x, 2, 8, 64, 0.125, 4)
