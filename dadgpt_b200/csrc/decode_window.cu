@@ -696,8 +696,9 @@ int launch(Params p, cudaStream_t st) {
   while (p.ranks < kMaxCluster && p.ranks * kBytesPerRank < bytes && pairs * p.ranks * 2 <= resident) p.ranks *= 2;
   const long long grid = p.ranks > 1 ? pairs * p.ranks : std::min(pairs, static_cast<long long>(resident));
   p.stages = grid <= kFewPerSm * sms ? kFewStages : kManyStages;
-  // Longest first pays once a CTA takes more than one item; the in-kernel ranking handles 32..256 sequences.
-  p.reorder = p.B >= 32 && p.B <= kMaxRanked && pairs > grid;
+  // Longest first pays once a CTA takes more than one item (not under a window, which makes them all alike); the in-kernel
+  // ranking, 0.9 us, handles 32..256 sequences.
+  p.reorder = p.B >= 32 && p.B <= kMaxRanked && pairs > grid && p.window == 0;
   auto kern = p.ranks > 1 ? decode_window_kernel<FP8, D, true, WEIGHTS> : decode_window_kernel<FP8, D, false, WEIGHTS>;
   DAD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(decode_smem(kMaxStages))));
   cudaLaunchConfig_t cfg = {};

@@ -6,16 +6,18 @@
 // One CTA per 128 query rows of one (batch, head) goes through the 64-key tiles that any of its rows sees: those of the
 // first tokens, then from the one where its first row's window begins to the diagonal. Tiles of 64 keys, not 128: a
 // narrow window has few interior tiles, and half a tile less of hidden keys at either end is a third of the work at
-// window 128. An SM holds two CTAs, whose pipelines hide each other's set-up, hand-overs and ends:
+// window 128.
 //   warp 0      TMA producer: Q once, K and V tiles through a ring
-//   warp 1      MMA issuer (one elected lane) and owner of the tensor memory (256 columns):
-//               S = Q K^T (128 x 64 fp32, two buffers), O += P V with P read back from tensor memory
-//   warps 2-    softmax. Head size 64: two threads per row with 32 columns of every tile each, a maximum, a sum and an
-//               accumulator of their own, merged at the end (as flash_fwd64_sm100.cu). Head size 128: one thread per
-//               row, since two accumulators of 128 columns would leave no room for a second CTA.
-// S of the next tile is formed while the exponentials of the current one are computed; the accumulator is rescaled only
-// when a row's maximum has grown by 2^8 (exact all the same); warps that see nothing of a tile store zeros.
-// Every wait is bounded (sm100_ptx.cuh). Barriers and their order are those of flash_bf16_sm100.cu.
+//   warp 1      MMA issuer (one elected lane) and owner of the tensor memory:
+//               S = Q K^T (128 x 64 fp32), O += P V with P read back from tensor memory
+//   warps 2-5   softmax, one thread per row
+// A CTA does six tiles or so, and setting up and ending take as long as four: what counts is that others work meanwhile. So
+// an SM holds four CTAs of head size 64: 128 columns of tensor memory, P over S in one score buffer, whose next scores follow
+// the product with it, and 80 registers, for which a thread reads half of its scores twice. (Two CTAs with two threads per
+// row and two buffers, 192 x 1024, window 256: 46.3 us.) At head size 128 two, whose scores have two buffers: S of the next
+// tile is formed while the exponentials of the current one are computed.
+// The accumulator is rescaled only when a row's maximum has grown by 2^8 (exact all the same); warps that see nothing of a
+// tile store zeros. Every wait is bounded (sm100_ptx.cuh). Barriers as in flash_bf16_sm100.cu.
 #include <cuda_bf16.h>
 
 #include <cfloat>
@@ -39,25 +41,24 @@ constexpr float kRescaleThreshold = 8.0f;  // log2 units: P stays below 2^8
 template <int D>
 struct WindowFwd {
   static constexpr int kPanels = D / 64;
-  static constexpr int kPerRow = D == 64 ? 2 : 1;          // softmax threads of a row
-  static constexpr int kCols = kBN / kPerRow;              // columns of a tile per thread
-  static constexpr int kSoftmax = kBM * kPerRow;
+  static constexpr int kBufs = D == 64 ? 1 : 2;            // score buffers
+  static constexpr int kPerSm = D == 64 ? 4 : 2;           // CTAs
+  static constexpr int kSoftmax = kBM;
   static constexpr int kThreads = 64 + kSoftmax;
-  static constexpr int kStages = D == 64 ? 4 : 2;          // K / V ring depth
+  static constexpr int kStages = 2;                        // K / V ring depth
   static constexpr int kTile = kPanels * kSubPanelBytes;   // a [64, D] tile
   static constexpr int kQ = 0;
   static constexpr int kK = kQ + kPanels * kPanelBytes;
   static constexpr int kV = kK + kStages * kTile;
-  static constexpr int kStat = kV + kStages * kTile;       // (max, sum) of every half of a row
-  static constexpr int kBars = kStat + (kPerRow == 2 ? 2 * kBM * 8 : 0);
+  static constexpr int kBars = kV + kStages * kTile;
   static constexpr int kBytes = kBars + 256;
-  static constexpr uint32_t kColS = 0, kColO = 2 * kBN, kTmemCols = 256;
-  static_assert(kColO + kPerRow * D <= kTmemCols && 2 * (kBytes + 1024) <= 228 * 1024, "two CTAs on an SM");
+  static constexpr uint32_t kColS = 0, kColO = kBufs * kBN, kTmemCols = kColO + D;
+  static_assert(kTmemCols * kPerSm <= 512 && kPerSm * (kBytes + 1024) <= 228 * 1024, "the CTAs of an SM");
 };
 
 struct WindowBars {
-  uint64_t q_full, k_full[4], v_full[4], k_empty[4], v_empty[4];
-  uint64_t s_full[2], p_full[2], o_done[2], stat_full, settled;
+  uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2];
+  uint64_t s_full[2], p_full[2], o_done[2], settled;
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -67,13 +68,13 @@ static_assert(sizeof(WindowBars) <= 256, "barrier block");
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
 template <int D>
-__global__ void __launch_bounds__(WindowFwd<D>::kThreads, 2)
+__global__ void __launch_bounds__(WindowFwd<D>::kThreads, WindowFwd<D>::kPerSm)
 flash_window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_out,
                         float* __restrict__ lse, int S, float scale, int window, int sinks, LeveledGrid order,
                         int* __restrict__ status) {
   using L = WindowFwd<D>;
-  constexpr int kStages = L::kStages, kCols = L::kCols, kPerRow = L::kPerRow;
+  constexpr int kStages = L::kStages, kBufs = L::kBufs;
   extern __shared__ __align__(1024) uint8_t smem[];
   WindowBars* bars = reinterpret_cast<WindowBars*>(smem + L::kBars);
   volatile int* abort_flag = &bars->abort_flag;
@@ -121,7 +122,6 @@ flash_window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       mbar_init(&bars->p_full[b], L::kSoftmax);
       mbar_init(&bars->o_done[b], 1);
     }
-    mbar_init(&bars->stat_full, L::kSoftmax);
     mbar_init(&bars->settled, 1);
     bars->abort_flag = 0;
     fence_mbar_init();
@@ -172,37 +172,36 @@ flash_window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       const SmemDescBase v_desc0 = make_desc_base_sw128(smem_u32(smem + L::kV), kSubPanelBytes);
       bool ok = mbar_wait(&bars->q_full, 0, abort_flag);
 
-      // O_h (+)= P_i[:, columns of h] V_i[rows of h, :], one accumulator for each thread of a row
+      // O (+)= P_i V_i
       auto issue_pv = [&](int i) -> bool {
-        const int s = i % kStages;
+        const int s = i % kStages, buf = i % kBufs;
         if (!mbar_wait(&bars->v_full[s], (i / kStages) & 1, abort_flag)) return false;
-        if (!mbar_wait(&bars->p_full[i & 1], (i >> 1) & 1, abort_flag)) return false;
+        if (!mbar_wait(&bars->p_full[buf], (i / kBufs) & 1, abort_flag)) return false;
         tc_fence_after_sync();
         const SmemDescBase v_desc{v_desc0.lo + s * (L::kTile >> 4), v_desc0.hi};
 #pragma unroll
-        for (int h = 0; h < kPerRow; ++h)
-#pragma unroll
-          for (int kk = 0; kk < kCols / 16; ++kk)
-            mma_ts(tmem + L::kColO + h * D, tmem + L::kColS + (i & 1) * kBN + h * kCols + kk * 8,
-                   desc_at(v_desc, (h * (kCols / 16) + kk) * 2048), idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
+        for (int kk = 0; kk < kBN / 16; ++kk)
+          mma_ts(tmem + L::kColO, tmem + L::kColS + buf * kBN + kk * 8, desc_at(v_desc, kk * 2048), idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
         mma_commit(&bars->v_empty[s]);
         mma_commit(&bars->o_done[i & 1]);
         return true;
       };
 
       for (int j = 0; ok && j < n; ++j) {
-        const int s = j % kStages;
-        // Score buffer j % 2 is overwritten by S_j only after P_{j-2} V_{j-2}, which this thread issued earlier
+        const int s = j % kStages, buf = j % kBufs;
+        // Two buffers: S_j goes over P_{j-2}, behind P_{j-2} V_{j-2}, which this thread issued earlier, and ahead of
+        // P_{j-1} V_{j-1}. One: behind P_{j-1} V_{j-1}.
+        if (kBufs == 1 && j > 0 && !(ok = issue_pv(j - 1))) break;
         if (!(ok = mbar_wait(&bars->k_full[s], (j / kStages) & 1, abort_flag))) break;
         tc_fence_after_sync();
         const SmemDescBase k_desc{k_desc0.lo + s * (L::kTile >> 4), k_desc0.hi};
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          mma_ss(tmem + L::kColS + (j & 1) * kBN, desc_at(q_desc, (kk / 4) * kPanelBytes + (kk % 4) * 32),
+          mma_ss(tmem + L::kColS + buf * kBN, desc_at(q_desc, (kk / 4) * kPanelBytes + (kk % 4) * 32),
                  desc_at(k_desc, (kk / 4) * kSubPanelBytes + (kk % 4) * 32), idesc_s, kk > 0 ? 1u : 0u);
         mma_commit(&bars->k_empty[s]);
-        mma_commit(&bars->s_full[j & 1]);
-        if (j > 0) ok = issue_pv(j - 1);
+        mma_commit(&bars->s_full[buf]);
+        if (kBufs == 2 && j > 0) ok = issue_pv(j - 1);
       }
       if (ok) issue_pv(n - 1);
       settle_products(&bars->settled);
@@ -210,53 +209,54 @@ flash_window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   } else {
     // ------------------------------ softmax ------------------------------
     const int quad = warp % 4;                 // TMEM lane quadrant this warp may touch
-    const int half = (warp - 2) / 4;           // which of a row's threads
     const int row = quad * 32 + lane, r = q0 + row;
     const uint32_t tlane = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    const uint32_t tO = tlane + L::kColO + half * D;
+    const uint32_t tO = tlane + L::kColO;
     const float scale_log2 = scale * kLog2e;
     auto wait_pv = [&](int i) { return mbar_wait(&bars->o_done[i & 1], (i >> 1) & 1, abort_flag); };
     float m = -INFINITY, l = 0.f;   // running max (log2 units, scaled) and sum
     bool ok = true;
 
     for (int j = 0; j < n; ++j) {
-      const int sb = j & 1, t0 = tile_at(j) * kBN, c0 = t0 + half * kCols;
-      const uint32_t tS = tlane + L::kColS + sb * kBN + half * kCols;
+      const int buf = j % kBufs, t0 = tile_at(j) * kBN;
+      const uint32_t tS = tlane + L::kColS + buf * kBN;
       // tiles in which any row of the CTA does not see a key: across the diagonal, or across the window's beginning
       const bool edge = t0 + kBN - 1 > q0 || (t0 <= q0 + kBM - 1 - window && t0 + kBN > sinks);
-      uint32_t seen[kCols / 32];
+      uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
       bool any = true;
       if (edge) {
 #pragma unroll
-        for (int w = 0; w < kCols / 32; ++w) {
-          const int c = c0 + 32 * w;
+        for (int w = 0; w < 2; ++w) {
+          const int c = t0 + 32 * w;
           seen[w] = low_bits(r - c + 1) & (~low_bits(r - window - c + 1) | low_bits(sinks - c));
         }
-        any = __any_sync(0xffffffffu, seen[0] != 0 || seen[kCols / 32 - 1] != 0);
+        any = __any_sync(0xffffffffu, (seen[0] | seen[1]) != 0);
       }
-      if (!(ok = mbar_wait(&bars->s_full[sb], (j >> 1) & 1, abort_flag))) break;
-      tc_fence_after_sync();
-      uint32_t pk[kCols / 2];   // packed P of this thread
-      if (any) {
-        uint32_t x[kCols / 32][32];
-#pragma unroll
-        for (int w = 0; w < kCols / 32; ++w) tmem_ld32(tS + 32 * w, x[w]);
+      // 32 of the thread's scores
+      auto load = [&](uint32_t (&x)[32], int w) {
+        tmem_ld32(tS + 32 * w, x);
         tmem_wait_ld();
         if (edge) {
 #pragma unroll
-          for (int w = 0; w < kCols / 32; ++w)
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!(seen[w] >> i & 1u)) x[w][i] = 0xff800000u;   // -inf
+          for (int i = 0; i < 32; ++i)
+            if (!(seen[w] >> i & 1u)) x[i] = 0xff800000u;   // -inf
         }
-        // max of the raw scores (scale > 0 commutes with max)
-        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      };
+      // max of the raw scores (scale > 0 commutes with max)
+      auto most_of = [&](const uint32_t (&x)[32], float most) -> float {
+        float mx[4] = {most, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int w = 0; w < kCols / 32; ++w)
-#pragma unroll
-          for (int i = 0; i < 32; i += 2)
-            mx4[(i >> 1) & 3] = fmax3(mx4[(i >> 1) & 3], __uint_as_float(x[w][i]), __uint_as_float(x[w][i + 1]));
-        const float mx = __fmul_rn(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), scale_log2);
+        for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+        return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      };
+      if (!(ok = mbar_wait(&bars->s_full[buf], (j / kBufs) & 1, abort_flag))) break;
+      tc_fence_after_sync();
+      if (any) {
+        uint32_t xa[32], xb[32];
+        load(xa, 0);
+        float mx = most_of(xa, -INFINITY);
+        load(xb, 1);
+        mx = __fmul_rn(most_of(xb, mx), scale_log2);
         if (j == 0) {
           m = mx;   // O is first written by an MMA with accumulate = 0: nothing to rescale
         } else if (__any_sync(0xffffffffu, mx > m + kRescaleThreshold)) {
@@ -266,13 +266,13 @@ flash_window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
           // m = -inf: nothing but zeros has been accumulated so far
           const float corr = (m == -INFINITY) ? 0.f : ex2(m - m_new);
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(tO + c * 32, o);
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld16(tO + c * 16, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-            tmem_st32(tO + c * 32, o);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+            tmem_st16(tO + c * 16, o);
           }
           tmem_wait_st();
           l = __fmul_rn(l, corr);
@@ -284,79 +284,63 @@ flash_window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         const float2 sl = make_float2(scale_log2, scale_log2);
         const float neg_m = (m == -INFINITY) ? 0.f : -m;
         const float2 nm = make_float2(neg_m, neg_m);
-#pragma unroll
-        for (int w = 0; w < kCols / 32; ++w)
+        auto weights = [&](const uint32_t (&x)[32], uint32_t (&pk)[16]) {   // packed P
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            const float2 e = ffma2(make_float2(__uint_as_float(x[w][i]), __uint_as_float(x[w][i + 1])), sl, nm);
+            const float2 e = ffma2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sl, nm);
             const float2 p = make_float2(ex2(e.x), ex2(e.y));
             sum2[(i >> 1) & 1] = fadd2(sum2[(i >> 1) & 1], p);
-            pk[w * 16 + i / 2] = pack_bf16(p.x, p.y);
+            pk[i / 2] = pack_bf16(p.x, p.y);
           }
+        };
+        // P goes over S, into its first 32 columns: the second half's scores are read by then, the first half's, where
+        // registers do not hold both, a second time
+        uint32_t pa[16], pb[16];
+        weights(xb, pb);
+        if (kBufs == 1) load(xa, 0);
+        weights(xa, pa);
         l += (sum2[0].x + sum2[1].x) + (sum2[0].y + sum2[1].y);
+        tmem_st16(tS, pa);
+        tmem_st16(tS + 16, pb);
       } else {
+        uint32_t none[16];
 #pragma unroll
-        for (int i = 0; i < kCols / 2; ++i) pk[i] = 0u;
+        for (int i = 0; i < 16; ++i) none[i] = 0u;
+        tmem_st16(tS, none);
+        tmem_st16(tS + 16, none);
       }
-      if constexpr (kCols == 64) tmem_st32(tS, pk);
-      else tmem_st16(tS, pk);
       tmem_wait_st();
       tc_fence_before_sync();
-      mbar_arrive(&bars->p_full[sb]);
+      mbar_arrive(&bars->p_full[buf]);
     }
 
-    // out = O / l, or (O_0 w_0 + O_1 w_1) / (l_0 w_0 + l_1 w_1) with w_h = exp2(m_h - max(m_0, m_1)); lse in natural-log
-    // units of the scaled scores. Results leave through the Q tile, which every product has read, and TMA.
-    float m_tot = m, l_tot = l, f0 = 1.f / l, f1 = 0.f;
-    if (kPerRow == 2 && ok) {
-      float2* stat = reinterpret_cast<float2*>(smem + L::kStat);
-      stat[half * kBM + row] = make_float2(m, l);
-      mbar_arrive(&bars->stat_full);
-      if ((ok = mbar_wait(&bars->stat_full, 0, abort_flag))) {
-        const float2 s0 = stat[row], s1 = stat[kBM + row];
-        m_tot = fmaxf(s0.x, s1.x);   // a row sees its own key: finite
-        const float w0 = (s0.x == -INFINITY) ? 0.f : ex2(s0.x - m_tot);
-        const float w1 = (s1.x == -INFINITY) ? 0.f : ex2(s1.x - m_tot);
-        l_tot = s0.y * w0 + s1.y * w1;
-        f0 = w0 / l_tot, f1 = w1 / l_tot;
-      }
-    }
+    // out = O / l; lse in natural-log units of the scaled scores. Results leave through the Q tile, which every product has
+    // read, and TMA.
     if (ok && wait_pv(n - 1)) {
       tc_fence_after_sync();
-      // a thread writes D / kPerRow columns, 32 at a time: head size 64 as boxes of 64-byte rows, 128 of 128-byte rows
-      constexpr int kRowBytes = kPerRow == 2 ? 64 : 128;
-      uint8_t* stage = smem + L::kQ + half * (kBM * kRowBytes) + quad * 32 * kRowBytes;
+      const float f = 1.f / l;   // (a row sees its own key)
+      uint8_t* stage = smem + L::kQ + quad * 32 * 128;
 #pragma unroll
-      for (int c = 0; c < D / kPerRow / 32; ++c) {
-        uint32_t oa[32], ob[32];
-        tmem_ld32(tlane + L::kColO + (half * (D / kPerRow) + c * 32), oa);
-        if (kPerRow == 2) tmem_ld32(tlane + L::kColO + D + (half * (D / kPerRow) + c * 32), ob);
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(tO + c * 32, o);
         tmem_wait_ld();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float y[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            y[e] = __uint_as_float(oa[8 * i + e]) * f0;
-            if (kPerRow == 2) y[e] = fmaf(__uint_as_float(ob[8 * i + e]), f1, y[e]);
-          }
-          const int at = kPerRow == 2 ? lane * 64 + ((i ^ (lane >> 1 & 3)) << 4)
-                                      : (c / 2) * kPanelBytes + lane * 128 + ((((c & 1) * 4 + i) ^ (lane & 7)) << 4);
-          *reinterpret_cast<uint4*>(stage + at) = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]),
-                                                             pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+          for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(o[8 * i + e]) * f;
+          *reinterpret_cast<uint4*>(stage + (c / 2) * kPanelBytes + lane * 128 + ((((c & 1) * 4 + i) ^ (lane & 7)) << 4)) =
+              make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0 && q0 + quad * 32 < S) {   // (rows beyond S are not written)
-        if (kPerRow == 2) {
-          tma_store_4d(&map_out, stage, half * 32, q0 + quad * 32, 0, bh);
-        } else {
-          for (int p = 0; p < L::kPanels; ++p) tma_store_3d(&map_out, stage + p * kPanelBytes, p * 64, q0 + quad * 32, bh);
-        }
+        for (int p = 0; p < L::kPanels; ++p) tma_store_3d(&map_out, stage + p * kPanelBytes, p * 64, q0 + quad * 32, bh);
         bulk_commit();
       }
-      if (half == 0 && r < S) lse[static_cast<size_t>(bh) * S + r] = (m_tot + log2f(l_tot)) * kLn2;
+      if (r < S) lse[static_cast<size_t>(bh) * S + r] = (m + log2f(l)) * kLn2;
       if (lane == 0) bulk_wait_read<0>();
     }
   }
@@ -380,9 +364,7 @@ int launch_window_fwd(uint16_t* out, float* lse, const uint16_t* q, const uint16
   if (int rc = make_tensor_map_bf16(&mq, q, BH, S, D, kBM)) return rc;
   if (int rc = make_tensor_map_bf16(&mk, k, BH, S, D, kBN)) return rc;
   if (int rc = make_tensor_map_bf16(&mv, v, BH, S, D, kBN)) return rc;
-  if (int rc = L::kPerRow == 2 ? make_tensor_map_rows64(&mo, out, false, BH, S, D, 32, unit_layout(BH, 1, S, D, false))
-                               : make_tensor_map_bf16(&mo, out, BH, S, D, 32))
-    return rc;
+  if (int rc = make_tensor_map_bf16(&mo, out, BH, S, D, 32)) return rc;
   int* status = device_status_word();
   if (!status) return DADATTN_E_CUDA;
   auto kern = flash_window_fwd_kernel<D>;

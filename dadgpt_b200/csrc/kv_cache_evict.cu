@@ -4,16 +4,20 @@
 // (equal ones: the lower index; NaN counts as the least). The rows that stay are moved together, in order, with their
 // weights, into another cache or within their own.
 //
-// The CTAs of a cluster share a (sequence, head): K or V, and columns of the rows. Each finds the selection for itself:
-//   * the weights become integers of the same order in shared memory, and the smallest kept one is found byte by byte from
-//     the top, by histograms of those that agree in the bytes before (four passes, whatever the values);
-//   * the rows are gone through 1024 at a time: a prefix sum over "larger than the smallest kept" and "equal to it" gives
-//     each kept row its place, and 16-byte pieces of the kept rows are copied.
-// Bound by HBM where there are enough (sequence, head) pairs: the weights once, each kept row in and out.
+// The CTAs of a cluster share a (sequence, head):
+//   * each turns the weights of its part of the rows into integers of the same order in shared memory; the smallest kept one is
+//     found byte by byte from the top, by histograms of those that agree in the bytes before, which the cluster adds up
+//     (four passes, whatever the values);
+//   * each counts and numbers the rows of its part that are larger than the smallest kept, and the first ones that are equal
+//     to it, and writes them into the list of every CTA of the cluster;
+//   * the rows of the list are copied in 16-byte pieces: into another cache by shares of the list, within one cache by columns.
+// Bound by HBM where there are enough (sequence, head) pairs: the weights once, each kept row in and out. (Each CTA selecting
+// for itself, and copying as it went through the rows 1024 at a time, took 65 us for 4 x 24 heads of up to 8000 rows, 20 of
+// them histograms and 20 the numbering.)
 //
 // Within one cache: a row's place is never behind the row, so rows that are loaded in order may be stored as soon as every
 // thread has loaded its pieces of the same batch; what is stored lies ahead of all that is loaded later. The columns of a
-// cluster's CTAs are their own. Weights are read by every CTA of the cluster and moved by one: behind a cluster barrier.
+// cluster's CTAs are their own, and the weights, which one of them moves, were read by all behind a cluster barrier.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -26,9 +30,11 @@ namespace dadattn {
 namespace {
 
 constexpr int kEvictThreads = 256;
-constexpr int kChunk = 4 * kEvictThreads;   // rows of a step
 constexpr int kBatch = 4;                   // 16-byte pieces that a thread has in registers
-constexpr int kMaxStaged = 49152;           // rows whose weights fit shared memory (192 KB)
+constexpr int kEvictPerSm = 6;              // CTAs that an SM holds
+constexpr int kMaxParts = 8;                // CTAs of a cluster
+constexpr int kMaxStaged = 24576;           // rows whose weights a CTA has in shared memory (96 KB),
+constexpr int kMaxListed = 24576;           // and kept rows that it has at a time
 
 struct EvictParams {
   uint16_t *k_dst, *v_dst;
@@ -38,16 +44,35 @@ struct EvictParams {
   const float* weights_src;
   const int32_t* lengths_src;
   int* status;
-  int H, D, max_len_dst, max_len_src, budget, recent, parts, staged;
+  int H, D, max_len_dst, max_len_src, budget, recent, parts, listed;
   bool in_place;
 };
 
 struct EvictShared {
-  int histogram[256];
+  int histogram[2][256];   // of this CTA's rows; passes take turns
+  int counts[kMaxParts];   // of every CTA: rows larger than the smallest kept, and equal to it
+  int equals[kMaxParts];
   int warp_total[kEvictThreads / 32];
-  int chosen, above;    // a pass's byte, and how many keys are larger
-  int list[kChunk];     // rows of the step that stay
+  int chosen, above;       // a pass's byte, and how many keys are larger
 };
+
+__device__ __forceinline__ void st_cluster_int(uint32_t addr, int v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ int ld_cluster_int(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+// All CTAs of the cluster
+__device__ __forceinline__ void meet(int parts) {
+  if (parts == 1) {
+    __syncthreads();
+  } else {
+    cluster_arrive();
+    cluster_wait();
+  }
+}
 
 // An integer of the same order; zeros of either sign are equal, NaN is the least.
 __device__ __forceinline__ uint32_t key_of(float w) {
@@ -79,13 +104,17 @@ __device__ __forceinline__ int prefix_sum(EvictShared& sh, int mine, int& total)
   return before + sum - mine;
 }
 
-__global__ void __launch_bounds__(kEvictThreads) kv_cache_evict_kernel(const EvictParams p) {
-  extern __shared__ __align__(16) uint32_t keys[];   // the weights of a staged call, then nothing
+__global__ void __launch_bounds__(kEvictThreads, kEvictPerSm) kv_cache_evict_kernel(const __grid_constant__ EvictParams p) {
+  extern __shared__ __align__(16) int dynamic[];   // the list, then the keys of this CTA's rows
+  int* list = dynamic;
+  uint32_t* keys = reinterpret_cast<uint32_t*>(dynamic + p.listed);
   __shared__ EvictShared sh;
+  const int parts = p.parts, part = static_cast<int>(blockIdx.x) % parts, bh = static_cast<int>(blockIdx.x) / parts, b = bh / p.H;
+  const int t = threadIdx.x, D = p.D;
+  sh.histogram[0][t] = 0;
+  sh.histogram[1][t] = 0;
   pdl_wait();
   pdl_launch_dependents();
-  const int part = static_cast<int>(blockIdx.x) % p.parts, bh = static_cast<int>(blockIdx.x) / p.parts, b = bh / p.H;
-  const int t = threadIdx.x;
   const int n = p.lengths_src[b];
   // (the same for all CTAs of a cluster, who leave together)
   if (n < 0 || n > p.max_len_src) {
@@ -99,11 +128,10 @@ __global__ void __launch_bounds__(kEvictThreads) kv_cache_evict_kernel(const Evi
   const bool all = n <= p.budget;
   const int candidates = all ? 0 : n - p.recent;   // rows that are chosen from; those behind stay
   const int wanted = all ? 0 : p.budget - p.recent;
-  auto key = [&](int row) { return p.staged ? keys[row] : key_of(weights[row]); };
-  if (p.staged) {
+  // this CTA's rows, and those of them that are chosen from
+  const int share = (n + parts - 1) / parts, row0 = min(part * share, n), row1 = min(row0 + share, n), end = min(row1, candidates);
 #pragma unroll 4
-    for (int row = t; row < candidates; row += kEvictThreads) keys[row] = key_of(weights[row]);
-  }
+  for (int row = row0 + t; row < end; row += kEvictThreads) keys[row - row0] = key_of(weights[row]);
 
   // The smallest kept key, and how many of the rows that have it stay (the first ones).
   uint32_t least = 0xffffffffu;
@@ -111,18 +139,30 @@ __global__ void __launch_bounds__(kEvictThreads) kv_cache_evict_kernel(const Evi
   if (wanted > 0) {
     uint32_t prefix = 0;
     int left = wanted;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      sh.histogram[t] = 0;
-      __syncthreads();
+    for (int shift = 24, turn = 0; shift >= 0; shift -= 8, turn ^= 1) {
+      __syncthreads();   // (the keys, and the cleared histogram)
+      int* histogram = sh.histogram[turn];
 #pragma unroll 4
-      for (int row = t; row < candidates; row += kEvictThreads) {
-        const uint32_t k = key(row);
+      for (int row = t; row < end - row0; row += kEvictThreads) {
+        const uint32_t k = keys[row];
         // (shift + 8 = 32 in the first pass: every key counts)
-        if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&sh.histogram[(k >> shift) & 255u], 1);
+        if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&histogram[(k >> shift) & 255u], 1);
       }
-      __syncthreads();
-      // thread t has byte 255 - t: the sums before it are of the larger bytes
-      const int mine = sh.histogram[255 - t];
+      meet(parts);
+      // thread t has byte 255 - t of all CTAs: the sums before it are of the larger bytes
+      int mine = 0;
+      if (parts == 1) {
+        mine = histogram[255 - t];
+      } else {
+        int of[kMaxParts];   // (all on their way together)
+#pragma unroll
+        for (int i = 0; i < kMaxParts; ++i)
+          if (i < parts) of[i] = ld_cluster_int(cluster_address(&histogram[255 - t], i));
+#pragma unroll
+        for (int i = 0; i < kMaxParts; ++i)
+          if (i < parts) mine += of[i];
+      }
+      sh.histogram[turn ^ 1][t] = 0;   // (everybody is past the pass before)
       int total;
       const int above = prefix_sum(sh, mine, total);
       if (above < left && left <= above + mine) {
@@ -136,77 +176,104 @@ __global__ void __launch_bounds__(kEvictThreads) kv_cache_evict_kernel(const Evi
     least = prefix;
     equal_wanted = left;
   }
-  if (p.parts > 1 && p.in_place) {   // (only staged calls come here: every CTA has its copy of the weights)
-    __syncthreads();
-    cluster_arrive();
-    cluster_wait();
+  auto is_larger = [&](int row) { return row >= candidates || (wanted > 0 && keys[row - row0] > least); };
+  auto is_equal = [&](int row) { return row < candidates && wanted > 0 && keys[row - row0] == least; };
+
+  // How many rows of the CTAs before this one stay
+  int counted = 0;
+  for (int row = row0 + t; row < row1; row += kEvictThreads) {
+    if (is_larger(row)) ++counted;
+    else if (is_equal(row)) counted += 1 << 16;
+  }
+  int larger = 0, equal = 0;
+  {   // (a part has no more than kMaxStaged < 2^16 rows)
+    int total;
+    prefix_sum(sh, counted, total);
+    if (t < parts) {
+      st_cluster_int(cluster_address(&sh.counts[part], t), total & 0xffff);
+      st_cluster_int(cluster_address(&sh.equals[part], t), total >> 16);
+    }
+    meet(parts);   // (and every CTA has read its weights: one of them may move them now)
+    for (int i = 0; i < part; ++i) larger += sh.counts[i], equal += sh.equals[i];
   }
 
-  const bool both = p.parts == 1;
-  const int slices = both ? 1 : p.parts / 2, pieces = p.D / 8 / slices;   // 16-byte pieces of a row that are this CTA's
-  const int shift = 31 - __clz(pieces), column = (both ? 0 : part / 2) * pieces;
-  const int row_pieces = p.D / 8;
-  int larger = 0, equal = 0;   // rows before the step that are larger than the least, and that are equal to it
-  int done = 0;                // rows kept before the step
-  for (int row0 = 0; row0 < n; row0 += kChunk) {
-    // a thread's four rows: bit i of `gt`, `eq`
-    int gt = 0, eq = 0;
-    float w[4];
+  const int row_pieces = D / 8;   // 16-byte pieces of a row
+  const size_t src0 = static_cast<size_t>(bh) * p.max_len_src, dst0 = static_cast<size_t>(bh) * p.max_len_dst;
+  for (int begin = 0; begin < kept; begin += p.listed) {   // (one turn, unless the budget is larger than the list)
+    const int count = min(kept - begin, p.listed);
+    // Numbers of this CTA's kept rows, into all lists: a thread has four rows in turn of 1024
+    int before_gt = larger, before_eq = equal;
+    for (int r0 = row0; r0 < row1; r0 += 4 * kEvictThreads) {
+      int gt = 0, eq = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = row0 + 4 * t + i;
-      w[i] = 0.f;
-      if (row < n) {
-        if (part == 0) w[i] = weights[row];
-        if (row >= candidates) {
-          gt |= 1 << i;
-        } else if (wanted > 0) {
-          const uint32_t k = key(row);
-          if (k > least) gt |= 1 << i;
-          else if (k == least) eq |= 1 << i;
+      for (int i = 0; i < 4; ++i) {
+        const int row = r0 + 4 * t + i;
+        if (row < row1) {
+          if (is_larger(row)) gt |= 1 << i;
+          else if (is_equal(row)) eq |= 1 << i;
         }
       }
-    }
-    int total;
-    const int before = prefix_sum(sh, __popc(gt) | __popc(eq) << 16, total);
-    int g = larger + (before & 0xffff), e = equal + (before >> 16);
-    const int first = done;
+      int total;
+      const int before = prefix_sum(sh, __popc(gt) | __popc(eq) << 16, total);
+      int g = before_gt + (before & 0xffff), e = before_eq + (before >> 16);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool is_gt = gt >> i & 1, is_eq = eq >> i & 1;
-      const int place = g + min(e, equal_wanted);
-      if (is_gt || (is_eq && e < equal_wanted)) {
-        sh.list[place - first] = row0 + 4 * t + i;
-        // (every thread has read its weights of this step, and what is stored lies ahead of the steps to come)
-        if (part == 0) p.weights_dst[static_cast<size_t>(bh) * p.max_len_dst + place] = w[i];
+      for (int i = 0; i < 4; ++i) {
+        const bool is_gt = gt >> i & 1, is_eq = eq >> i & 1;
+        const int place = g + min(e, equal_wanted) - begin;
+        if ((is_gt || (is_eq && e < equal_wanted)) && place >= 0 && place < count)
+          for (int j = 0; j < parts; ++j) st_cluster_int(cluster_address(&list[place], j), r0 + 4 * t + i);
+        g += is_gt;
+        e += is_eq;
       }
-      g += is_gt;
-      e += is_eq;
+      before_gt += total & 0xffff;
+      before_eq += total >> 16;
     }
-    larger += total & 0xffff;
-    equal += total >> 16;
-    done = larger + min(equal, equal_wanted);
-    __syncthreads();
-    const int count = (done - first) << shift;
-    for (int side = both ? 0 : part % 2; side < (both ? 2 : part % 2 + 1); ++side) {
-      const uint4* src = reinterpret_cast<const uint4*>(side ? p.v_src : p.k_src) + static_cast<size_t>(bh) * p.max_len_src * row_pieces + column;
-      uint4* dst = reinterpret_cast<uint4*>(side ? p.v_dst : p.k_dst) + (static_cast<size_t>(bh) * p.max_len_dst + first) * row_pieces + column;
-      for (int i0 = 0; i0 < count; i0 += kBatch * kEvictThreads) {
+    meet(parts);   // the list is there
+
+    // another cache: a share of the rows; the same: a share of the columns, of K or of V where the cluster is large enough
+    const bool by_rows = !p.in_place;
+    const int sides = by_rows || parts == 1 ? 2 : 1, slices = by_rows || parts == 1 ? 1 : parts / 2;
+    const int pieces = row_pieces / slices, shift = 31 - __clz(pieces);
+    const int column = by_rows || parts == 1 ? 0 : part / 2 * pieces;
+    const int first = by_rows ? static_cast<int>(static_cast<long long>(count) * part / parts) : 0;
+    const int last = by_rows ? static_cast<int>(static_cast<long long>(count) * (part + 1) / parts) : count;
+    const int work = (last - first) << shift;
+    for (int i = 0; i < sides; ++i) {
+      const bool is_v = sides == 2 ? i : part % 2;
+      const uint4* src = reinterpret_cast<const uint4*>(is_v ? p.v_src : p.k_src) + src0 * row_pieces + column;
+      uint4* dst = reinterpret_cast<uint4*>(is_v ? p.v_dst : p.k_dst) + (dst0 + begin + first) * row_pieces + column;
+      for (int i0 = 0; i0 < work; i0 += kBatch * kEvictThreads) {
         uint4 x[kBatch];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int at = i0 + i * kEvictThreads + t;
-          if (at < count) x[i] = src[static_cast<size_t>(sh.list[at >> shift]) * row_pieces + (at & (pieces - 1))];
+        for (int j = 0; j < kBatch; ++j) {
+          const int at = i0 + j * kEvictThreads + t;
+          if (at < work) x[j] = src[static_cast<size_t>(list[first + (at >> shift)]) * row_pieces + (at & (pieces - 1))];
         }
         if (p.in_place) __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int at = i0 + i * kEvictThreads + t;
-          if (at < count) dst[static_cast<size_t>(at >> shift) * row_pieces + (at & (pieces - 1))] = x[i];
+        for (int j = 0; j < kBatch; ++j) {
+          const int at = i0 + j * kEvictThreads + t;
+          if (at < work) dst[static_cast<size_t>(at >> shift) * row_pieces + (at & (pieces - 1))] = x[j];
         }
       }
     }
-    __syncthreads();   // the list is read
+    if (by_rows || part == 0) {
+      for (int i0 = first; i0 < last; i0 += kBatch * kEvictThreads) {
+        float x[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int at = i0 + j * kEvictThreads + t;
+          if (at < last) x[j] = weights[list[at]];
+        }
+        if (p.in_place) __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int at = i0 + j * kEvictThreads + t;
+          if (at < last) p.weights_dst[dst0 + begin + at] = x[j];
+        }
+      }
+    }
+    if (begin + p.listed < kept) meet(parts);   // the list is read
   }
 }
 
@@ -239,8 +306,8 @@ extern "C" int dadattn_kv_cache_evict_bf16(uint16_t* k_dst, uint16_t* v_dst, flo
     if (!dst[i] || !src[i]) return fail(DADATTN_E_ARG, "cache eviction: null pointer");
   if (B <= 0 || H <= 0 || max_len_dst <= 0 || max_len_src <= 0 || static_cast<long long>(B) * H > 0x7fffffffLL / 8)
     return fail(DADATTN_E_ARG, "cache eviction: bad sizes B=%d H=%d max_len %d and %d", B, H, max_len_dst, max_len_src);
-  if (max_len_dst > DADATTN_MAX_CACHE_LEN || max_len_src > DADATTN_MAX_CACHE_LEN)
-    return fail(DADATTN_E_UNSUPPORTED, "cache eviction: max_len may not exceed %d", DADATTN_MAX_CACHE_LEN);
+  if (max_len_dst > DADATTN_MAX_CACHE_LEN || max_len_src > kMaxParts * kMaxStaged)
+    return fail(DADATTN_E_UNSUPPORTED, "cache eviction: max_len of the source may not exceed %d", kMaxParts * kMaxStaged);
   if (D != 64 && D != 128) return fail(DADATTN_E_UNSUPPORTED, "cache eviction: unsupported D %d", D);
   if (budget < 1 || budget > max_len_dst || recent < 0 || recent > budget)
     return fail(DADATTN_E_ARG, "cache eviction: budget %d must be in [1, %d], recent %d in [0, budget]", budget, max_len_dst, recent);
@@ -266,13 +333,13 @@ extern "C" int dadattn_kv_cache_evict_bf16(uint16_t* k_dst, uint16_t* v_dst, flo
   DAD_CUDA(cudaGetDevice(&dev));
   DAD_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
   EvictParams p = {k_dst, v_dst, weights_dst, lengths_dst, k_src, v_src, weights_src, lengths_src, device_status_word(),
-                   H, D, max_len_dst, max_len_src, budget, recent, 1, max_len_src <= kMaxStaged, in_place};
+                   H, D, max_len_dst, max_len_src, budget, recent, 1, std::min(std::min(budget, max_len_src), kMaxListed), in_place};
   if (!p.status) return DADATTN_E_CUDA;
-  while (p.parts < 8 && static_cast<long long>(pairs) * p.parts * 2 <= 8LL * sms) p.parts *= 2;
-  if (in_place && !p.staged) p.parts = 1;   // the weights are read all along, by the CTA that moves them
+  // CTAs for each pair: as many as fit the GPU at once, and as the weights need room
+  while (p.parts < kMaxParts && (static_cast<long long>(pairs) * p.parts * 2 <= static_cast<long long>(kEvictPerSm) * sms || max_len_src > p.parts * kMaxStaged)) p.parts *= 2;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const size_t smem = p.staged ? static_cast<size_t>(max_len_src) * 4 : 0;
-  DAD_CUDA(cudaFuncSetAttribute(kv_cache_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxStaged * 4));
+  const size_t smem = sizeof(int) * (p.listed + static_cast<size_t>(max_len_src + p.parts - 1) / p.parts);
+  DAD_CUDA(cudaFuncSetAttribute(kv_cache_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kMaxListed + kMaxStaged) * 4));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(pairs * p.parts));
   cfg.blockDim = dim3(kEvictThreads);

@@ -358,7 +358,8 @@ int dadattn_decode_bf16_window(uint16_t* out, const uint16_t* q, const uint16_t*
  * last `recent` rows and, of the others, the budget - recent with the largest weights (equal ones: the lower index; NaN
  * counts as the least). What stays is moved to rows 0.. of the destination, in order, K, V and weight alike, and
  * lengths_dst[b] becomes min(n, budget). Other rows of the destination are left as they were.
- * k, v [B,H,max_len,D] bf16, weights [B,H,max_len] fp32, 1 <= budget <= max_len_dst, 0 <= recent <= budget. The destination
+ * k, v [B,H,max_len,D] bf16, weights [B,H,max_len] fp32, 1 <= budget <= max_len_dst, 0 <= recent <= budget,
+ * max_len_src <= 196608. The destination
  * is another cache, or the source itself (all four arrays the same; the arrays do not overlap otherwise). A sequence whose
  * length is outside [0, max_len_src] is left untouched and reported through DADATTN_E_ARG at the next
  * dadattn_device_status(). Every head keeps rows of its own choice: only for models whose keys do not depend on the row they

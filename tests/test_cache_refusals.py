@@ -54,7 +54,7 @@ BAD += [(_fill, c, rc) for c, rc in [
     (dict(v_heads=P + 8), -1), (dict(counts=P + 1), -1), (dict(k_scale=P + 2), -1), (dict(max_len=-4), -1)]]
 BAD += [(_evict, c, rc) for c, rc in [
     (dict(ws=None), -1), (dict(budget=0), -1), (dict(budget=101), -1), (dict(recent=51), -1), (dict(recent=-1), -1),
-    (dict(D=256), -2), (dict(kd=_far(0) + 8), -1), (dict(kd=_far(4)), -1), (dict(kd=_far(4) + 1024), -1),
+    (dict(D=256), -2), (dict(max_src=196609), -2), (dict(kd=_far(0) + 8), -1), (dict(kd=_far(4)), -1), (dict(kd=_far(4) + 1024), -1),
     (dict(vd=_far(0)), -1), (dict(wd=_far(6)), -1), (dict(ld=_far(7)), -1),
     (dict(kd=_far(4), vd=_far(5), wd=_far(6), ld=_far(7)), -1)]]   # (the two max_len differ)
 

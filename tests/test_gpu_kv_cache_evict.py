@@ -51,7 +51,7 @@ def _check(dst, src, before, lengths, budget, recent):
 
 CASES = [(1, 3, 9000, 64, [8999], 2048, 256), (2, 5, 2500, 128, [2500, 1024], 1024, 0), (7, 3, 300, 64, [0, 1, 63, 64, 65, 300, 299], 64, 64),
          (3, 2, 40, 128, [40, 10, 11], 10, 3), (5, 300, 130, 64, [130, 5, 64, 100, 129], 100, 99), (2, 2, 1030, 64, [1030, 1025], 1, 0),
-         (2, 2, 60000, 64, [60000, 50000], 700, 50)]
+         (2, 2, 60000, 64, [60000, 50000], 700, 50), (1, 1, 60000, 64, [59999], 40000, 7), (1, 2, 196608, 64, [196608], 1500, 1500)]
 
 
 @pytest.mark.parametrize("ties", [False, True], ids=["", "ties"])
