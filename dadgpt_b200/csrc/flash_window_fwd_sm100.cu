@@ -30,6 +30,9 @@ namespace {
 
 using namespace ptx;
 
+// (four polls ahead of the suspending wait: 1 %)
+#define window_wait(bar, parity, abort_flag) mbar_wait_at<4>(bar, parity, abort_flag, __LINE__)
+
 constexpr int kBM = 128;                   // query rows per CTA
 constexpr int kBN = 64;                    // keys per tile
 constexpr int kPanelBytes = kBM * 128;     // [128 rows][64 bf16], swizzled
@@ -151,10 +154,10 @@ flash_window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       int n_k = 1, n_v = 1;   // tiles loaded
       for (int j = 1; j < n; ++j) {
         const int s = j % kStages, use = j / kStages;
-        if (use > 0 && !mbar_wait(&bars->k_empty[s], (use - 1) & 1, abort_flag)) break;
+        if (use > 0 && !window_wait(&bars->k_empty[s], (use - 1) & 1, abort_flag)) break;
         load_k(s, j);
         ++n_k;
-        if (use > 0 && !mbar_wait(&bars->v_empty[s], (use - 1) & 1, abort_flag)) break;
+        if (use > 0 && !window_wait(&bars->v_empty[s], (use - 1) & 1, abort_flag)) break;
         load_v(s, j);
         ++n_v;
       }
@@ -170,13 +173,13 @@ flash_window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       const SmemDescBase q_desc = make_desc_base_sw128(smem_u32(smem + L::kQ), 0);
       const SmemDescBase k_desc0 = make_desc_base_sw128(smem_u32(smem + L::kK), 0);
       const SmemDescBase v_desc0 = make_desc_base_sw128(smem_u32(smem + L::kV), kSubPanelBytes);
-      bool ok = mbar_wait(&bars->q_full, 0, abort_flag);
+      bool ok = window_wait(&bars->q_full, 0, abort_flag);
 
       // O (+)= P_i V_i
       auto issue_pv = [&](int i) -> bool {
         const int s = i % kStages, buf = i % kBufs;
-        if (!mbar_wait(&bars->v_full[s], (i / kStages) & 1, abort_flag)) return false;
-        if (!mbar_wait(&bars->p_full[buf], (i / kBufs) & 1, abort_flag)) return false;
+        if (!window_wait(&bars->v_full[s], (i / kStages) & 1, abort_flag)) return false;
+        if (!window_wait(&bars->p_full[buf], (i / kBufs) & 1, abort_flag)) return false;
         tc_fence_after_sync();
         const SmemDescBase v_desc{v_desc0.lo + s * (L::kTile >> 4), v_desc0.hi};
 #pragma unroll
@@ -192,7 +195,7 @@ flash_window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         // Two buffers: S_j goes over P_{j-2}, behind P_{j-2} V_{j-2}, which this thread issued earlier, and ahead of
         // P_{j-1} V_{j-1}. One: behind P_{j-1} V_{j-1}.
         if (kBufs == 1 && j > 0 && !(ok = issue_pv(j - 1))) break;
-        if (!(ok = mbar_wait(&bars->k_full[s], (j / kStages) & 1, abort_flag))) break;
+        if (!(ok = window_wait(&bars->k_full[s], (j / kStages) & 1, abort_flag))) break;
         tc_fence_after_sync();
         const SmemDescBase k_desc{k_desc0.lo + s * (L::kTile >> 4), k_desc0.hi};
 #pragma unroll
@@ -213,7 +216,7 @@ flash_window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     const uint32_t tlane = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const uint32_t tO = tlane + L::kColO;
     const float scale_log2 = scale * kLog2e;
-    auto wait_pv = [&](int i) { return mbar_wait(&bars->o_done[i & 1], (i >> 1) & 1, abort_flag); };
+    auto wait_pv = [&](int i) { return window_wait(&bars->o_done[i & 1], (i >> 1) & 1, abort_flag); };
     float m = -INFINITY, l = 0.f;   // running max (log2 units, scaled) and sum
     bool ok = true;
 
@@ -223,7 +226,7 @@ flash_window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       // tiles in which any row of the CTA does not see a key: across the diagonal, or across the window's beginning
       const bool edge = t0 + kBN - 1 > q0 || (t0 <= q0 + kBM - 1 - window && t0 + kBN > sinks);
       uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-      bool any = true;
+      bool any = true, masked = false;   // whether the warp's rows see anything, and not everything
       if (edge) {
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
@@ -231,12 +234,13 @@ flash_window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
           seen[w] = low_bits(r - c + 1) & (~low_bits(r - window - c + 1) | low_bits(sinks - c));
         }
         any = __any_sync(0xffffffffu, (seen[0] | seen[1]) != 0);
+        masked = __any_sync(0xffffffffu, (seen[0] & seen[1]) != 0xffffffffu);
       }
       // 32 of the thread's scores
       auto load = [&](uint32_t (&x)[32], int w) {
         tmem_ld32(tS + 32 * w, x);
         tmem_wait_ld();
-        if (edge) {
+        if (masked) {
 #pragma unroll
           for (int i = 0; i < 32; ++i)
             if (!(seen[w] >> i & 1u)) x[i] = 0xff800000u;   // -inf
@@ -249,7 +253,7 @@ flash_window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
         return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       };
-      if (!(ok = mbar_wait(&bars->s_full[buf], (j / kBufs) & 1, abort_flag))) break;
+      if (!(ok = window_wait(&bars->s_full[buf], (j / kBufs) & 1, abort_flag))) break;
       tc_fence_after_sync();
       if (any) {
         uint32_t xa[32], xb[32];
