@@ -43,6 +43,7 @@ constexpr int kManyStages = 3, kManyPerSm = 4;
 constexpr int kMaxStages = 4;
 constexpr int kItemRing = 2;                  // items a CTA's producer may be ahead
 constexpr int kMaxCluster = 8;
+constexpr int kMaxPaired = 64;                // sequences of a call up to which clusters share two
 constexpr long long kBytesPerRank = 65536;    // K + V bytes that are worth a CTA of a cluster
 
 // The workspace: the item counter and 1 + kTicketGroups counters of the lengths' tickets (uint32, zero between calls), in
@@ -69,8 +70,9 @@ struct Shared {
       int place[kMaxRanked];
       int order[kMaxRanked];
     };
-    float record[kMaxCluster][130];      // clusters: every CTA's partial result, in the CTA of rank 0
+    float record[kMaxCluster][130];      // clusters: every CTA's partial result, in the CTA that merges it
   };
+  int2 member[2];                        // paired: (sequence or -1, length)
   float2 state[kMaxCluster];             // clusters with weights: every CTA's (m, l), in every CTA
 };
 
@@ -88,7 +90,7 @@ struct Params {
   unsigned* counters;
   int* status;
   int B, H, max_len, blocks, window, sinks;
-  int ranks, stages, reorder;
+  int ranks, stages, reorder, paired;
   float scale;
 };
 
@@ -219,6 +221,7 @@ __global__ void __launch_bounds__(kThreads, kManyPerSm) decode_window_kernel(con
       sh.lens[i] = i < B ? p.lengths[i] : INT_MIN;
       if (!CLUSTER && p.reorder) sh.place[i] = 0;
     }
+  if (CLUSTER && threadIdx.x < 2) sh.member[threadIdx.x] = make_int2(-1, 0);
   __syncthreads();
   if (!CLUSTER && p.reorder) rank_by_length(sh.lens, sh.place, sh.order, B, kThreads);
   if (CLUSTER) cluster_arrive();   // "this CTA has started": waited for before the first remote store
@@ -230,21 +233,62 @@ __global__ void __launch_bounds__(kThreads, kManyPerSm) decode_window_kernel(con
     bool good;
   };
   const int n_items = B * H, n_lanes = static_cast<int>(gridDim.x);
-  auto item = [&](int e) -> Item {
-    const int place = e / H, b = !CLUSTER && p.reorder ? sh.order[place] : place;
-    Item s{b, e - place * H, snapshot ? sh.lens[b] : p.lengths[b], 0, 0, false};
-    s.good = s.len >= 0 && s.len < max_len;
+  // CTA `share` of the `shares` that share sequence b's head h
+  auto share_of = [&](int b, int h, int len, int share, int shares) -> Item {
+    Item s{b, h, len, 0, 0, len >= 0 && len < max_len};
     if (!s.good) {
       s.len = 0;
     } else {
-      const int n = V(s.len, p.window, p.sinks).tiles();
+      const int n = V(len, p.window, p.sinks).tiles();
       // (64 bits: not needed by any cache that fits the GPU, and free here)
-      s.t0 = static_cast<int>(static_cast<long long>(n) * rank / ranks);
-      s.t1 = static_cast<int>(static_cast<long long>(n) * (rank + 1) / ranks);
+      s.t0 = static_cast<int>(static_cast<long long>(n) * share / shares);
+      s.t1 = static_cast<int>(static_cast<long long>(n) * (share + 1) / shares);
     }
     return s;
   };
-  const Item first = item(static_cast<int>(blockIdx.x) / ranks);
+  int share = rank, shares = ranks;             // this CTA among those that share its sequence
+  int merges = rank == 0 ? 0 : -1, from = 0;    // clusters: which of its sequences a CTA merges, whose first CTA has rank `from`
+  auto item = [&](int e) -> Item {
+    const int place = e / H, b = !CLUSTER && p.reorder ? sh.order[place] : place;
+    return share_of(b, e - place * H, snapshot ? sh.lens[b] : p.lengths[b], share, shares);
+  };
+  Item first, merged;
+  bool second = false;                          // whether the CTA's share is of its cluster's second sequence
+  if (!CLUSTER || !p.paired) {
+    first = merged = item(static_cast<int>(blockIdx.x) / ranks);
+  } else {
+    // Cluster c takes head c % H of the c / H-th longest and the c / H-th shortest sequence (one, in the middle of an odd
+    // number), as decode.cu's; its CTAs are divided by their tiles, so that the largest share is as small as it can be.
+    const int e = static_cast<int>(blockIdx.x) / ranks, nth = e / H, h = e - nth * H, t = threadIdx.x;
+    if (t < B) {
+      const int mine = sh.lens[t];
+      int place = 0;
+#pragma unroll 4
+      for (int j = 0; j < B; ++j)
+        place += static_cast<int>(sh.lens[j] > mine) | (static_cast<int>(sh.lens[j] == mine) & static_cast<int>(j < t));
+      if (place == nth) sh.member[0] = make_int2(t, mine);
+      else if (place == B - 1 - nth) sh.member[1] = make_int2(t, mine);
+    }
+    __syncthreads();
+    const int2 a = sh.member[0], b = sh.member[1];
+    auto tiles_of = [&](const int2& x) { return x.x >= 0 && x.y >= 0 && x.y < max_len ? V(x.y, p.window, p.sinks).tiles() + 1 : 0; };
+    const int tiles_a = tiles_of(a), tiles_b = tiles_of(b);
+    int cut = b.x < 0 || tiles_b == 0 ? ranks : 0;   // CTAs for the first
+    if (tiles_a > 0 && tiles_b > 0) {
+      // the whole number below or above what is in proportion, whichever has the smaller largest share
+      const float fa = static_cast<float>(tiles_a), fb = static_cast<float>(tiles_b);
+      const int below = min(max(static_cast<int>(__fdividef(fa * ranks, fa + fb)), 1), ranks - 1), above = min(below + 1, ranks - 1);
+      cut = fa * (ranks - above) <= fb * below ? below : above;
+    }
+    second = rank >= cut;
+    share = second ? rank - cut : rank;
+    shares = second ? ranks - cut : cut;
+    first = second ? share_of(b.x, h, b.y, share, shares) : share_of(a.x, h, a.y, share, shares);
+    merges = rank == 0 ? 0 : rank == 1 && b.x >= 0 ? 1 : -1;
+    merged = merges == 1 ? share_of(b.x, h, b.y, 0, max(ranks - cut, 1)) : share_of(a.x, h, a.y, 0, max(cut, 1));
+    from = merges == 1 ? cut : 0;
+  }
+  const int merged_shares = CLUSTER && p.paired ? (merges == 1 ? ranks - from : second ? 0 : shares) : ranks;
 
   const LengthTickets tickets{p.counters + 1};
   volatile int* abort_flag = &sh.abort_flag;
@@ -423,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, kManyPerSm) decode_window_kernel(con
       using One = std::integral_constant<int, 1>;
 
       // the token being appended: its vectors are used and stored by the CTA of the last share
-      if (warp == 0 && s.good && rank == ranks - 1) {
+      if (warp == 0 && s.good && share == shares - 1) {
         const bool mine = slot == 0;
         Raw kr[1], vr[1];
 #pragma unroll
@@ -559,9 +603,9 @@ __global__ void __launch_bounds__(kThreads, kManyPerSm) decode_window_kernel(con
         if (!CLUSTER) {
           if (s.good) p.out[bh * D + d] = Elem<bf16>::from_float(aa / ll);
         } else {
-          // hand the share to rank 0, which is known to run once the cluster's first barrier is through
+          // hand the share to the CTA that merges it, which is known to run once the cluster's first barrier is through
           cluster_wait();
-          const uint32_t rec = cluster_address(&sh.record[rank][0], 0);
+          const uint32_t rec = cluster_address(&sh.record[rank][0], second ? 1 : 0);
           st_cluster(rec + d * 4, aa);
           if (d == 0) {
             st_cluster(rec + D * 4, mm);
@@ -584,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, kManyPerSm) decode_window_kernel(con
         rows(min(s.t0, view.a) * V::kRows, min(min(s.t1, view.a) * V::kRows, view.sinks));
         rows(view.first + max(s.t0 - view.a, 0) * V::kRows,
              min(view.first + max(s.t1 - view.a, 0) * V::kRows, s.len));
-        if (rank == ranks - 1 && d == 0) weights[s.len] = ex2(scores[s.len] - m_all) * inv;
+        if (share == shares - 1 && d == 0) weights[s.len] = ex2(scores[s.len] - m_all) * inv;
       };
       if (WEIGHTS && !CLUSTER && s.good && ok) add_weights(mm, ll);
       if (WEIGHTS && CLUSTER) {
@@ -594,13 +638,14 @@ __global__ void __launch_bounds__(kThreads, kManyPerSm) decode_window_kernel(con
         cluster_wait();
         if (s.good && ok) {
           float m_all = -FLT_MAX, l_all = 0.f;
-          for (int j = 0; j < ranks; ++j) m_all = fmaxf(m_all, sh.state[j].x);
-          for (int j = 0; j < ranks; ++j) l_all += sh.state[j].y * ex2(sh.state[j].x - m_all);
+          const int j0 = rank - share;
+          for (int j = j0; j < j0 + shares; ++j) m_all = fmaxf(m_all, sh.state[j].x);
+          for (int j = j0; j < j0 + shares; ++j) l_all += sh.state[j].y * ex2(sh.state[j].x - m_all);
           add_weights(m_all, l_all);
         }
       }
       // the token filled the tail: it becomes a block
-      if (FP8 && s.good && ok && rank == ranks - 1 && s.len % kFp8Block == kFp8Block - 1) {
+      if (FP8 && s.good && ok && share == shares - 1 && s.len % kFp8Block == kFp8Block - 1) {
         constexpr int kPieces = kFp8Block * D / 8 / (kWarps * 32);   // 16-byte pieces of the tail per thread
         const size_t from = bh * kFp8Block * D, to = (bh * max_len + view.full) * D;
 #pragma unroll
@@ -643,20 +688,20 @@ __global__ void __launch_bounds__(kThreads, kManyPerSm) decode_window_kernel(con
       cluster_arrive();
       cluster_wait();
     }
-    if (rank == 0) {
-      if (first.good) {
+    if (merges >= 0) {
+      if (merged.good) {
         if (d < D) {
           float mm = -FLT_MAX;
-          for (int j = 0; j < ranks; ++j) mm = fmaxf(mm, sh.record[j][D]);
+          for (int j = from; j < from + merged_shares; ++j) mm = fmaxf(mm, sh.record[j][D]);
           float ll = 0.f, aa = 0.f;
-          for (int j = 0; j < ranks; ++j) {
+          for (int j = from; j < from + merged_shares; ++j) {
             const float c = ex2(sh.record[j][D] - mm);   // a share without rows has m = -FLT_MAX: 0
             ll += sh.record[j][D + 1] * c;
             aa += sh.record[j][d] * c;
           }
-          p.out[(static_cast<size_t>(first.b) * H + first.h) * D + d] = Elem<bf16>::from_float(aa / ll);
+          p.out[(static_cast<size_t>(merged.b) * H + merged.h) * D + d] = Elem<bf16>::from_float(aa / ll);
         }
-      } else if (first.h == 0 && d == 0) {
+      } else if (merged.h == 0 && d == 0) {
         atomicExch(p.status, DADATTN_E_ARG);
       }
     }
@@ -694,7 +739,15 @@ int launch(Params p, cudaStream_t st) {
   const int resident = kManyPerSm * sms;
   p.ranks = 1;
   while (p.ranks < kMaxCluster && p.ranks * kBytesPerRank < bytes && pairs * p.ranks * 2 <= resident) p.ranks *= 2;
-  const long long grid = p.ranks > 1 ? pairs * p.ranks : std::min(pairs, static_cast<long long>(resident));
+  long long grid = p.ranks > 1 ? pairs * p.ranks : std::min(pairs, static_cast<long long>(resident));
+  // Clusters of four or eight for two sequences in place of two or four CTAs for each, where lengths may differ and some room
+  // is left on the GPU; decode.cu has both sides of the limits. Here: 4 sequences x 24 heads x 128 in 8 bits, of 1000, 3000,
+  // 5000 and 7000 rows: 33.0 us with four CTAs for each, 25.2 so, and 25.2 both ways where each has 4000 rows. Under a window
+  // the sequences are alike.
+  const long long paired = static_cast<long long>((p.B + 1) / 2) * p.H * p.ranks * 2;
+  p.paired = p.window == 0 && p.ranks > 1 && p.ranks < kMaxCluster && p.B >= 2 && p.B <= kMaxPaired &&
+             paired * 100 <= resident * (p.ranks * 2 == kMaxCluster ? 84LL : 92LL);
+  if (p.paired) p.ranks *= 2, grid = paired;
   p.stages = grid <= kFewPerSm * sms ? kFewStages : kManyStages;
   // Longest first pays once a CTA takes more than one item (not under a window, which makes them all alike); the in-kernel
   // ranking, 0.9 us, handles 32..256 sequences.

@@ -73,6 +73,38 @@ def test_steps_against_float64(cuda, shape, window, sinks, weights):
     assert device_status() == 0
 
 
+# two sequences to a cluster of eight and of four, with one in the middle and without
+PAIRED = [(4, 24, 1300, 64, [1298, 0, 17, 900]), (4, 24, 1300, 64, [500] * 4), (5, 20, 1300, 128, [3, 1297, 640, 0, 1250]),
+          (9, 20, 600, 64, [0, 597, 1, 300, 300, 300, 64, 63, 590])]
+
+
+@pytest.mark.parametrize("weights", [False, True], ids=["", "weights"])
+@pytest.mark.parametrize("shape", PAIRED, ids=["halves", "alike", "odd", "fours"])
+def test_two_sequences_of_a_cluster(cuda, shape, weights):
+    B, H, max_len, D, lengths = shape
+    c, g = _cache(cuda, B, H, max_len, D, lengths, B, weights)
+    _hide(c, lengths, 0, 0)
+    _step(c, g, _step(c, g, lengths, 0, 0, weights), 0, 0, weights)
+    # no token for a full and for an invalid length, whichever of the two sequences has it
+    c.k.normal_(generator=g)
+    c.v.normal_(generator=g)
+    for bad in ([0], [1], [B - 1], [0, 1], [2, 3], list(range(B))):
+        lengths = [(1300 if i % 2 else -5) if i in bad else 10 * i for i in range(B)]
+        c.lengths.copy_(torch.tensor(lengths, dtype=torch.int32))
+        q, kn, vn = (torch.randn(B, H, D, device=cuda, generator=g).bfloat16() for _ in range(3))
+        out, k0 = torch.full_like(q, 7.0), c.k.clone()
+        dad.decode_attention_bf16_window(out, q, kn, vn, c, D ** -0.5, weights=weights)
+        assert device_status() == -1 and c.lengths.tolist() == [n if i in bad else n + 1 for i, n in enumerate(lengths)]
+        for i, n in enumerate(lengths):
+            if i in bad:
+                assert bool((out[i] == 7.0).all())
+            else:
+                k0[i, :, n] = kn[i]
+                want, _, bound, largest = attend(q[i], c.k[i], c.v[i], visible(n, max_len, 0, 0), D ** -0.5)
+                check_out(out[i], want, bound, largest)
+        assert torch.equal(c.k.view(torch.int16), k0.view(torch.int16))
+
+
 def test_without_a_window_it_is_the_decode_call(cuda):
     lengths = [0, 5, 299, 130]
     a, g = _cache(cuda, 4, 12, 300, 64, lengths, 1, False)

@@ -14,9 +14,9 @@ def _kept(weights, n, budget, recent):
     """The rows of one head that stay, by sorting in Python."""
     if n <= budget:
         return list(range(n))
-    w = [float("-inf") if x != x else x for x in weights[:n].tolist()]
+    w = weights[:n].tolist()
     # NaN counts as less than everything, -inf too: a NaN comes behind a -inf
-    order = sorted(range(n - recent), key=lambda j: (weights[j].item() != weights[j].item(), -w[j], j))
+    order = sorted(range(n - recent), key=lambda j: (w[j] != w[j], -w[j] if w[j] == w[j] else 0, j))
     return sorted(order[:budget - recent]) + list(range(n - recent, n))
 
 

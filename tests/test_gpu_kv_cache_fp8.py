@@ -151,6 +151,29 @@ def test_steps_against_float64(cuda, shape, window, sinks):
     assert device_status() == 0
 
 
+# two sequences to a cluster of eight and of four, with one in the middle and without
+@pytest.mark.parametrize("shape", [(4, 24, 1300, 64, [1298, 0, 63, 900]), (4, 24, 1300, 64, [511] * 4), (5, 20, 1300, 128, [3, 1297, 639, 0, 1250]),
+                                   (9, 20, 600, 64, [0, 597, 1, 300, 319, 300, 64, 63, 575])], ids=["halves", "alike", "odd", "fours"])
+def test_two_sequences_of_a_cluster(cuda, shape):
+    B, H, max_len, D, lengths = shape
+    c, g = _filled(cuda, B, H, max_len, D, lengths, B)
+    _step(c, g, _step(c, g, lengths, 0, 0), 0, 0)
+    lengths = [10 + 50 * b for b in range(B)]
+    c, g = _filled(cuda, B, H, max_len, D, lengths, B + 1)
+    c.lengths[0], c.lengths[B - 2] = -1, max_len
+    lengths[0], lengths[B - 2] = -1, max_len
+    q, kn, vn = (torch.randn(B, H, D, device=cuda, generator=g).bfloat16() for _ in range(3))
+    out, before = torch.full_like(q, 7.0), c.k_tail.clone()
+    dad.decode_attention_fp8(out, q, kn, vn, c, D ** -0.5)
+    assert device_status() == -1
+    for b, n in enumerate(lengths):
+        bad = b in (0, B - 2)
+        assert bool((out[b] == 7.0).all()) == bad and c.lengths[b].item() == n + (not bad)
+        if not bad:
+            before[b, :, n % BLOCK] = kn[b]
+    assert torch.equal(c.k_tail.view(torch.int16), before.view(torch.int16))
+
+
 @pytest.mark.parametrize("B,H,D", [(2, 3, 64), (2, 3, 128), (40, 16, 64), (160, 4, 128)])
 def test_tokens_and_prompts_leave_the_same_bytes(cuda, B, H, D):
     # prompts of every length modulo a block, then as many single tokens as reach two blocks more
