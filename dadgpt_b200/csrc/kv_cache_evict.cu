@@ -4,16 +4,21 @@
 // (equal ones: the lower index; NaN counts as the least). The rows that stay are moved together, in order, with their
 // weights, into another cache or within their own.
 //
-// The CTAs of a cluster share a (sequence, head):
+// A CTA has a (sequence, head), or the CTAs of a cluster share it where there are few:
 //   * each turns the weights of its part of the rows into integers of the same order in shared memory; the smallest kept one is
-//     found byte by byte from the top, by histograms of those that agree in the bytes before, which the cluster adds up
-//     (four passes, whatever the values);
+//     found byte by byte from the top, by histograms of those that agree in the bytes before, which the cluster adds up. Four
+//     passes at most: the search ends where all that agree so far stay. After the second the rows that stay for certain are
+//     asked for in L2.
 //   * each counts and numbers the rows of its part that are larger than the smallest kept, and the first ones that are equal
-//     to it, and writes them into the list of every CTA of the cluster;
-//   * the rows of the list are copied in 16-byte pieces: into another cache by shares of the list, within one cache by columns.
-// Bound by HBM where there are enough (sequence, head) pairs: the weights once, each kept row in and out. (Each CTA selecting
-// for itself, and copying as it went through the rows 1024 at a time, took 65 us for 4 x 24 heads of up to 8000 rows, 20 of
-// them histograms and 20 the numbering.)
+//     to it, and writes them into the list of the CTA that will copy them;
+//   * the rows of the list are copied in 16-byte pieces: into another cache by shares of the list, within one cache by columns
+//     (there every CTA of the cluster has the whole list).
+// Bound by HBM where there are enough (sequence, head) pairs: the weights once, each kept row in and out. Where all heads are as
+// long as they can be, the selections of all CTAs come first and the copies after them: 64 x 12 heads of 64, 1024 rows to 512,
+// take 45.6 us, 9 of them selection, and 38.5 where nothing is to be selected (203 MB: 5.3 TB/s). 4 x 24 heads of 128, 8000 rows to 2048:
+// 52.4 us, 38.8 with nothing to select. (There each CTA selecting for itself, and copying as it went through the rows 1024 at a
+// time, took 87; all four passes 61.7; every list written by all CTAs 57; two waves of clusters of two for 64 x 12 heads 55.
+// Adding up equal bytes of a warp by votes before the shared atomics cost 1 to 3 us.)
 //
 // Within one cache: a row's place is never behind the row, so rows that are loaded in order may be stored as soon as every
 // thread has loaded its pieces of the same batch; what is stored lies ahead of all that is loaded later. The columns of a
@@ -30,8 +35,11 @@ namespace dadattn {
 namespace {
 
 constexpr int kEvictThreads = 256;
-constexpr int kBatch = 4;                   // 16-byte pieces that a thread has in registers
-constexpr int kEvictPerSm = 6;              // CTAs that an SM holds
+// 16-byte pieces that a thread has in registers, and CTAs that an SM holds. Clusters: six on an SM (40 registers), so that
+// their waits for each other are covered. One CTA for each pair: 64 x 12 heads of 1 .. 1024 rows to 512 take 32.4 us with four
+// that have 8 pieces in flight (all of 1024 rows: 45.6), 35.2 with six of 4 (45.6), 34.7 with five of 4 (57.1: a second wave).
+constexpr int kClusterBatch = 4, kClusterPerSm = 6;
+constexpr int kSingleBatch = 8, kSinglePerSm = 4;
 constexpr int kMaxParts = 8;                // CTAs of a cluster
 constexpr int kMaxStaged = 24576;           // rows whose weights a CTA has in shared memory (96 KB),
 constexpr int kMaxListed = 24576;           // and kept rows that it has at a time
@@ -53,7 +61,7 @@ struct EvictShared {
   int counts[kMaxParts];   // of every CTA: rows larger than the smallest kept, and equal to it
   int equals[kMaxParts];
   int warp_total[kEvictThreads / 32];
-  int chosen, above;       // a pass's byte, and how many keys are larger
+  int chosen, above, of_chosen;   // a pass's byte, how many keys are larger, and how many have it
 };
 
 __device__ __forceinline__ void st_cluster_int(uint32_t addr, int v) {
@@ -104,12 +112,14 @@ __device__ __forceinline__ int prefix_sum(EvictShared& sh, int mine, int& total)
   return before + sum - mine;
 }
 
-__global__ void __launch_bounds__(kEvictThreads, kEvictPerSm) kv_cache_evict_kernel(const __grid_constant__ EvictParams p) {
+template <bool CLUSTER>
+__global__ void __launch_bounds__(kEvictThreads, CLUSTER ? kClusterPerSm : kSinglePerSm) kv_cache_evict_kernel(const __grid_constant__ EvictParams p) {
   extern __shared__ __align__(16) int dynamic[];   // the list, then the keys of this CTA's rows
   int* list = dynamic;
   uint32_t* keys = reinterpret_cast<uint32_t*>(dynamic + p.listed);
   __shared__ EvictShared sh;
-  const int parts = p.parts, part = static_cast<int>(blockIdx.x) % parts, bh = static_cast<int>(blockIdx.x) / parts, b = bh / p.H;
+  constexpr int kBatch = CLUSTER ? kClusterBatch : kSingleBatch;
+  const int parts = CLUSTER ? p.parts : 1, part = static_cast<int>(blockIdx.x) % parts, bh = static_cast<int>(blockIdx.x) / parts, b = bh / p.H;
   const int t = threadIdx.x, D = p.D;
   sh.histogram[0][t] = 0;
   sh.histogram[1][t] = 0;
@@ -168,27 +178,43 @@ __global__ void __launch_bounds__(kEvictThreads, kEvictPerSm) kv_cache_evict_ker
       if (above < left && left <= above + mine) {
         sh.chosen = 255 - t;
         sh.above = above;
+        sh.of_chosen = mine;
       }
       __syncthreads();
       prefix = prefix << 8 | static_cast<uint32_t>(sh.chosen);
       left -= sh.above;
+      least = prefix;
+      if (sh.of_chosen == left && prefix > 0) {   // all that agree stay
+        least = (prefix << shift) - 1;
+        left = 0;
+        break;
+      }
+      if (shift == 16) {   // rows that stay for certain: on their way while the rest is found
+        for (int row = t; row < end - row0; row += kEvictThreads)
+          if ((keys[row] >> 16) > prefix) {
+            const size_t at = (static_cast<size_t>(bh) * p.max_len_src + row0 + row) * D;
+            for (int i = 0; i < D; i += 64) {   // 128 bytes
+              asm volatile("prefetch.global.L2 [%0];" ::"l"(p.k_src + at + i));
+              asm volatile("prefetch.global.L2 [%0];" ::"l"(p.v_src + at + i));
+            }
+          }
+      }
     }
-    least = prefix;
     equal_wanted = left;
   }
   auto is_larger = [&](int row) { return row >= candidates || (wanted > 0 && keys[row - row0] > least); };
   auto is_equal = [&](int row) { return row < candidates && wanted > 0 && keys[row - row0] == least; };
 
   // How many rows of the CTAs before this one stay
-  int counted = 0;
-  for (int row = row0 + t; row < row1; row += kEvictThreads) {
-    if (is_larger(row)) ++counted;
-    else if (is_equal(row)) counted += 1 << 16;
-  }
   int larger = 0, equal = 0;
-  {   // (a part has no more than kMaxStaged < 2^16 rows)
-    int total;
+  if (CLUSTER && !all) {   // (a part has no more than kMaxStaged < 2^16 rows)
+    int counted = 0, total;
+    for (int row = row0 + t; row < row1; row += kEvictThreads) {
+      if (is_larger(row)) ++counted;
+      else if (is_equal(row)) counted += 1 << 16;
+    }
     prefix_sum(sh, counted, total);
+    if (wanted == 0) meet(parts);   // (no pass has met yet: a CTA has to run before another one stores to it)
     if (t < parts) {
       st_cluster_int(cluster_address(&sh.counts[part], t), total & 0xffff);
       st_cluster_int(cluster_address(&sh.equals[part], t), total >> 16);
@@ -199,16 +225,25 @@ __global__ void __launch_bounds__(kEvictThreads, kEvictPerSm) kv_cache_evict_ker
 
   const int row_pieces = D / 8;   // 16-byte pieces of a row
   const size_t src0 = static_cast<size_t>(bh) * p.max_len_src, dst0 = static_cast<size_t>(bh) * p.max_len_dst;
+  const bool by_rows = !p.in_place, with_list = !all && !CLUSTER;   // weights that move as their rows are listed
   for (int begin = 0; begin < kept; begin += p.listed) {   // (one turn, unless the budget is larger than the list)
-    const int count = min(kept - begin, p.listed);
-    // Numbers of this CTA's kept rows, into all lists: a thread has four rows in turn of 1024
+    const int count = min(kept - begin, p.listed), chunk = (count + parts - 1) / parts;
+    // another cache: a share of the rows; the same: a share of the columns, of K or of V where the cluster is large enough
+    const int first = by_rows ? min(part * chunk, count) : 0, last = by_rows ? min(first + chunk, count) : count;
+    if (all) {
+      for (int i = first + t; i < last; i += kEvictThreads) list[i] = begin + i;
+      __syncthreads();
+    }
+    // Numbers of this CTA's kept rows: a thread has four rows in turn of 1024
     int before_gt = larger, before_eq = equal;
-    for (int r0 = row0; r0 < row1; r0 += 4 * kEvictThreads) {
+    for (int r0 = row0; !all && r0 < row1; r0 += 4 * kEvictThreads) {
       int gt = 0, eq = 0;
+      float w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = r0 + 4 * t + i;
         if (row < row1) {
+          if (with_list) w[i] = weights[row];
           if (is_larger(row)) gt |= 1 << i;
           else if (is_equal(row)) eq |= 1 << i;
         }
@@ -220,23 +255,26 @@ __global__ void __launch_bounds__(kEvictThreads, kEvictPerSm) kv_cache_evict_ker
       for (int i = 0; i < 4; ++i) {
         const bool is_gt = gt >> i & 1, is_eq = eq >> i & 1;
         const int place = g + min(e, equal_wanted) - begin;
-        if ((is_gt || (is_eq && e < equal_wanted)) && place >= 0 && place < count)
-          for (int j = 0; j < parts; ++j) st_cluster_int(cluster_address(&list[place], j), r0 + 4 * t + i);
+        if ((is_gt || (is_eq && e < equal_wanted)) && place >= 0 && place < count) {
+          if (with_list) p.weights_dst[dst0 + begin + place] = w[i];
+          if (!CLUSTER) {
+            list[place] = r0 + 4 * t + i;
+          } else {
+            const int owner = by_rows ? place / chunk : 0;
+            for (int j = owner; j < (by_rows ? owner + 1 : parts); ++j) st_cluster_int(cluster_address(&list[place], j), r0 + 4 * t + i);
+          }
+        }
         g += is_gt;
         e += is_eq;
       }
       before_gt += total & 0xffff;
       before_eq += total >> 16;
     }
-    meet(parts);   // the list is there
+    if (!all) meet(parts);   // the list is there
 
-    // another cache: a share of the rows; the same: a share of the columns, of K or of V where the cluster is large enough
-    const bool by_rows = !p.in_place;
     const int sides = by_rows || parts == 1 ? 2 : 1, slices = by_rows || parts == 1 ? 1 : parts / 2;
     const int pieces = row_pieces / slices, shift = 31 - __clz(pieces);
     const int column = by_rows || parts == 1 ? 0 : part / 2 * pieces;
-    const int first = by_rows ? static_cast<int>(static_cast<long long>(count) * part / parts) : 0;
-    const int last = by_rows ? static_cast<int>(static_cast<long long>(count) * (part + 1) / parts) : count;
     const int work = (last - first) << shift;
     for (int i = 0; i < sides; ++i) {
       const bool is_v = sides == 2 ? i : part % 2;
@@ -257,7 +295,7 @@ __global__ void __launch_bounds__(kEvictThreads, kEvictPerSm) kv_cache_evict_ker
         }
       }
     }
-    if (by_rows || part == 0) {
+    if (!with_list && (by_rows || part == 0)) {
       for (int i0 = first; i0 < last; i0 += kBatch * kEvictThreads) {
         float x[kBatch];
 #pragma unroll
@@ -336,10 +374,11 @@ extern "C" int dadattn_kv_cache_evict_bf16(uint16_t* k_dst, uint16_t* v_dst, flo
                    H, D, max_len_dst, max_len_src, budget, recent, 1, std::min(std::min(budget, max_len_src), kMaxListed), in_place};
   if (!p.status) return DADATTN_E_CUDA;
   // CTAs for each pair: as many as fit the GPU at once, and as the weights need room
-  while (p.parts < kMaxParts && (static_cast<long long>(pairs) * p.parts * 2 <= static_cast<long long>(kEvictPerSm) * sms || max_len_src > p.parts * kMaxStaged)) p.parts *= 2;
+  while (p.parts < kMaxParts && (static_cast<long long>(pairs) * p.parts * 2 <= static_cast<long long>(kClusterPerSm) * sms || max_len_src > p.parts * kMaxStaged)) p.parts *= 2;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const size_t smem = sizeof(int) * (p.listed + static_cast<size_t>(max_len_src + p.parts - 1) / p.parts);
-  DAD_CUDA(cudaFuncSetAttribute(kv_cache_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kMaxListed + kMaxStaged) * 4));
+  auto kern = p.parts > 1 ? kv_cache_evict_kernel<true> : kv_cache_evict_kernel<false>;
+  DAD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (kMaxListed + kMaxStaged) * 4));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(pairs * p.parts));
   cfg.blockDim = dim3(kEvictThreads);
@@ -352,7 +391,7 @@ extern "C" int dadattn_kv_cache_evict_bf16(uint16_t* k_dst, uint16_t* v_dst, flo
   attrs[1].val.clusterDim = {static_cast<unsigned>(p.parts), 1, 1};
   cfg.attrs = attrs;
   cfg.numAttrs = p.parts > 1 ? 2 : 1;
-  DAD_CUDA(cudaLaunchKernelEx(&cfg, kv_cache_evict_kernel, p));
+  DAD_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
   if (in_place)
     DAD_CUDA(launch_pdl(evict_lengths_kernel, dim3((B + 255) / 256), dim3(256), 0, st, lengths_dst, B, max_len_src, budget));
   return DADATTN_OK;
