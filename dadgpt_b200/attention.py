@@ -180,7 +180,8 @@ def decode_attention_bf16(out, q, k_new, v_new, cache: KVCacheBF16, scale):
 def decode_attention_bf16_window(out, q, k_new, v_new, cache: KVCacheBF16, scale, *, window=0, sinks=0, weights=False):
     """:func:`decode_attention_bf16` over a sliding window: the token at row L of its sequence sees row j <= L iff
     L - j < window or j < sinks (window = 0: every row). With ``weights``, each visible row's probability is added to
-    ``cache.weights`` (and the appended row's weight set to its own); the cache was made with ``weights=True``."""
+    ``cache.weights`` (and the appended row's weight set to its own); the cache was made with ``weights=True``, and rows
+    that a prompt filled begin with the weights that the caller puts there (zeros, say)."""
     if weights and cache.weights is None:
         raise ValueError("the cache has no weights: make it with weights=True")
     _native().decode_bf16_window(cache.B, cache.H, cache.D, cache.max_len, scale, window, sinks, out, q, k_new, v_new,

@@ -652,12 +652,10 @@ __global__ void __launch_bounds__(kThreads, kManyPerSm) decode_window_kernel(con
         for (int side = 0; side < 2; ++side) {
           const uint4* tail = reinterpret_cast<const uint4*>((side ? p.v_tail : p.k_tail) + from);
           uint4 raw[kPieces];
-          float most = 0.f;
 #pragma unroll
-          for (int i = 0; i < kPieces; ++i) {
-            raw[i] = tail[i * kWarps * 32 + d];
-            most = fmaxf(most, most_of_bf16(raw[i]));
-          }
+          for (int i = 0; i < kPieces; ++i) raw[i] = tail[i * kWarps * 32 + d];
+          bool plain;
+          float most = most_of_bf16(raw, plain);
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
           consumers_sync();   // (sh.m is read: the output's sums, or the other side's block)
@@ -668,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, kManyPerSm) decode_window_kernel(con
           const int e = fp8_exponent(most);
           uint2* codes = reinterpret_cast<uint2*>(static_cast<uint8_t*>(side ? p.v : p.k) + to);
 #pragma unroll
-          for (int i = 0; i < kPieces; ++i) codes[i * kWarps * 32 + d] = fp8_of_bf16(raw[i], power_of_two(-e));
+          for (int i = 0; i < kPieces; ++i) codes[i * kWarps * 32 + d] = fp8_of_bf16(raw[i], power_of_two(-e), plain);
           if (d == 0) (side ? p.v_scale : p.k_scale)[bh * p.blocks + s.len / kFp8Block] = power_of_two(e);
         }
       }

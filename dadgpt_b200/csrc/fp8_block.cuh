@@ -38,31 +38,39 @@ __device__ __forceinline__ int fp8_exponent(float most) {
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
-// Two codes, the first in the low byte. `inv` = 2^-e.
-__device__ __forceinline__ uint32_t fp8_pair(float a, float b, float inv) {
-  a *= inv;
-  b *= inv;
-  if (fabsf(a) == INFINITY) a = NAN;   // (the conversion would make it 448)
-  if (fabsf(b) == INFINITY) b = NAN;
-  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+// Largest finite |x| of a thread's pieces of eight bf16 elements; `plain`: none is infinite or NaN. Absolute values are
+// compared as 16-bit integers, two at a time, and looked at one by one only where one of them is not finite.
+template <int N>
+__device__ __forceinline__ float most_of_bf16(const uint4 (&raw)[N], bool& plain) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    for (const uint32_t w : {raw[i].x, raw[i].y, raw[i].z, raw[i].w}) m = __vmaxu2(m, w & 0x7fff7fffu);
+  const uint32_t top = max(m >> 16, m & 0xffffu);
+  plain = top < 0x7f80u;
+  if (plain) return __uint_as_float(top << 16);
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    for (const uint32_t w : {raw[i].x, raw[i].y, raw[i].z, raw[i].w})
+      most = fmaxf(most, fmaxf(finite_abs(__uint_as_float(w << 16)), finite_abs(__uint_as_float(w & 0xffff0000u))));
+  return most;
 }
 
-// Eight bf16 elements -> eight codes.
-__device__ __forceinline__ uint2 fp8_of_bf16(const uint4& raw, float inv) {
+// Eight bf16 elements -> eight codes, the first in the lowest byte. `inv` = 2^-e.
+__device__ __forceinline__ uint2 fp8_of_bf16(const uint4& raw, float inv, bool plain) {
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
   uint32_t c[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    c[i] = fp8_pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u), inv);
+  for (int i = 0; i < 4; ++i) {
+    float a = __uint_as_float(w[i] << 16) * inv, b = __uint_as_float(w[i] & 0xffff0000u) * inv;
+    if (!plain) {   // (the conversion would make an infinity 448)
+      if (fabsf(a) == INFINITY) a = NAN;
+      if (fabsf(b) == INFINITY) b = NAN;
+    }
+    c[i] = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  }
   return make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
-}
-__device__ __forceinline__ float most_of_bf16(const uint4& raw) {
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  float m = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    m = fmaxf(m, fmaxf(finite_abs(__uint_as_float(w[i] << 16)), finite_abs(__uint_as_float(w[i] & 0xffff0000u))));
-  return m;
 }
 
 }  // namespace

@@ -342,7 +342,8 @@ int dadattn_decode_noalloc_status(dadattn_stream_t stream);
  * Rows that are not seen are not read. The token is appended and lengths[b] advanced as in dadattn_decode_bf16, a sequence
  * with L outside [0, max_len) is left untouched and reported the same way.
  * weights (may be NULL): [B,H,max_len] fp32. Each visible row's softmax probability is added to its weight, and the
- * appended row's weight is set to its probability, so that nothing has to be cleared when a sequence starts.
+ * appended row's weight is set to its probability, so that nothing has to be cleared when a sequence starts from its first
+ * token. Rows that a prompt put there (dadattn_kv_cache_fill) begin with the weights that the caller gives them: zeros, say.
  * max_len is at most DADATTN_MAX_CACHE_LEN, here and in the calls below.
  * workspace: at least dadattn_decode_window_workspace_bytes(B, H, D, max_len, weights != NULL) bytes, 16-byte aligned, with
  * the rules of dadattn_decode_bf16's: zero-filled once, to be zero-filled again when B, H or max_len change, not shared by
@@ -359,12 +360,11 @@ int dadattn_decode_bf16_window(uint16_t* out, const uint16_t* q, const uint16_t*
  * counts as the least). What stays is moved to rows 0.. of the destination, in order, K, V and weight alike, and
  * lengths_dst[b] becomes min(n, budget). Other rows of the destination are left as they were.
  * k, v [B,H,max_len,D] bf16, weights [B,H,max_len] fp32, 1 <= budget <= max_len_dst, 0 <= recent <= budget,
- * max_len_src <= 196608. The destination
- * is another cache, or the source itself (all four arrays the same; the arrays do not overlap otherwise). A sequence whose
- * length is outside [0, max_len_src] is left untouched and reported through DADATTN_E_ARG at the next
- * dadattn_device_status(). Every head keeps rows of its own choice: only for models whose keys do not depend on the row they
- * lie in (positions added to the embeddings, as in GPT-2, or rotated into the keys before they are cached), and without
- * dadattn_decode_bf16_window's window, which counts rows. No counterpart in the reference. */
+ * max_len_src <= 196608. The destination is another cache, or the source itself (all four arrays the same; the arrays do
+ * not overlap otherwise). A sequence whose length is outside [0, max_len_src] is left untouched and reported through
+ * DADATTN_E_ARG at the next dadattn_device_status(). Every head keeps rows of its own choice: only for models whose keys do
+ * not depend on the row they lie in (positions added to the embeddings, as in GPT-2, or rotated into the keys before they are
+ * cached), and without dadattn_decode_bf16_window's window, which counts rows. No counterpart in the reference. */
 int dadattn_kv_cache_evict_bf16(uint16_t* k_dst, uint16_t* v_dst, float* weights_dst, int32_t* lengths_dst,
                                 const uint16_t* k_src, const uint16_t* v_src, const float* weights_src,
                                 const int32_t* lengths_src, int B, int H, int D, int max_len_dst, int max_len_src, int budget,
