@@ -621,9 +621,22 @@ __global__ void __launch_bounds__(kThreads, kManyPerSm) decode_window_kernel(con
       auto add_weights = [&](float m_all, float l_all) {
         const float inv = 1.f / l_all;
         float* weights = p.weights + bh * max_len;
+        // Several rows of a thread on their way together. One after the other 4 x 24 heads of 128 (clusters), 4000 rows, took
+        // 41.7 us, so 38.8; 64 x 12 heads of 64, 1000 rows, 47.5 / 45.0 (8 at a time 49.0: the next item's vectors are spilt).
+        constexpr int kAhead = CLUSTER ? 8 : 4;
         auto rows = [&](int from, int to) {
-#pragma unroll 4
-          for (int j = from + d; j < to; j += kWarps * 32) weights[j] += ex2(scores[j] - m_all) * inv;
+          for (int j = from + d; j < to; j += kAhead * kWarps * 32) {
+            float sc[kAhead], w[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+              if (j + u * kWarps * 32 < to) {
+                sc[u] = scores[j + u * kWarps * 32];
+                w[u] = weights[j + u * kWarps * 32];
+              }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+              if (j + u * kWarps * 32 < to) weights[j + u * kWarps * 32] = w[u] + ex2(sc[u] - m_all) * inv;
+          }
         };
         rows(min(s.t0, view.a) * V::kRows, min(min(s.t1, view.a) * V::kRows, view.sinks));
         rows(view.first + max(s.t0 - view.a, 0) * V::kRows,
