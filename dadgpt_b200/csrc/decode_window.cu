@@ -14,6 +14,17 @@
 //                 from bf16, and holds the same bytes whether a prompt filled it or single tokens did.
 // Weights: a row's score is written to scratch as it is formed; once the item's m and l are known the CTA that formed it
 // adds exp(s - m) / l to the row's weight. 12 bytes a row beside 4 D of K and V.
+//
+// Measured in a graph of such calls on rotating caches (us; 64 x 12 heads of 64, 4 x 24 of 128):
+//   64 sequences of 9 .. 1017 rows   bf16 22.1 (4.5 TB/s), with weights 26.0, 8 bits 18.5 (2.7 TB/s)
+//   64 of 1000                       bf16 36.8 (5.3 TB/s), with weights 45.0; 8 bits, 1024 rows, 26.2 (3.8 TB/s)
+//   64 of 600, window 256            13.6 (3.7 TB/s)
+//   4 of 4000                        bf16 34.3 (5.7 TB/s), with weights 38.8, 8 bits 25.2 (3.9 TB/s); one of 650: 4.7 either way
+// What bounds the 8-bit form is not HBM but instruction issue (two conversions of every element beside its product; 53 % of
+// the slots, which are not filled while a call starts and ends) and the time to the first tile, 4.4 us of the 18.5. Tried for
+// it and not faster: rings of every warp's own filled by 16-byte copies (20-22 us), both products by warp-wide matrix
+// instructions (20-29) or K's alone (19.7), even shares of all rows for every CTA with partial results in memory (25-34), two
+// consumer warps with 4 KB tiles (26).
 #include <cuda_bf16.h>
 
 #include <cfloat>
@@ -44,7 +55,6 @@ constexpr int kMaxStages = 4;
 constexpr int kItemRing = 2;                  // items a CTA's producer may be ahead
 constexpr int kMaxCluster = 8;
 constexpr int kMaxPaired = 64;                // sequences of a call up to which clusters share two
-constexpr long long kBytesPerRank = 65536;    // K + V bytes that are worth a CTA of a cluster
 
 // The workspace: the item counter and 1 + kTicketGroups counters of the lengths' tickets (uint32, zero between calls), in
 // the space that decode.cu has for its own, so that the calls of both can share a workspace; with weights, the scores
@@ -743,13 +753,17 @@ int launch(Params p, cudaStream_t st) {
   DAD_CUDA(cudaGetDevice(&dev));
   DAD_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
   const long long pairs = static_cast<long long>(p.B) * p.H;
-  // CTAs per (sequence, head): as many as the most rows that a token can see have 64 KB of K and V for, while all of the
-  // call's CTAs still fit on the GPU at once (decode.cu has both sides).
+  // CTAs per (sequence, head): one for each tile (16 KB of K and V) of the rows that a token can see at most, while all of the
+  // call's CTAs still fit on the GPU at once; but no cluster for 64 KB, or 32 KB of 8-bit rows, and less, where meeting costs
+  // more than it saves. us, 12 heads of 64 (a CTA for each 64 KB / for each 16 KB): one sequence of 650 rows of 1024 5.05 /
+  // 4.70, 8 bits 6.10 / 4.70; 400 of 512 5.56 / 4.20, 8 bits 5.36 / 4.86; two sequences 5.77 / 4.88, 8 bits 6.71 / 5.12; 8 the
+  // same. 200 of 256 3.99 with one CTA, 4.20 with four, 8 bits 4.87 with one, 5.55 with two.
   const long long rows = p.window > 0 ? std::min<long long>(p.max_len, static_cast<long long>(p.window) + p.sinks) : p.max_len;
   const long long bytes = rows * 2 * D * (FP8 ? 1 : 2);
   const int resident = kManyPerSm * sms;
   p.ranks = 1;
-  while (p.ranks < kMaxCluster && p.ranks * kBytesPerRank < bytes && pairs * p.ranks * 2 <= resident) p.ranks *= 2;
+  if (bytes > (FP8 ? 32768 : 65536))
+    while (p.ranks < kMaxCluster && p.ranks * 2LL * kTileBytes < bytes && pairs * p.ranks * 2 <= resident) p.ranks *= 2;
   long long grid = p.ranks > 1 ? pairs * p.ranks : std::min(pairs, static_cast<long long>(resident));
   // Clusters of four or eight for two sequences in place of two or four CTAs for each, where lengths may differ and some room
   // is left on the GPU; decode.cu has both sides of the limits. Here: 4 sequences x 24 heads x 128 in 8 bits, of 1000, 3000,
