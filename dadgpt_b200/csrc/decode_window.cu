@@ -16,9 +16,9 @@
 // adds exp(s - m) / l to the row's weight. 12 bytes a row beside 4 D of K and V.
 //
 // Measured in a graph of such calls on rotating caches (us; 64 x 12 heads of 64, 4 x 24 of 128):
-//   64 sequences of 9 .. 1017 rows   bf16 22.1 (4.5 TB/s), with weights 26.0, 8 bits 18.5 (2.7 TB/s)
-//   64 of 1000                       bf16 36.8 (5.3 TB/s), with weights 45.0; 8 bits, 1024 rows, 26.2 (3.8 TB/s)
-//   64 of 600, window 256            13.6 (3.7 TB/s)
+//   64 sequences of 9 .. 1017 rows   bf16 21.8 (4.6 TB/s), with weights 25.3, 8 bits 18.5 (2.7 TB/s)
+//   64 of 1000                       bf16 35.7 (5.5 TB/s), with weights 42.0; 8 bits, 1024 rows, 26.2 (3.8 TB/s)
+//   64 of 600, window 256            13.3 (3.8 TB/s)
 //   4 of 4000                        bf16 34.3 (5.7 TB/s), with weights 38.8, 8 bits 25.2 (3.9 TB/s); one of 650: 4.7 either way
 // What bounds the 8-bit form is not HBM but instruction issue (two conversions of every element beside its product; 53 % of
 // the slots, which are not filled while a call starts and ends) and the time to the first tile, 4.4 us of the 18.5. Tried for
@@ -138,6 +138,14 @@ __device__ __forceinline__ void unpack_fp8(float2 (&f)[8], const uint4& raw) {
     f[2 * i] = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i] & 0xffffu), __NV_E4M3)));
     f[2 * i + 1] = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i] >> 16), __NV_E4M3)));
   }
+}
+
+// acc += a b for both elements of the words: bf16 factors, exact products, fp32 sums, no conversion ahead of them
+__device__ __forceinline__ void fma_bf16(float2& acc, uint32_t a, uint32_t b) {
+  asm("{\n\t.reg .b16 al, ah, bl, bh;\n\tmov.b32 {al, ah}, %2;\n\tmov.b32 {bl, bh}, %3;\n\t"
+      "fma.rn.f32.bf16 %0, al, bl, %0;\n\tfma.rn.f32.bf16 %1, ah, bh, %1;\n\t}"
+      : "+f"(acc.x), "+f"(acc.y)
+      : "r"(a), "r"(b));
 }
 
 // The visible rows of a sequence of `len` rows as tiles.
@@ -416,7 +424,25 @@ __global__ void __launch_bounds__(kThreads, kManyPerSm) decode_window_kernel(con
           for (int e = 0; e < 4; ++e) f[4 * i + e] = x[e];
         }
       };
-      unpack_bf16(qf, q_raw);
+      if (FP8) unpack_bf16(qf, q_raw);
+      // q k of a lane's part of a row: bf16 without a conversion (64 x 12 heads of 64, 512 rows each: 23.1 -> 22.2 us, with
+      // weights and 1000 rows 45.1 -> 42.0), 8-bit rows as fp32. (Those as f16, with q scaled to f16 once, was 2 % faster on
+      // some calls and 3 % slower on others.)
+      auto dot_of = [&](const auto& k, auto unpack) -> float {
+        float2 dot = make_float2(0.f, 0.f);
+        if constexpr (FP8) {
+          float2 kf[EPL / 2];
+          unpack(kf, k);
+#pragma unroll
+          for (int e = 0; e < EPL / 2; ++e) dot = ffma2(qf[e], kf[e], dot);
+        } else {
+          const uint4 &qx = q_raw[0], &kx = *reinterpret_cast<const uint4*>(&k.x);   // (one piece, whichever way it came)
+          const uint32_t a[4] = {qx.x, qx.y, qx.z, qx.w}, b[4] = {kx.x, kx.y, kx.z, kx.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) fma_bf16(dot, a[e], b[e]);
+        }
+        return dot.x + dot.y;
+      };
 #pragma unroll
       for (int e = 0; e < EPL / 2; ++e) acc[e] = make_float2(0.f, 0.f);
       float* scores = WEIGHTS ? p.scores + bh * max_len : nullptr;
@@ -429,14 +455,7 @@ __global__ void __launch_bounds__(kThreads, kManyPerSm) decode_window_kernel(con
         constexpr bool ALL = decltype(all)::value;
         float sc[NR], pr[NR];
 #pragma unroll
-        for (int u = 0; u < NR; ++u) {
-          float2 kf[EPL / 2];
-          unpack(kf, kr[u]);
-          float2 dot = fmul2(qf[0], kf[0]);
-#pragma unroll
-          for (int e = 1; e < EPL / 2; ++e) dot = ffma2(qf[e], kf[e], dot);
-          sc[u] = dot.x + dot.y;
-        }
+        for (int u = 0; u < NR; ++u) sc[u] = dot_of(kr[u], unpack);
 #pragma unroll
         for (int o = LPK / 2; o > 0; o >>= 1)
 #pragma unroll
