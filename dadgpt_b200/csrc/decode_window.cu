@@ -140,14 +140,6 @@ __device__ __forceinline__ void unpack_fp8(float2 (&f)[8], const uint4& raw) {
   }
 }
 
-// acc += a b for both elements of the words: bf16 factors, exact products, fp32 sums, no conversion ahead of them
-__device__ __forceinline__ void fma_bf16(float2& acc, uint32_t a, uint32_t b) {
-  asm("{\n\t.reg .b16 al, ah, bl, bh;\n\tmov.b32 {al, ah}, %2;\n\tmov.b32 {bl, bh}, %3;\n\t"
-      "fma.rn.f32.bf16 %0, al, bl, %0;\n\tfma.rn.f32.bf16 %1, ah, bh, %1;\n\t}"
-      : "+f"(acc.x), "+f"(acc.y)
-      : "r"(a), "r"(b));
-}
-
 // The visible rows of a sequence of `len` rows as tiles.
 template <bool FP8, int D>
 struct View {
@@ -651,7 +643,8 @@ __global__ void __launch_bounds__(kThreads, kManyPerSm) decode_window_kernel(con
         const float inv = 1.f / l_all;
         float* weights = p.weights + bh * max_len;
         // Several rows of a thread on their way together. One after the other 4 x 24 heads of 128 (clusters), 4000 rows, took
-        // 41.7 us, so 38.8; 64 x 12 heads of 64, 1000 rows, 47.5 / 45.0 (8 at a time 49.0: the next item's vectors are spilt).
+        // 41.7 us, so 39; 64 x 12 heads of 64, 1000 rows, 47.5 / 45.0 (42.0 with the bf16 products; with 8 at a time 48.2: the
+        // next item's vectors are spilt).
         constexpr int kAhead = CLUSTER ? 8 : 4;
         auto rows = [&](int from, int to) {
           for (int j = from + d; j < to; j += kAhead * kWarps * 32) {

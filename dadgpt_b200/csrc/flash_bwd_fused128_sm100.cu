@@ -30,9 +30,11 @@
 #include <cuda_bf16.h>
 
 #include <cfloat>
+#include <type_traits>
 
 #include "common.cuh"
 #include "sm100_ptx.cuh"
+#include "window_delta.cuh"
 
 namespace dadattn {
 namespace {
@@ -464,31 +466,56 @@ flash_bwd_fused128_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
 // lanes per row of 128. Also zeros into the workspace, 32 bytes per thread (a memset of its own between two
 // kernels costs short calls about 3 us). From the last row on, as the pass that rounds: the gradient kernel starts with
 // the first, whose lines L2 then still holds (64 x 2048 backward 269-274 -> 261-268 us, 192 x 1024 260-264 -> 258-259).
-__global__ void fused128_prepare_kernel(float* __restrict__ delta, float* __restrict__ dq_ws,
+// With a window, FEW, the last of those blocks (the first to start) take the rows that see few keys.
+// Those need registers, so that half as many threads are on an SM, which then have two pieces each on their way.
+template <class FEW>
+constexpr int kPreparePieces = std::is_same_v<FEW, FewKeys> ? 2 : 1;
+template <class FEW>
+__global__ void __launch_bounds__(kPrepareThreads, 8 / kPreparePieces<FEW>)
+fused128_prepare_kernel(float* __restrict__ delta, float* __restrict__ dq_ws,
                                         const __nv_bfloat16* __restrict__ dout,
-                                        const __nv_bfloat16* __restrict__ out, int64_t rows) {
-  constexpr int D = kGD, Lr = D / 8;
+                                        const __nv_bfloat16* __restrict__ out, int64_t rows, const FEW few) {
+  constexpr int D = kGD, Lr = D / 8, N = kPreparePieces<FEW>;
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t block = gridDim.x - 1 - blockIdx.x, t = block * blockDim.x + threadIdx.x;
-  const int64_t r = t / Lr;
-  const int c = static_cast<int>(t % Lr) * 8;
-  float4* zero = reinterpret_cast<float4*>(dq_ws) + block * (2 * kPrepareThreads);
-  zero[threadIdx.x] = zero[threadIdx.x + kPrepareThreads] = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
-  if (r < rows) {
-    const uint4 a = *reinterpret_cast<const uint4*>(dout + r * D + c);
-    const uint4 b = *reinterpret_cast<const uint4*>(out + r * D + c);
-    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+  const int64_t block = gridDim.x - 1 - blockIdx.x;
+  if constexpr (N > 1)
+    if (block >= few.first_block) {
+      few_keys_delta<D>(few, block - few.first_block, dout, delta);
+      return;
+    }
+  const int c = static_cast<int>(threadIdx.x % Lr) * 8;
+  int64_t r[N];
+  uint4 a[N], b[N];
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    const int64_t t = (block * N + u) * blockDim.x + threadIdx.x;
+    r[u] = t / Lr;
+    // (a tile of the workspace is cleared by a multiple of N blocks' pieces)
+    float4* zero = reinterpret_cast<float4*>(dq_ws) + (block * N + u) * (2 * kPrepareThreads);
+    zero[threadIdx.x] = zero[threadIdx.x + kPrepareThreads] = make_float4(0.f, 0.f, 0.f, 0.f);
+    a[u] = b[u] = make_uint4(0, 0, 0, 0);
+    if (r[u] < rows) {
+      a[u] = *reinterpret_cast<const uint4*>(dout + r[u] * D + c);
+      b[u] = *reinterpret_cast<const uint4*>(out + r[u] * D + c);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    float sum = 0.f;
+    const uint32_t aw[4] = {a[u].x, a[u].y, a[u].z, a[u].w}, bw[4] = {b[u].x, b[u].y, b[u].z, b[u].w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       sum = fmaf(__uint_as_float(aw[i] << 16), __uint_as_float(bw[i] << 16), sum);
       sum = fmaf(__uint_as_float(aw[i] & 0xffff0000u), __uint_as_float(bw[i] & 0xffff0000u), sum);
     }
-  }
 #pragma unroll
-  for (int o = Lr / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (r < rows && c == 0) delta[r] = sum;
+    for (int o = Lr / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    bool mine = true;
+    if constexpr (N > 1)   // (2^31 rows would be 549 GB of bf16)
+      mine = static_cast<uint32_t>(r[u]) % static_cast<uint32_t>(few.S) >= static_cast<uint32_t>(few.rows);
+    if (r[u] < rows && c == 0 && mine) delta[r[u]] = sum;
+  }
 }
 
 // Workspace tile [16 groups of 4 queries][128 dims][4 queries] fp32 -> dq[q][128] bf16. One CTA of 256 threads
@@ -556,8 +583,18 @@ static int launch_bwd_d128(uint16_t* dq, uint16_t* dk, uint16_t* dv, void* works
   stage_event(0, st);
   const int64_t rows = static_cast<int64_t>(BH) * S;
   const int64_t blocks = static_cast<int64_t>(BH) * n_sub * (kGDqTileBytes / (32 * kPrepareThreads));
-  DAD_CUDA(launch_pdl(fused128_prepare_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kPrepareThreads), 0, st, delta,
-                      dq_ws, reinterpret_cast<const BF*>(dout), reinterpret_cast<const BF*>(out), rows));
+  if (window > 0) {
+    static_assert(FewKeys::kThreads == kPrepareThreads, "one block size");
+    static_assert(kGDqTileBytes / (32 * kPrepareThreads) % kPreparePieces<FewKeys> == 0, "blocks of a tile");
+    const int64_t half = blocks / kPreparePieces<FewKeys>;
+    const FewKeys few = few_keys(q, k, v, lse, BH, S, scale, window, sinks, half);
+    DAD_CUDA(launch_pdl(fused128_prepare_kernel<FewKeys>, dim3(static_cast<unsigned>(half + few_keys_blocks(few))),
+                        dim3(kPrepareThreads), 0, st, delta, dq_ws, reinterpret_cast<const BF*>(dout),
+                        reinterpret_cast<const BF*>(out), rows, few));
+  } else {
+    DAD_CUDA(launch_pdl(fused128_prepare_kernel<NoRows>, dim3(static_cast<unsigned>(blocks)), dim3(kPrepareThreads), 0, st, delta,
+                        dq_ws, reinterpret_cast<const BF*>(dout), reinterpret_cast<const BF*>(out), rows, NoRows{}));
+  }
   stage_event(1, st);
   const PhiloxRounds rng = make_philox_rounds(seed, offset, rate, static_cast<uint32_t>(S));
   // Key tiles level by level over groups of units, whatever the number of CTAs. Backward alone, us (medians), level

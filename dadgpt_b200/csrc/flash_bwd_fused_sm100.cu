@@ -36,9 +36,11 @@
 #include <cuda_bf16.h>
 
 #include <cfloat>
+#include <type_traits>
 
 #include "common.cuh"
 #include "sm100_ptx.cuh"
+#include "window_delta.cuh"
 
 namespace dadattn {
 namespace {
@@ -736,42 +738,64 @@ flash_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 // Blocks take the rows from the end, here and in the pass that rounds: the gradient kernel starts with the first units,
 // whose lines are then the last to have come into L2, and leaves those of the last ones there (192 x 1024 step 168.9
 // -> 167.7 us, behind fp32 tensors 74.1 -> 73.7).
-template <bool INTERLEAVED>
-__global__ void fused_prepare_kernel(float* __restrict__ delta, float* __restrict__ dq_ws,
+// With a window, FEW, the last of those blocks (the first to start) take the rows that see few keys.
+// Those need registers, so that half as many threads are on an SM, which then have two pieces each on their way.
+template <class FEW>
+constexpr int kPreparePieces = std::is_same_v<FEW, FewKeys> ? 2 : 1;
+template <bool INTERLEAVED, class FEW>
+__global__ void __launch_bounds__(256, 8 / kPreparePieces<FEW>)
+fused_prepare_kernel(float* __restrict__ delta, float* __restrict__ dq_ws,
                                      int* __restrict__ item_counter,
                                      const __nv_bfloat16* __restrict__ dout,
                                      const __nv_bfloat16* __restrict__ out, int64_t rows, int S,
-                                     UnitLayout lay) {
+                                     UnitLayout lay, const FEW few) {
   constexpr int D = kFD, Lr = D / 8;  // 8 lanes per row
-  const int64_t t = static_cast<int64_t>(gridDim.x - 1 - blockIdx.x) * blockDim.x + threadIdx.x;
-  const int64_t r = t / Lr;   // row of the [BH, S] index space: delta and the workspace are heads-split
-  const int c = static_cast<int>(t % Lr) * 8;
+  constexpr int N = kPreparePieces<FEW>;
+  const int64_t block = gridDim.x - 1 - blockIdx.x;
   pdl_wait();
   pdl_launch_dependents();
-  if (t == 0) *item_counter = 0;
-  float sum = 0.f;
-  if (r < rows) {
-    zero_32_bytes(dq_ws + r * D + c);   // (whole sectors)
-    // where row r = (unit, s) lies in dO and O: heads-split rows are simply consecutive
-    int64_t at = r * D + c;
-    if (INTERLEAVED) {
-      // (32-bit: 2^31 rows would be 274 GB of bf16, and 64-bit divisions took a fifth of this pass's time)
-      const int unit = static_cast<uint32_t>(r) / static_cast<uint32_t>(S), srow = static_cast<int>(r) - unit * S;
-      const int ub = unit / lay.heads, uh = unit - ub * lay.heads;
-      at = ub * lay.batch + uh * lay.head + srow * lay.row + c;
+  if (block == 0 && threadIdx.x == 0) *item_counter = 0;
+  if constexpr (N > 1)
+    if (block >= few.first_block) {
+      few_keys_delta<D>(few, block - few.first_block, dout, delta);
+      return;
     }
-    const uint4 a = *reinterpret_cast<const uint4*>(dout + at);
-    const uint4 b = *reinterpret_cast<const uint4*>(out + at);
-    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+  const int c = static_cast<int>(threadIdx.x % Lr) * 8;
+  int64_t r[N];   // rows of the [BH, S] index space: delta and the workspace are heads-split
+  uint4 a[N], b[N];
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    r[u] = ((block * N + u) * blockDim.x + threadIdx.x) / Lr;
+    a[u] = b[u] = make_uint4(0, 0, 0, 0);
+    if (r[u] < rows) {
+      zero_32_bytes(dq_ws + r[u] * D + c);   // (whole sectors)
+      // where row r = (unit, s) lies in dO and O: heads-split rows are simply consecutive
+      int64_t at = r[u] * D + c;
+      if (INTERLEAVED) {
+        // (32-bit: 2^31 rows would be 274 GB of bf16, and 64-bit divisions took a fifth of this pass's time)
+        const int unit = static_cast<uint32_t>(r[u]) / static_cast<uint32_t>(S), srow = static_cast<int>(r[u]) - unit * S;
+        const int ub = unit / lay.heads, uh = unit - ub * lay.heads;
+        at = ub * lay.batch + uh * lay.head + srow * lay.row + c;
+      }
+      a[u] = *reinterpret_cast<const uint4*>(dout + at);
+      b[u] = *reinterpret_cast<const uint4*>(out + at);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    float sum = 0.f;
+    const uint32_t aw[4] = {a[u].x, a[u].y, a[u].z, a[u].w}, bw[4] = {b[u].x, b[u].y, b[u].z, b[u].w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       sum = fmaf(__uint_as_float(aw[i] << 16), __uint_as_float(bw[i] << 16), sum);
       sum = fmaf(__uint_as_float(aw[i] & 0xffff0000u), __uint_as_float(bw[i] & 0xffff0000u), sum);
     }
-  }
 #pragma unroll
-  for (int o = Lr / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (r < rows && c == 0) delta[r] = sum;
+    for (int o = Lr / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    bool mine = true;
+    if constexpr (N > 1) mine = static_cast<uint32_t>(r[u]) % static_cast<uint32_t>(S) >= static_cast<uint32_t>(few.rows);   // (32 bits: as above)
+    if (r[u] < rows && c == 0 && mine) delta[r[u]] = sum;
+  }
 }
 
 // dQ workspace (fp32) -> dq (bf16). The sums are read for the last time: their lines, which would go out to memory
@@ -917,10 +941,19 @@ static int launch_bwd_d64(uint16_t* dq, uint16_t* dk, uint16_t* dv, void* worksp
   const int64_t rows = static_cast<int64_t>(BH) * S;
   const int64_t prep_threads = rows * (kFD / 8);
   stage_event(0, st);
-  DAD_CUDA(launch_pdl(heads > 0 ? fused_prepare_kernel<true> : fused_prepare_kernel<false>,
-                      dim3(static_cast<unsigned>((prep_threads + 255) / 256)),
-                      dim3(256), 0, st, delta, dq_ws, item_counter, reinterpret_cast<const BF*>(dout),
-                      reinterpret_cast<const BF*>(out), rows, S, lay));
+  const int64_t prep_blocks = (prep_threads + 255) / 256;
+  if (window > 0) {
+    const int64_t blocks = (prep_blocks + kPreparePieces<FewKeys> - 1) / kPreparePieces<FewKeys>;
+    const FewKeys few = few_keys(q, k, v, lse, BH, S, scale, window, sinks, blocks);
+    DAD_CUDA(launch_pdl(fused_prepare_kernel<false, FewKeys>, dim3(static_cast<unsigned>(blocks + few_keys_blocks(few))), dim3(256),
+                        0, st, delta, dq_ws, item_counter, reinterpret_cast<const BF*>(dout), reinterpret_cast<const BF*>(out), rows,
+                        S, lay, few));
+  } else {
+    DAD_CUDA(launch_pdl(heads > 0 ? fused_prepare_kernel<true, NoRows> : fused_prepare_kernel<false, NoRows>,
+                        dim3(static_cast<unsigned>(prep_blocks)),
+                        dim3(256), 0, st, delta, dq_ws, item_counter, reinterpret_cast<const BF*>(dout),
+                        reinterpret_cast<const BF*>(out), rows, S, lay, NoRows{}));
+  }
   stage_event(1, st);
   if (int rc = launch_fused_kernel(dq_ws, dk, dv, nullptr, nullptr, delta, item_counter, dout, lse, q, k, v, BH, S, lay,
                                    scale, rate, make_philox(seed, offset), unit0, mask_bits, window, sinks, st))

@@ -105,6 +105,21 @@ def test_what_no_query_reaches_does_not_matter(cuda, D):
         assert torch.equal(a[:, 512:], b[:, 512:])
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("S,window", [(200, 1), (1, 7), (777, 1)])
+def test_a_row_that_sees_one_key_has_no_gradient_of_scores(cuda, D, S, window):
+    """P = 1 and dS = dP - delta = 0 for such rows. Two sums of D products in fp32, in whichever order and rounded or cut off
+    (2^-23 a step), and P's own error (`rel` of bounds()) are what is left, not the rounding of out to bf16."""
+    inputs = _inputs(cuda, 2, S, D, 11)
+    scale = D ** -0.5
+    _, lse, dq, dk, _ = _run(*inputs, scale, window, 0)
+    q, k, v, do = (t.double() for t in inputs)
+    size = (q * k).abs().sum(2) * scale
+    rel = 2 * (D + 4) * 2.0 ** -24 * size + 2 * (S + 4) * 2.0 ** -24 + 4 * 2.0 ** -24 * lse.double().abs() + 2.0 ** -20
+    ds = (2 * D * 2.0 ** -23 + 2 * rel) * (do * v).abs().sum(2) * scale * (1 + 2.0 ** -6)   # (and the roundings to bf16)
+    assert bool((dq.double().abs() <= ds[..., None] * k.abs()).all()) and bool((dk.double().abs() <= ds[..., None] * q.abs()).all())
+
+
 def test_a_directional_difference(cuda):
     S, D, window, sinks, scale = 150, 64, 40, 3, 0.125
     inputs = _inputs(cuda, 1, S, D, 7)
