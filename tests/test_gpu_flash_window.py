@@ -39,7 +39,7 @@ def _check(got, inputs, scale, window, sinks, units):
 
 SHAPES = [(1, 1, 0), (2, 1, 1), (63, 64, 0), (64, 17, 3), (65, 64, 1), (127, 1, 0), (128, 65, 64), (129, 128, 0), (129, 2, 130),
           (200, 63, 65), (256, 129, 4), (300, 0, 0), (300, 300, 7), (300, 5000, 0), (300, 30, 5000), (511, 128, 4),
-          (513, 100, 129), (640, 64, 64), (777, 256, 4), (777, 33, 300), (1000, 1, 1), (1100, 500, 0)]
+          (500, 8, 24), (333, 32, 0), (333, 31, 2), (513, 100, 129), (640, 64, 64), (777, 256, 4), (777, 33, 300), (1000, 1, 1), (1100, 500, 0)]
 
 
 @pytest.mark.parametrize("D", [64, 128])

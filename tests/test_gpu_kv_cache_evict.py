@@ -159,3 +159,28 @@ def test_the_kernel_ahead_may_write_weights_and_lengths(cuda):
         dad.kv_cache_evict_bf16(dst, src, 100, 10)
         for x in ("k", "v", "weights", "lengths"):
             assert torch.equal(getattr(dst, x), getattr(want, x))
+
+
+def test_two_caches_on_two_streams_at_once(cuda):
+    """Steps and evictions of two caches, each on its own stream, leave what they leave one after the other."""
+    def run(at_once):
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()] if at_once else [torch.cuda.current_stream()] * 2
+        caches = [_made(cuda, 40, 12, 400, 64, [(b * 7 + 13 * i) % 300 for b in range(40)], 31 + i) for i in range(2)]
+        small = [dad.KVCacheFP8(3, 12, 1000, 64, device=cuda) for _ in range(2)]
+        g = torch.Generator(device=cuda).manual_seed(33)
+        heads = torch.randn(3, 12, 700, 64, device=cuda, generator=g).bfloat16()
+        x = torch.randn(2, 4, 40, 12, 64, device=cuda, generator=g).bfloat16()
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for i, (st, c, f) in enumerate(zip(streams, caches, small)):
+                with torch.cuda.stream(st):
+                    dad.decode_attention_bf16_window(x[i, 3], x[i, 0], x[i, 1], x[i, 2], c, 0.125, weights=True)
+                    dad.kv_cache_evict_bf16(c, c, 150, 20)
+                    dad.kv_cache_fill_fp8(f, heads, heads)
+                    dad.decode_attention_fp8(x[i, 3, :3], x[i, 0, :3], x[i, 1, :3], x[i, 2, :3], f, 0.125)
+        torch.cuda.synchronize()
+        assert device_status() == 0
+        return [t for c, f in zip(caches, small) for t in (c.k, c.v, c.weights, c.lengths, f.k.view(torch.uint8), f.k_tail, f.lengths)] + [x]
+
+    for a, b in zip(run(False), run(True)):
+        assert torch.equal(a, b)
