@@ -606,7 +606,9 @@ __global__ void __launch_bounds__(kThreads, kManyPerSm) decode_window_kernel(con
           sh.l[warp] = l;
         }
       }
-      consumers_sync();   // (the scores and the appended row are there for the whole CTA, too)
+      // The warps go on with one `ok`: barriers follow that only an item in order has. (The scores and the appended row are
+      // there for the whole CTA, too.)
+      ok = !consumers_any(!ok);
       const int d = threadIdx.x;
       float mm = -FLT_MAX, ll = 0.f;
 #pragma unroll
@@ -707,8 +709,8 @@ __global__ void __launch_bounds__(kThreads, kManyPerSm) decode_window_kernel(con
       }
       if (!CLUSTER) {
         if (!s.good && s.h == 0 && threadIdx.x == 0) atomicExch(p.status, DADATTN_E_ARG);
-        // sh.acc / sh.m are read: the next item may write them. The warps go on together or not at all.
-        if (consumers_any(!ok)) have = false;
+        consumers_sync();   // sh.acc / sh.m are read: the next item may write them
+        have = have && ok;
       }
     }
   }
