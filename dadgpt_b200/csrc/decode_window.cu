@@ -538,8 +538,10 @@ __global__ void __launch_bounds__(kThreads, kManyPerSm) decode_window_kernel(con
           float ks = scale_unit, vs = 1.f;
           if (FP8) {
             const int i = warp * (V::kRows / kWarps) / kFp8Block;   // the warp's block within the tile
-            ks *= sh.scales[st][i];
-            vs = sh.scales[st][2 + i];
+            if (r.base + i * kFp8Block < r.hi) {                    // (of one that the tile has no row of, no scale was loaded)
+              ks *= sh.scales[st][i];
+              vs = sh.scales[st][2 + i];
+            }
           }
           auto unpack = [&](float2 (&f)[EPL / 2], const Row& w) {
             if constexpr (FP8) unpack_fp8(f, w.x);
@@ -556,8 +558,6 @@ __global__ void __launch_bounds__(kThreads, kManyPerSm) decode_window_kernel(con
               valid[u] = view.sees(r, row(u));
               if (!valid[u]) kr[u].x = vr[u].x = make_uint4(0, 0, 0, 0);
             }
-            // (the scale of a block that the tile has no row of was not loaded)
-            if (FP8 && !(vs < INFINITY)) vs = 0.f;
             absorb(kr, vr, unpack, valid, Count{}, std::false_type{}, ks, vs, row);
           }
         }
