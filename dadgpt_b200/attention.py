@@ -181,7 +181,9 @@ def decode_attention_bf16_window(out, q, k_new, v_new, cache: KVCacheBF16, scale
     """:func:`decode_attention_bf16` over a sliding window: the token at row L of its sequence sees row j <= L iff
     L - j < window or j < sinks (window = 0: every row). With ``weights``, each visible row's probability is added to
     ``cache.weights`` (and the appended row's weight set to its own); the cache was made with ``weights=True``, and rows
-    that a prompt filled begin with the weights that the caller puts there (zeros, say)."""
+    that a prompt filled begin with the weights that the caller puts there (zeros, say). Without ``weights`` none is written,
+    on a cache that has them neither: the appended row's is then what an earlier row left in its place, until the caller
+    sets it."""
     if weights and cache.weights is None:
         raise ValueError("the cache has no weights: make it with weights=True")
     _native().decode_bf16_window(cache.B, cache.H, cache.D, cache.max_len, scale, window, sinks, out, q, k_new, v_new,
@@ -191,7 +193,9 @@ def decode_attention_bf16_window(out, q, k_new, v_new, cache: KVCacheBF16, scale
 def kv_cache_evict_bf16(dst: KVCacheBF16, src: KVCacheBF16, budget, recent=0):
     """Keeps ``budget`` rows of every sequence and head of ``src`` that has more: the last ``recent`` ones and the
     heaviest of the others by ``src.weights`` (equal ones: the lower index). K, V and weights of the rows that stay go,
-    in order, to rows 0.. of ``dst``, another cache or ``src`` itself, and ``dst.lengths`` becomes min(length, budget)."""
+    in order, to rows 0.. of ``dst``, another cache or ``src`` itself, and ``dst.lengths`` becomes min(length, budget).
+    Every row needs a weight of its own, from steps with ``weights`` or from the caller: see
+    :func:`decode_attention_bf16_window`."""
     if dst.weights is None or src.weights is None:
         raise ValueError("eviction goes by the weights: make the caches with weights=True")
     _native().evict_bf16(src.B, src.H, src.D, dst.max_len, src.max_len, budget, recent, dst.k, dst.v, dst.weights,

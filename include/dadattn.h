@@ -344,6 +344,8 @@ int dadattn_decode_noalloc_status(dadattn_stream_t stream);
  * weights (may be NULL): [B,H,max_len] fp32. Each visible row's softmax probability is added to its weight, and the
  * appended row's weight is set to its probability, so that nothing has to be cleared when a sequence starts from its first
  * token. Rows that a prompt put there (dadattn_kv_cache_fill) begin with the weights that the caller gives them: zeros, say.
+ * (The weight that the prompt's own queries give them is formed by no call.) With weights NULL, as by dadattn_decode_bf16, no
+ * weight is written, and the appended row's stays what it was: dadattn_kv_cache_evict_bf16 says what that means.
  * max_len is at most DADATTN_MAX_CACHE_LEN, here and in the calls below.
  * workspace: at least dadattn_decode_window_workspace_bytes(B, H, D, max_len, weights != NULL) bytes, 16-byte aligned, with
  * the rules of dadattn_decode_bf16's: zero-filled once, to be zero-filled again when B, H or max_len change, not shared by
@@ -361,7 +363,12 @@ int dadattn_decode_bf16_window(uint16_t* out, const uint16_t* q, const uint16_t*
  * lengths_dst[b] becomes min(n, budget). Other rows of the destination are left as they were.
  * k, v [B,H,max_len,D] bf16, weights [B,H,max_len] fp32, 1 <= budget <= max_len_dst, 0 <= recent <= budget,
  * max_len_src <= 196608. The destination is another cache, or the source itself (all four arrays the same; the arrays do
- * not overlap otherwise). A sequence whose length is outside [0, max_len_src] is left untouched and reported through
+ * not overlap otherwise).
+ * Every row that is chosen from needs a weight of its own: from steps with weights, or put there by the caller. A row that a
+ * prompt or a step without weights left behind has what lay in that place: zero in a new cache, but the weight of an earlier
+ * row where a cache is used again or was evicted from in place (rows from the budget on keep their old weights). Equal weights
+ * keep the first rows: behind a prompt whose rows all have zero, the prompt's first ones.
+ * A sequence whose length is outside [0, max_len_src] is left untouched and reported through
  * DADATTN_E_ARG at the next dadattn_device_status(). Every head keeps rows of its own choice: only for models whose keys do
  * not depend on the row they lie in (positions added to the embeddings, as in GPT-2, or rotated into the keys before they are
  * cached), and without dadattn_decode_bf16_window's window, which counts rows. No counterpart in the reference. */
