@@ -13,18 +13,21 @@
 //                 CTA that appended it turns it into a block behind the item's arithmetic: every block is rounded once,
 //                 from bf16, and holds the same bytes whether a prompt filled it or single tokens did.
 // Weights: a row's score is written to scratch as it is formed; once the item's m and l are known the CTA that formed it
-// adds exp(s - m) / l to the row's weight. 12 bytes a row beside 4 D of K and V.
+// adds exp(s - m) / l to the row's weight. 16 bytes a row (the score out and, from L2, in again; the weight in and out) beside
+// 4 D of K and V.
 //
 // Measured in a graph of such calls on rotating caches (us; 64 x 12 heads of 64, 4 x 24 of 128):
 //   64 sequences of 9 .. 1017 rows   bf16 21.8 (4.6 TB/s), with weights 25.3, 8 bits 18.5 (2.7 TB/s)
 //   64 of 1000                       bf16 35.7 (5.5 TB/s), with weights 42.0; 8 bits, 1024 rows, 26.2 (3.8 TB/s)
 //   64 of 600, window 256            13.3 (3.8 TB/s)
 //   4 of 4000                        bf16 34.3 (5.7 TB/s), with weights 38.8, 8 bits 25.2 (3.9 TB/s); one of 650: 4.7 either way
-// What bounds the 8-bit form is not HBM but instruction issue (two conversions of every element beside its product; 53 % of
-// the slots, which are not filled while a call starts and ends) and the time to the first tile, 4.4 us of the 18.5. Tried for
-// it and not faster: rings of every warp's own filled by 16-byte copies (20-22 us), both products by warp-wide matrix
-// instructions (20-29) or K's alone (19.7), even shares of all rows for every CTA with partial results in memory (25-34), two
-// consumer warps with 4 KB tiles (26).
+// The 8-bit form is at no unit's limit (HBM 41 %, issue slots 53 %): its time is the start and end of a call, 4.4 us of the
+// 18.5 to the first tile, and in between waits of few warps for their own earlier steps (2.4 cycles an instruction for memory,
+// 1.4 for results). It executes 5.8 instructions for a cached element, where two conversions to a pair and the product are 2 to
+// 2.5: tiles whose last rows are missing are computed whole, and every item is merged and ranked. Its persistent instances
+// spill (94 registers, 128 bytes out and 160 in). Tried for it and not faster: rings of every warp's own filled by 16-byte
+// copies (20-22 us), both products by warp-wide matrix instructions (20-29) or K's alone (19.7), even shares of all rows for
+// every CTA with partial results in memory (25-34), two consumer warps with 4 KB tiles (26).
 #include <cuda_bf16.h>
 
 #include <cfloat>
@@ -782,14 +785,16 @@ int launch(Params p, cudaStream_t st) {
   // Clusters of four or eight for two sequences in place of two or four CTAs for each, where lengths may differ and some room
   // is left on the GPU; decode.cu has both sides of the limits. Here: 4 sequences x 24 heads x 128 in 8 bits, of 1000, 3000,
   // 5000 and 7000 rows: 33.0 us with four CTAs for each, 25.2 so, and 25.2 both ways where each has 4000 rows. Under a window
-  // the sequences are alike.
+  // the sequences that are longer than it are alike. (The rule does not see a window that most are shorter than: the same
+  // sequences with one as long as the cache take 34.1 us, 26.3 without.)
   const long long paired = static_cast<long long>((p.B + 1) / 2) * p.H * p.ranks * 2;
   p.paired = p.window == 0 && p.ranks > 1 && p.ranks < kMaxCluster && p.B >= 2 && p.B <= kMaxPaired &&
              paired * 100 <= resident * (p.ranks * 2 == kMaxCluster ? 84LL : 92LL);
   if (p.paired) p.ranks *= 2, grid = paired;
   p.stages = grid <= kFewPerSm * sms ? kFewStages : kManyStages;
-  // Longest first pays once a CTA takes more than one item (not under a window, which makes them all alike); the in-kernel
-  // ranking, 0.9 us, handles 32..256 sequences.
+  // Longest first pays once a CTA takes more than one item (not under a window, behind which sequences are alike; 64 x 12 heads
+  // of 9 .. 1017 rows in 8 bits with a window that hides nothing 20.8 us, 18.9 ranked); the in-kernel ranking, 0.9 us, handles
+  // 32..256 sequences.
   p.reorder = p.B >= 32 && p.B <= kMaxRanked && pairs > grid && p.window == 0;
   auto kern = p.ranks > 1 ? decode_window_kernel<FP8, D, true, WEIGHTS> : decode_window_kernel<FP8, D, false, WEIGHTS>;
   DAD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(decode_smem(kMaxStages))));

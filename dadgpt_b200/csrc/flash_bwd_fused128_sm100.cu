@@ -467,7 +467,8 @@ flash_bwd_fused128_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
 // kernels costs short calls about 3 us). From the last row on, as the pass that rounds: the gradient kernel starts with
 // the first, whose lines L2 then still holds (64 x 2048 backward 269-274 -> 261-268 us, 192 x 1024 260-264 -> 258-259).
 // With a window, FEW, the last of those blocks (the first to start) take the rows that see few keys.
-// Those need registers, so that half as many threads are on an SM, which then have two pieces each on their way.
+// Those need registers (64, with 64 bytes spilt), so that half as many threads are on an SM, which then have two pieces each on
+// their way.
 template <class FEW>
 constexpr int kPreparePieces = std::is_same_v<FEW, FewKeys> ? 2 : 1;
 template <class FEW>
@@ -608,6 +609,7 @@ static int launch_bwd_d128(uint16_t* dq, uint16_t* dk, uint16_t* dv, void* works
   // With a window all units are one group: the tiles of the first tokens, which every query sees, are the only long ones
   // and start ahead of all others (backward, 24 x 8192, window 1024, 4 first tokens, in groups of 24 / 12 / 8 / 4 units:
   // 372 / 378 / 429 / 468 us; without first tokens all the same). As long as the grid's second dimension holds the levels.
+  // Measured for windows up to S / 4 or so; with one that hides nothing the same units take 1237 us, causal 1168.
   const bool one_group = window > 0 && (S + kGKeys - 1) / kGKeys <= 65535;
   const LeveledGrid order = one_group ? LeveledGrid{BH, BH} : leveled_grid(32768, S, BH);
   const int variant = window > 0 ? 2 : rate > 0.f ? 1 : 0;

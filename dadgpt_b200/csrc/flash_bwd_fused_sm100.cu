@@ -739,7 +739,8 @@ flash_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 // whose lines are then the last to have come into L2, and leaves those of the last ones there (192 x 1024 step 168.9
 // -> 167.7 us, behind fp32 tensors 74.1 -> 73.7).
 // With a window, FEW, the last of those blocks (the first to start) take the rows that see few keys.
-// Those need registers, so that half as many threads are on an SM, which then have two pieces each on their way.
+// Those need registers (64, with 40 bytes spilt), so that half as many threads are on an SM, which then have two pieces each on
+// their way.
 template <class FEW>
 constexpr int kPreparePieces = std::is_same_v<FEW, FewKeys> ? 2 : 1;
 template <bool INTERLEAVED, class FEW>
@@ -900,7 +901,8 @@ static int launch_fused_kernel(float* dq_ws, uint16_t* dk, uint16_t* dv, float* 
   dim3 grid(static_cast<unsigned>(n_items < sms ? n_items : sms));
   // With a window the tiles of the first tokens, which every query sees, are the only long ones: all units in one group (192
   // x 1024, window 256, 4 first tokens, in groups of 192 / 64 / 32 / 16: 101.8 / 101.3 / 107.9 / 115.1 us; 72 x 777, window
-  // 128, 72 / 36 / 24: 36.6 / 43.0 / 46.1; without first tokens all the same).
+  // 128, 72 / 36 / 24: 36.6 / 43.0 / 46.1; without first tokens all the same). Measured for windows up to S / 4 or so; where all
+  // tiles are long the rule gives away what groups are for (192 x 1024, window 512: 128 us, 1024: 134, causal 127).
   const int group_bh = window > 0 || static_cast<int64_t>(BH) * S <= kFAllInL2 ? BH : leveled_grid(65536, S, BH).group;
   const int variant = window > 0 ? 4 : f32_dk ? 3 : rate > 0.f ? (mask_bits ? 2 : 1) : 0;
   auto kern = variant == 4 ? flash_bwd_fused_kernel<0, false, true>

@@ -19,8 +19,11 @@
 // The accumulator is rescaled only when a row's maximum has grown by 2^8 (exact all the same); warps that see nothing of a
 // tile store zeros.
 // Measured (us): 192 x 1024 x 64, window 256, 4 first tokens 41 (101 MB and 11.4 GFLOP), 72 x 777 x 64, window 128 14,
-// 24 x 8192 x 128, window 1024 114 (97 GFLOP: 850 TFLOP/s). Bound by instruction issue and exponentials with latency between
-// (slots 50 %, exp2 unit 41 %, tensor pipe 24 % in the first case; of six tiles or so of 64 keys a third is hidden).
+// 24 x 8192 x 128, window 1024 114 (97 GFLOP: 850 TFLOP/s). No unit is near its limit in either (issue slots 50 %, exp2 41 %,
+// tensor pipe 24 % in the first, 40, 48 and 50 % in the last): a tile's steps wait for each other, and a CTA's start and end
+// are as long as some tiles. Of six tiles or so of 64 keys a third is hidden in the first case. A window that hides little is
+// better taken by the causal kernels, to which nothing here turns: 192 x 1024 x 64 60 us with a window of 1024 and 46 there,
+// 53 with 512; 24 x 8192 x 128 413 and 409.
 // Every wait is bounded (sm100_ptx.cuh). Barriers as in flash_bf16_sm100.cu.
 #include <cuda_bf16.h>
 

@@ -20,6 +20,11 @@
 // time, took 87; all four passes 61.7; every list written by all CTAs 57; two waves of clusters of two for 64 x 12 heads 55.
 // Adding up equal bytes of a warp by votes before the shared atomics cost 1 to 3 us.)
 //
+// Within one cache it is about as fast where CTAs have a (sequence, head) each, 64 x 12 heads of 64, 1024 rows to 512: 48.0 us,
+// of 9 .. 1017 rows 26.7 (33.6 into another: short sequences stay as they are), and slower for clusters, whose CTAs copy a few
+// pieces of every row each, batch by batch: 4 x 24 heads of 128, 8000 rows to 2048 63.4, 2056 to 2048 66.7 (into another 52.9
+// and 47.9). The second launch, for the lengths, is in these.
+//
 // Within one cache: a row's place is never behind the row, so rows that are loaded in order may be stored as soon as every
 // thread has loaded its pieces of the same batch; what is stored lies ahead of all that is loaded later. The columns of a
 // cluster's CTAs are their own, and the weights, which one of them moves, were read by all behind a cluster barrier.
@@ -35,8 +40,8 @@ namespace dadattn {
 namespace {
 
 constexpr int kEvictThreads = 256;
-// 16-byte pieces that a thread has in registers, and CTAs that an SM holds. Clusters: six on an SM (40 registers), so that
-// their waits for each other are covered. One CTA for each pair: 64 x 12 heads of 1 .. 1024 rows to 512 take 32.4 us with four
+// 16-byte pieces that a thread has in registers, and CTAs that an SM holds. Clusters: six on an SM (40 registers, 64 bytes
+// spilt), so that their waits for each other are covered. One CTA for each pair: 64 x 12 heads of 1 .. 1024 rows to 512 take 32.4 us with four
 // that have 8 pieces in flight (all of 1024 rows: 45.6), 35.2 with six of 4 (45.6), 34.7 with five of 4 (57.1: a second wave).
 constexpr int kClusterBatch = 4, kClusterPerSm = 6;
 constexpr int kSingleBatch = 8, kSinglePerSm = 4;

@@ -37,9 +37,9 @@ __device__ __forceinline__ uint4 load_eight(const void* heads, size_t at) {
 }
 
 // Block x of (sequence, head) z, of K or V (y) or of both; the last x of a sequence is its open block. Both for bf16: half as
-// many CTAs, as long as their registers (48) leave the SM as many bytes on their way: the two cases above 46.4 -> 45.8 and
-// 28.4 -> 26.5 us. One from fp32, whose elements take twice the registers ahead of the conversion: 77.3 against 73.6, and
-// 50.7 against 44.1 for 16 x 24 heads of 128, of lengths 1 .. 1024.
+// many CTAs, as long as their registers (48 at head size 64, 80 at 128) leave the SM as many bytes on their way: the two cases
+// above 46.4 -> 45.8 and 28.4 -> 26.5 us. One from fp32, whose elements take twice the registers ahead of the conversion: 77.3
+// against 73.6, and 50.7 against 44.1 for 16 x 24 heads of 128, of lengths 1 .. 1024.
 template <bool BF16>
 constexpr int kSides = BF16 ? 2 : 1;
 template <bool BF16, int D>

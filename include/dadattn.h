@@ -179,7 +179,8 @@ int dadattn_flash_bwd_bf16_strided(uint16_t* dq, uint16_t* dk, uint16_t* dv, voi
  * sinks. Keys outside every query's reach cost nothing: work goes by the 64-key tiles (backward: 128-key tiles and the
  * queries that reach them) with a visible pair in them. As in the calls above, a row that is infinite or NaN makes NaN
  * of the rows that share a tile with one that sees it. The backward must be the single-pass one (the default), its
- * workspace is 256-byte aligned. */
+ * workspace is 256-byte aligned. BH is at most 65535, S at most DADATTN_MAX_CACHE_LEN. A window that hides nothing (0, or S
+ * and more) is taken as it stands, by these kernels: where no pair is hidden the causal calls are the faster ones as a rule. */
 int dadattn_flash_fwd_bf16_window(uint16_t* out, float* lse, const uint16_t* q, const uint16_t* k, const uint16_t* v, int BH,
                                   int S, int D, float scale, int window, int sinks, dadattn_stream_t stream);
 size_t dadattn_flash_bwd_bf16_window_workspace_bytes(int BH, int S, int D);
@@ -394,8 +395,8 @@ int dadattn_fp8_scale_blocks(int max_len);   /* max_len / 64, one at least */
 /* Fills the first counts[b] rows of every sequence from a prefill's heads k_heads, v_heads [B,H,S,D] (fp32, or bf16 when
  * heads_are_bf16; rows behind counts[b] are padding and not read) and sets lengths[b] = counts[b]. counts NULL: S rows of
  * every sequence (S <= max_len). A sequence with counts[b] outside [0, min(S, max_len)] is left untouched and reported
- * through DADATTN_E_ARG at the next dadattn_device_status(). D 64 or 128; one sequence of a larger cache: pointers to its
- * part and B = 1. */
+ * through DADATTN_E_ARG at the next dadattn_device_status(). D 64 or 128, B * H at most 65535 per call (the other calls of
+ * this cache take more); one sequence of a larger cache: pointers to its part and B = 1. */
 int dadattn_kv_cache_fill_fp8(uint8_t* k_cache, uint8_t* v_cache, float* k_scale, float* v_scale, uint16_t* k_tail,
                               uint16_t* v_tail, int32_t* lengths, const void* k_heads, const void* v_heads,
                               const int32_t* counts, int B, int H, int S, int max_len, int D, int heads_are_bf16,
