@@ -540,8 +540,8 @@ __global__ void __launch_bounds__(kThreads, kManyPerSm) decode_window_kernel(con
           for (int u = 0; u < kGroups; ++u) vr[u].x = *reinterpret_cast<const uint4*>(vt + at + u * 512);
           float ks = scale_unit, vs = 1.f;
           if (FP8) {
-            const int i = warp * (V::kRows / kWarps) / kFp8Block;   // the warp's block within the tile
-            if (r.base + i * kFp8Block < r.hi) {                    // (of one that the tile has no row of, no scale was loaded)
+            const int i = warp * (V::kRows / kWarps) / kFp8Block;           // the warp's block within the tile
+            if (V::kRows == kFp8Block || r.base + i * kFp8Block < r.hi) {   // (of one without a row no scale was loaded)
               ks *= sh.scales[st][i];
               vs = sh.scales[st][2 + i];
             }
