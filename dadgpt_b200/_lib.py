@@ -10,6 +10,7 @@ NATIVE_PATH = os.path.join(PKG, "_native.so")
 SHIM_PATH = os.path.join(PKG, "libdadattn_gpuops.so")
 
 P, I, F, U64, I64, SZ = C.c_void_p, C.c_int, C.c_float, C.c_uint64, C.c_int64, C.c_size_t
+F64 = C.c_double
 
 # name -> (restype, argtypes); mirrors include/dadattn.h one to one.
 SIGNATURES = {
@@ -56,6 +57,12 @@ SIGNATURES = {
     "dadattn_fp8_scale_blocks": (I, [I]),
     "dadattn_kv_cache_fill_fp8": (I, [P] * 10 + [I] * 6 + [P]),
     "dadattn_decode_fp8": (I, [P] * 11 + [I, I, I, I, F, I, I, P, SZ, P]),
+    "dadattn_rotary_frequencies": (I, [P, I, F64, I, F64, F64, F64, F64]),
+    "dadattn_rotary": (I, [P] * 9 + [I64] + [I] * 5 + [P, F, I, I, I, I, P]),
+    "dadattn_paged_append_bf16": (I, [P] * 13 + [I] * 8 + [P, F, I, I, I, P]),
+    "dadattn_paged_attention_bf16": (I, [P] * 10 + [I] * 9 + [F, P]),
+    "dadattn_decode_paged_bf16": (I, [P] * 13 + [I] * 7 + [F, P, F, I, I, P]),
+    "dadattn_paged_advance": (I, [P, P, I, I, I, I, P]),
     "dadattn_device_status": (I, [P]),
 }
 

@@ -7,6 +7,8 @@ raise (the reference throws std::runtime_error / std::out_of_range).
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _lib
@@ -239,6 +241,111 @@ def decode_attention_fp8(out, q, k_new, v_new, cache: KVCacheFP8, scale, *, wind
     _native().decode_fp8(cache.B, cache.H, cache.D, cache.max_len, scale, window, sinks, out, q, k_new, v_new, cache.k,
                          cache.v, cache.k_scale, cache.v_scale, cache.k_tail, cache.v_tail, cache.lengths,
                          cache.workspace)
+
+
+class RotaryPositions:
+    """How heads are turned by their positions: the first ``rot_dim`` elements of each, in pairs (i, i + rot_dim / 2) or,
+    ``interleaved``, (2 i, 2 i + 1), pair i by ``position * freq[i]`` radians. ``scaling`` for contexts ``stretch`` times as
+    long as those trained on: None, "linear", "base" or "parts" (by turns over ``trained_len``, from ``low`` to ``high``);
+    include/dadattn.h has the formulas. ``factor`` multiplies the turned elements; None: 0.1 ln(stretch) + 1 with "parts",
+    else 1."""
+
+    SCALINGS = {None: 0, "linear": 1, "base": 2, "parts": 3}   # DADATTN_ROTARY_*
+
+    def __init__(self, rot_dim, *, base=10000.0, interleaved=False, scaling=None, stretch=1.0, trained_len=0, low=1.0,
+                 high=32.0, factor=None, device="cuda"):
+        if scaling not in self.SCALINGS:
+            raise ValueError(f"unknown scaling {scaling!r}")
+        host = torch.empty(max(rot_dim, 0) // 2, dtype=torch.float64)
+        _lib.check(_lib.load().dadattn_rotary_frequencies(host.data_ptr() or 8, rot_dim, base, self.SCALINGS[scaling], stretch,
+                                                          trained_len, low, high))
+        self.rot_dim, self.interleaved = rot_dim, bool(interleaved)
+        if factor is None:
+            factor = 0.1 * math.log(stretch) + 1.0 if scaling == "parts" else 1.0
+        self.factor = float(factor)
+        self.freq = host.to(device)
+
+
+def _turn(backward, q_out, k_out, q, k, rotary, positions, first):
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
+        raise ValueError("q and k must be [B, S, heads, D]")
+    B, S, H, D = q.shape
+    _native().rotary(backward, B, S, H, 0 if k is None else k.shape[2], D, first, rotary.freq, rotary.factor, rotary.rot_dim,
+                     rotary.interleaved, q_out, k_out, q, k, positions)
+
+
+def rotary_forward(q_out, k_out, q, k, rotary: RotaryPositions, *, positions=None, first=0):
+    """Queries [B,S,H,D] and keys [B,S,Hk,D] (fp32 or bf16) turned by their positions: ``positions`` [B,S] int32 on the device,
+    or first + s. Any order in memory with neighbouring elements in a row: heads-split tensors are passed as
+    ``x.view(B, H, S, D).transpose(1, 2)``, activations [B*S, H*D] as ``x.view(B, S, H, D)``. The results may be the tensors
+    themselves; k and k_out may be None."""
+    _turn(0, q_out, k_out, q, k, rotary, positions, first)
+
+
+def rotary_backward(dq, dk, dq_turned, dk_turned, rotary: RotaryPositions, *, positions=None, first=0):
+    """Backward of the call above: gradients of the turned tensors to those of the tensors."""
+    _turn(1, dq, dk, dq_turned, dk_turned, rotary, positions, first)
+
+
+class KVCachePagedBF16:
+    """A cache of one layer in pages: k, v [pages,H,page_size,D] bf16. Row j of sequence b is row j % page_size of page
+    ``page_table[b, j // page_size]`` (int32 [B,max_pages], filled by the caller); ``lengths`` [B] int32 rows are there ahead
+    of a call. Layers of a model share table and lengths: pass those of the first. H: key heads."""
+
+    def __init__(self, B, H, pages, page_size, max_pages, D, device="cuda", page_table=None, lengths=None):
+        self.B, self.H, self.pages, self.page_size, self.max_pages, self.D = B, H, pages, page_size, max_pages, D
+        self.k = torch.zeros(pages, H, page_size, D, dtype=torch.bfloat16, device=device)
+        self.v = torch.zeros_like(self.k)
+        self.page_table = torch.zeros(B, max_pages, dtype=torch.int32, device=device) if page_table is None else page_table
+        self.lengths = torch.zeros(B, dtype=torch.int32, device=device) if lengths is None else lengths
+
+    def _args(self):
+        return (self.B, self.H, self.D, self.pages, self.page_size, self.max_pages, self.k, self.v, self.page_table,
+                self.lengths)
+
+
+def _rotary_args(rotary):
+    return (None, 1.0, 0, 0) if rotary is None else (rotary.freq, rotary.factor, rotary.rot_dim, rotary.interleaved)
+
+
+def _packed(name, x):
+    if x.dim() != 3:
+        raise ValueError(f"{name} must be [tokens, heads, D], got {tuple(x.shape)}")
+    return x.shape
+
+
+def kv_cache_append_paged(cache: KVCachePagedBF16, k_new, v_new, starts=None, *, q=None, q_out=None, rotary=None):
+    """The new rows of a packed batch, k_new and v_new [T,H,D] bf16 or fp32, to their pages: sequence b's are rows
+    starts[b] .. starts[b+1]-1 (int32 [B+1]; None: one for each sequence) and become its rows lengths[b] and on, which stay the
+    lengths until :func:`kv_cache_advance_paged`. With ``rotary``, keys are turned by their rows, and so are queries q
+    [T,Hq,D], into q_out (bf16)."""
+    T = _packed("k_new", k_new)[0]
+    Hq = 0 if q is None else _packed("q", q)[1]
+    _native().append_paged(*cache._args(), *_rotary_args(rotary), T, Hq, starts, q_out, q, k_new, v_new)
+
+
+def paged_attention_bf16(out, q, cache: KVCachePagedBF16, starts, max_new, scale, *, lse=None):
+    """Causal attention of a packed batch's new tokens, q [T,Hq,D] bf16, over all rows of their sequences, whose pages hold
+    theirs already (:func:`kv_cache_append_paged`): token i of sequence b sees rows j <= lengths[b] + i. ``max_new``: no sequence
+    brings more tokens. Hq a multiple of the cache's heads. out [T,Hq,D]; lse [T,Hq] fp32 where it is wanted."""
+    T, Hq, _ = _packed("q", q)
+    _native().paged_attention(*cache._args(), T, max_new, Hq, scale, starts, out, lse, q)
+
+
+def decode_attention_paged_bf16(out, q, k_new, v_new, cache: KVCachePagedBF16, scale, *, rotary=None, lse=None):
+    """One decode step for every sequence of a paged cache: the token is turned by its row (with ``rotary``), appended and
+    attended for, q, out [B,Hq,D], k_new, v_new [B,H,D] bf16. The lengths stay what they are until
+    :func:`kv_cache_advance_paged`: layers share them."""
+    _native().decode_paged(*cache._args(), *_rotary_args(rotary), _packed("q", q)[1], scale, out, lse, q, k_new, v_new)
+
+
+def kv_cache_advance_paged(cache: KVCachePagedBF16, starts=None, tokens=None):
+    """The end of a step, behind its last layer: every sequence becomes longer by its new tokens (``starts`` and ``tokens``, the
+    packed batch's rows, as for the step; None: one for each)."""
+    T = cache.B if starts is None else tokens
+    if T is None:
+        raise ValueError("tokens, the rows of the packed batch, goes with starts")
+    _native().advance_paged(cache.B, T, cache.page_size, cache.max_pages, cache.lengths, starts)
 
 
 def set_decode_early_start(on: bool) -> None:

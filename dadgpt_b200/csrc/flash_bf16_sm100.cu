@@ -99,6 +99,22 @@ int make_tensor_map_bf16_units(CUtensorMap* map, const void* base, int units, in
                                const UnitLayout& lay) {
   return encode_units(map, base, false, units, S, D, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B, lay);
 }
+int make_tensor_map_bf16_tokens(CUtensorMap* map, const void* base, int T, int heads, int D, int64_t token_stride,
+                                int64_t head_stride, int box_heads, int box_tokens) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return fail(DADATTN_E_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(T)};
+  // a dimension of extent 1 still needs a legal stride (a multiple of 16 bytes)
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(heads > 1 ? head_stride : D) * 2,
+                                 static_cast<cuuint64_t>(T > 1 ? token_stride : D) * 2};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens)};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(DADATTN_E_CUDA, "cuTensorMapEncodeTiled (tokens) failed (%d)", (int)r);
+  return DADATTN_OK;
+}
 int make_tensor_map_rows64(CUtensorMap* map, const void* base, bool f32, int units, int S, int D, int box_rows,
                            const UnitLayout& lay) {
   return encode_units(map, base, f32, units, S, D, f32 ? 16 : 32, box_rows, CU_TENSOR_MAP_SWIZZLE_64B, lay);

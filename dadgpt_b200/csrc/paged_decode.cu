@@ -1,0 +1,547 @@
+// One decode step over a paged KV cache: the token of every sequence is turned by its position, appended to its page and
+// attended for, in one launch.
+//
+//   out_r = sum_j p_rj v_j,  p_rj = exp(scale q_r.k_j - m_r) / l_r   over rows j = 0 .. lengths[b]
+//
+// for the `group` query heads r that share a key head: they are the rows of one 16-row operand of the warp-wide matrix
+// instruction (m16n8k16, bf16 in, fp32 sums), so that K and V are read once for all of them. Bound by HBM: 4 D bytes a cached
+// row and key head, 2 to 16 FLOPs a byte; what counts is that enough of them are on their way. tcgen05 would need its scores
+// back from tensor memory with one row a lane, and 128 of them for each product, where there are 1 to 16.
+//   * a CTA (a cluster, where few items share the GPU) per sequence, key head and 16 query heads. Of a cluster each CTA takes
+//     a run of the 64-row tiles, and they join their maxima, sums and accumulators through distributed shared memory: no
+//     workspace, and nothing that two calls could share.
+//   * one producer warp: lane i fetches the i-th box of a tile (TMA, 128-byte swizzle, boxes as high as a page, up to the
+//     tile; 16 rows in a sequence's last tile, of which only those with a row are fetched), and looks its page up a tile ahead.
+//   * four consumer warps, 16 rows of a tile each, with a running maximum and sum of their own: scores and probabilities stay
+//     in registers, whose layout as a result is the one of the next product's operand. Accumulators are rescaled only when
+//     the maximum has grown by 2^8.
+//   * the new token needs no row of the cache: its scores, with k as rounded for the cache, are where one warp's running
+//     maximum begins, and v its accumulator.
+// Rows behind the last one are not trusted: their scores are masked and their V set to zero in shared memory.
+// Every wait is bounded (sm100_ptx.cuh).
+#include <cuda_bf16.h>
+
+#include "decode_common.cuh"
+#include "paged.cuh"
+#include "rotary.cuh"
+
+namespace dadattn {
+namespace {
+
+using namespace ptx;
+using bf16 = __nv_bfloat16;
+
+constexpr int kWarps = 4;                     // consumer warps
+constexpr int kThreads = (kWarps + 1) * 32;   // and one producer warp
+constexpr int kTile = 64;                     // cache rows of a stage
+constexpr int kWarpRows = kTile / kWarps;     // 16
+constexpr int kRows = 16;                     // query rows of an item
+constexpr int kMaxCluster = 16;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kRescaleAt = 8.0f;
+
+template <int D>
+struct Plan {
+  static constexpr int kStages = 3;
+  static constexpr int kPerSm = D == 64 ? 4 : 2;
+  static constexpr int kPanels = D / 64;
+  static constexpr int kPanelBytes = kTile * 128;            // [64 rows][64 bf16], swizzled
+  static constexpr int kSide = kPanels * kPanelBytes;        // K or V of a tile
+  static constexpr int kStageBytes = 2 * kSide;
+  // Behind the ring, or in its place once it has been read: accumulators of the warps and the CTA's.
+  static constexpr int kPitch = D + 4;                       // floats of a row (banks)
+  static constexpr int kWarpAcc = kRows * kPitch;
+  static constexpr int kBytes = kStages * kStageBytes;
+  static_assert((kWarps + 1) * kWarpAcc * 4 <= kBytes, "accumulators in the ring's place");
+};
+
+template <int D>
+struct DecodeShared {
+  uint64_t full[Plan<D>::kStages], empty[Plan<D>::kStages];
+  int abort_flag, bad;
+  float m[kWarps][kRows], l[kWarps][kRows];
+  float m_all[kRows], l_all[kRows];           // of the CTA, read by the cluster's others
+  __align__(16) float2 table[kMaxRotaryHead / 4];   // (cos, sin): D / 2 at most
+  __align__(16) bf16 q[kRows][D + 8];
+  __align__(16) bf16 k_new[D], v_new[D];
+};
+
+struct DecodeParams {
+  bf16* out;
+  float* lse;
+  const bf16 *q, *k_new, *v_new;
+  bf16 *k_pages, *v_pages;
+  int64_t out_token, out_head, q_token, q_head, k_token, k_head, v_token, v_head;
+  PagedCache cache;
+  int heads_q, group, parts;   // query heads of a key head, in `parts` items of up to 16
+  int chunk;                   // rows of a box: those of a page, up to a tile
+  float scale;
+  RotaryParams r;
+  int* status;
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// c (16 x 8) += a (16 x 16) b (16 x 8)
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ int ld_cluster_int(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int D, int CLUSTER>
+__global__ void __launch_bounds__(kThreads, Plan<D>::kPerSm)
+paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                    const __grid_constant__ CUtensorMap map_k16, const __grid_constant__ CUtensorMap map_v16,
+                    const DecodeParams p) {
+  using L = Plan<D>;
+  constexpr int kStages = L::kStages, kSteps = D / 16;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ DecodeShared<D> sh;
+  volatile int* abort_flag = &sh.abort_flag;
+  const PagedCache& c = p.cache;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = CLUSTER > 1 ? blockIdx.x % CLUSTER : 0;
+  const int item = blockIdx.x / CLUSTER;
+  const int per_seq = c.heads * p.parts;
+  const int b = item / per_seq, kv_head = (item - b * per_seq) / p.parts, part = item % p.parts;
+  const int head0 = kv_head * p.group + part * kRows, rows = min(p.group - part * kRows, kRows);
+
+  if ((smem_u32(smem) & 1023u) != 0) {
+    if (threadIdx.x == 0) atomicExch(p.status, DADATTN_E_CUDA);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&sh.full[s], 1);
+      mbar_init(&sh.empty[s], kWarps);
+    }
+    sh.abort_flag = 0;
+    sh.bad = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  pdl_wait();
+  pdl_launch_dependents();
+
+  const int ahead = c.lengths[b];
+  // (the same for every CTA of a cluster: nobody waits for one that has left)
+  if (ahead < 0 || ahead >= c.max_pages << c.page_shift) {
+    if (threadIdx.x == 0) atomicExch(p.status, DADATTN_E_ARG);
+    return;
+  }
+  const int n_tiles = (ahead + kTile - 1) / kTile;
+  const int first_tile = static_cast<int>(static_cast<int64_t>(n_tiles) * rank / CLUSTER);
+  const int end_tile = static_cast<int>(static_cast<int64_t>(n_tiles) * (rank + 1) / CLUSTER);
+  const int n = end_tile - first_tile;
+  const bool last_rank = rank == CLUSTER - 1;   // has the new token
+
+  float o[kSteps * 2][4];          // O: 8 columns each, rows lane / 4 and + 8
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  if (warp == kWarps) {
+    // ------------------------------ producer ------------------------------
+    const int32_t* table = c.table + static_cast<int64_t>(b) * c.max_pages;
+    int issued = 0;
+    auto plan = [&](int tile, int& box_rows, int& boxes) {   // boxes of one side and panel
+      const int there = min(ahead - tile * kTile, kTile);
+      box_rows = there < kTile ? 16 : p.chunk;
+      boxes = (there + box_rows - 1) / box_rows;
+    };
+    // the page of this lane's box of a tile
+    auto look_up = [&](int tile) -> int {
+      int box_rows, boxes;
+      plan(tile, box_rows, boxes);
+      const int i = lane % boxes;
+      return lane < boxes * L::kPanels * 2 ? table[(tile * kTile + i * box_rows) >> c.page_shift] : 0;
+    };
+    int page = n > 0 ? look_up(first_tile) : 0;
+    for (int j = 0; j < n; ++j) {
+      const int s = j % kStages, tile = first_tile + j;
+      int box_rows, boxes;
+      plan(tile, box_rows, boxes);
+      const int count = boxes * L::kPanels * 2, mine = page;
+      if (j + 1 < n) page = look_up(tile + 1);
+      if (j >= kStages && !warp_wait(&sh.empty[s], (j / kStages - 1) & 1, abort_flag)) break;
+      if (lane == 0) mbar_arrive_expect_tx(&sh.full[s], count * box_rows * 128);
+      __syncwarp();
+      if (lane < count) {
+        const int i = lane % boxes, panel = lane / boxes % L::kPanels, side = lane / (boxes * L::kPanels);
+        const int row = tile * kTile + i * box_rows;
+        const bool good = mine >= 0 && mine < c.pages;
+        if (!good) sh.bad = 1;
+        // (a row coordinate outside the pool reads zeros)
+        const int y = good ? ((mine * c.heads + kv_head) << c.page_shift) + (row & ((1 << c.page_shift) - 1)) : -kMaxPage;
+        const CUtensorMap* map = side ? (box_rows == 16 ? &map_v16 : &map_v) : (box_rows == 16 ? &map_k16 : &map_k);
+        tma_load_3d(smem + s * L::kStageBytes + side * L::kSide + panel * L::kPanelBytes + i * box_rows * 128, map, &sh.full[s],
+                    panel * 64, y, 0);
+      }
+      __syncwarp();
+      ++issued;
+    }
+    if (lane == 0) settle_ring(sh.full, kStages, issued);
+  } else {
+    // ------------------------------ set-up of the consumers ------------------------------
+    const int t = threadIdx.x;
+    constexpr int kConsumers = kWarps * 32, kUnits = D / kTurnUnit;
+    const int half = p.r.rot / 2;
+    // pieces of 16 elements: of the query rows, then of k and v
+    const int pieces = (kRows + 2) * kUnits;
+    for (int e = t; e < half; e += kConsumers) sh.table[cos_sin_place(e)] = cos_sin<false>(ahead, turns_of(p.r.freq[e]), p.r.factor);
+    // (not the producer, who is at work)
+    auto consumers_meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers) : "memory"); };
+    consumers_meet();
+    const int new_page = last_rank ? c.table[static_cast<int64_t>(b) * c.max_pages + (ahead >> c.page_shift)] : 0;
+    const bool can_append = new_page >= 0 && new_page < c.pages;
+    if (!can_append) sh.bad = 1;
+    const int64_t new_row = (((static_cast<int64_t>(new_page) * c.heads + kv_head) << c.page_shift) +
+                             (ahead & ((1 << c.page_shift) - 1))) * D;
+    for (int i = t; i < pieces; i += kConsumers) {
+      const int row = i / kUnits, u = i % kUnits;
+      const bool is_v = row == kRows + 1;
+      const int first = is_v ? u * kTurnUnit : unit_first(u, p.r), second = is_v ? 8 : unit_second(u, p.r);
+      if (row >= kRows && !last_rank) continue;
+      Sixteen<bf16> x;
+      if (row < kRows) {
+        if (row < rows) x.load(p.q, b * p.q_token + (head0 + row) * p.q_head + first, second);
+        else x.a = x.b = make_uint4(0, 0, 0, 0);
+      } else if (is_v) {
+        x.load(p.v_new, b * p.v_token + kv_head * p.v_head + first, second);
+      } else {
+        x.load(p.k_new, b * p.k_token + kv_head * p.k_head + first, second);
+      }
+      if (!is_v && u * kTurnUnit < p.r.rot) {
+        float f[16];
+        x.to_floats(f);
+        turn_unit(f, sh.table, u, p.r);
+        x.from_floats(f);
+      }
+      x.store(row < kRows ? sh.q[row] : is_v ? sh.v_new : sh.k_new, first, second);
+      if (row >= kRows && part == 0 && can_append) x.store(is_v ? p.v_pages : p.k_pages, new_row + first, second);
+    }
+    consumers_meet();
+
+    uint32_t qf[kSteps][4];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int col = s * 16 + (lane % 4) * 2;
+      qf[s][0] = *reinterpret_cast<const uint32_t*>(&sh.q[lane / 4][col]);
+      qf[s][1] = *reinterpret_cast<const uint32_t*>(&sh.q[lane / 4 + 8][col]);
+      qf[s][2] = *reinterpret_cast<const uint32_t*>(&sh.q[lane / 4][col + 8]);
+      qf[s][3] = *reinterpret_cast<const uint32_t*>(&sh.q[lane / 4 + 8][col + 8]);
+    }
+    const float scale_log2 = p.scale * kLog2e;
+#pragma unroll
+    for (int i = 0; i < kSteps * 2; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    if (last_rank && warp == 0) {
+      float2 dot[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const int col = s * 16 + (lane % 4) * 2;
+        const uint32_t k0 = *reinterpret_cast<const uint32_t*>(&sh.k_new[col]);
+        const uint32_t k1 = *reinterpret_cast<const uint32_t*>(&sh.k_new[col + 8]);
+        fma_bf16(dot[0], qf[s][0], k0);
+        fma_bf16(dot[0], qf[s][2], k1);
+        fma_bf16(dot[1], qf[s][1], k0);
+        fma_bf16(dot[1], qf[s][3], k1);
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        float d = dot[x].x + dot[x].y;
+        d += __shfl_xor_sync(0xffffffffu, d, 1);
+        d += __shfl_xor_sync(0xffffffffu, d, 2);
+        m[x] = __fmul_rn(d, scale_log2);
+        // (1; NaN where the score is infinite or NaN, 0 for minus infinity. The four lanes' parts are added up.)
+        l[x] = lane % 4 == 0 && m[x] != -INFINITY ? ex2(m[x] - m[x]) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < kSteps * 2; ++i) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(&sh.v_new[i * 8 + (lane % 4) * 2]);
+        const float v0 = __uint_as_float(w << 16), v1 = __uint_as_float(w & 0xffff0000u);
+        o[i][0] = m[0] == -INFINITY ? 0.f : v0, o[i][1] = m[0] == -INFINITY ? 0.f : v1;
+        o[i][2] = m[1] == -INFINITY ? 0.f : v0, o[i][3] = m[1] == -INFINITY ? 0.f : v1;
+      }
+    }
+
+    // ------------------------------ the tiles ------------------------------
+    const uint32_t ring = smem_u32(smem);
+    for (int j = 0; j < n; ++j) {
+      const int s = j % kStages, tile = first_tile + j;
+      const int there = min(ahead - tile * kTile - warp * kWarpRows, kWarpRows);   // rows of this warp's 16
+      if (!warp_wait(&sh.full[s], (j / kStages) & 1, abort_flag)) break;
+      if (there > 0) {
+        const uint32_t k_tile = ring + s * L::kStageBytes + warp * kWarpRows * 128, v_tile = k_tile + L::kSide;
+        float sc[2][4] = {};
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step) {
+          // matrices: keys 0-7 and 8-15, 16-byte chunks 2 step and 2 step + 1
+          uint32_t kf[4];
+          const int key = (lane & 7) + (lane >> 4) * 8, ch = step * 2 + ((lane >> 3) & 1);
+          ldmatrix4(k_tile + (ch / 8) * L::kPanelBytes + key * 128 + (((ch & 7) ^ (key & 7)) << 4), kf);
+          mma_16816(sc[0], qf[step], kf[0], kf[1]);
+          mma_16816(sc[1], qf[step], kf[2], kf[3]);
+        }
+        if (there < kWarpRows) {
+          // Rows that are not there: no score, and a V of zeros (what the page holds there could be anything).
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (h * 8 + (lane % 4) * 2 + (e & 1) >= there) sc[h][e] = -INFINITY;
+          for (int i = lane; i < (kWarpRows - there) * D / 8; i += 32) {
+            const int row = there + i / (D / 8), ch = i % (D / 8);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_tile + (ch / 8) * L::kPanelBytes + row * 128 + ((ch & 7) << 4)),
+                         "r"(0)
+                         : "memory");
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        float mx[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          mx[x] = __fmul_rn(fmaxf(fmaxf(sc[0][2 * x], sc[0][2 * x + 1]), fmaxf(sc[1][2 * x], sc[1][2 * x + 1])), scale_log2);
+        if (__any_sync(0xffffffffu, mx[0] > m[0] + kRescaleAt || mx[1] > m[1] + kRescaleAt || m[0] == -INFINITY || m[1] == -INFINITY)) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
+            mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
+            const float m_new = fmaxf(m[x], mx[x]);
+            const float corr = m[x] == -INFINITY ? 0.f : ex2(m[x] - m_new);
+            m[x] = m_new;
+            l[x] = __fmul_rn(l[x], corr);
+#pragma unroll
+            for (int i = 0; i < kSteps * 2; ++i) o[i][2 * x] *= corr, o[i][2 * x + 1] *= corr;
+          }
+        }
+        uint32_t pf[4];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float neg = m[x] == -INFINITY ? 0.f : -m[x];
+          float e[4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) e[2 * h + k] = ex2(fmaf(sc[h][2 * x + k], scale_log2, neg));
+          l[x] += (e[0] + e[1]) + (e[2] + e[3]);
+          pf[x] = pack_bf16(e[0], e[1]);
+          pf[2 + x] = pack_bf16(e[2], e[3]);
+        }
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          uint32_t vf[4];
+          const int key = lane & 15, ch = i * 2 + (lane >> 4);
+          ldmatrix4_trans(v_tile + (ch / 8) * L::kPanelBytes + key * 128 + (((ch & 7) ^ (key & 7)) << 4), vf);
+          mma_16816(o[2 * i], pf, vf[0], vf[1]);
+          mma_16816(o[2 * i + 1], pf, vf[2], vf[3]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.empty[s]);
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+    }
+  }
+
+  // ------------------------------ the warps', then the CTAs' results together ------------------------------
+  __syncthreads();   // (nobody reads the ring any more; the producer has seen its copies land)
+  float* acc = reinterpret_cast<float*>(smem);               // [warps][rows][kPitch]
+  float* sum = acc + kWarps * L::kWarpAcc;                   // [rows][kPitch]
+  if (warp < kWarps) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int row = lane / 4 + 8 * x;
+      if (row < rows) {
+#pragma unroll
+        for (int i = 0; i < kSteps * 2; ++i)
+          *reinterpret_cast<float2*>(acc + warp * L::kWarpAcc + row * L::kPitch + i * 8 + (lane % 4) * 2) =
+              make_float2(o[i][2 * x], o[i][2 * x + 1]);
+        if (lane % 4 == 0) sh.m[warp][row] = m[x], sh.l[warp][row] = l[x];
+      }
+    }
+  }
+  __syncthreads();
+  auto write_out = [&](int row, int col, float a, float b2, float l_tot) {
+    const float f = 1.0f / l_tot;
+    *reinterpret_cast<uint32_t*>(p.out + b * p.out_token + (head0 + row) * p.out_head + col) = pack_bf16(a * f, b2 * f);
+  };
+  for (int i = threadIdx.x; i < rows * (D / 2); i += kThreads) {
+    const int row = i / (D / 2), col = i % (D / 2) * 2;
+    float m_tot = sh.m[0][row];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) m_tot = fmaxf(m_tot, sh.m[w][row]);
+    float l_tot = 0.f, a = 0.f, b2 = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float mw = sh.m[w][row], f = mw == -INFINITY ? 0.f : ex2(mw - m_tot);
+      const float2 v = *reinterpret_cast<const float2*>(acc + w * L::kWarpAcc + row * L::kPitch + col);
+      l_tot = fmaf(sh.l[w][row], f, l_tot);
+      a = fmaf(v.x, f, a);
+      b2 = fmaf(v.y, f, b2);
+    }
+    if (CLUSTER == 1) {
+      if (!sh.bad && !sh.abort_flag) {
+        write_out(row, col, a, b2, l_tot);
+        if (p.lse && col == 0) p.lse[static_cast<int64_t>(b) * p.heads_q + head0 + row] = (m_tot + log2f(l_tot)) * kLn2;
+      }
+    } else {
+      *reinterpret_cast<float2*>(sum + row * L::kPitch + col) = make_float2(a, b2);
+      if (col == 0) sh.m_all[row] = m_tot, sh.l_all[row] = l_tot;
+    }
+  }
+  if (CLUSTER > 1) {
+    cluster_arrive();
+    cluster_wait();
+    int bad = 0;
+#pragma unroll 1
+    for (int r = 0; r < CLUSTER; ++r)
+      bad |= ld_cluster_int(cluster_address(&sh.bad, r)) | ld_cluster_int(cluster_address(&sh.abort_flag, r));
+    // this CTA's share of the results
+    const int all = rows * (D / 2), share = (all + CLUSTER - 1) / CLUSTER;
+    for (int i = rank * share + threadIdx.x; i < min(all, (rank + 1) * share); i += kThreads) {
+      const int row = i / (D / 2), col = i % (D / 2) * 2;
+      float mr[CLUSTER], m_tot = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < CLUSTER; ++r) mr[r] = ld_cluster(cluster_address(&sh.m_all[row], r));
+#pragma unroll
+      for (int r = 0; r < CLUSTER; ++r) m_tot = fmaxf(m_tot, mr[r]);
+      float l_tot = 0.f, a = 0.f, b2 = 0.f;
+#pragma unroll
+      for (int r = 0; r < CLUSTER; ++r) {
+        const float f = mr[r] == -INFINITY ? 0.f : ex2(mr[r] - m_tot);
+        const uint32_t at = cluster_address(sum + row * L::kPitch + col, r);
+        l_tot = fmaf(ld_cluster(cluster_address(&sh.l_all[row], r)), f, l_tot);
+        a = fmaf(ld_cluster(at), f, a);
+        b2 = fmaf(ld_cluster(at + 4), f, b2);
+      }
+      if (!bad) {
+        write_out(row, col, a, b2, l_tot);
+        if (p.lse && col == 0) p.lse[static_cast<int64_t>(b) * p.heads_q + head0 + row] = (m_tot + log2f(l_tot)) * kLn2;
+      }
+    }
+    cluster_arrive();
+    cluster_wait();   // (the others' shared memory stays until it has been read)
+  }
+  if (threadIdx.x == 0) {
+    if (sh.abort_flag) report_timeout(p.status, sh.abort_flag);
+    else if (sh.bad) atomicExch(p.status, DADATTN_E_ARG);
+  }
+}
+
+struct Maps {
+  CUtensorMap k, v, k16, v16;
+};
+
+template <int D, int CLUSTER>
+int launch_decode(const Maps& maps, const DecodeParams& p, int items, cudaStream_t st) {
+  using L = Plan<D>;
+  auto kern = paged_decode_kernel<D, CLUSTER>;
+  DAD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
+  if (CLUSTER > 8) DAD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(items) * CLUSTER);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = L::kBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CLUSTER;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CLUSTER > 1 ? 2 : 1;
+  DAD_CUDA(cudaLaunchKernelEx(&cfg, kern, maps.k, maps.v, maps.k16, maps.v16, p));
+  return DADATTN_OK;
+}
+
+// CTAs of a cluster: so many that they fill the GPU, and no more than there may be tiles for.
+int cluster_for(long long items, long long most_rows, int per_sm) {
+  const long long slots = static_cast<long long>(current_sm_count()) * per_sm;
+  int c = 1;
+  while (c < kMaxCluster && items * c * 2 <= slots && static_cast<long long>(c) * 2 * kTile <= most_rows) c *= 2;
+  return c;
+}
+
+template <int D>
+int launch_decode_d(const Maps& maps, const DecodeParams& p, int items, long long most_rows, cudaStream_t st) {
+  switch (cluster_for(items, most_rows, Plan<D>::kPerSm)) {
+    case 1: return launch_decode<D, 1>(maps, p, items, st);
+    case 2: return launch_decode<D, 2>(maps, p, items, st);
+    case 4: return launch_decode<D, 4>(maps, p, items, st);
+    case 8: return launch_decode<D, 8>(maps, p, items, st);
+    default: return launch_decode<D, 16>(maps, p, items, st);
+  }
+}
+
+}  // namespace
+}  // namespace dadattn
+
+using namespace dadattn;
+
+extern "C" int dadattn_decode_paged_bf16(uint16_t* out, float* lse, const uint16_t* q, const uint16_t* k_new,
+                                         const uint16_t* v_new, const int64_t* out_strides, const int64_t* q_strides,
+                                         const int64_t* k_strides, const int64_t* v_strides, uint16_t* k_pages,
+                                         uint16_t* v_pages, const int32_t* page_table, const int32_t* lengths, int B, int Hq,
+                                         int Hkv, int D, int pages, int page_size, int max_pages, float scale,
+                                         const double* freq, float factor, int rot_dim, int interleaved,
+                                         dadattn_stream_t stream) {
+  const char* name = "paged decode";
+  if (int rc = check_paged(name, k_pages, v_pages, page_table, lengths, nullptr, B, Hkv, D, pages, page_size, max_pages)) return rc;
+  if (Hq <= 0 || Hq % Hkv) return fail(DADATTN_E_ARG, "%s: Hq=%d must be a multiple of Hkv=%d", name, Hq, Hkv);
+  if (!(scale > 0.0f && scale < INFINITY)) return fail(DADATTN_E_ARG, "%s: scale must be positive and finite", name);
+  if (int rc = check_rotary(name, freq, factor, rot_dim, D)) return rc;
+  if (int rc = check_packed(name, out, out_strides, 8, true, B, Hq)) return rc;
+  if (int rc = check_packed(name, q, q_strides, 8, false, B, Hq)) return rc;
+  if (int rc = check_packed(name, k_new, k_strides, 8, false, B, Hkv)) return rc;
+  if (int rc = check_packed(name, v_new, v_strides, 8, false, B, Hkv)) return rc;
+  if (!aligned(lse, 4)) return fail(DADATTN_E_ARG, "%s: lse must be 4-byte aligned", name);
+  const int group = Hq / Hkv, parts = (group + kRows - 1) / kRows;
+  const long long items = static_cast<long long>(B) * Hkv * parts;
+  if (items * kMaxCluster > 0x7fffffffll) return fail(DADATTN_E_UNSUPPORTED, "%s: B=%d and Hkv=%d are too many", name, B, Hkv);
+  DecodeParams p = {};
+  p.out = reinterpret_cast<bf16*>(out), p.lse = lse;
+  p.q = reinterpret_cast<const bf16*>(q), p.k_new = reinterpret_cast<const bf16*>(k_new), p.v_new = reinterpret_cast<const bf16*>(v_new);
+  p.k_pages = reinterpret_cast<bf16*>(k_pages), p.v_pages = reinterpret_cast<bf16*>(v_pages);
+  p.out_token = out_strides[0], p.out_head = out_strides[1], p.q_token = q_strides[0], p.q_head = q_strides[1];
+  p.k_token = k_strides[0], p.k_head = k_strides[1], p.v_token = v_strides[0], p.v_head = v_strides[1];
+  p.cache = PagedCache{page_table, lengths, nullptr, B, pages, log2_of(page_size), max_pages, Hkv};
+  p.heads_q = Hq, p.group = group, p.parts = parts, p.chunk = page_size < kTile ? page_size : kTile;
+  p.scale = scale;
+  p.r = RotaryParams{freq, factor, rot_dim, interleaved != 0, 0};
+  p.status = device_status_word();
+  if (!p.status) return DADATTN_E_CUDA;
+  const int rows = pages * Hkv * page_size;
+  Maps maps;
+  if (int rc = make_tensor_map_bf16(&maps.k, k_pages, 1, rows, D, p.chunk)) return rc;
+  if (int rc = make_tensor_map_bf16(&maps.v, v_pages, 1, rows, D, p.chunk)) return rc;
+  if (int rc = make_tensor_map_bf16(&maps.k16, k_pages, 1, rows, D, 16)) return rc;
+  if (int rc = make_tensor_map_bf16(&maps.v16, v_pages, 1, rows, D, 16)) return rc;
+  const long long most_rows = static_cast<long long>(max_pages) * page_size;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return D == 64 ? launch_decode_d<64>(maps, p, static_cast<int>(items), most_rows, st)
+                 : launch_decode_d<128>(maps, p, static_cast<int>(items), most_rows, st);
+}

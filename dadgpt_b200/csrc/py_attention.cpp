@@ -31,6 +31,7 @@ const char* type_name(at::ScalarType t) {
     case at::kBFloat16: return "torch.bfloat16";
     case at::kByte: return "torch.uint8";
     case at::kInt: return "torch.int32";
+    case at::kDouble: return "torch.float64";
     case at::kFloat8_e4m3fn: return "torch.float8_e4m3fn";
     default: return c10::toString(t);
   }
@@ -69,6 +70,9 @@ class Args {
     }
     return t;
   }
+  // a CUDA tensor of the given type and shape on the current device, its elements next to each other, its other strides into
+  // `strides` (those of dimensions of extent 1 as 0 where they do not matter)
+  const at::Tensor& strided(const char* name, at::ScalarType type, std::initializer_list<int64_t> shape, int64_t* strides);
   // the same, on the current device and of the given shape
   const at::Tensor& here(const char* name, at::ScalarType type, std::initializer_list<int64_t> shape);
   const at::Tensor& workspace() {
@@ -142,6 +146,24 @@ const at::Tensor& Args::here(const char* name, at::ScalarType type, std::initial
   const at::Tensor& t = need(name, type);
   need_current(name, t);
   need_shape(name, t, shape);
+  return t;
+}
+
+const at::Tensor& Args::strided(const char* name, at::ScalarType type, std::initializer_list<int64_t> shape, int64_t* strides) {
+  const at::Tensor& t = tensor(name);
+  if (!t.is_cuda()) {
+    PyErr_Format(PyExc_ValueError, "%s must be a CUDA tensor (there is no CPU path)", name);
+    throw Bad{};
+  }
+  need_current(name, t);
+  need_shape(name, t, shape);
+  const int64_t last = t.dim() - 1;
+  if (t.scalar_type() != type || (t.size(last) > 1 && t.stride(last) != 1)) {
+    PyErr_Format(PyExc_ValueError, "%s must be %s with rows of neighbouring elements, got %s, last stride %lld", name,
+                 type_name(type), type_name(t.scalar_type()), static_cast<long long>(t.stride(last)));
+    throw Bad{};
+  }
+  for (int64_t i = 0; i < last; ++i) strides[i] = t.size(i) > 1 ? t.stride(i) : 0;
   return t;
 }
 
@@ -571,6 +593,142 @@ PyObject* evict_bf16(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// freq, factor, rot_dim, interleaved of a RotaryPositions; freq None: no rotation
+struct Rotary {
+  const double* freq = nullptr;
+  float factor = 1.f;
+  int rot = 0, interleaved = 0;
+  explicit Rotary(Args& p) {
+    if (!p.none()) {
+      const at::Tensor& f = p.need("freq", at::kDouble);
+      Args::need_current("freq", f);
+      freq = static_cast<const double*>(f.data_ptr());
+      n = f.numel();
+    }
+    factor = p.real();
+    rot = p.integer();
+    interleaved = p.integer();
+    if (freq && n != rot / 2) {
+      PyErr_Format(PyExc_ValueError, "freq has %lld elements, expected %d", static_cast<long long>(n), rot / 2);
+      throw Bad{};
+    }
+  }
+  int64_t n = 0;
+};
+const int32_t* ints(const at::Tensor& t) { return static_cast<const int32_t*>(t.data_ptr()); }
+
+// backward, B, S, Hq, Hk, D, first, freq, factor, rot_dim, interleaved, q_out, k_out or None, q, k or None, positions or None
+PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args p(a, n, 16, "rotary");
+    const int back = p.integer(), B = p.integer(), S = p.integer(), Hq = p.integer(), Hk = p.integer(), D = p.integer();
+    const int64_t first = p.integer64();
+    const Rotary r(p);
+    const at::ScalarType type = p.peek_type("q_out") == kB ? kB : kF;
+    int64_t s[4][3] = {};   // q_out, k_out, q, k
+    void *qo = ptr(p.strided("q_out", type, {B, S, Hq, D}, s[0])), *ko = nullptr;
+    if (!p.none()) ko = ptr(p.strided("k_out", type, {B, S, Hk, D}, s[1]));
+    const void *q = ptr(p.strided("q", type, {B, S, Hq, D}, s[2])), *k = nullptr;
+    if (!p.none()) k = ptr(p.strided("k", type, {B, S, Hk, D}, s[3]));
+    const int32_t* const positions = p.none() ? nullptr : ints(p.here("positions", at::kInt, {B, S}));
+    const dadattn_stream_t st = stream();
+    return done(without_gil([&] {
+      return dadattn_rotary(qo, ko, q, k, s[0], s[1], s[2], s[3], positions, first, B, S, Hq, Hk, D, r.freq, r.factor, r.rot,
+                            r.interleaved, back, type == kB, st);
+    }));
+  });
+}
+
+// The paged cache's arguments: B, Hkv, D, pages, page_size, max_pages, k_pages, v_pages, page_table, lengths
+struct Paged {
+  int B, H, D, pages, page_size, max_pages;
+  uint16_t *k, *v;
+  const int32_t *table, *lengths;
+  explicit Paged(Args& p)
+      : B(p.integer()), H(p.integer()), D(p.integer()), pages(p.integer()), page_size(p.integer()), max_pages(p.integer()),
+        k(b16(p.here("k_pages", kB, {pages, H, page_size, D}))), v(b16(p.here("v_pages", kB, {pages, H, page_size, D}))),
+        table(ints(p.here("page_table", at::kInt, {B, max_pages}))), lengths(ints(p.here("lengths", at::kInt, {B}))) {}
+};
+
+// paged cache, rotary, T, Hq, starts or None, q_out or None, q or None, k_new, v_new
+PyObject* append_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args p(a, n, 21, "append_paged");
+    const Paged c(p);
+    const Rotary r(p);
+    const int T = p.integer(), Hq = p.integer();
+    const int32_t* const starts = p.none() ? nullptr : ints(p.here("starts", at::kInt, {int64_t(c.B) + 1}));
+    int64_t s[4][2] = {};
+    uint16_t* const qo = p.none() ? nullptr : b16(p.strided("q_out", kB, {T, Hq, c.D}, s[0]));
+    at::ScalarType type = kF;
+    const void* q = nullptr;
+    if (!p.none()) {
+      type = p.peek_type("q") == kB ? kB : kF;
+      q = ptr(p.strided("q", type, {T, Hq, c.D}, s[1]));
+    }
+    if (!q) type = p.peek_type("k_new") == kB ? kB : kF;
+    const void *kn = ptr(p.strided("k_new", type, {T, c.H, c.D}, s[2])), *vn = ptr(p.strided("v_new", type, {T, c.H, c.D}, s[3]));
+    const dadattn_stream_t st = stream();
+    return done(without_gil([&] {
+      return dadattn_paged_append_bf16(c.k, c.v, c.table, c.lengths, starts, qo, q, kn, vn, s[0], s[1], s[2], s[3], c.B, T, Hq, c.H,
+                                       c.D, c.pages, c.page_size, c.max_pages, r.freq, r.factor, r.rot, r.interleaved, type == kB, st);
+    }));
+  });
+}
+
+// paged cache, T, max_new, Hq, scale, starts or None, out, lse or None, q
+PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args p(a, n, 18, "paged_attention");
+    const Paged c(p);
+    const int T = p.integer(), max_new = p.integer(), Hq = p.integer();
+    const float scale = p.real();
+    const int32_t* const starts = p.none() ? nullptr : ints(p.here("starts", at::kInt, {int64_t(c.B) + 1}));
+    int64_t s[2][2] = {};
+    uint16_t* const out = b16(p.strided("out", kB, {T, Hq, c.D}, s[0]));
+    float* const lse = p.none() ? nullptr : f32(p.here("lse", kF, {T, Hq}));
+    const uint16_t* const q = b16(p.strided("q", kB, {T, Hq, c.D}, s[1]));
+    const dadattn_stream_t st = stream();
+    return done(without_gil([&] {
+      return dadattn_paged_attention_bf16(out, lse, q, s[0], s[1], c.k, c.v, c.table, c.lengths, starts, c.B, T, max_new, Hq, c.H,
+                                          c.D, c.pages, c.page_size, c.max_pages, scale, st);
+    }));
+  });
+}
+
+// paged cache, rotary, Hq, scale, out, lse or None, q, k_new, v_new
+PyObject* decode_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args p(a, n, 21, "decode_paged");
+    const Paged c(p);
+    const Rotary r(p);
+    const int Hq = p.integer();
+    const float scale = p.real();
+    int64_t s[4][2] = {};
+    uint16_t* const out = b16(p.strided("out", kB, {c.B, Hq, c.D}, s[0]));
+    float* const lse = p.none() ? nullptr : f32(p.here("lse", kF, {c.B, Hq}));
+    const uint16_t *q = b16(p.strided("q", kB, {c.B, Hq, c.D}, s[1])), *kn = b16(p.strided("k_new", kB, {c.B, c.H, c.D}, s[2])),
+                   *vn = b16(p.strided("v_new", kB, {c.B, c.H, c.D}, s[3]));
+    const dadattn_stream_t st = stream();
+    return done(without_gil([&] {
+      return dadattn_decode_paged_bf16(out, lse, q, kn, vn, s[0], s[1], s[2], s[3], c.k, c.v, c.table, c.lengths, c.B, Hq, c.H, c.D,
+                                       c.pages, c.page_size, c.max_pages, scale, r.freq, r.factor, r.rot, r.interleaved, st);
+    }));
+  });
+}
+
+// B, T, page_size, max_pages, lengths, starts or None
+PyObject* advance_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args p(a, n, 6, "advance_paged");
+    const int B = p.integer(), T = p.integer(), page_size = p.integer(), max_pages = p.integer();
+    int32_t* const lengths = static_cast<int32_t*>(ptr(p.here("lengths", at::kInt, {B})));
+    const int32_t* const starts = p.none() ? nullptr : ints(p.here("starts", at::kInt, {int64_t(B) + 1}));
+    const dadattn_stream_t st = stream();
+    return done(without_gil([&] { return dadattn_paged_advance(lengths, starts, B, T, page_size, max_pages, st); }));
+  });
+}
+
 PyObject* set_error_class(PyObject*, PyObject* cls) {
   Py_XINCREF(cls);
   Py_XDECREF(g_error_class);
@@ -582,7 +740,8 @@ PyObject* set_error_class(PyObject*, PyObject* cls) {
 PyMethodDef g_methods[] = {FAST(fwd_f32), FAST(bwd_f32), FAST(fwd_bf16), FAST(bwd_bf16), FAST(fwd_bf16_strided),
                            FAST(bwd_bf16_strided), FAST(fwd_bf16_window), FAST(bwd_bf16_window), FAST(fwd_via_bf16), FAST(bwd_via_bf16), FAST(mask_bits),
                            FAST(decode_f32), FAST(decode_bf16), FAST(decode_bf16_window), FAST(decode_fp8), FAST(fill_fp8),
-                           FAST(evict_bf16),
+                           FAST(evict_bf16), FAST(rotary), FAST(append_paged), FAST(paged_attention), FAST(decode_paged),
+                           FAST(advance_paged),
                            {"set_error_class", set_error_class, METH_O, nullptr},
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

@@ -134,14 +134,17 @@ __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 // x = innermost coordinate in elements; x * element size must be a multiple of 16 bytes.
-__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar,
-                                            int x, int y, int z) {
+__device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes "
       "[%0], [%1, {%3, %4, %5}], [%2];"
-      ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x),
+      ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x),
       "r"(y), "r"(z)
       : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+  tma_load_3d(smem_u32(smem_dst), map, bar, x, y, z);
 }
 
 // TMA stores out of shared memory: issued, made a group, waited for. The memory may be written again, and the CTA leave,
@@ -507,7 +510,11 @@ inline UnitLayout unit_layout(int B, int H, int S, int D, bool interleaved) {
 // pass units = B*H: the map is then (D, S, 1, B*H).
 int make_tensor_map_bf16_units(CUtensorMap* map, const void* base, int units, int S, int D, int box_rows,
                                const UnitLayout& lay);
-// The same over a bf16 or fp32 tensor with boxes of 64-byte rows (32 or 16 columns) and 64-byte swizzle.
+// 3-D map (d, head, token) of a packed [T, heads, D] bf16 tensor with strides in elements; box 64 x box_heads x box_tokens,
+// 128-byte swizzle; tokens beyond T read as zero.
+int make_tensor_map_bf16_tokens(CUtensorMap* map, const void* base, int T, int heads, int D, int64_t token_stride,
+                                int64_t head_stride, int box_heads, int box_tokens);
+// make_tensor_map_bf16_units over a bf16 or fp32 tensor with boxes of 64-byte rows (32 or 16 columns) and 64-byte swizzle.
 int make_tensor_map_rows64(CUtensorMap* map, const void* base, bool f32, int units, int S, int D, int box_rows,
                            const UnitLayout& lay);
 

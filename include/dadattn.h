@@ -409,6 +409,101 @@ int dadattn_decode_fp8(uint16_t* out, const uint16_t* q, const uint16_t* k_new, 
                        int32_t* lengths, int B, int H, int D, int max_len, float scale, int window, int sinks,
                        void* workspace, size_t workspace_bytes, dadattn_stream_t stream);
 
+/* ---- rotary positions ------------------------------------------------------------------------------ */
+
+/* Rotary positions (no counterpart in the reference, whose positions are added to the embeddings): of each head of D elements
+ * the first rot_dim are rot_dim / 2 pairs, and pair i of the token at position p is turned by the angle p * freq[i]:
+ *   y1 = factor (x1 cos - x2 sin),  y2 = factor (x2 cos + x1 sin),
+ * (x1, x2) being elements (i, i + rot_dim / 2), or (2 i, 2 i + 1) when `interleaved`. Elements from rot_dim on pass unchanged.
+ * Angles are formed without rounding (a 64-bit fraction of a turn), so that far positions lose nothing.
+ *
+ * Frequencies, radians per position, into a HOST array of rot_dim / 2 (which the caller copies to the device):
+ * w_i = base^(-2 i / rot_dim), and for contexts `stretch` times as long as the model was trained for
+ *   DADATTN_ROTARY_LINEAR  w_i / stretch (positions interpolated)
+ *   DADATTN_ROTARY_BASE    the base times stretch^(rot_dim / (rot_dim - 2)): the slowest pair is slowed by `stretch`, the
+ *                          fastest not at all
+ *   DADATTN_ROTARY_PARTS   with r_i = trained_len w_i / 2 pi turns over the trained length and
+ *                          g = clamp((r_i - low) / (high - low), 0, 1):  g w_i + (1 - g) w_i / stretch
+ * The attention factor that goes with the last (0.1 ln(stretch) + 1, where a model has one) is the calls' `factor`. */
+#define DADATTN_ROTARY_PLAIN 0
+#define DADATTN_ROTARY_LINEAR 1
+#define DADATTN_ROTARY_BASE 2
+#define DADATTN_ROTARY_PARTS 3
+int dadattn_rotary_frequencies(double* freq, int rot_dim, double base, int scaling, double stretch, double trained_len,
+                               double low, double high);
+
+/* Queries and keys of a training step, or of any batch, turned; with `backward` by the negative angle, which takes the
+ * gradients of the turned tensors to those of the tensors. q [B,S,Hq,D], k [B,S,Hk,D] in any order of the dimensions but the
+ * last: element (b, s, h, d) lies at b strides[0] + s strides[1] + h strides[2] + d (host arrays of three, in elements). So
+ * heads split, [B*H, S, D], and as the projections write them, [B*S, H*D], are both taken. bf16 when is_bf16, else fp32; the
+ * arithmetic is fp32. The position of token (b, s) is positions[b S + s] (int32 on the device, may be negative), or first + s
+ * with positions NULL. freq: device array. q_out may be q and k_out k (same strides); results do not overlap anything else.
+ * Hk = 0: no k. D and rot_dim are multiples of 16, D at most 256; every row begins at a multiple of 16 bytes; results'
+ * strides are not zero. (Hq + Hk) D at most 524288. */
+int dadattn_rotary(void* q_out, void* k_out, const void* q, const void* k, const int64_t* q_out_strides,
+                   const int64_t* k_out_strides, const int64_t* q_strides, const int64_t* k_strides, const int32_t* positions,
+                   int64_t first, int B, int S, int Hq, int Hk, int D, const double* freq, float factor, int rot_dim,
+                   int interleaved, int backward, int is_bf16, dadattn_stream_t stream);
+
+/* ---- KV cache in pages ----------------------------------------------------------------------------- */
+
+/* A cache in pages (no counterpart in the reference), which sequences take as they grow and may share where they agree:
+ *   k_pages, v_pages [pages,Hkv,page_size,D] bf16; page_size a power of two from 16 to 1024, D 64 or 128
+ *   page_table [B,max_pages] int32: row j of sequence b is row j % page_size of page page_table[b, j / page_size]. Entries
+ *     behind a sequence's last row are not read
+ *   lengths [B] int32: the rows that are there AHEAD of a call. No call but dadattn_paged_advance changes them, so that the
+ *     layers of a model, each with pages of its own, share one table and one set of lengths.
+ * A batch's new tokens lie packed: sequence b's are rows starts[b] .. starts[b + 1] - 1 of [T, heads, D] (starts [B + 1] int32,
+ * not falling, starts[B] <= T), none, one or many, and are its rows lengths[b] and on. starts NULL: one token for each sequence,
+ * T = B. Packed tensors have strides (host arrays of two: token, head, in elements), every row beginning at a multiple of 16
+ * bytes; those of results and of the attention's queries are not zero. Rows of the packed results that belong to no sequence
+ * (behind starts[B]) are left as they were. Hq query heads share Hkv key heads, Hq / Hkv neighbours each.
+ * A sequence whose numbers do not fit (lengths[b] below 0, rows beyond max_pages * page_size, starts[b + 1] below starts[b]) is
+ * left untouched, and so is a row whose page is outside [0, pages); both are reported through DADATTN_E_ARG at the next
+ * dadattn_device_status(). (Where starts fall, whose the rows are that two sequences claim is not said.) Nothing outside the pages is read or written for any contents of the device arrays.
+ * No call needs a workspace; calls may overlap on the GPU unless one writes what the other reads or writes. */
+
+/* New rows to their pages: k_new, v_new [T,Hkv,D] (bf16 when new_is_bf16, else fp32, rounded to bf16 once), keys turned by
+ * their rows in their sequences where rot_dim > 0 (as in dadattn_rotary; freq NULL and rot_dim 0: learned positions). Hq > 0:
+ * q [T,Hq,D] of the same type is turned too, into q_out (bf16; may be q where that is bf16 with the same strides). A sequence's pages of
+ * these rows belong to it alone. rot_dim a multiple of 16; (Hq + 2 Hkv) D at most 524288. A prefill's heads [H,n,D] are taken
+ * with the strides (D, n D) and B = 1. */
+int dadattn_paged_append_bf16(uint16_t* k_pages, uint16_t* v_pages, const int32_t* page_table, const int32_t* lengths,
+                              const int32_t* starts, uint16_t* q_out, const void* q, const void* k_new, const void* v_new,
+                              const int64_t* q_out_strides, const int64_t* q_strides, const int64_t* k_strides,
+                              const int64_t* v_strides, int B, int T, int Hq, int Hkv, int D, int pages, int page_size,
+                              int max_pages, const double* freq, float factor, int rot_dim, int interleaved, int new_is_bf16,
+                              dadattn_stream_t stream);
+
+/* Attention of the new tokens over all rows of their sequences, theirs among them, which are in their pages already: token i
+ * of sequence b sees rows j <= lengths[b] + i. out, q [T,Hq,D] bf16; lse [T,Hq] fp32 (natural log of the sum of exp of the
+ * scaled scores; may be NULL). scale > 0. max_new: no sequence brings more tokens than this (one that does is left untouched
+ * and reported); it bounds the launch. Hq / Hkv at most 128. Where a page is outside the pool, the rows of the 128-row query
+ * tiles that would read it (256 rows where two tiles share their keys) are left untouched. What pages hold behind a sequence's
+ * last row has no influence; an infinite or NaN row of a sequence makes NaN of the rows of a 128-row query tile that reads its
+ * tile of 128 keys, as in dadattn_flash_fwd_bf16. */
+int dadattn_paged_attention_bf16(uint16_t* out, float* lse, const uint16_t* q, const int64_t* out_strides,
+                                 const int64_t* q_strides, const uint16_t* k_pages, const uint16_t* v_pages,
+                                 const int32_t* page_table, const int32_t* lengths, const int32_t* starts, int B, int T,
+                                 int max_new, int Hq, int Hkv, int D, int pages, int page_size, int max_pages, float scale,
+                                 dadattn_stream_t stream);
+
+/* One decode step in one launch: the token of every sequence (q [B,Hq,D], k_new, v_new [B,Hkv,D] bf16, strides as above) is
+ * turned by its row where rot_dim > 0, appended at row lengths[b] and attended for over rows 0 .. lengths[b]; out [B,Hq,D],
+ * lse [B,Hq] or NULL. The same as dadattn_paged_append_bf16 and dadattn_paged_attention_bf16 with starts NULL, up to the order of
+ * the sums. Where a page that holds a row of the sequence is outside the pool, out of that sequence and key head is left
+ * untouched. */
+int dadattn_decode_paged_bf16(uint16_t* out, float* lse, const uint16_t* q, const uint16_t* k_new, const uint16_t* v_new,
+                              const int64_t* out_strides, const int64_t* q_strides, const int64_t* k_strides,
+                              const int64_t* v_strides, uint16_t* k_pages, uint16_t* v_pages, const int32_t* page_table,
+                              const int32_t* lengths, int B, int Hq, int Hkv, int D, int pages, int page_size, int max_pages,
+                              float scale, const double* freq, float factor, int rot_dim, int interleaved,
+                              dadattn_stream_t stream);
+
+/* The end of a step, behind its last layer: lengths[b] += the tokens that sequence b brought (starts as above). */
+int dadattn_paged_advance(int32_t* lengths, const int32_t* starts, int B, int T, int page_size, int max_pages,
+                          dadattn_stream_t stream);
+
 /* Synchronises the stream and returns the sticky device-side status word of this device
  * (0, or a DADATTN_E_* code recorded by a kernel: a bounded wait that ran out, a sequence at
  * max_len). Clears the word. For a wait that ran out dadattn_last_error() names the source line
