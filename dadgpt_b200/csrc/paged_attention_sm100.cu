@@ -6,17 +6,21 @@
 // a key head are rows of one tile: a 128-row tile is 128 / group tokens of all of them, so K and V are read once for the group
 // and a short piece of a prompt still fills tiles.
 //
-// A CTA has two softmax groups of 128 threads (a row each), two tensor-core issuers and one ring of 128-key K and V tiles:
-//   * pairs (CLUSTER = 1): two adjacent query tiles, A and B, of a sequence and key head. Both use every K / V tile of the
-//     ring; while the threads of one compute exponentials the tensor pipe runs the products of the other;
-//   * one tile: where a sequence has no second one, the two groups share its keys, A the even tiles of the ring, B the odd
-//     ones, and join their maxima, sums and accumulators at the end;
-//   * clusters: where the tiles do not fill the GPU every CTA of a cluster takes a run of one tile's keys, both groups as above,
-//     and the results are joined through distributed shared memory: no workspace.
+// A CTA has two softmax groups of 128 threads (a row each), two tensor-core issuers and one ring of 128-key K and V tiles. An
+// item is
+//   * a pair of adjacent query tiles, A and B, of a sequence and key head. Both use every K / V tile of the ring; while the
+//     threads of one compute exponentials the tensor pipe runs the products of the other;
+//   * or one tile, where a sequence has no second one: the groups share its keys, A the even tiles of the ring, B the odd ones,
+//     and join their maxima, sums and accumulators, which each finds in tensor memory, at the end.
+// CTAs are persistent and take items from the grid's own queue (clusterlaunchcontrol): keys of the next item are on their way
+// while the current one ends. Where the tiles do not fill the GPU (CLUSTER > 1), every CTA of a cluster takes a run of one tile's
+// keys, both groups as above, and the results are joined through distributed shared memory: no workspace.
+// The two groups' exponentials take turns: left to themselves they fall into step, each at half the exp2 unit's rate, and the
+// tensor pipe idles (a count in shared memory says how far the other is; it is waited for with a limit and nothing depends on it).
 // Keys come through the page table: lane i of the producer warp fetches the i-th box of a tile (as high as a page, up to the
 // tile), and looks its page up a tile ahead. Rows behind a sequence's last are not trusted: their scores are masked, and the
 // softmax threads set their V to zero in shared memory before they hand over the probabilities of that tile.
-//   warp 0       K / V producer                    warp 1     issuer of group A, tensor memory
+//   warp 0       scheduler + K / V producer        warp 1     issuer of group A, tensor memory
 //   warp 2       issuer of group B                 warp 3     Q
 //   warps 4-7    softmax group A                   warps 8-11 softmax group B
 // Every wait is bounded (sm100_ptx.cuh).
@@ -30,7 +34,6 @@
 #include "sm100_ptx.cuh"
 
 namespace dadattn {
-
 namespace {
 
 using namespace ptx;
@@ -40,6 +43,7 @@ constexpr int kT = 128;                 // tile edge: query rows of a group, key
 constexpr int kPanel = 128 * 128;       // [128 rows][64 bf16]: 16 KB, 128-byte rows, swizzled
 constexpr int kThreads = 12 * 32;
 constexpr int kGroup = 128;             // threads of a softmax group
+constexpr int kItems = 4;               // items a CTA knows of (a power of two)
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -57,26 +61,29 @@ struct Plan {
   static constexpr int kTileBytes = kPanels * kPanel;
   static constexpr int kSlots = D == 128 ? 5 : 10;          // ring of K and V tiles, K0 V0 K1 V1 ...
   static constexpr int kQ = 0;                              // [A, B]
-  static constexpr int kKV = kQ + 2 * kTileBytes;           // (from Q's second tile on where there is one)
-  static constexpr int kHalf = D == 128 ? 3 : 5;            // slots of a group's own ring, where there is one tile
+  static constexpr int kKV = kQ + 2 * kTileBytes;
   static constexpr int kBars = kKV + kSlots * kTileBytes;
-  static constexpr int kBytes = kBars + 1024 + 2 * 2 * 128 * 4;
-  static constexpr int kPitch = D + 4;                      // floats of a row of the accumulators that are joined (banks)
-  static constexpr int kAcc = kT * kPitch * 4;              // in the ring's place
+  static constexpr int kStats = kBars + 1024;               // [group][row] (maximum, sum)
+  static constexpr int kBytes = kStats + 2 * 128 * 8;
+  static constexpr int kPitch = D + 4;                      // floats of a row of an accumulator that a cluster joins (banks)
   static_assert(kBytes <= 232448, "shared memory budget of one CTA exceeded");
-  static_assert(2 * kAcc <= kSlots * kTileBytes, "accumulators in the ring's place");
-  static_assert(2 * kHalf <= kSlots + 1, "the groups' rings");
+  static_assert(kT * kPitch * 4 <= kSlots * kTileBytes, "the accumulator in the ring's place");
 };
 
-constexpr int kMaxSlots = 10;   // of either way of using the ring
-static_assert(Plan<64>::kSlots <= kMaxSlots && Plan<128>::kSlots <= kMaxSlots && 2 * Plan<64>::kHalf <= kMaxSlots &&
-              2 * Plan<128>::kHalf <= kMaxSlots, "barriers of the slots");
+constexpr int kMaxSlots = 10;
+static_assert(Plan<64>::kSlots <= kMaxSlots && Plan<128>::kSlots <= kMaxSlots, "barriers of the slots");
 struct Bars {
-  uint64_t q_full[2], slot_full[kMaxSlots], slot_empty[kMaxSlots];
+  __align__(16) uint4 stolen;             // answer to a request for another block
+  uint64_t stolen_full;
+  uint64_t item_ready[kItems], item_free[kItems];
+  uint64_t q_full[2], q_empty[2], slot_full[kMaxSlots], slot_empty[kMaxSlots];
   uint64_t s_full[2], p_full[2][2], o_done[2], settled[2];   // [group]; p_full: [group][half of the keys]
+  uint64_t joined, parted;                // groups that share a tile: results are there; have been read
   uint32_t tmem_base;
-  int abort_flag, bad;
-  int item[5];   // sequence, first token of the item in it, rows ahead, first row in the packed tensors, tokens of the sequence
+  int abort_flag;
+  int any_bad;                            // a page outside the pool, in any item
+  int exps[2][4];                         // tiles whose exponentials a warp of a group is through with
+  int item[kItems][8];                    // sequence (-1: the end), first token, rows ahead, first packed row, tokens, key head, bad
 };
 static_assert(sizeof(Bars) <= 1024, "barrier block");
 
@@ -86,25 +93,9 @@ struct ChunkParams {
   int64_t out_token, out_head;
   PagedCache cache;
   int T, max_new, heads_q, group, tile_tokens;   // tokens of a tile: 128 / group
-  int chunk;                            // rows of a K / V box
+  int chunk;                                     // rows of a K / V box
   float scale;
   int* status;
-};
-
-// A tile of a group: its rows, and how many key tiles it needs.
-struct Tile {
-  int token0, rows, n;
-};
-
-// K and V tiles in shared memory, K0 V0 K1 V1 ... The two tiles of a pair use one ring, each tile of which both issuers give
-// back. Groups that share the keys of one tile have a ring each: an issuer that passed over the other's tiles without
-// holding them could not tell their uses apart by the barriers' parity.
-struct Ring {
-  uint64_t *full, *empty;
-  uint32_t at;   // shared-memory address of the first slot
-  int len;
-  __device__ __forceinline__ int slot(int i) const { return i % len; }
-  __device__ __forceinline__ uint32_t use(int i) const { return (i / len) & 1; }
 };
 
 __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
@@ -112,9 +103,9 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
   return v;
 }
 __device__ __forceinline__ int ld_cluster_int(uint32_t addr) {
@@ -123,12 +114,47 @@ __device__ __forceinline__ int ld_cluster_int(uint32_t addr) {
   return v;
 }
 
-// The lowest-numbered sequence whose items, `tokens` tokens each, reach index x; by one warp. item[0] < 0: there is none.
-// Sequences that are refused have no items.
-__device__ __forceinline__ void find_item(const ChunkParams& p, int x, int tokens, int (&item)[5]) {
+// A tile of a group, or what is left of one: its rows, and how many key tiles they see.
+struct Tile {
+  int token0, rows, n;
+};
+struct Item {
+  int b, token0, ahead, first, count, kv_head;
+  template <int CLUSTER>
+  __device__ __forceinline__ bool single(const ChunkParams& p) const { return CLUSTER > 1 || token0 + p.tile_tokens >= count; }
+  __device__ __forceinline__ Tile tile(const ChunkParams& p, int at) const {   // at: 0, or 1 for the second of a pair
+    Tile t;
+    t.token0 = token0 + at * p.tile_tokens;
+    const int tokens = min(count - t.token0, p.tile_tokens);
+    t.rows = tokens * p.group;
+    t.n = (ahead + t.token0 + tokens + kT - 1) / kT;
+    return t;
+  }
+};
+// What a CTA does of an item: key tiles lo .. lo + n_kv - 1, of which group x takes n(x), its i-th being the CTA's at(x, i)-th.
+struct Share {
+  bool single;
+  int lo, n_kv, n_first;
+  __device__ __forceinline__ int n(int x) const { return single ? (n_kv - x + 1) / 2 : x ? n_kv : n_first; }
+  __device__ __forceinline__ int at(int x, int i) const { return single ? 2 * i + x : i; }
+};
+template <int CLUSTER>
+__device__ __forceinline__ Share share_of(const Item& it, const ChunkParams& p, int rank) {
+  Share s;
+  s.single = it.single<CLUSTER>(p);
+  const int n = it.tile(p, s.single ? 0 : 1).n;
+  s.lo = CLUSTER > 1 ? static_cast<int>(static_cast<int64_t>(n) * rank / CLUSTER) : 0;
+  s.n_kv = (CLUSTER > 1 ? static_cast<int>(static_cast<int64_t>(n) * (rank + 1) / CLUSTER) : n) - s.lo;
+  s.n_first = s.single ? 0 : it.tile(p, 0).n;
+  return s;
+}
+
+// The item of index x, `tokens` tokens each, among those of all sequences; by one warp. b < 0: there is none. Sequences that
+// are refused have no items.
+__device__ __forceinline__ Item find_item(const ChunkParams& p, int x, int kv_head, int tokens) {
   const PagedCache& c = p.cache;
   const int lane = threadIdx.x % 32;
-  item[0] = -1;
+  Item it = {-1, 0, 0, 0, 0, kv_head};
   int64_t before = 0;   // items of the sequences so far
   for (int base = 0; base < c.B; base += 32) {
     int ahead = 0, first = 0, count = 0;
@@ -148,16 +174,68 @@ __device__ __forceinline__ void find_item(const ChunkParams& p, int x, int token
       const int at = __ffs(reached) - 1;
       // the last tokens first: their rows see the most keys
       const int index = mine - 1 - static_cast<int>(x - before - (upto - mine));
-      item[0] = base + at;
-      item[1] = __shfl_sync(0xffffffffu, index, at) * tokens;
-      item[2] = __shfl_sync(0xffffffffu, ahead, at);
-      item[3] = __shfl_sync(0xffffffffu, first, at);
-      item[4] = __shfl_sync(0xffffffffu, count, at);
-      return;
+      it.b = base + at;
+      it.token0 = __shfl_sync(0xffffffffu, index, at) * tokens;
+      it.ahead = __shfl_sync(0xffffffffu, ahead, at);
+      it.first = __shfl_sync(0xffffffffu, first, at);
+      it.count = __shfl_sync(0xffffffffu, count, at);
+      return it;
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
   }
+  return it;
 }
+
+// ---- the grid's queue -------------------------------------------------------------------------------
+// Asks for a block of this grid that has not started yet, in its place; the answer (16 bytes) completes on `bar`.
+// Not asked again once the answer was that there is none.
+__device__ __forceinline__ void request_block(uint4* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+               ::"r"(smem_u32(answer)), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ bool read_answer(const uint4* answer, int& x, int& y) {
+  uint32_t ok, bx = 0, by = 0;
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 h, [%3];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, _, _}, h;\n\t}"
+      : "=&r"(ok), "=&r"(bx), "=&r"(by)
+      : "r"(smem_u32(answer))
+      : "memory");
+  x = bx, y = by;
+  return ok != 0;
+}
+
+// Every role reads the CTA's items, in order, from the ring that the scheduler fills, and gives each back.
+struct Feed {
+  Bars* bars;
+  volatile int* abort_flag;
+  int n;
+  __device__ __forceinline__ const volatile int* entry() const { return bars->item[n & (kItems - 1)]; }
+  __device__ __forceinline__ bool next(Item& it) {
+    if (!mbar_wait(&bars->item_ready[n & (kItems - 1)], (n / kItems) & 1, abort_flag)) return false;
+    const volatile int* e = entry();
+    it = Item{e[0], e[1], e[2], e[3], e[4], e[5]};
+    return it.b >= 0;
+  }
+  __device__ __forceinline__ void give_back() { mbar_arrive(&bars->item_free[n++ & (kItems - 1)]); }
+};
+
+// Which slot of the ring a tile's K (m = 0) or V is in, and the parity of that use. tile: of all that the CTA has gone through.
+template <int D>
+struct Slot {
+  int at;
+  uint32_t parity;
+  __device__ __forceinline__ Slot(int tile, int m) {
+    const uint32_t i = 2u * tile + m;
+    at = i % Plan<D>::kSlots;
+    parity = (i / Plan<D>::kSlots) & 1;
+  }
+};
 
 template <int D, int CLUSTER>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -169,69 +247,40 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256;
   extern __shared__ __align__(1024) uint8_t smem[];
   Bars* bars = reinterpret_cast<Bars*>(smem + L::kBars);
-  float* stats = reinterpret_cast<float*>(smem + L::kBars + 1024);   // [group][m, l][128]
+  float2* stats = reinterpret_cast<float2*>(smem + L::kStats);
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int rank = CLUSTER > 1 ? blockIdx.x % CLUSTER : 0, kv_head = blockIdx.y;
+  const int rank = CLUSTER > 1 ? blockIdx.x % CLUSTER : 0;
   const PagedCache& c = p.cache;
 
   if ((smem_u32(smem) & 1023u) != 0) {  // the swizzled layouts need a 1024-byte aligned base
     if (threadIdx.x == 0) atomicExch(p.status, DADATTN_E_CUDA);
     return;
   }
-  const int item_tokens = (CLUSTER > 1 ? 1 : 2) * p.tile_tokens;
-  if (warp == 0) {
-    pdl_wait();
-    int item[5];
-    find_item(p, blockIdx.x / CLUSTER, item_tokens, item);
-    if (lane == 0) {
-#pragma unroll
-      for (int i = 0; i < 5; ++i) bars->item[i] = item[i];
-    }
-  }
-  __syncthreads();
-  const int b = bars->item[0];
-  if (b < 0) return;   // (the same for a whole cluster)
-  const int token0 = bars->item[1], ahead = bars->item[2], first = bars->item[3], count = bars->item[4];
-  // One tile, whose keys the groups share, or two.
-  const bool single = CLUSTER > 1 || token0 + p.tile_tokens >= count;
-  auto tile_of = [&](int x) {
-    Tile t;
-    t.token0 = token0 + (single ? 0 : x * p.tile_tokens);
-    const int tokens = min(count - t.token0, p.tile_tokens);
-    t.rows = tokens * p.group;
-    t.n = (ahead + t.token0 + tokens + kT - 1) / kT;
-    return t;
-  };
-  // K / V tiles of this CTA: lo .. lo + n_kv - 1
-  const int n_last = tile_of(1).n;
-  const int lo = CLUSTER > 1 ? static_cast<int>(static_cast<int64_t>(n_last) * rank / CLUSTER) : 0;
-  const int n_kv = (CLUSTER > 1 ? static_cast<int>(static_cast<int64_t>(n_last) * (rank + 1) / CLUSTER) : n_last) - lo;
-  // Those of group x: every `stride`-th from `from`, `n` of them.
-  const int stride = single ? 2 : 1;
-  auto from_of = [&](int x) { return single ? x : 0; };
-  auto tiles_of = [&](int x) { return single ? (n_kv - x + 1) / 2 : tile_of(x).n; };
-  auto ring_of = [&](int x) {
-    const int s = single ? x * L::kHalf : 0;
-    return Ring{bars->slot_full + s, bars->slot_empty + s,
-                smem_u32(smem) + L::kQ + (single ? 1 : 2) * L::kTileBytes + s * L::kTileBytes, single ? L::kHalf : kSlots};
-  };
-
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kMaxSlots; ++i) {
+    mbar_init(&bars->stolen_full, 1);
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(&bars->item_ready[i], 1);
+      mbar_init(&bars->item_free[i], 2 * kGroup + 3);   // softmax, issuers, Q
+    }
+    for (int i = 0; i < kSlots; ++i) {
       mbar_init(&bars->slot_full[i], 1);
-      mbar_init(&bars->slot_empty[i], single ? 1 : 2);   // one arrival per issuer of the ring
+      mbar_init(&bars->slot_empty[i], 2);               // one arrival per issuer
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&bars->q_full[x], 1);
+      mbar_init(&bars->q_empty[x], 1);
       mbar_init(&bars->s_full[x], 1);
       mbar_init(&bars->p_full[x][0], kGroup);
       mbar_init(&bars->p_full[x][1], kGroup);
       mbar_init(&bars->o_done[x], 1);
       mbar_init(&bars->settled[x], 1);
+      for (int w = 0; w < 4; ++w) bars->exps[x][w] = 0;
     }
+    mbar_init(&bars->joined, 2 * kGroup);
+    mbar_init(&bars->parted, 2 * kGroup);
     bars->abort_flag = 0;
-    bars->bad = 0;
+    bars->any_bad = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -245,63 +294,119 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   pdl_wait();
   pdl_launch_dependents();
 
-  const int total = ahead + count;   // rows of the sequence
+  Feed feed{bars, abort_flag, 0};
+  Item it;
   if (warp < 4) {
     setmaxnreg_dec<kRegsHelper>();
     if (warp == 0) {
-      // ------------------------------ K / V producer ------------------------------
-      const int32_t* table = c.table + static_cast<int64_t>(b) * c.max_pages;
-      const int per_tile = kT / p.chunk;
+      // ------------------------------ scheduler + K / V producer ------------------------------
+      const int item_tokens = (CLUSTER > 1 ? 1 : 2) * p.tile_tokens;
+      const int per_tile = kT / p.chunk;   // boxes
       const int box = lane % per_tile, panel = lane / per_tile;
-      // the page of this lane's box; -1: no row of it is there
-      auto look_up = [&](int tile) -> int {
-        const int row = tile * kT + box * p.chunk;
-        if (panel >= L::kPanels || row >= total) return -1;
-        const int page = table[row >> c.page_shift];
-        if (page >= 0 && page < c.pages) return page;
-        bars->bad = 1;
-        return -2;
-      };
-      int page = n_kv > 0 ? look_up(lo) : -1, issued0 = 0, issued1 = 0;   // tiles, by ring
+      int n_pub = 0, n_asked = 0, n_loaded = 0, slot = 0;
+      uint32_t parity = 0;
       bool ok = true;
-      for (int j = 0; ok && j < n_kv; ++j) {
-        const int tile = lo + j, mine = page;
-        if (j + 1 < n_kv) page = look_up(tile + 1);
-        const int boxes = min((total - tile * kT + p.chunk - 1) / p.chunk, per_tile);
-        const int row = tile * kT + box * p.chunk;
-        // (a row coordinate outside the pool reads zeros)
-        const int y = mine >= 0 ? ((mine * c.heads + kv_head) << c.page_shift) + (row & ((1 << c.page_shift) - 1)) : -kMaxPage;
-        const int x = single ? j & 1 : 0;
-        const Ring r = ring_of(x);
-        int& issued = x ? issued1 : issued0;
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          const int i = issued, slot = r.slot(i);
-          if (i >= r.len && !(ok = warp_wait(&r.empty[slot], r.use(i) ^ 1u, abort_flag))) break;
-          if (lane == 0) mbar_arrive_expect_tx(&r.full[slot], boxes * L::kPanels * p.chunk * 128);
-          __syncwarp();
-          if (mine != -1)
-            tma_load_3d(r.at + slot * L::kTileBytes + panel * kPanel + box * p.chunk * 128, m ? &map_v : &map_k, &r.full[slot],
-                        panel * 64, y, 0);
-          __syncwarp();
-          ++issued;
+      auto ask = [&]() {
+        if (lane == 0) {
+          fence_proxy_async_smem();   // (the last answer has been read)
+          mbar_arrive_expect_tx(&bars->stolen_full, 16);
+          request_block(&bars->stolen, &bars->stolen_full);
         }
+        __syncwarp();
+        ++n_asked;
+      };
+      // the next block's item; b < 0 and `more` false: nothing left
+      auto answer = [&](bool& more) {
+        int x, y;
+        ok = warp_wait(&bars->stolen_full, (n_asked - 1) & 1, abort_flag);
+        more = ok && read_answer(&bars->stolen, x, y);
+        __syncwarp();
+        if (more) it = find_item(p, x, y, item_tokens);
+        else it.b = -1;
+      };
+      it = find_item(p, blockIdx.x / CLUSTER, blockIdx.y, item_tokens);
+      bool more = CLUSTER == 1;
+      while (ok) {
+        while (ok && it.b < 0 && more) {
+          ask();
+          answer(more);
+        }
+        if (!ok) break;
+        const int e = n_pub & (kItems - 1);
+        if (n_pub >= kItems && !(ok = warp_wait(&bars->item_free[e], (n_pub / kItems - 1) & 1, abort_flag))) break;
+        if (lane == 0) {
+          volatile int* to = bars->item[e];
+          to[0] = it.b, to[1] = it.token0, to[2] = it.ahead, to[3] = it.first, to[4] = it.count, to[5] = it.kv_head, to[6] = 0;
+          mbar_arrive(&bars->item_ready[e]);
+        }
+        __syncwarp();
+        ++n_pub;
+        if (it.b < 0) break;
+        const Share s = share_of<CLUSTER>(it, p, rank);
+        const int total = it.ahead + it.count;   // rows of the sequence
+        const int32_t* table = c.table + static_cast<int64_t>(it.b) * c.max_pages;
+        // the page of this lane's box; -1: no row of it is there
+        auto look_up = [&](int tile) -> int {
+          const int row = tile * kT + box * p.chunk;
+          if (panel >= L::kPanels || row >= total) return -1;
+          const int page = table[row >> c.page_shift];
+          if (page >= 0 && page < c.pages) return page;
+          bars->item[e][6] = bars->any_bad = 1;
+          return -2;
+        };
+        int page = s.n_kv > 0 ? look_up(s.lo) : -1;
+        for (int j = 0; ok && j < s.n_kv; ++j) {
+          const int tile = s.lo + j, mine = page;
+          // The next block is asked for only now: what a CTA holds in advance no idle CTA can take.
+          if (j + 1 < s.n_kv) page = look_up(tile + 1);
+          else if (CLUSTER == 1) ask();
+          const int boxes = min((total - tile * kT + p.chunk - 1) / p.chunk, per_tile);
+          const int row = tile * kT + box * p.chunk;
+          // (a row coordinate outside the pool reads zeros)
+          const int y = mine >= 0 ? ((mine * c.heads + it.kv_head) << c.page_shift) + (row & ((1 << c.page_shift) - 1)) : -kMaxPage;
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            if (n_loaded >= kSlots && !(ok = warp_wait(&bars->slot_empty[slot], parity ^ 1u, abort_flag))) break;
+            if (lane == 0) mbar_arrive_expect_tx(&bars->slot_full[slot], boxes * L::kPanels * p.chunk * 128);
+            __syncwarp();
+            if (mine != -1)
+              tma_load_3d(smem + L::kKV + slot * L::kTileBytes + panel * kPanel + box * p.chunk * 128, m ? &map_v : &map_k,
+                          &bars->slot_full[slot], panel * 64, y, 0);
+            __syncwarp();
+            ++n_loaded;
+            if (++slot == kSlots) slot = 0, parity ^= 1u;
+          }
+        }
+        if (CLUSTER == 1 && ok) answer(more);
+        else it.b = -1;
       }
       if (lane == 0) {
-        settle_ring(ring_of(0).full, ring_of(0).len, issued0);
-        if (single) settle_ring(ring_of(1).full, ring_of(1).len, issued1);
+        if (n_asked > 0) settle(&bars->stolen_full, (n_asked - 1) & 1);
+        settle_ring(bars->slot_full, kSlots, n_loaded);
       }
     } else if (warp == 3) {
       // ------------------------------ Q ------------------------------
       if (lane == 0) {
-        const int copies = single ? 1 : 2;
-        for (int x = 0; x < copies; ++x) {
-          mbar_arrive_expect_tx(&bars->q_full[x], L::kPanels * p.tile_tokens * p.group * 128);
-          for (int h = 0; h < L::kPanels; ++h)
-            tma_load_3d(smem + L::kQ + x * L::kTileBytes + h * kPanel, &map_q, &bars->q_full[x], h * 64, kv_head * p.group,
-                        first + tile_of(x).token0);
+        prefetch_tensormap(&map_q);
+        int n[2] = {0, 0};
+        bool ok = true;
+        while (ok && feed.next(it)) {
+          const Share s = share_of<CLUSTER>(it, p, rank);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (s.n(x) == 0) continue;
+            if (n[x] > 0 && !(ok = mbar_wait(&bars->q_empty[x], (n[x] - 1) & 1, abort_flag))) break;
+            mbar_arrive_expect_tx(&bars->q_full[x], L::kPanels * p.tile_tokens * p.group * 128);
+            for (int h = 0; h < L::kPanels; ++h)
+              tma_load_3d(smem + L::kQ + x * L::kTileBytes + h * kPanel, &map_q, &bars->q_full[x], h * 64, it.kv_head * p.group,
+                          it.first + it.tile(p, s.single ? 0 : x).token0);
+            ++n[x];
+          }
+          feed.give_back();
         }
-        for (int x = 0; x < copies; ++x) settle(&bars->q_full[x], 0);
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if (n[x] > 0) settle(&bars->q_full[x], (n[x] - 1) & 1);
       }
     } else {
       // ------------------------------ MMA issuers ------------------------------
@@ -309,51 +414,71 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       if (elect_one()) {
         constexpr uint32_t idesc_s = make_idesc_bf16(kT, kT, 0, 0);   // Q, K: K-major
         constexpr uint32_t idesc_o = make_idesc_bf16(kT, D, 0, 1);    // P K-major, V MN-major
-        const int q_at = single ? 0 : x;
-        const SmemDescBase q_desc = make_desc_base_sw128(smem_u32(smem + L::kQ) + q_at * L::kTileBytes, 0);
+        const SmemDescBase q_desc = make_desc_base_sw128(smem_u32(smem + L::kQ) + x * L::kTileBytes, 0);
         // (read MN-major, a V tile's two 64-column panels are kPanel apart; K-major operands ignore that offset)
-        const Ring ring = ring_of(x);
-        const SmemDescBase kv_desc0 = make_desc_base_sw128(ring.at, kPanel);
+        const SmemDescBase kv_desc0 = make_desc_base_sw128(smem_u32(smem + L::kKV), kPanel);
         const uint32_t tS = tmem + kColS + x * 128, tO = tmem + kColO + x * D;
-        const int n = tiles_of(x);
+        uint32_t g = 0, u = 0;   // key tiles and items of this group so far
+        int gone = 0;            // key tiles of the CTA so far
         bool ok = true;
-        auto wait_slot = [&](int i) -> bool { return mbar_wait(&ring.full[ring.slot(i)], ring.use(i), abort_flag); };
-        auto issue_s = [&](int i) -> bool {
-          if (!wait_slot(2 * i)) return false;
-          const int slot = ring.slot(2 * i);
+        auto wait_slot = [&](const Slot<D>& s) -> bool { return mbar_wait(&bars->slot_full[s.at], s.parity, abort_flag); };
+        // a tile that this group has nothing to do with: given back once it is there, as the others are
+        auto skip = [&](int tile) -> bool {
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            const Slot<D> s(tile, m);
+            if (!wait_slot(s)) return false;
+            mbar_arrive(&bars->slot_empty[s.at]);
+          }
+          return true;
+        };
+        auto issue_s = [&](int tile, bool last) -> bool {
+          const Slot<D> s(tile, 0);
+          if (!wait_slot(s)) return false;
           tc_fence_after_sync();
-          const SmemDescBase k_desc{kv_desc0.lo + slot * (L::kTileBytes >> 4), kv_desc0.hi};
+          const SmemDescBase k_desc{kv_desc0.lo + s.at * (L::kTileBytes >> 4), kv_desc0.hi};
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t off = (kk / 4) * kPanel + (kk % 4) * 32;
             mma_ss(tS, desc_at(q_desc, off), desc_at(k_desc, off), idesc_s, kk > 0 ? 1u : 0u);
           }
-          mma_commit(&ring.empty[slot]);
+          mma_commit(&bars->slot_empty[s.at]);
+          if (last) mma_commit(&bars->q_empty[x]);
           mma_commit(&bars->s_full[x]);
           return true;
         };
-        ok = n == 0 || (mbar_wait(&bars->q_full[q_at], 0, abort_flag) && issue_s(0));
-        for (int i = 0; ok && i < n; ++i) {
-          if (!(ok = wait_slot(2 * i + 1))) break;
-          const int slot = ring.slot(2 * i + 1);
-          const SmemDescBase v_desc{kv_desc0.lo + slot * (L::kTileBytes >> 4), kv_desc0.hi};
+        while (ok && feed.next(it)) {
+          const Share s = share_of<CLUSTER>(it, p, rank);
+          const int n = s.n(x);
+          if (s.single && x == 1 && s.n_kv > 0) ok = skip(gone);
+          if (ok && n > 0) ok = mbar_wait(&bars->q_full[x], u++ & 1, abort_flag) && issue_s(gone + s.at(x, 0), n == 1);
+          for (int i = 0; ok && i < n; ++i, ++g) {
+            const int at = s.at(x, i);
+            // (the other's next tile, ahead of the wait for the probabilities: its slots are not to wait for those)
+            if (s.single && at + 1 < s.n_kv && !(ok = skip(gone + at + 1))) break;
+            const Slot<D> v(gone + at, 1);
+            if (!(ok = wait_slot(v))) break;
+            // (a new item's first P V may overwrite O: its probabilities come after the last results have been read)
+            const SmemDescBase v_desc{kv_desc0.lo + v.at * (L::kTileBytes >> 4), kv_desc0.hi};
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {   // O (+)= P[:, 64 h .. 64 h + 63] V[64 h .. 64 h + 63, :]
-            if (!(ok = mbar_wait(&bars->p_full[x][h], i & 1, abort_flag))) break;
-            tc_fence_after_sync();
+            for (int h = 0; h < 2; ++h) {   // O (+)= P[:, 64 h .. 64 h + 63] V[64 h .. 64 h + 63, :]
+              if (!(ok = mbar_wait(&bars->p_full[x][h], g & 1, abort_flag))) break;
+              tc_fence_after_sync();
 #pragma unroll
-            for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
-              mma_ts(tO, tS + kk * 8, desc_at(v_desc, kk * 2048), idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
+              for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
+                mma_ts(tO, tS + kk * 8, desc_at(v_desc, kk * 2048), idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
+            }
+            if (!ok) break;
+            mma_commit(&bars->slot_empty[v.at]);
+            if (i + 1 < n) ok = issue_s(gone + s.at(x, i + 1), i + 2 == n);   // over the probabilities, whose product is ahead in the pipe
+            else mma_commit(&bars->o_done[x]);
           }
-          if (!ok) break;
-          mma_commit(&ring.empty[slot]);
-          if (i + 1 < n) ok = issue_s(i + 1);   // over the probabilities, whose product is ahead in the pipe
-          else mma_commit(&bars->o_done[x]);
+          // tiles that only the pair's other group sees
+          if (!s.single)
+            for (int j = n; ok && j < s.n_kv; ++j) ok = skip(gone + j);
+          gone += s.n_kv;
+          feed.give_back();
         }
-        // tiles of the pair's other group: given back once they are there
-        if (!single)
-          for (int i = 2 * n; ok && i < 2 * n_kv; ++i)
-            if ((ok = wait_slot(i))) mbar_arrive(&ring.empty[ring.slot(i)]);
         settle_products(&bars->settled[x]);
       }
     }
@@ -366,154 +491,185 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const uint32_t tlane = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const uint32_t tS = tlane + kColS + x * 128, tO = tlane + kColO + x * D;
     const float scale_log2 = p.scale * kLog2e;
-    const Tile t = tile_of(x);
-    const int n = tiles_of(x);
-    const bool active = quad * 32 < t.rows;          // whether the warp has a row
-    const int mine = min(row, t.rows - 1);           // (rows that are not there take the last one's mask)
-    const int token = t.token0 + mine / p.group, limit = ahead + token;
-    float m = -INFINITY, l = 0.f;   // running max (log2 units, scaled) and sum
+    uint32_t g = 0, u = 0, joins = 0;     // key tiles, items with any and shared tiles of this group so far
+    int gone = 0, others = 0;             // key tiles of the CTA and of the other group so far
     bool ok = true;
-    int j = from_of(x);
-    for (int i = 0; i < n; ++i, j += stride) {
-      if (!(ok = mbar_wait(&bars->s_full[x], i & 1, abort_flag))) break;
-      tc_fence_after_sync();
-      const int key0 = (lo + j) * kT;
-      uint32_t s[4][32];
-      if (active) {
+    while (ok && feed.next(it)) {
+      const Share s = share_of<CLUSTER>(it, p, rank);
+      const Tile t = it.tile(p, s.single ? 0 : x);
+      const int n = s.n(x), total = it.ahead + it.count;
+      const bool active = quad * 32 < t.rows;          // whether the warp has a row
+      const int token = t.token0 + min(row, t.rows - 1) / p.group, limit = it.ahead + token;   // (rows that are not there: the last one's mask)
+      float m = -INFINITY, l = 0.f;   // running max (log2 units, scaled) and sum
+      for (int i = 0; i < n; ++i, ++g) {
+        if (!(ok = mbar_wait(&bars->s_full[x], g & 1, abort_flag))) break;
+        tc_fence_after_sync();
+        const int key0 = (s.lo + s.at(x, i)) * kT;
+        uint32_t sc[4][32];
+        if (active) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) tmem_ld32(tS + q * 32, s[q]);
-        tmem_wait_ld();
-        const int seen = limit - key0;   // the last column that the row sees
-        if (__any_sync(0xffffffffu, seen < kT - 1)) {
+          for (int q = 0; q < 4; ++q) tmem_ld32(tS + q * 32, sc[q]);
+          tmem_wait_ld();
+          const int seen = limit - key0;   // the last column that the row sees
+          if (__any_sync(0xffffffffu, seen < kT - 1)) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (q * 32 + e > seen) sc[q][e] = 0xff800000u;  // -inf
+          }
+          // max of the raw scores (scale > 0 commutes with max)
+          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int q = 0; q < 4; q += 2)
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (q * 32 + e > seen) s[q][e] = 0xff800000u;  // -inf
-        }
-        // max of the raw scores (scale > 0 commutes with max)
-        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int q = 0; q < 4; q += 2)
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            mx4[e & 3] = fmax3(mx4[e & 3], __uint_as_float(s[q][e]), __uint_as_float(s[q + 1][e]));
-        const float mx = __fmul_rn(fmaxf(fmax3(mx4[0], mx4[1], mx4[2]), mx4[3]), scale_log2);
-        if (i == 0) {
-          m = mx;  // O is first written by a product that does not accumulate: nothing to rescale
-        } else if (__any_sync(0xffffffffu, row < t.rows && mx > m + kRescaleAt)) {   // (nobody else's rows decide)
-          // (P V of the tile before is through: these scores were issued behind it)
-          const float m_new = fmaxf(m, mx);
-          // m = -inf: nothing but zeros has been accumulated so far
-          const float corr = (m == -INFINITY) ? 0.f : ex2(m - m_new);
+              mx4[e & 3] = fmax3(mx4[e & 3], __uint_as_float(sc[q][e]), __uint_as_float(sc[q + 1][e]));
+          const float mx = __fmul_rn(fmaxf(fmax3(mx4[0], mx4[1], mx4[2]), mx4[3]), scale_log2);
+          if (i == 0) {
+            m = mx;  // O is first written by a product that does not accumulate: nothing to rescale
+          } else if (__any_sync(0xffffffffu, row < t.rows && mx > m + kRescaleAt)) {   // (nobody else's rows decide)
+            // (P V of the tile before is through: these scores were issued behind it)
+            const float m_new = fmaxf(m, mx);
+            // m = -inf: nothing but zeros has been accumulated so far
+            const float corr = (m == -INFINITY) ? 0.f : ex2(m - m_new);
 #pragma unroll 1
+            for (int q = 0; q < D / 32; ++q) {
+              uint32_t o[32];
+              tmem_ld32(tO + q * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+              tmem_st32(tO + q * 32, o);
+            }
+            tmem_wait_st();
+            l = __fmul_rn(l, corr);
+            m = m_new;
+          }
+        }
+        if (total - key0 < kT) {
+          // The sequence ends in this tile: V of the rows behind it.
+          const Slot<D> v(gone + s.at(x, i), 1);
+          const int there = total - key0;
+          if (!(ok = mbar_wait(&bars->slot_full[v.at], v.parity, abort_flag))) break;
+          uint8_t* rows = smem + L::kKV + v.at * L::kTileBytes;
+          for (int e = threadIdx.x % kGroup; e < (kT - there) * (D / 8); e += kGroup) {
+            const int r = there + e / (D / 8), ch = e % (D / 8);
+            *reinterpret_cast<uint4*>(rows + (ch / 8) * kPanel + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+        // A's turn is behind B's tile before, B's behind A's tile of the same place.
+        {
+          const int due = x == 0 ? min(i, s.n(1)) : min(i + 1, s.n(0));
+          const volatile int* done = &bars->exps[1 - x][quad];
+          for (int k = 0; k < 256 && *done < others + due; ++k) {}
+        }
+        // p = exp2(s scale log2e - m). A row whose scores are all -inf so far must give p = 0, not exp2(NaN).
+        float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        const float2 sl = make_float2(scale_log2, scale_log2);
+        const float neg_m = (m == -INFINITY) ? 0.f : -m;
+        const float2 nm = make_float2(neg_m, neg_m);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (active) {
+            uint32_t pk[16];   // bf16 pairs (k, k + 1) per column
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 y = ffma2(make_float2(__uint_as_float(sc[q][e]), __uint_as_float(sc[q][e + 1])), sl, nm);
+              const float2 w = make_float2(ex2(y.x), ex2(y.y));
+              sum2[(e >> 1) & 1] = fadd2(sum2[(e >> 1) & 1], w);
+              pk[e / 2] = pack_bf16(w.x, w.y);
+            }
+            tmem_st16(tS + q * 16, pk);
+          }
+          if (q & 1) {
+            if (active) tmem_wait_st();
+            tc_fence_before_sync();
+            mbar_arrive(&bars->p_full[x][q / 2]);
+          }
+        }
+        if (lane == 0) *const_cast<volatile int*>(&bars->exps[x][quad]) = static_cast<int>(g) + 1;
+        l += (sum2[0].x + sum2[1].x) + (sum2[0].y + sum2[1].y);
+      }
+      if (ok && n > 0) ok = mbar_wait(&bars->o_done[x], u++ & 1, abort_flag);
+      if (!ok) break;
+      tc_fence_after_sync();
+      const int64_t to_token = it.first + token;
+      const int to_head = it.kv_head * p.group + min(row, t.rows - 1) % p.group;
+      bf16* to = p.out + to_token * p.out_token + to_head * p.out_head;
+      const bool write = row < t.rows && !feed.entry()[6];
+      l *= ex2(m == -INFINITY ? 0.f : m - m);   // (NaN where the max is not finite)
+      if (!s.single) {
+        // out = O / l, lse in natural-log units of the scaled scores
+        const float f = 1.0f / l;
+        if (active) {
+#pragma unroll
           for (int q = 0; q < D / 32; ++q) {
             uint32_t o[32];
             tmem_ld32(tO + q * 32, o);
             tmem_wait_ld();
+            if (write) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-            tmem_st32(tO + q * 32, o);
+              for (int e = 0; e < 32; e += 8) {
+                float y[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) y[k] = __uint_as_float(o[e + k]) * f;
+                *reinterpret_cast<uint4*>(to + q * 32 + e) =
+                    make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+              }
+            }
           }
-          tmem_wait_st();
-          l = __fmul_rn(l, corr);
-          m = m_new;
         }
-      }
-      if (total - key0 < kT) {
-        // The sequence ends in this tile: V of the rows behind it.
-        const Ring ring = ring_of(x);
-        const int slot = ring.slot(2 * i + 1), there = total - key0;
-        if (!(ok = mbar_wait(&ring.full[slot], ring.use(2 * i + 1), abort_flag))) break;
-        const uint32_t v = ring.at + slot * L::kTileBytes;
-        for (int e = threadIdx.x % kGroup; e < (kT - there) * (D / 8); e += kGroup) {
-          const int r = there + e / (D / 8), ch = e % (D / 8);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v + (ch / 8) * kPanel + r * 128 + (ch & 7) * 16), "r"(0)
-                       : "memory");
-        }
-        fence_proxy_async_smem();
-      }
-      // p = exp2(s scale log2e - m). A row whose scores are all -inf so far must give p = 0, not exp2(NaN).
-      float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      const float2 sl = make_float2(scale_log2, scale_log2);
-      const float neg_m = (m == -INFINITY) ? 0.f : -m;
-      const float2 nm = make_float2(neg_m, neg_m);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
+        if (write && p.lse) p.lse[to_token * p.heads_q + to_head] = (m + log2f(l)) * kLn2;
+      } else {
+        // The other group has the rest of the row's keys: each group joins one half of the columns.
+        stats[x * 128 + row] = make_float2(m, l);
+        tc_fence_before_sync();
+        mbar_arrive(&bars->joined);
+        if (!(ok = mbar_wait(&bars->joined, joins & 1, abort_flag))) break;
+        tc_fence_after_sync();
+        const float2 other = stats[(1 - x) * 128 + row];
+        const float m_all = fmaxf(m, other.x);
+        // (a part that has seen nothing has nothing but garbage)
+        const float f0 = m == -INFINITY ? 0.f : ex2(m - m_all), f1 = other.x == -INFINITY ? 0.f : ex2(other.x - m_all);
+        const float l_all = l * f0 + other.y * f1;
+        const float norm = CLUSTER == 1 ? 1.0f / l_all : 1.0f;
+        float* acc = reinterpret_cast<float*>(smem + L::kKV) + row * L::kPitch;
         if (active) {
-          uint32_t pk[16];   // bf16 pairs (k, k + 1) per column
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float2 y = ffma2(make_float2(__uint_as_float(s[q][e]), __uint_as_float(s[q][e + 1])), sl, nm);
-            const float2 w = make_float2(ex2(y.x), ex2(y.y));
-            sum2[(e >> 1) & 1] = fadd2(sum2[(e >> 1) & 1], w);
-            pk[e / 2] = pack_bf16(w.x, w.y);
-          }
-          tmem_st16(tS + q * 16, pk);
-        }
-        if (q & 1) {
-          if (active) tmem_wait_st();
-          tc_fence_before_sync();
-          mbar_arrive(&bars->p_full[x][q / 2]);
-        }
-      }
-      l += (sum2[0].x + sum2[1].x) + (sum2[0].y + sum2[1].y);
-    }
-    if (ok && n > 0) ok = mbar_wait(&bars->o_done[x], 0, abort_flag);
-    tc_fence_after_sync();
-    const int q_head = kv_head * p.group + mine % p.group;
-    if (!single) {
-      // Results: out = O / l, lse in natural-log units of the scaled scores. They leave through the group's Q tile, which
-      // nobody reads any more: every Q K^T has completed before the last s_full was observed.
-      if (ok && active && !bars->bad) {
-        const float l_tot = l * ex2(m - m);   // (NaN where the max is not finite)
-        const float f = 1.0f / l_tot;
-        uint8_t* stage = smem + L::kQ + x * L::kTileBytes + quad * 32 * 128;   // this warp's rows
+          for (int q = x * (D / 64); q < (x + 1) * (D / 64); ++q) {
+            uint32_t o[32], o1[32];
+            tmem_ld32(tO + q * 32, o);
+            tmem_ld32(tlane + kColO + (1 - x) * D + q * 32, o1);
+            tmem_wait_ld();
 #pragma unroll
-        for (int q = 0; q < D / 32; ++q) {
-          uint32_t o[32];
-          tmem_ld32(tO + q * 32, o);
-          tmem_wait_ld();
-          uint8_t* dst = stage + (q / 2) * kPanel + lane * 128;
+            for (int e = 0; e < 32; e += 8) {
+              float y[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float y[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(o[8 * i + e]) * f;
-            *reinterpret_cast<uint4*>(dst + ((((q & 1) * 4 + i) ^ (lane & 7)) << 4)) =
-                make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+              for (int k = 0; k < 8; ++k) {
+                const float a = f0 == 0.f ? 0.f : __uint_as_float(o[e + k]) * f0;
+                y[k] = (f1 == 0.f ? a : fmaf(__uint_as_float(o1[e + k]), f1, a)) * norm;
+              }
+              if (CLUSTER > 1) {
+                *reinterpret_cast<float4*>(acc + q * 32 + e) = make_float4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<float4*>(acc + q * 32 + e + 4) = make_float4(y[4], y[5], y[6], y[7]);
+              } else if (write) {
+                *reinterpret_cast<uint4*>(to + q * 32 + e) =
+                    make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+              }
+            }
           }
         }
-        if (p.lse && row < t.rows) p.lse[static_cast<int64_t>(first + token) * p.heads_q + q_head] = (m + log2f(l_tot)) * kLn2;
-        __syncwarp();
-        constexpr int kPieces = D / 8;   // 16-byte pieces of a row
-#pragma unroll 4
-        for (int i = lane; i < 32 * kPieces; i += 32) {
-          const int r = i / kPieces, ch = i % kPieces, at = quad * 32 + r;
-          if (at >= t.rows) break;
-          const uint4 v = *reinterpret_cast<const uint4*>(stage + (ch / 8) * kPanel + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
-          bf16* dst = p.out + static_cast<int64_t>(first + t.token0 + at / p.group) * p.out_token +
-                      static_cast<int64_t>(kv_head * p.group + at % p.group) * p.out_head + ch * 8;
-          *reinterpret_cast<uint4*>(dst) = v;
-        }
+        if (CLUSTER == 1 && x == 0 && write && p.lse) p.lse[to_token * p.heads_q + to_head] = (m_all + log2f(l_all)) * kLn2;
+        tc_fence_before_sync();
+        mbar_arrive(&bars->parted);
+        if (!(ok = mbar_wait(&bars->parted, joins++ & 1, abort_flag))) break;
+        if (CLUSTER > 1 && x == 0) stats[row] = make_float2(m_all, l_all);
       }
-    } else {
-      // Both groups are through with the ring: accumulators, maxima and sums go there.
-      asm volatile("bar.sync 1, %0;" ::"n"(2 * kGroup) : "memory");
-      stats[x * 256 + row] = ok && n > 0 ? m : -INFINITY;
-      stats[x * 256 + 128 + row] = l * ex2(m == -INFINITY ? 0.f : m - m);
-      if (ok && n > 0 && active) {
-        float* acc = reinterpret_cast<float*>(smem + L::kKV + x * L::kAcc) + row * L::kPitch;
-#pragma unroll
-        for (int q = 0; q < D / 32; ++q) {
-          uint32_t o[32];
-          tmem_ld32(tO + q * 32, o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<uint4*>(acc + q * 32 + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-        }
-      }
+      gone += s.n_kv;
+      others += s.n(1 - x);
+      feed.give_back();
     }
   }
 
@@ -525,55 +681,52 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     tc_fence_after_sync();
     tmem_dealloc(tmem, kTmemCols);
   }
-  if (single) {
-    int bad = bars->bad | bars->abort_flag;
-    if (CLUSTER > 1) {
-      cluster_arrive();
-      cluster_wait();
-      bad = 0;
+  if (CLUSTER > 1) {
+    const volatile int* e = bars->item[0];
+    it = Item{e[0], e[1], e[2], e[3], e[4], e[5]};
+    cluster_arrive();
+    cluster_wait();
+    int bad = it.b < 0;   // (there is no item, or nobody published one)
 #pragma unroll 1
-      for (int r = 0; r < CLUSTER; ++r)
-        bad |= ld_cluster_int(cluster_address(&bars->bad, r)) | ld_cluster_int(cluster_address(&bars->abort_flag, r));
-    }
+    for (int r = 0; r < CLUSTER; ++r)
+      bad |= ld_cluster_int(cluster_address(&bars->any_bad, r)) | ld_cluster_int(cluster_address(&bars->abort_flag, r));
     // This CTA's share of the rows, eight columns a thread.
     constexpr int kPieces = D / 8;
-    const Tile t = tile_of(0);
+    const Tile t = it.tile(p, 0);
     const int share = (t.rows + CLUSTER - 1) / CLUSTER, row0 = rank * share, row1 = min(t.rows, row0 + share);
     for (int i = threadIdx.x; !bad && i < (row1 - row0) * kPieces; i += kThreads) {
       const int row = row0 + i / kPieces, col = i % kPieces * 8;
-      float m_tot = -INFINITY, l_tot = 0.f, y[8] = {};
-#pragma unroll 1
-      for (int r = 0; r < 2 * CLUSTER; ++r) m_tot = fmaxf(m_tot, ld_cluster(cluster_address(&stats[(r & 1) * 256 + row], r / 2)));
-#pragma unroll 2
-      for (int r = 0; r < 2 * CLUSTER; ++r) {
-        const float mr = ld_cluster(cluster_address(&stats[(r & 1) * 256 + row], r / 2));
-        const float lr = ld_cluster(cluster_address(&stats[(r & 1) * 256 + 128 + row], r / 2));
-        if (mr == -INFINITY) continue;   // (nothing was accumulated)
-        const float f = ex2(mr - m_tot);
-        l_tot = fmaf(lr, f, l_tot);
-        const uint32_t at = cluster_address(smem + L::kKV + (r & 1) * L::kAcc + (row * L::kPitch + col) * 4, r / 2);
+      float2 ml[CLUSTER];
+      float m_all = -INFINITY, l_all = 0.f, y[8] = {};
+#pragma unroll
+      for (int r = 0; r < CLUSTER; ++r) ml[r] = ld_cluster2(cluster_address(&stats[row], r));
+#pragma unroll
+      for (int r = 0; r < CLUSTER; ++r) m_all = fmaxf(m_all, ml[r].x);
+#pragma unroll
+      for (int r = 0; r < CLUSTER; ++r) {
+        const float f = ml[r].x == -INFINITY ? 0.f : ex2(ml[r].x - m_all);
+        l_all = fmaf(ml[r].y, f, l_all);
+        const uint32_t at = cluster_address(smem + L::kKV + (row * L::kPitch + col) * 4, r);
         const float4 a = ld_cluster4(at), b4 = ld_cluster4(at + 16);
         const float v[8] = {a.x, a.y, a.z, a.w, b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = fmaf(v[e], f, y[e]);
+        for (int k = 0; k < 8; ++k) y[k] = f == 0.f ? y[k] : fmaf(v[k], f, y[k]);
       }
-      const float f = 1.0f / l_tot;
+      const float f = 1.0f / l_all;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] *= f;
-      const int64_t token = first + t.token0 + row / p.group;
-      const int head = kv_head * p.group + row % p.group;
+      for (int k = 0; k < 8; ++k) y[k] *= f;
+      const int64_t token = it.first + t.token0 + row / p.group;
+      const int head = it.kv_head * p.group + row % p.group;
       *reinterpret_cast<uint4*>(p.out + token * p.out_token + head * p.out_head + col) =
           make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
-      if (p.lse && col == 0) p.lse[token * p.heads_q + head] = (m_tot + log2f(l_tot)) * kLn2;
+      if (p.lse && col == 0) p.lse[token * p.heads_q + head] = (m_all + log2f(l_all)) * kLn2;
     }
-    if (CLUSTER > 1) {
-      cluster_arrive();
-      cluster_wait();   // (the others' shared memory stays until it has been read)
-    }
+    cluster_arrive();
+    cluster_wait();   // (the others' shared memory stays until it has been read)
   }
   if (threadIdx.x == 0) {
     if (bars->abort_flag) report_timeout(p.status, bars->abort_flag);
-    else if (bars->bad) atomicExch(p.status, DADATTN_E_ARG);
+    else if (bars->any_bad) atomicExch(p.status, DADATTN_E_ARG);
   }
 }
 
