@@ -27,6 +27,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <climits>
 
 #include "decode_common.cuh"
 #include "paged.cuh"
@@ -44,40 +45,43 @@ constexpr int kPanel = 128 * 128;       // [128 rows][64 bf16]: 16 KB, 128-byte 
 constexpr int kThreads = 12 * 32;
 constexpr int kGroup = 128;             // threads of a softmax group
 constexpr int kItems = 4;               // items a CTA knows of (a power of two)
+constexpr int kSlots = 5;               // ring of K and V tiles, K0 V0 K1 V1 ...
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kRescaleAt = 8.0f;      // log2 units: O is rescaled only when the maximum grew by 2^8
-// Registers per thread once the warpgroups have rebalanced (a softmax thread holds 128 scores).
-constexpr int kRegsLaunch = 168, kRegsSoftmax = 208, kRegsHelper = 88;
-static_assert(2 * kGroup * kRegsSoftmax + 128 * kRegsHelper <= kThreads * kRegsLaunch,
-              "the warpgroups ask for more registers than the CTA owns");
-static_assert(kThreads * kRegsLaunch <= 65536 && (kRegsLaunch + 8) * kThreads > 65536,
-              "kRegsLaunch is not what the compiler gives a CTA of this size");
 
 template <int D>
 struct Plan {
+  static constexpr int kPerSm = D == 128 ? 1 : 2;           // CTAs
+  static constexpr int kN = D == 128 ? 128 : 64;            // keys of a step
+  static constexpr int kSteps = kT / kN;                    // steps of a key tile
   static constexpr int kPanels = D / 64;
   static constexpr int kTileBytes = kPanels * kPanel;
-  static constexpr int kSlots = D == 128 ? 5 : 10;          // ring of K and V tiles, K0 V0 K1 V1 ...
   static constexpr int kQ = 0;                              // [A, B]
   static constexpr int kKV = kQ + 2 * kTileBytes;
   static constexpr int kBars = kKV + kSlots * kTileBytes;
-  static constexpr int kStats = kBars + 1024;               // [group][row] (maximum, sum)
-  static constexpr int kBytes = kStats + 2 * 128 * 8;
+  static constexpr int kBytes = kBars + 1024;
   static constexpr int kPitch = D + 4;                      // floats of a row of an accumulator that a cluster joins (banks)
-  static_assert(kBytes <= 232448, "shared memory budget of one CTA exceeded");
-  static_assert(kT * kPitch * 4 <= kSlots * kTileBytes, "the accumulator in the ring's place");
+  static constexpr int kStats = kKV + kT * kPitch * 4;      // and the rows' maxima and sums behind them, in the ring's place
+  static constexpr uint32_t kTmemCols = 512 / kPerSm, kColS = 0, kColO = 2 * kN;
+  // Registers per thread at launch, and once the warpgroups have rebalanced.
+  static constexpr int kRegsLaunch = D == 128 ? 168 : 80, kRegsSoftmax = D == 128 ? 208 : 88, kRegsHelper = D == 128 ? 88 : 64;
+  static_assert(kPerSm * (kBytes + 1024) <= 228 * 1024, "shared memory of an SM exceeded");
+  static_assert(kStats + kT * 8 <= kBars, "the accumulator in the ring's place");
+  static_assert(2 * (kN + D) <= kTmemCols, "tensor memory");
+  static_assert(2 * kGroup * kRegsSoftmax + 128 * kRegsHelper <= kThreads * kRegsLaunch,
+                "the warpgroups ask for more registers than the CTA owns");
+  static_assert(kPerSm * kThreads * kRegsLaunch <= 65536 && kPerSm * kThreads * (kRegsLaunch + 8) > 65536,
+                "kRegsLaunch is not what the compiler gives a CTA of this size");
 };
 
-constexpr int kMaxSlots = 10;
-static_assert(Plan<64>::kSlots <= kMaxSlots && Plan<128>::kSlots <= kMaxSlots, "barriers of the slots");
 struct Bars {
   __align__(16) uint4 stolen;             // answer to a request for another block
   uint64_t stolen_full;
   uint64_t item_ready[kItems], item_free[kItems];
-  uint64_t q_full[2], q_empty[2], slot_full[kMaxSlots], slot_empty[kMaxSlots];
-  uint64_t s_full[2], p_full[2][2], o_done[2], settled[2];   // [group]; p_full: [group][half of the keys]
+  uint64_t q_full[2], q_empty[2], slot_full[kSlots], slot_empty[kSlots];
+  uint64_t s_full[2], p_full[2][2], o_done[2], settled[2];   // [group]; p_full: [group][64 keys of a step]
   uint64_t joined, parted;                // groups that share a tile: results are there; have been read
   uint32_t tmem_base;
   int abort_flag;
@@ -88,11 +92,14 @@ struct Bars {
 static_assert(sizeof(Bars) <= 1024, "barrier block");
 
 struct ChunkParams {
+  int wide;     // rows of out begin at multiples of 32 bytes
+  int sorted;   // items do not all start at once
   bf16* out;
   float* lse;
   int64_t out_token, out_head;
   PagedCache cache;
   int T, max_new, heads_q, group, tile_tokens;   // tokens of a tile: 128 / group
+  int token_shift;                               // log2 of the tokens of two tiles, -1: not a power of two
   int chunk;                                     // rows of a K / V box
   float scale;
   int* status;
@@ -108,15 +115,38 @@ __device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
   return v;
 }
+// Two columns of a lane's
+__device__ __forceinline__ void tmem_st2(uint32_t taddr, uint32_t a, uint32_t b) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};" ::"r"(taddr), "r"(a), "r"(b) : "memory");
+}
+__device__ __forceinline__ void tmem_ld2(uint32_t taddr, float& a, float& b) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=f"(a), "=f"(b) : "r"(taddr) : "memory");
+}
 __device__ __forceinline__ int ld_cluster_int(uint32_t addr) {
   int v;
   asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
 
+// 16 floats to bf16, 32 bytes of a row: a thread has a row to itself, and a store costs the lines it touches.
+__device__ __forceinline__ void store_16(bf16* to, const float (&y)[16], bool wide) {
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = pack_bf16(y[2 * i], y[2 * i + 1]);
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(to)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(to)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+
 // A tile of a group, or what is left of one: its rows, and how many key tiles they see.
 struct Tile {
   int token0, rows, n;
+  bool half;   // of the last key tile only the first half is seen
 };
 struct Item {
   int b, token0, ahead, first, count, kv_head;
@@ -127,7 +157,9 @@ struct Item {
     t.token0 = token0 + at * p.tile_tokens;
     const int tokens = min(count - t.token0, p.tile_tokens);
     t.rows = tokens * p.group;
-    t.n = (ahead + t.token0 + tokens + kT - 1) / kT;
+    const int keys = ahead + t.token0 + tokens;
+    t.n = (keys + kT - 1) / kT;
+    t.half = keys % kT != 0 && keys % kT <= kT / 2;
     return t;
   }
 };
@@ -135,53 +167,107 @@ struct Item {
 struct Share {
   bool single;
   int lo, n_kv, n_first;
+  int half;   // the CTA's tile (of group x: bit x) of which only the first half is seen is its last one
   __device__ __forceinline__ int n(int x) const { return single ? (n_kv - x + 1) / 2 : x ? n_kv : n_first; }
   __device__ __forceinline__ int at(int x, int i) const { return single ? 2 * i + x : i; }
+  // steps of group x, `per_tile` to a tile but for a last half that nothing is seen of
+  __device__ __forceinline__ int steps(int x, int per_tile) const {
+    const int tiles = n(x);
+    const bool has_last = single ? tiles > 0 && at(x, tiles - 1) == n_kv - 1 : true;
+    return per_tile * tiles - (per_tile == 2 && has_last && (half >> x & 1) ? 1 : 0);
+  }
 };
 template <int CLUSTER>
 __device__ __forceinline__ Share share_of(const Item& it, const ChunkParams& p, int rank) {
   Share s;
   s.single = it.single<CLUSTER>(p);
-  const int n = it.tile(p, s.single ? 0 : 1).n;
+  const Tile last = it.tile(p, s.single ? 0 : 1);
+  const int n = last.n;
   s.lo = CLUSTER > 1 ? static_cast<int>(static_cast<int64_t>(n) * rank / CLUSTER) : 0;
   s.n_kv = (CLUSTER > 1 ? static_cast<int>(static_cast<int64_t>(n) * (rank + 1) / CLUSTER) : n) - s.lo;
-  s.n_first = s.single ? 0 : it.tile(p, 0).n;
+  s.n_first = 0;
+  s.half = last.half && s.lo + s.n_kv == n ? 3 : 0;
+  if (!s.single) {
+    const Tile first = it.tile(p, 0);
+    s.n_first = first.n;
+    s.half = (s.half & 2) | (first.half ? 1 : 0);
+  }
   return s;
 }
 
-// The item of index x, `tokens` tokens each, among those of all sequences; by one warp. b < 0: there is none. Sequences that
-// are refused have no items.
-__device__ __forceinline__ Item find_item(const ChunkParams& p, int x, int kv_head, int tokens) {
+// Block `block` is key head block % heads of an item (of `tokens` tokens) of this place in the order; by one warp. b < 0: there
+// is none. Sequences that are refused have no items. The order: of 32 sequences at a time the items with the most keys, so
+// that what starts last is short (one sequence after the other, each key head by itself: 16 prompts of up to 1024 tokens 46 us
+// instead of 36). An item's weight is twice its keys; one tile counts half, since both groups work on it. How many items of a
+// sequence reach a weight is an expression, so that the 64th of the range of weights in which the x-th falls is found by
+// halving, and the item in it by counting. (To the last bit of the weight the search took 1.6 us, 4-8 % of whole calls; this
+// one a third of that.) Where all items start at once (`sorted` false) the order does not matter.
+__device__ __forceinline__ Item find_item(const ChunkParams& p, unsigned block, int tokens, bool sorted) {
   const PagedCache& c = p.cache;
   const int lane = threadIdx.x % 32;
-  Item it = {-1, 0, 0, 0, 0, kv_head};
-  int64_t before = 0;   // items of the sequences so far
+  const int place = block / c.heads;
+  Item it = {-1, 0, 0, 0, 0, static_cast<int>(block - static_cast<unsigned>(place) * c.heads)};
+  int64_t x = place;
   for (int base = 0; base < c.B; base += 32) {
     int ahead = 0, first = 0, count = 0;
     if (base + lane < c.B && (!sequence_rows(c, base + lane, p.T, ahead, first, count) || count > p.max_new)) {
       atomicExch(p.status, DADATTN_E_ARG);
       count = 0;
     }
-    const int mine = (count + tokens - 1) / tokens;
-    int upto = mine;
+    const int mine = (count + tokens - 1) / tokens;   // items: the i-th of them from token i * tokens on
+    const int all = __reduce_add_sync(0xffffffffu, mine);
+    if (x >= all) {
+      x -= all;
+      continue;
+    }
+    int at, index;
+    if (!sorted) {
+      int upto = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int other = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += other;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += other;
+      }
+      at = __ffs(__ballot_sync(0xffffffffu, upto > x)) - 1;
+      index = __shfl_sync(0xffffffffu, upto, at) - 1 - static_cast<int>(x);
+    } else {
+      // (keys are 2^30 at most, DADATTN_MAX_CACHE_LEN: weights are unsigned)
+      const bool one = count - (mine - 1) * tokens <= tokens / 2;   // the last item is one tile
+      const unsigned keys = ahead + count, last = one ? keys : 2 * keys;
+      const unsigned most = __reduce_max_sync(0xffffffffu, mine ? 2 * keys : 0u);
+      const int unit = max(0, 26 - __clz(most));   // most < 64 << unit
+      // the first of the sequence's whole items that reaches so many units, behind which all do; the last one is its own
+      auto from = [&](unsigned units) -> int {
+        const int need = static_cast<int>((static_cast<uint64_t>(units) << unit) + 1 >> 1) - ahead;   // keys
+        const int i = need <= tokens ? 0 : (p.token_shift >= 0 ? (need + tokens - 1) >> p.token_shift : (need + tokens - 1) / tokens) - 1;
+        return min(i, max(mine - 1, 0));
+      };
+      auto last_reaches = [&](unsigned units) -> bool { return mine > 0 && last >> unit >= units; };
+      auto reach = [&](unsigned units) -> int { return max(mine - 1, 0) - from(units) + last_reaches(units); };
+      unsigned low = 0;   // the most units that more than x items reach
+#pragma unroll 1
+      for (unsigned step = 32; step; step >>= 1)
+        if (__reduce_add_sync(0xffffffffu, reach(low + step)) > x) low += step;
+      const int above = __reduce_add_sync(0xffffffffu, reach(low + 1)), here = from(low + 1);
+      const bool with_last = last_reaches(low) && !last_reaches(low + 1);
+      const int with = here - from(low) + with_last;   // the sequence's items of so many units
+      int upto = with;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += other;
+      }
+      const int rest = static_cast<int>(x) - above;
+      at = __ffs(__ballot_sync(0xffffffffu, upto > rest)) - 1;
+      const int nth = rest - (upto - with);   // of them: the last one, then the others from behind
+      index = __shfl_sync(0xffffffffu, with_last && nth == 0 ? mine - 1 : here - 1 - nth + with_last, at);
     }
-    const unsigned reached = __ballot_sync(0xffffffffu, before + upto > x);
-    if (reached) {
-      const int at = __ffs(reached) - 1;
-      // the last tokens first: their rows see the most keys
-      const int index = mine - 1 - static_cast<int>(x - before - (upto - mine));
-      it.b = base + at;
-      it.token0 = __shfl_sync(0xffffffffu, index, at) * tokens;
-      it.ahead = __shfl_sync(0xffffffffu, ahead, at);
-      it.first = __shfl_sync(0xffffffffu, first, at);
-      it.count = __shfl_sync(0xffffffffu, count, at);
-      return it;
-    }
-    before += __shfl_sync(0xffffffffu, upto, 31);
+    it.b = base + at;
+    it.token0 = index * tokens;
+    it.ahead = __shfl_sync(0xffffffffu, ahead, at);
+    it.first = __shfl_sync(0xffffffffu, first, at);
+    it.count = __shfl_sync(0xffffffffu, count, at);
+    return it;
   }
   return it;
 }
@@ -194,19 +280,18 @@ __device__ __forceinline__ void request_block(uint4* answer, uint64_t* bar) {
                ::"r"(smem_u32(answer)), "r"(smem_u32(bar))
                : "memory");
 }
-__device__ __forceinline__ bool read_answer(const uint4* answer, int& x, int& y) {
-  uint32_t ok, bx = 0, by = 0;
+__device__ __forceinline__ bool read_answer(const uint4* answer, unsigned& block) {
+  uint32_t ok;
   asm volatile(
       "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
-      "ld.shared.b128 h, [%3];\n\t"
+      "ld.shared.b128 h, [%2];\n\t"
       "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t"
-      "mov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\t"
-      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, _, _}, h;\n\t}"
-      : "=&r"(ok), "=&r"(bx), "=&r"(by)
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, _, _, _}, h;\n\t}"
+      : "=&r"(ok), "=&r"(block)
       : "r"(smem_u32(answer))
       : "memory");
-  x = bx, y = by;
   return ok != 0;
 }
 
@@ -222,7 +307,10 @@ struct Feed {
     it = Item{e[0], e[1], e[2], e[3], e[4], e[5]};
     return it.b >= 0;
   }
-  __device__ __forceinline__ void give_back() { mbar_arrive(&bars->item_free[n++ & (kItems - 1)]); }
+  __device__ __forceinline__ void give_back(bool arrives = true) {
+    if (arrives) mbar_arrive(&bars->item_free[n & (kItems - 1)]);
+    ++n;
+  }
 };
 
 // Which slot of the ring a tile's K (m = 0) or V is in, and the parity of that use. tile: of all that the CTA has gone through.
@@ -232,22 +320,21 @@ struct Slot {
   uint32_t parity;
   __device__ __forceinline__ Slot(int tile, int m) {
     const uint32_t i = 2u * tile + m;
-    at = i % Plan<D>::kSlots;
-    parity = (i / Plan<D>::kSlots) & 1;
+    at = i % kSlots;
+    parity = (i / kSlots) & 1;
   }
 };
 
 template <int D, int CLUSTER>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, Plan<D>::kPerSm)
 paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const ChunkParams p) {
   using L = Plan<D>;
-  constexpr int kSlots = L::kSlots;
-  // Tensor memory: the scores of group X at 128 X (its probabilities in the first 64 columns of them), O at 256 + D X.
-  constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256;
+  // Tensor memory: the scores of group X at kN X (its probabilities in the first half of these columns), O at kColO + D X.
+  constexpr int kN = L::kN, kSteps = L::kSteps;
+  constexpr uint32_t kTmemCols = L::kTmemCols, kColS = L::kColS, kColO = L::kColO;
   extern __shared__ __align__(1024) uint8_t smem[];
   Bars* bars = reinterpret_cast<Bars*>(smem + L::kBars);
-  float2* stats = reinterpret_cast<float2*>(smem + L::kStats);
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int rank = CLUSTER > 1 ? blockIdx.x % CLUSTER : 0;
@@ -261,7 +348,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     mbar_init(&bars->stolen_full, 1);
     for (int i = 0; i < kItems; ++i) {
       mbar_init(&bars->item_ready[i], 1);
-      mbar_init(&bars->item_free[i], 2 * kGroup + 3);   // softmax, issuers, Q
+      mbar_init(&bars->item_free[i], 8 + 3);            // softmax warps, issuers, Q
     }
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(&bars->slot_full[i], 1);
@@ -271,14 +358,14 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       mbar_init(&bars->q_full[x], 1);
       mbar_init(&bars->q_empty[x], 1);
       mbar_init(&bars->s_full[x], 1);
-      mbar_init(&bars->p_full[x][0], kGroup);
-      mbar_init(&bars->p_full[x][1], kGroup);
+      mbar_init(&bars->p_full[x][0], 4);                // one arrival per warp
+      mbar_init(&bars->p_full[x][1], 4);
       mbar_init(&bars->o_done[x], 1);
       mbar_init(&bars->settled[x], 1);
       for (int w = 0; w < 4; ++w) bars->exps[x][w] = 0;
     }
-    mbar_init(&bars->joined, 2 * kGroup);
-    mbar_init(&bars->parted, 2 * kGroup);
+    mbar_init(&bars->joined, 8);
+    mbar_init(&bars->parted, 8);
     bars->abort_flag = 0;
     bars->any_bad = 0;
     fence_mbar_init();
@@ -297,10 +384,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   Feed feed{bars, abort_flag, 0};
   Item it;
   if (warp < 4) {
-    setmaxnreg_dec<kRegsHelper>();
+    setmaxnreg_dec<L::kRegsHelper>();
     if (warp == 0) {
       // ------------------------------ scheduler + K / V producer ------------------------------
       const int item_tokens = (CLUSTER > 1 ? 1 : 2) * p.tile_tokens;
+      const bool sorted = CLUSTER == 1 && p.sorted;
       const int per_tile = kT / p.chunk;   // boxes
       const int box = lane % per_tile, panel = lane / per_tile;
       int n_pub = 0, n_asked = 0, n_loaded = 0, slot = 0;
@@ -316,20 +404,20 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         ++n_asked;
       };
       // the next block's item; b < 0 and `more` false: nothing left
-      auto answer = [&](bool& more) {
-        int x, y;
+      auto answer = [&](Item& it, bool& more) {
+        unsigned block;
         ok = warp_wait(&bars->stolen_full, (n_asked - 1) & 1, abort_flag);
-        more = ok && read_answer(&bars->stolen, x, y);
+        more = ok && read_answer(&bars->stolen, block);
         __syncwarp();
-        if (more) it = find_item(p, x, y, item_tokens);
+        if (more) it = find_item(p, block, item_tokens, sorted);
         else it.b = -1;
       };
-      it = find_item(p, blockIdx.x / CLUSTER, blockIdx.y, item_tokens);
+      it = find_item(p, blockIdx.x / CLUSTER, item_tokens, sorted);
       bool more = CLUSTER == 1;
       while (ok) {
         while (ok && it.b < 0 && more) {
           ask();
-          answer(more);
+          answer(it, more);
         }
         if (!ok) break;
         const int e = n_pub & (kItems - 1);
@@ -377,7 +465,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             if (++slot == kSlots) slot = 0, parity ^= 1u;
           }
         }
-        if (CLUSTER == 1 && ok) answer(more);
+        if (CLUSTER == 1 && ok) answer(it, more);
         else it.b = -1;
       }
       if (lane == 0) {
@@ -412,14 +500,14 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       // ------------------------------ MMA issuers ------------------------------
       const int x = warp - 1;
       if (elect_one()) {
-        constexpr uint32_t idesc_s = make_idesc_bf16(kT, kT, 0, 0);   // Q, K: K-major
+        constexpr uint32_t idesc_s = make_idesc_bf16(kT, kN, 0, 0);   // Q, K: K-major
         constexpr uint32_t idesc_o = make_idesc_bf16(kT, D, 0, 1);    // P K-major, V MN-major
         const SmemDescBase q_desc = make_desc_base_sw128(smem_u32(smem + L::kQ) + x * L::kTileBytes, 0);
         // (read MN-major, a V tile's two 64-column panels are kPanel apart; K-major operands ignore that offset)
         const SmemDescBase kv_desc0 = make_desc_base_sw128(smem_u32(smem + L::kKV), kPanel);
-        const uint32_t tS = tmem + kColS + x * 128, tO = tmem + kColO + x * D;
-        uint32_t g = 0, u = 0;   // key tiles and items of this group so far
-        int gone = 0;            // key tiles of the CTA so far
+        const uint32_t tS = tmem + kColS + x * kN, tO = tmem + kColO + x * D;
+        uint32_t g = 0, u = 0, joins = 0;   // steps, items and shared tiles of this group so far
+        int gone = 0;                       // key tiles of the CTA so far
         bool ok = true;
         auto wait_slot = [&](const Slot<D>& s) -> bool { return mbar_wait(&bars->slot_full[s.at], s.parity, abort_flag); };
         // a tile that this group has nothing to do with: given back once it is there, as the others are
@@ -432,50 +520,57 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
           }
           return true;
         };
-        auto issue_s = [&](int tile, bool last) -> bool {
-          const Slot<D> s(tile, 0);
-          if (!wait_slot(s)) return false;
-          tc_fence_after_sync();
-          const SmemDescBase k_desc{kv_desc0.lo + s.at * (L::kTileBytes >> 4), kv_desc0.hi};
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk / 4) * kPanel + (kk % 4) * 32;
-            mma_ss(tS, desc_at(q_desc, off), desc_at(k_desc, off), idesc_s, kk > 0 ? 1u : 0u);
-          }
-          mma_commit(&bars->slot_empty[s.at]);
-          if (last) mma_commit(&bars->q_empty[x]);
-          mma_commit(&bars->s_full[x]);
-          return true;
-        };
         while (ok && feed.next(it)) {
           const Share s = share_of<CLUSTER>(it, p, rank);
-          const int n = s.n(x);
-          if (s.single && x == 1 && s.n_kv > 0) ok = skip(gone);
-          if (ok && n > 0) ok = mbar_wait(&bars->q_full[x], u++ & 1, abort_flag) && issue_s(gone + s.at(x, 0), n == 1);
-          for (int i = 0; ok && i < n; ++i, ++g) {
-            const int at = s.at(x, i);
-            // (the other's next tile, ahead of the wait for the probabilities: its slots are not to wait for those)
-            if (s.single && at + 1 < s.n_kv && !(ok = skip(gone + at + 1))) break;
-            const Slot<D> v(gone + at, 1);
-            if (!(ok = wait_slot(v))) break;
-            // (a new item's first P V may overwrite O: its probabilities come after the last results have been read)
-            const SmemDescBase v_desc{kv_desc0.lo + v.at * (L::kTileBytes >> 4), kv_desc0.hi};
+          const int steps = s.steps(x, kSteps);
+          // Scores of the k-th step: part k % kSteps of the group's k / kSteps-th tile
+          auto issue_s = [&](int k) -> bool {
+            const int at = s.at(x, k / kSteps), h = k % kSteps;
+            const Slot<D> slot(gone + at, 0);
+            if (h == 0 && !wait_slot(slot)) return false;
+            tc_fence_after_sync();
+            const SmemDescBase k_desc{kv_desc0.lo + slot.at * (L::kTileBytes >> 4) + h * (kN * 128 >> 4), kv_desc0.hi};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {   // O (+)= P[:, 64 h .. 64 h + 63] V[64 h .. 64 h + 63, :]
-              if (!(ok = mbar_wait(&bars->p_full[x][h], g & 1, abort_flag))) break;
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = (kk / 4) * kPanel + (kk % 4) * 32;
+              mma_ss(tS, desc_at(q_desc, off), desc_at(k_desc, off), idesc_s, kk > 0 ? 1u : 0u);
+            }
+            const bool last = k + 1 == steps, through = h == kSteps - 1 || last;
+            if (through) mma_commit(&bars->slot_empty[slot.at]);
+            if (last) mma_commit(&bars->q_empty[x]);
+            mma_commit(&bars->s_full[x]);
+            // (the other's next tile, ahead of the wait for these probabilities: its slots are not to wait for those)
+            if (s.single && through && at + 1 < s.n_kv) return skip(gone + at + 1);
+            return true;
+          };
+          if (s.single && x == 1 && s.n_kv > 0) ok = skip(gone);
+          if (ok && steps > 0) ok = mbar_wait(&bars->q_full[x], u++ & 1, abort_flag) && issue_s(0);
+          for (int k = 0; ok && k < steps; ++k, ++g) {
+            const int h = k % kSteps;
+            const Slot<D> v(gone + s.at(x, k / kSteps), 1);
+            if (h == 0 && !(ok = wait_slot(v))) break;
+            // O (+)= P V, 64 keys at a time. (A new item's first may overwrite O: its probabilities come after the last results
+            // have been read.)
+            const SmemDescBase v_desc{kv_desc0.lo + v.at * (L::kTileBytes >> 4) + h * (kN * 128 >> 4), kv_desc0.hi};
+#pragma unroll
+            for (int part = 0; part < kN / 64; ++part) {
+              if (!(ok = mbar_wait(&bars->p_full[x][part], g & 1, abort_flag))) break;
               tc_fence_after_sync();
 #pragma unroll
-              for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
-                mma_ts(tO, tS + kk * 8, desc_at(v_desc, kk * 2048), idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
+              for (int kk = 4 * part; kk < 4 * part + 4; ++kk)
+                mma_ts(tO, tS + kk * 8, desc_at(v_desc, kk * 2048), idesc_o, (k > 0 || kk > 0) ? 1u : 0u);
             }
             if (!ok) break;
-            mma_commit(&bars->slot_empty[v.at]);
-            if (i + 1 < n) ok = issue_s(gone + s.at(x, i + 1), i + 2 == n);   // over the probabilities, whose product is ahead in the pipe
-            else mma_commit(&bars->o_done[x]);
+            const bool last = k + 1 == steps;
+            if (h == kSteps - 1 || last) mma_commit(&bars->slot_empty[v.at]);
+            if (last) mma_commit(&bars->o_done[x]);
+            else ok = issue_s(k + 1);   // over the probabilities, whose product is ahead in the pipe
           }
           // tiles that only the pair's other group sees
           if (!s.single)
-            for (int j = n; ok && j < s.n_kv; ++j) ok = skip(gone + j);
+            for (int j = s.n(x); ok && j < s.n_kv; ++j) ok = skip(gone + j);
+          // (the groups' maxima and sums change hands where the next item's scores go)
+          if (s.single && CLUSTER == 1) ok = ok && mbar_wait(&bars->parted, joins++ & 1, abort_flag);
           gone += s.n_kv;
           feed.give_back();
         }
@@ -484,72 +579,91 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     }
   } else {
     // ------------------------------ softmax ------------------------------
-    setmaxnreg_inc<kRegsSoftmax>();
+    setmaxnreg_inc<L::kRegsSoftmax>();
     const int x = warp / 4 - 1;
     const int quad = warp % 4;            // TMEM lane quadrant of this warp
     const int row = quad * 32 + lane;     // row within the tile = TMEM lane
     const uint32_t tlane = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    const uint32_t tS = tlane + kColS + x * 128, tO = tlane + kColO + x * D;
+    const uint32_t tS = tlane + kColS + x * kN, tO = tlane + kColO + x * D;
     const float scale_log2 = p.scale * kLog2e;
-    uint32_t g = 0, u = 0, joins = 0;     // key tiles, items with any and shared tiles of this group so far
-    int gone = 0, others = 0;             // key tiles of the CTA and of the other group so far
+    uint32_t g = 0, u = 0, joins = 0;     // steps, items with any and shared tiles of this group so far
+    int gone = 0, others = 0;             // key tiles of the CTA and steps of the other group so far
     bool ok = true;
     while (ok && feed.next(it)) {
       const Share s = share_of<CLUSTER>(it, p, rank);
       const Tile t = it.tile(p, s.single ? 0 : x);
-      const int n = s.n(x), total = it.ahead + it.count;
+      const int steps = s.steps(x, kSteps), total = it.ahead + it.count;
       const bool active = quad * 32 < t.rows;          // whether the warp has a row
       const int token = t.token0 + min(row, t.rows - 1) / p.group, limit = it.ahead + token;   // (rows that are not there: the last one's mask)
       float m = -INFINITY, l = 0.f;   // running max (log2 units, scaled) and sum
-      for (int i = 0; i < n; ++i, ++g) {
+      for (int k = 0; k < steps; ++k, ++g) {
         if (!(ok = mbar_wait(&bars->s_full[x], g & 1, abort_flag))) break;
         tc_fence_after_sync();
-        const int key0 = (s.lo + s.at(x, i)) * kT;
-        uint32_t sc[4][32];
-        if (active) {
+        const int tile = s.at(x, k / kSteps), key0 = (s.lo + tile) * kT;
+        const int seen = limit - key0 - (k % kSteps) * kN;   // the last column that the row sees
+        const bool masked = __any_sync(0xffffffffu, seen < kN - 1);
+        // 32 of the thread's scores
+        auto load = [&](uint32_t (&sc)[32], int q) { tmem_ld32(tS + q * 32, sc); };
+        auto mask = [&](uint32_t (&sc)[32], int q) {
+          if (!masked) return;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) tmem_ld32(tS + q * 32, sc[q]);
-          tmem_wait_ld();
-          const int seen = limit - key0;   // the last column that the row sees
-          if (__any_sync(0xffffffffu, seen < kT - 1)) {
+          for (int e = 0; e < 32; ++e)
+            if (q * 32 + e > seen) sc[e] = 0xff800000u;  // -inf
+        };
+        // max of the raw scores (scale > 0 commutes with max)
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto max_of = [&](const uint32_t (&sc)[32]) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (q * 32 + e > seen) sc[q][e] = 0xff800000u;  // -inf
-          }
-          // max of the raw scores (scale > 0 commutes with max)
-          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int q = 0; q < 4; q += 2)
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              mx4[e & 3] = fmax3(mx4[e & 3], __uint_as_float(sc[q][e]), __uint_as_float(sc[q + 1][e]));
+          for (int e = 0; e < 32; e += 2)
+            mx4[(e >> 1) & 3] = fmax3(mx4[(e >> 1) & 3], __uint_as_float(sc[e]), __uint_as_float(sc[e + 1]));
+        };
+        // The step's maximum, and the accumulator to it where it has grown; false: a wait ran out.
+        auto new_max = [&] {
           const float mx = __fmul_rn(fmaxf(fmax3(mx4[0], mx4[1], mx4[2]), mx4[3]), scale_log2);
-          if (i == 0) {
+          if (k == 0) {
             m = mx;  // O is first written by a product that does not accumulate: nothing to rescale
           } else if (__any_sync(0xffffffffu, row < t.rows && mx > m + kRescaleAt)) {   // (nobody else's rows decide)
-            // (P V of the tile before is through: these scores were issued behind it)
+            // (P V of the step before is through: these scores were issued behind it)
             const float m_new = fmaxf(m, mx);
             // m = -inf: nothing but zeros has been accumulated so far
             const float corr = (m == -INFINITY) ? 0.f : ex2(m - m_new);
 #pragma unroll 1
-            for (int q = 0; q < D / 32; ++q) {
-              uint32_t o[32];
-              tmem_ld32(tO + q * 32, o);
+            for (int q = 0; q < D / 16; ++q) {
+              uint32_t o[16];
+              tmem_ld16(tO + q * 16, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-              tmem_st32(tO + q * 32, o);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+              tmem_st16(tO + q * 16, o);
             }
             tmem_wait_st();
             l = __fmul_rn(l, corr);
             m = m_new;
           }
-        }
-        if (total - key0 < kT) {
+        };
+        // p = exp2(s scale log2e - m). A row whose scores are all -inf so far must give p = 0, not exp2(NaN).
+        float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        auto weights = [&](const uint32_t (&sc)[32], uint32_t (&pk)[16]) {   // bf16 pairs (k, k + 1) per column
+          const float2 sl = make_float2(scale_log2, scale_log2);
+          const float neg_m = (m == -INFINITY) ? 0.f : -m;
+          const float2 nm = make_float2(neg_m, neg_m);
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float2 y = ffma2(make_float2(__uint_as_float(sc[e]), __uint_as_float(sc[e + 1])), sl, nm);
+            const float2 w = make_float2(ex2(y.x), ex2(y.y));
+            sum2[(e >> 1) & 1] = fadd2(sum2[(e >> 1) & 1], w);
+            pk[e / 2] = pack_bf16(w.x, w.y);
+          }
+        };
+        auto hand_over = [&](int part) {
+          if (active) tmem_wait_st();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->p_full[x][part]);
+        };
+        if (k % kSteps == 0 && total - key0 < kT) {
           // The sequence ends in this tile: V of the rows behind it.
-          const Slot<D> v(gone + s.at(x, i), 1);
+          const Slot<D> v(gone + tile, 1);
           const int there = total - key0;
           if (!(ok = mbar_wait(&bars->slot_full[v.at], v.parity, abort_flag))) break;
           uint8_t* rows = smem + L::kKV + v.at * L::kTileBytes;
@@ -559,40 +673,60 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
           }
           fence_proxy_async_smem();
         }
-        // A's turn is behind B's tile before, B's behind A's tile of the same place.
-        {
-          const int due = x == 0 ? min(i, s.n(1)) : min(i + 1, s.n(0));
-          const volatile int* done = &bars->exps[1 - x][quad];
-          for (int k = 0; k < 256 && *done < others + due; ++k) {}
-        }
-        // p = exp2(s scale log2e - m). A row whose scores are all -inf so far must give p = 0, not exp2(NaN).
-        float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        const float2 sl = make_float2(scale_log2, scale_log2);
-        const float neg_m = (m == -INFINITY) ? 0.f : -m;
-        const float2 nm = make_float2(neg_m, neg_m);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        if (D == 128) {
+          uint32_t sc[4][32];
           if (active) {
-            uint32_t pk[16];   // bf16 pairs (k, k + 1) per column
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float2 y = ffma2(make_float2(__uint_as_float(sc[q][e]), __uint_as_float(sc[q][e + 1])), sl, nm);
-              const float2 w = make_float2(ex2(y.x), ex2(y.y));
-              sum2[(e >> 1) & 1] = fadd2(sum2[(e >> 1) & 1], w);
-              pk[e / 2] = pack_bf16(w.x, w.y);
-            }
-            tmem_st16(tS + q * 16, pk);
+            for (int q = 0; q < 4; ++q) load(sc[q], q);
+            tmem_wait_ld();
+#pragma unroll
+            for (int q = 0; q < 4; ++q) mask(sc[q], q);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) max_of(sc[q]);
+            new_max();
           }
-          if (q & 1) {
-            if (active) tmem_wait_st();
-            tc_fence_before_sync();
-            mbar_arrive(&bars->p_full[x][q / 2]);
+          // A's turn is behind B's step before, B's behind A's of the same place.
+          {
+            const int due = x == 0 ? min(k, s.steps(1, kSteps)) : min(k + 1, s.steps(0, kSteps));
+            const volatile int* done = &bars->exps[1 - x][quad];
+            for (int i = 0; i < 256 && *done < others + due; ++i) {}
           }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t pk[16];
+            if (active) weights(sc[q], pk);
+            // (the first half's stores are through by now; waited for where they are issued they cost 4 %)
+            if (q == 2) hand_over(0);
+            if (active) tmem_st16(tS + q * 16, pk);
+          }
+          if (lane == 0) *const_cast<volatile int*>(&bars->exps[x][quad]) = static_cast<int>(g) + 1;
+          hand_over(1);
+        } else {
+          if (active) {
+            // (the probabilities go over the scores; 88 registers hold half of these, so the first half is read twice)
+            uint32_t sc[32], first[16], second[16];
+            load(sc, 0);
+            tmem_wait_ld();
+            mask(sc, 0);
+            max_of(sc);
+            load(sc, 1);
+            tmem_wait_ld();
+            mask(sc, 1);
+            max_of(sc);
+            new_max();
+            weights(sc, second);
+            load(sc, 0);
+            tmem_wait_ld();
+            mask(sc, 0);
+            tmem_st16(tS + 16, second);
+            weights(sc, first);
+            tmem_st16(tS, first);
+          }
+          hand_over(0);
         }
-        if (lane == 0) *const_cast<volatile int*>(&bars->exps[x][quad]) = static_cast<int>(g) + 1;
         l += (sum2[0].x + sum2[1].x) + (sum2[0].y + sum2[1].y);
       }
-      if (ok && n > 0) ok = mbar_wait(&bars->o_done[x], u++ & 1, abort_flag);
+      if (ok && steps > 0) ok = mbar_wait(&bars->o_done[x], u++ & 1, abort_flag);
       if (!ok) break;
       tc_fence_after_sync();
       const int64_t to_token = it.first + token;
@@ -611,65 +745,69 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             tmem_wait_ld();
             if (write) {
 #pragma unroll
-              for (int e = 0; e < 32; e += 8) {
-                float y[8];
+              for (int e = 0; e < 32; e += 16) {
+                float y[16];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) y[k] = __uint_as_float(o[e + k]) * f;
-                *reinterpret_cast<uint4*>(to + q * 32 + e) =
-                    make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+                for (int i = 0; i < 16; ++i) y[i] = __uint_as_float(o[e + i]) * f;
+                store_16(to + q * 32 + e, y, p.wide);
               }
             }
           }
         }
         if (write && p.lse) p.lse[to_token * p.heads_q + to_head] = (m + log2f(l)) * kLn2;
       } else {
-        // The other group has the rest of the row's keys: each group joins one half of the columns.
-        stats[x * 128 + row] = make_float2(m, l);
+        // The other group has the rest of the row's keys: each group joins one half of the columns. The rows' maxima and sums
+        // change hands in the first columns of the scores.
+        tmem_st2(tS, __float_as_uint(m), __float_as_uint(l));
+        tmem_wait_st();
         tc_fence_before_sync();
-        mbar_arrive(&bars->joined);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->joined);
         if (!(ok = mbar_wait(&bars->joined, joins & 1, abort_flag))) break;
         tc_fence_after_sync();
-        const float2 other = stats[(1 - x) * 128 + row];
-        const float m_all = fmaxf(m, other.x);
+        float m1, l1;
+        tmem_ld2(tlane + kColS + (1 - x) * kN, m1, l1);
+        tmem_wait_ld();
+        const float m_all = fmaxf(m, m1);
         // (a part that has seen nothing has nothing but garbage)
-        const float f0 = m == -INFINITY ? 0.f : ex2(m - m_all), f1 = other.x == -INFINITY ? 0.f : ex2(other.x - m_all);
-        const float l_all = l * f0 + other.y * f1;
+        const float f0 = m == -INFINITY ? 0.f : ex2(m - m_all), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - m_all);
+        const float l_all = l * f0 + l1 * f1;
         const float norm = CLUSTER == 1 ? 1.0f / l_all : 1.0f;
         float* acc = reinterpret_cast<float*>(smem + L::kKV) + row * L::kPitch;
         if (active) {
 #pragma unroll
-          for (int q = x * (D / 64); q < (x + 1) * (D / 64); ++q) {
-            uint32_t o[32], o1[32];
-            tmem_ld32(tO + q * 32, o);
-            tmem_ld32(tlane + kColO + (1 - x) * D + q * 32, o1);
+          for (int q = x * (D / 32); q < (x + 1) * (D / 32); ++q) {
+            uint32_t o[16], o1[16];
+            tmem_ld16(tO + q * 16, o);
+            tmem_ld16(tlane + kColO + (1 - x) * D + q * 16, o1);
             tmem_wait_ld();
+            float y[16];
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              float y[8];
+            for (int i = 0; i < 16; ++i) {
+              const float a = f0 == 0.f ? 0.f : __uint_as_float(o[i]) * f0;
+              y[i] = (f1 == 0.f ? a : fmaf(__uint_as_float(o1[i]), f1, a)) * norm;
+            }
+            if (CLUSTER > 1) {
 #pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                const float a = f0 == 0.f ? 0.f : __uint_as_float(o[e + k]) * f0;
-                y[k] = (f1 == 0.f ? a : fmaf(__uint_as_float(o1[e + k]), f1, a)) * norm;
-              }
-              if (CLUSTER > 1) {
-                *reinterpret_cast<float4*>(acc + q * 32 + e) = make_float4(y[0], y[1], y[2], y[3]);
-                *reinterpret_cast<float4*>(acc + q * 32 + e + 4) = make_float4(y[4], y[5], y[6], y[7]);
-              } else if (write) {
-                *reinterpret_cast<uint4*>(to + q * 32 + e) =
-                    make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
-              }
+              for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<float4*>(acc + q * 16 + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+            } else if (write) {
+              store_16(to + q * 16, y, p.wide);
             }
           }
         }
         if (CLUSTER == 1 && x == 0 && write && p.lse) p.lse[to_token * p.heads_q + to_head] = (m_all + log2f(l_all)) * kLn2;
+        if (CLUSTER > 1 && x == 0) reinterpret_cast<float2*>(smem + L::kStats)[row] = make_float2(m_all, l_all);
         tc_fence_before_sync();
-        mbar_arrive(&bars->parted);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->parted);
         if (!(ok = mbar_wait(&bars->parted, joins++ & 1, abort_flag))) break;
-        if (CLUSTER > 1 && x == 0) stats[row] = make_float2(m_all, l_all);
+        tc_fence_after_sync();
       }
       gone += s.n_kv;
-      others += s.n(1 - x);
-      feed.give_back();
+      others += s.steps(1 - x, kSteps);
+      __syncwarp();
+      feed.give_back(lane == 0);
     }
   }
 
@@ -699,7 +837,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       float2 ml[CLUSTER];
       float m_all = -INFINITY, l_all = 0.f, y[8] = {};
 #pragma unroll
-      for (int r = 0; r < CLUSTER; ++r) ml[r] = ld_cluster2(cluster_address(&stats[row], r));
+      for (int r = 0; r < CLUSTER; ++r) ml[r] = ld_cluster2(cluster_address(smem + L::kStats + row * 8, r));
 #pragma unroll
       for (int r = 0; r < CLUSTER; ++r) m_all = fmaxf(m_all, ml[r].x);
 #pragma unroll
@@ -735,14 +873,15 @@ struct Maps {
 };
 
 template <int D, int CLUSTER>
-int launch_chunk(const Maps& maps, const ChunkParams& p, long long items, cudaStream_t st) {
+int launch_chunk(const Maps& maps, ChunkParams p, long long items, cudaStream_t st) {
   using L = Plan<D>;
+  p.sorted = items * p.cache.heads > static_cast<long long>(current_sm_count()) * L::kPerSm;
   auto kern = paged_attention_kernel<D, CLUSTER>;
   DAD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
   static std::atomic<int> regs_seen;
-  if (int rc = check_launch_registers(reinterpret_cast<const void*>(kern), kRegsLaunch, regs_seen)) return rc;
+  if (int rc = check_launch_registers(reinterpret_cast<const void*>(kern), L::kRegsLaunch, regs_seen)) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(items * CLUSTER), static_cast<unsigned>(p.cache.heads));
+  cfg.gridDim = dim3(static_cast<unsigned>(items * p.cache.heads * CLUSTER));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = L::kBytes;
   cfg.stream = st;
@@ -793,7 +932,6 @@ extern "C" int dadattn_paged_attention_bf16(uint16_t* out, float* lse, const uin
   if (!starts && T != B) return fail(DADATTN_E_ARG, "%s: without starts T=%d is B=%d", name, T, B);
   if (Hq <= 0 || Hq % Hkv) return fail(DADATTN_E_ARG, "%s: Hq=%d must be a multiple of Hkv=%d", name, Hq, Hkv);
   if (Hq / Hkv > kT) return fail(DADATTN_E_UNSUPPORTED, "%s: %d query heads share a key head, more than %d", name, Hq / Hkv, kT);
-  if (Hkv > 65535) return fail(DADATTN_E_UNSUPPORTED, "%s: Hkv=%d exceeds 65535", name, Hkv);
   if (!(scale > 0.0f && scale < INFINITY)) return fail(DADATTN_E_ARG, "%s: scale must be positive and finite", name);
   if (int rc = check_packed(name, out, out_strides, 8, true, T, Hq)) return rc;
   if (int rc = check_packed(name, q, q_strides, 8, false, T, Hq)) return rc;
@@ -804,12 +942,14 @@ extern "C" int dadattn_paged_attention_bf16(uint16_t* out, float* lse, const uin
   p.out = reinterpret_cast<bf16*>(out), p.lse = lse;
   p.out_token = out_strides[0], p.out_head = out_strides[1];
   p.cache = PagedCache{page_table, lengths, starts, B, pages, log2_of(page_size), max_pages, Hkv};
+  p.wide = aligned(out, 32) && out_strides[0] % 16 == 0 && out_strides[1] % 16 == 0;
   p.T = T, p.max_new = max_new, p.heads_q = Hq, p.group = Hq / Hkv, p.tile_tokens = kT / p.group;
   p.chunk = page_size < kT ? page_size : kT;
+  p.token_shift = (p.tile_tokens & (p.tile_tokens - 1)) ? -1 : log2_of(2 * p.tile_tokens);
   p.scale = scale;
   if (max_new > T) max_new = T;   // (bounds the items)
-  if ((static_cast<long long>(T) / p.tile_tokens + B) * kMaxCluster > 0x7fffffffll)
-    return fail(DADATTN_E_UNSUPPORTED, "%s: T=%d and B=%d are too many", name, T, B);
+  if ((static_cast<long long>(T) / p.tile_tokens + B) * kMaxCluster > 0x7fffffffll / Hkv)
+    return fail(DADATTN_E_UNSUPPORTED, "%s: T=%d, B=%d and Hkv=%d are too many", name, T, B, Hkv);
   p.status = device_status_word();
   if (!p.status) return DADATTN_E_CUDA;
   const int rows = pages * Hkv * page_size;

@@ -73,7 +73,7 @@ BAD += [(_attention, c, rc) for c, rc in [
     (dict(out=None), -1), (dict(q=None), -1), (dict(T=0), -1), (dict(max_new=0), -1), (dict(starts=None), -1), (dict(Hq=6), -1),
     (dict(Hq=0), -1), (dict(Hq=4 * 129), -2), (dict(scale=0.0), -1), (dict(scale=-1.0), -1), (dict(scale=NAN), -1),
     (dict(scale=INF), -1), (dict(out=P + 8), -1), (dict(lse=P + 2), -1), (dict(os=_strides(0, 64)), -1), (dict(qs=_strides(0, 64)), -1),
-    (dict(qs=_strides(512, 0)), -1), (dict(qs=_strides(512, 4)), -1), (dict(T=1 << 30, B=1 << 29), -2), (dict(Hkv=65536, Hq=65536), -2)]]
+    (dict(qs=_strides(512, 0)), -1), (dict(qs=_strides(512, 4)), -1), (dict(T=1 << 30, B=1 << 29), -2), (dict(T=1 << 26, Hkv=1024, Hq=1024), -2)]]
 BAD += [(_decode, c, rc) for c, rc in [
     (dict(out=None), -1), (dict(v_new=None), -1), (dict(Hq=6), -1), (dict(scale=0.0), -1), (dict(scale=NAN), -1), (dict(rot=24), -2),
     (dict(freq=None), -1), (dict(lse=P + 1), -1), (dict(q=P + 4), -1), (dict(os=_strides(512, 0)), -1), (dict(B=1 << 27), -2)]]
