@@ -28,6 +28,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cmath>
 
 #include "decode_common.cuh"
 #include "paged.cuh"
@@ -99,7 +100,7 @@ struct ChunkParams {
   int64_t out_token, out_head;
   PagedCache cache;
   int T, max_new, heads_q, group, tile_tokens;   // tokens of a tile: 128 / group
-  int token_shift;                               // log2 of the tokens of two tiles, -1: not a power of two
+  int item_tokens, token_shift;                  // of an item, two tiles or one; their log2, -1: not a power of two
   int chunk;                                     // rows of a K / V box
   float scale;
   int* status;
@@ -150,8 +151,9 @@ struct Tile {
 };
 struct Item {
   int b, token0, ahead, first, count, kv_head;
-  template <int CLUSTER>
-  __device__ __forceinline__ bool single(const ChunkParams& p) const { return CLUSTER > 1 || token0 + p.tile_tokens >= count; }
+  __device__ __forceinline__ bool single(const ChunkParams& p) const {
+    return p.item_tokens == p.tile_tokens || token0 + p.tile_tokens >= count;
+  }
   __device__ __forceinline__ Tile tile(const ChunkParams& p, int at) const {   // at: 0, or 1 for the second of a pair
     Tile t;
     t.token0 = token0 + at * p.tile_tokens;
@@ -180,7 +182,7 @@ struct Share {
 template <int CLUSTER>
 __device__ __forceinline__ Share share_of(const Item& it, const ChunkParams& p, int rank) {
   Share s;
-  s.single = it.single<CLUSTER>(p);
+  s.single = CLUSTER > 1 || it.single(p);
   const Tile last = it.tile(p, s.single ? 0 : 1);
   const int n = last.n;
   s.lo = CLUSTER > 1 ? static_cast<int>(static_cast<int64_t>(n) * rank / CLUSTER) : 0;
@@ -195,16 +197,16 @@ __device__ __forceinline__ Share share_of(const Item& it, const ChunkParams& p, 
   return s;
 }
 
-// Block `block` is key head block % heads of an item (of `tokens` tokens) of this place in the order; by one warp. b < 0: there
+// Block `block` is key head block % heads of the item of place block / heads in the order; by one warp. b < 0: there
 // is none. Sequences that are refused have no items. The order: of 32 sequences at a time the items with the most keys, so
 // that what starts last is short (one sequence after the other, each key head by itself: 16 prompts of up to 1024 tokens 46 us
 // instead of 36). An item's weight is twice its keys; one tile counts half, since both groups work on it. How many items of a
 // sequence reach a weight is an expression, so that the 64th of the range of weights in which the x-th falls is found by
 // halving, and the item in it by counting. (To the last bit of the weight the search took 1.6 us, 4-8 % of whole calls; this
 // one a third of that.) Where all items start at once (`sorted` false) the order does not matter.
-__device__ __forceinline__ Item find_item(const ChunkParams& p, unsigned block, int tokens, bool sorted) {
+__device__ __forceinline__ Item find_item(const ChunkParams& p, unsigned block, bool sorted) {
   const PagedCache& c = p.cache;
-  const int lane = threadIdx.x % 32;
+  const int lane = threadIdx.x % 32, tokens = p.item_tokens;
   const int place = block / c.heads;
   Item it = {-1, 0, 0, 0, 0, static_cast<int>(block - static_cast<unsigned>(place) * c.heads)};
   int64_t x = place;
@@ -232,7 +234,7 @@ __device__ __forceinline__ Item find_item(const ChunkParams& p, unsigned block, 
       index = __shfl_sync(0xffffffffu, upto, at) - 1 - static_cast<int>(x);
     } else {
       // (keys are 2^30 at most, DADATTN_MAX_CACHE_LEN: weights are unsigned)
-      const bool one = count - (mine - 1) * tokens <= tokens / 2;   // the last item is one tile
+      const bool one = count - (mine - 1) * tokens <= p.tile_tokens && tokens > p.tile_tokens;   // the last item is one tile
       const unsigned keys = ahead + count, last = one ? keys : 2 * keys;
       const unsigned most = __reduce_max_sync(0xffffffffu, mine ? 2 * keys : 0u);
       const int unit = max(0, 26 - __clz(most));   // most < 64 << unit
@@ -387,7 +389,6 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     setmaxnreg_dec<L::kRegsHelper>();
     if (warp == 0) {
       // ------------------------------ scheduler + K / V producer ------------------------------
-      const int item_tokens = (CLUSTER > 1 ? 1 : 2) * p.tile_tokens;
       const bool sorted = CLUSTER == 1 && p.sorted;
       const int per_tile = kT / p.chunk;   // boxes
       const int box = lane % per_tile, panel = lane / per_tile;
@@ -409,10 +410,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         ok = warp_wait(&bars->stolen_full, (n_asked - 1) & 1, abort_flag);
         more = ok && read_answer(&bars->stolen, block);
         __syncwarp();
-        if (more) it = find_item(p, block, item_tokens, sorted);
+        if (more) it = find_item(p, block, sorted);
         else it.b = -1;
       };
-      it = find_item(p, blockIdx.x / CLUSTER, item_tokens, sorted);
+      it = find_item(p, blockIdx.x / CLUSTER, sorted);
       bool more = CLUSTER == 1;
       while (ok) {
         while (ok && it.b < 0 && more) {
@@ -897,22 +898,59 @@ int launch_chunk(const Maps& maps, ChunkParams p, long long items, cudaStream_t 
   return DADATTN_OK;
 }
 
+// How a call's tiles (of every key head) are shared out: pairs of them to a CTA, or each to a CTA or to a cluster of 2, 4 or 8.
+// Pairs read a key tile once for two, and win where there are many (us, pairs / single tiles): 512 tiles of 2048 tokens behind
+// 14336 of head size 128 466 / 539, 1024 tiles of 4096 128 / 147; at head size 64, where two CTAs are on an SM, 1536 of 16 x
+// 1024 56 / 65, 768 of 8 x 1024 36 / 37, 384 of 4 x 1024 33 / 22. Of fewer tiles the cheapest in key tiles, 2 us each, that a
+// group goes through: its items' own, and something for joining, by how often an SM is filled. One tile a CTA / 2 / 4 / 8:
+//   head size 128   16 tiles, 8033 rows 70 / 40 / 27 / 38    64, 8256 72 / 43 / 57 / 109     128, 16512 142 / 147 / 175 / 274
+//                   8, 60001 485 / 245 / 128 / 70            64, 256 8.8 / 11 / 25 / 71      160, 4001 87 / 83 / 90 / 150
+//   head size 64    12, 1024 13.6 / 10.2 / 8.6 / 9.0         36, 1001 17 / 13 / 14 / 24      192, 4096 65 / 61 / 72 / 115
+// The sequences' counts and lengths are on the device, so tiles and rows are the most that there may be.
+struct Sharing {
+  bool pairs;
+  int cluster;
+};
+Sharing share_out(long long tiles, long long pairs, long long most_rows, bool alike, int per_sm, int sms) {
+  if (tiles >= (per_sm == 1 ? 2 : 8) * sms) return {true, 1};
+  const long long n = (most_rows + kT - 1) / kT;
+  // how often `ctas` fill the GPU, or the part of it that clusters of their size can have (of eight: 14 clusters on 148 SMs)
+  auto fills = [&](double ctas, double slots) {
+    const double x = ctas / slots;
+    if (x <= 1.0) return 1.0;
+    if (per_sm == 2) return std::max(1.5, 0.75 * x + 0.35);   // (two CTAs on an SM take half as long again as one)
+    return alike ? std::ceil(x) : x + 0.5;
+  };
+  Sharing best = {true, 1};
+  double least = fills(pairs, sms) * n;
+  const struct { int cluster; double slots, join; } ways[] = {{1, 1.0, 0.5}, {2, 1.0, 1.5}, {4, 0.97, 1.75}, {8, 0.76, 2.5}};
+  for (const auto& w : ways) {
+    const double each = static_cast<double>((n + 2 * w.cluster - 1) / (2 * w.cluster)) + w.join;
+    const double cost = fills(static_cast<double>(tiles * w.cluster), w.slots * sms) * each;
+    if (cost < least) least = cost, best = {false, w.cluster};
+  }
+  return best;
+}
+
 template <int D>
-int launch_chunk_d(const Maps& maps, const ChunkParams& p, int max_new, long long most_rows, cudaStream_t st) {
-  // Items of every key head: no more than these (the sequences' counts are on the device).
+int launch_chunk_d(const Maps& maps, ChunkParams p, int max_new, long long most_rows, cudaStream_t st) {
+  // Items of a key head: no more than these.
   const int tt = p.tile_tokens, B = p.cache.B;
   auto most_items = [&](int tokens) -> long long {
     const long long each = (max_new + tokens - 1) / tokens;   // of one sequence
     return std::min<long long>(each * B, p.T / tokens + B);
   };
-  const long long tiles = most_items(tt), sms = current_sm_count();
-  int cluster = 1;
-  while (cluster < kMaxCluster && tiles * p.cache.heads * cluster * 2 <= sms && cluster * 4ll * kT <= most_rows) cluster *= 2;
-  switch (cluster) {
-    case 1: return launch_chunk<D, 1>(maps, p, most_items(2 * tt), st);
-    case 2: return launch_chunk<D, 2>(maps, p, tiles, st);
-    case 4: return launch_chunk<D, 4>(maps, p, tiles, st);
-    default: return launch_chunk<D, 8>(maps, p, tiles, st);
+  // (items are as long as each other, about, where one sequence has most of its rows ahead of the call)
+  const Sharing how = share_out(most_items(tt) * p.cache.heads, most_items(2 * tt) * p.cache.heads, most_rows,
+                                B == 1 && 2ll * max_new <= most_rows, Plan<D>::kPerSm, current_sm_count());
+  p.item_tokens = how.pairs ? 2 * tt : tt;
+  p.token_shift = (tt & (tt - 1)) ? -1 : log2_of(p.item_tokens);
+  const long long items = most_items(p.item_tokens);
+  switch (how.cluster) {
+    case 1: return launch_chunk<D, 1>(maps, p, items, st);
+    case 2: return launch_chunk<D, 2>(maps, p, items, st);
+    case 4: return launch_chunk<D, 4>(maps, p, items, st);
+    default: return launch_chunk<D, 8>(maps, p, items, st);
   }
 }
 
@@ -945,7 +983,6 @@ extern "C" int dadattn_paged_attention_bf16(uint16_t* out, float* lse, const uin
   p.wide = aligned(out, 32) && out_strides[0] % 16 == 0 && out_strides[1] % 16 == 0;
   p.T = T, p.max_new = max_new, p.heads_q = Hq, p.group = Hq / Hkv, p.tile_tokens = kT / p.group;
   p.chunk = page_size < kT ? page_size : kT;
-  p.token_shift = (p.tile_tokens & (p.tile_tokens - 1)) ? -1 : log2_of(2 * p.tile_tokens);
   p.scale = scale;
   if (max_new > T) max_new = T;   // (bounds the items)
   if ((static_cast<long long>(T) / p.tile_tokens + B) * kMaxCluster > 0x7fffffffll / Hkv)
