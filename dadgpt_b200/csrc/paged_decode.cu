@@ -3,23 +3,32 @@
 //
 //   out_r = sum_j p_rj v_j,  p_rj = exp(scale q_r.k_j - m_r) / l_r   over rows j = 0 .. lengths[b]
 //
-// for the `group` query heads r that share a key head: they are the rows of one 16-row operand of the warp-wide matrix
-// instruction (m16n8k16, bf16 in, fp32 sums), so that K and V are read once for all of them. Bound by HBM: 4 D bytes a cached
-// row and key head, 2 to 16 FLOPs a byte; what counts is that enough of them are on their way. tcgen05 would need its scores
-// back from tensor memory with one row a lane, and 128 of them for each product, where there are 1 to 16.
+// for the `group` query heads r that share a key head: they are the 8 columns (up to 16: two times 8) of the second operand of
+// the warp-wide matrix instruction (m16n8k16, bf16 in, fp32 sums), so that K and V are read once for all of them. The products are
+// transposed, S^T = K Q^T and O^T = V^T P^T: 16 rows of the cache, not 16 of 1 to 8 query rows, fill the instruction's 16 (3 %
+// faster than the other way round, and 32 registers fewer). Bound by HBM: 4 D bytes a cached row and key head, 2 to 16 FLOPs a
+// byte; what counts is that enough of them are on their way, and that a call is over soon after its longest sequence. tcgen05
+// would need its scores back from tensor memory, and 128 rows for each product.
 //   * a CTA (a cluster, where few items share the GPU) per sequence, key head and 16 query heads. Of a cluster each CTA takes
 //     a run of the 64-row tiles, and they join their maxima, sums and accumulators through distributed shared memory: no
 //     workspace, and nothing that two calls could share.
 //   * one producer warp: lane i fetches the i-th box of a tile (TMA, 128-byte swizzle, boxes as high as a page, up to the
 //     tile; 16 rows in a sequence's last tile, of which only those with a row are fetched), and looks its page up a tile ahead.
-//   * four consumer warps, 16 rows of a tile each, with a running maximum and sum of their own: scores and probabilities stay
-//     in registers, whose layout as a result is the one of the next product's operand. Accumulators are rescaled only when
-//     the maximum has grown by 2^8.
+//   * four consumer warps, 16 rows of a tile each, with a running maximum and sum of their own. Scores and probabilities stay in
+//     registers: as a result they lie transposed to the next product's operand, which movmatrix puts right. Accumulators are
+//     rescaled only when the maximum has grown by 2^8.
 //   * the new token needs no row of the cache: its scores, with k as rounded for the cache, are where one warp's running
 //     maximum begins, and v its accumulator.
+// Measured (us, rotating caches): 64 sequences of 9 .. 1023 rows, 12 heads of 64 21 (4.9 TB/s), all of 1000 38-39 (5.1); 8 of
+// 1000 .. 15999, 8 key heads of 128 for 32 46 (5.8), one of 60000 55 (4.5); 12 heads of 64, 699 rows 5.6. Two warps a CTA,
+// seven CTAs an SM: 31 for the first; eight warps, two CTAs: 23, and 5.2 for the last, but 53 for 128 sequences of up to 999
+// (45); persistent CTAs that take a long and a short item each 24. A CTA by itself draws 44 GB/s, what its ring of 64 KB gives
+// at 1.4 us from request to use.
 // Rows behind the last one are not trusted: their scores are masked and their V set to zero in shared memory.
 // Every wait is bounded (sm100_ptx.cuh).
 #include <cuda_bf16.h>
+
+#include <climits>
 
 #include "decode_common.cuh"
 #include "paged.cuh"
@@ -33,36 +42,36 @@ using bf16 = __nv_bfloat16;
 
 constexpr int kWarps = 4;                     // consumer warps
 constexpr int kThreads = (kWarps + 1) * 32;   // and one producer warp
-constexpr int kTile = 64;                     // cache rows of a stage
-constexpr int kWarpRows = kTile / kWarps;     // 16
-constexpr int kRows = 16;                     // query rows of an item
+constexpr int kWarpRows = 16;                 // cache rows of a warp in a stage
+constexpr int kTile = kWarps * kWarpRows;
+constexpr int kRows = 16;                     // query rows of an item, at most
 constexpr int kMaxCluster = 16;
+constexpr int kRanked = 4;                    // sequences of a lane that are ranked: 128 of a call
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kRescaleAt = 8.0f;
 
-template <int D>
+template <int D, int NT>
 struct Plan {
-  static constexpr int kStages = 3;
-  static constexpr int kPerSm = D == 64 ? 4 : 2;
+  static constexpr int kStages = D == 64 ? 3 : 2;            // with kPerSm: 192 KB on their way into an SM
+  static constexpr int kPerSm = D == 64 ? 4 : 3;
   static constexpr int kPanels = D / 64;
   static constexpr int kPanelBytes = kTile * 128;            // [64 rows][64 bf16], swizzled
   static constexpr int kSide = kPanels * kPanelBytes;        // K or V of a tile
   static constexpr int kStageBytes = 2 * kSide;
   // Behind the ring, or in its place once it has been read: accumulators of the warps and the CTA's.
   static constexpr int kPitch = D + 4;                       // floats of a row (banks)
-  static constexpr int kWarpAcc = kRows * kPitch;
-  static constexpr int kBytes = kStages * kStageBytes;
-  static_assert((kWarps + 1) * kWarpAcc * 4 <= kBytes, "accumulators in the ring's place");
+  static constexpr int kWarpAcc = 8 * NT * kPitch;
+  static constexpr int kBytes = kStages * kStageBytes > (kWarps + 1) * kWarpAcc * 4 ? kStages * kStageBytes : (kWarps + 1) * kWarpAcc * 4;
 };
 
-template <int D>
+template <int D, int NT>
 struct DecodeShared {
-  uint64_t full[Plan<D>::kStages], empty[Plan<D>::kStages];
+  uint64_t full[Plan<D, NT>::kStages], empty[Plan<D, NT>::kStages];
   int abort_flag, bad;
   float m[kWarps][kRows], l[kWarps][kRows];
   float m_all[kRows], l_all[kRows];           // of the CTA, read by the cluster's others
   __align__(16) float2 table[kMaxRotaryHead / 4];   // (cos, sin): D / 2 at most
-  __align__(16) bf16 q[kRows][D + 8];
+  __align__(16) bf16 q[8 * NT][D + 8];
   __align__(16) bf16 k_new[D], v_new[D];
 };
 
@@ -78,6 +87,7 @@ struct DecodeParams {
   float scale;
   RotaryParams r;
   int* status;
+  int ranked;   // items do not all start at once: they are taken by length
 };
 
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
@@ -99,6 +109,12 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// An 8 x 8 block of 16-bit elements in the operands' layout (row lane / 4, columns 2 (lane % 4) and the next), transposed.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 __device__ __forceinline__ float ld_cluster(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
@@ -110,22 +126,60 @@ __device__ __forceinline__ int ld_cluster_int(uint32_t addr) {
   return v;
 }
 
-template <int D, int CLUSTER>
-__global__ void __launch_bounds__(kThreads, Plan<D>::kPerSm)
+// The sequence of this place in an order by length, in 64ths of the longest's (so that what starts last is short), and its
+// length; by every warp for itself.
+__device__ __forceinline__ void by_length(const PagedCache& c, int place, int& b, int& ahead) {
+  const int lane = threadIdx.x % 32;
+  int lens[kRanked], units[kRanked], most = 0;
+#pragma unroll
+  for (int i = 0; i < kRanked; ++i) {
+    lens[i] = lane + 32 * i < c.B ? c.lengths[lane + 32 * i] : INT_MIN;
+    most = max(most, lens[i]);
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  const int unit = max(0, 26 - __clz(most));   // most < 64 << unit
+#pragma unroll
+  for (int i = 0; i < kRanked; ++i) units[i] = lane + 32 * i < c.B ? max(lens[i], 0) >> unit : -1;
+  auto reach = [&](int least) -> int {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kRanked; ++i) n += units[i] >= least;
+    return __reduce_add_sync(0xffffffffu, n);
+  };
+  int low = 0;   // the most units that more than `place` sequences reach
+#pragma unroll 1
+  for (int step = 32; step; step >>= 1)
+    if (reach(low + step) > place) low += step;
+  int rest = place - reach(low + 1);
+#pragma unroll
+  for (int i = 0; i < kRanked; ++i) {
+    const unsigned have = __ballot_sync(0xffffffffu, units[i] == low);
+    const int many = __popc(have);
+    if (rest >= 0 && rest < many) {
+      const int at = __fns(have, 0, rest + 1);
+      b = at + 32 * i;
+      ahead = __shfl_sync(0xffffffffu, lens[i], at);
+    }
+    rest -= many;
+  }
+}
+
+template <int D, int NT, int CLUSTER>
+__global__ void __launch_bounds__(kThreads, Plan<D, NT>::kPerSm)
 paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                     const __grid_constant__ CUtensorMap map_k16, const __grid_constant__ CUtensorMap map_v16,
                     const DecodeParams p) {
-  using L = Plan<D>;
+  using L = Plan<D, NT>;
   constexpr int kStages = L::kStages, kSteps = D / 16;
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ DecodeShared<D> sh;
+  __shared__ DecodeShared<D, NT> sh;
   volatile int* abort_flag = &sh.abort_flag;
   const PagedCache& c = p.cache;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int rank = CLUSTER > 1 ? blockIdx.x % CLUSTER : 0;
   const int item = blockIdx.x / CLUSTER;
   const int per_seq = c.heads * p.parts;
-  const int b = item / per_seq, kv_head = (item - b * per_seq) / p.parts, part = item % p.parts;
+  const int place = item / per_seq, kv_head = (item - place * per_seq) / p.parts, part = item % p.parts;
   const int head0 = kv_head * p.group + part * kRows, rows = min(p.group - part * kRows, kRows);
 
   if ((smem_u32(smem) & 1023u) != 0) {
@@ -145,7 +199,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   pdl_wait();
   pdl_launch_dependents();
 
-  const int ahead = c.lengths[b];
+  int b = place, ahead;
+  if (p.ranked) by_length(c, place, b, ahead);
+  else ahead = c.lengths[b];
   // (the same for every CTA of a cluster: nobody waits for one that has left)
   if (ahead < 0 || ahead >= c.max_pages << c.page_shift) {
     if (threadIdx.x == 0) atomicExch(p.status, DADATTN_E_ARG);
@@ -157,8 +213,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   const int n = end_tile - first_tile;
   const bool last_rank = rank == CLUSTER - 1;   // has the new token
 
-  float o[kSteps * 2][4];          // O: 8 columns each, rows lane / 4 and + 8
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  // Transposed: O^T is 16 columns of O and 8 query rows at a time. A lane has query rows 2 (lane % 4) and the one behind it,
+  // of elements (o[..][0], o[..][1]) lane / 4 and (o[..][2], o[..][3]) 8 behind that.
+  float o[kSteps][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) m[t][0] = m[t][1] = -INFINITY, l[t][0] = l[t][1] = 0.f;
   if (warp == kWarps) {
     // ------------------------------ producer ------------------------------
     const int32_t* table = c.table + static_cast<int64_t>(b) * c.max_pages;
@@ -206,7 +265,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     constexpr int kConsumers = kWarps * 32, kUnits = D / kTurnUnit;
     const int half = p.r.rot / 2;
     // pieces of 16 elements: of the query rows, then of k and v
-    const int pieces = (kRows + 2) * kUnits;
+    const int pieces = (8 * NT + 2) * kUnits;
     for (int e = t; e < half; e += kConsumers) sh.table[cos_sin_place(e)] = cos_sin<false>(ahead, turns_of(p.r.freq[e]), p.r.factor);
     // (not the producer, who is at work)
     auto consumers_meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers) : "memory"); };
@@ -218,11 +277,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                              (ahead & ((1 << c.page_shift) - 1))) * D;
     for (int i = t; i < pieces; i += kConsumers) {
       const int row = i / kUnits, u = i % kUnits;
-      const bool is_v = row == kRows + 1;
+      const bool is_v = row == (8 * NT) + 1;
       const int first = is_v ? u * kTurnUnit : unit_first(u, p.r), second = is_v ? 8 : unit_second(u, p.r);
-      if (row >= kRows && !last_rank) continue;
+      if (row >= (8 * NT) && !last_rank) continue;
       Sixteen<bf16> x;
-      if (row < kRows) {
+      if (row < (8 * NT)) {
         if (row < rows) x.load(p.q, b * p.q_token + (head0 + row) * p.q_head + first, second);
         else x.a = x.b = make_uint4(0, 0, 0, 0);
       } else if (is_v) {
@@ -236,51 +295,51 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         turn_unit(f, sh.table, u, p.r);
         x.from_floats(f);
       }
-      x.store(row < kRows ? sh.q[row] : is_v ? sh.v_new : sh.k_new, first, second);
-      if (row >= kRows && part == 0 && can_append) x.store(is_v ? p.v_pages : p.k_pages, new_row + first, second);
+      x.store(row < (8 * NT) ? sh.q[row] : is_v ? sh.v_new : sh.k_new, first, second);
+      if (row >= (8 * NT) && part == 0 && can_append) x.store(is_v ? p.v_pages : p.k_pages, new_row + first, second);
     }
     consumers_meet();
 
-    uint32_t qf[kSteps][4];
+    uint32_t qf[kSteps][NT][2];
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const int col = s * 16 + (lane % 4) * 2;
-      qf[s][0] = *reinterpret_cast<const uint32_t*>(&sh.q[lane / 4][col]);
-      qf[s][1] = *reinterpret_cast<const uint32_t*>(&sh.q[lane / 4 + 8][col]);
-      qf[s][2] = *reinterpret_cast<const uint32_t*>(&sh.q[lane / 4][col + 8]);
-      qf[s][3] = *reinterpret_cast<const uint32_t*>(&sh.q[lane / 4 + 8][col + 8]);
-    }
+    for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          qf[s][t][h] = *reinterpret_cast<const uint32_t*>(&sh.q[8 * t + lane / 4][s * 16 + (lane % 4) * 2 + 8 * h]);
     const float scale_log2 = p.scale * kLog2e;
 #pragma unroll
-    for (int i = 0; i < kSteps * 2; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) o[i][t][0] = o[i][t][1] = o[i][t][2] = o[i][t][3] = 0.f;
     if (last_rank && warp == 0) {
-      float2 dot[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const int col = s * 16 + (lane % 4) * 2;
-        const uint32_t k0 = *reinterpret_cast<const uint32_t*>(&sh.k_new[col]);
-        const uint32_t k1 = *reinterpret_cast<const uint32_t*>(&sh.k_new[col + 8]);
-        fma_bf16(dot[0], qf[s][0], k0);
-        fma_bf16(dot[0], qf[s][2], k1);
-        fma_bf16(dot[1], qf[s][1], k0);
-        fma_bf16(dot[1], qf[s][3], k1);
-      }
+      for (int t = 0; t < NT; ++t) {
+        float2 dot = make_float2(0.f, 0.f);   // of query row lane / 4, by the quad
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        float d = dot[x].x + dot[x].y;
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            fma_bf16(dot, qf[s][t][h], *reinterpret_cast<const uint32_t*>(&sh.k_new[s * 16 + (lane % 4) * 2 + 8 * h]));
+        float d = dot.x + dot.y;
         d += __shfl_xor_sync(0xffffffffu, d, 1);
         d += __shfl_xor_sync(0xffffffffu, d, 2);
-        m[x] = __fmul_rn(d, scale_log2);
-        // (1; NaN where the score is infinite or NaN, 0 for minus infinity. The four lanes' parts are added up.)
-        l[x] = lane % 4 == 0 && m[x] != -INFINITY ? ex2(m[x] - m[x]) : 0.f;
+        d = __fmul_rn(d, scale_log2);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          m[t][x] = __shfl_sync(0xffffffffu, d, 4 * (2 * (lane % 4) + x));
+          // (1; NaN where the score is infinite or NaN, 0 for minus infinity. The lanes' parts are added up.)
+          l[t][x] = lane / 4 == 0 && m[t][x] != -INFINITY ? ex2(m[t][x] - m[t][x]) : 0.f;
+        }
       }
 #pragma unroll
-      for (int i = 0; i < kSteps * 2; ++i) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(&sh.v_new[i * 8 + (lane % 4) * 2]);
-        const float v0 = __uint_as_float(w << 16), v1 = __uint_as_float(w & 0xffff0000u);
-        o[i][0] = m[0] == -INFINITY ? 0.f : v0, o[i][1] = m[0] == -INFINITY ? 0.f : v1;
-        o[i][2] = m[1] == -INFINITY ? 0.f : v0, o[i][3] = m[1] == -INFINITY ? 0.f : v1;
-      }
+      for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            o[i][t][e] = m[t][e & 1] == -INFINITY ? 0.f : __bfloat162float(sh.v_new[i * 16 + lane / 4 + 8 * (e >> 1)]);
     }
 
     // ------------------------------ the tiles ------------------------------
@@ -291,23 +350,23 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       if (!warp_wait(&sh.full[s], (j / kStages) & 1, abort_flag)) break;
       if (there > 0) {
         const uint32_t k_tile = ring + s * L::kStageBytes + warp * kWarpRows * 128, v_tile = k_tile + L::kSide;
-        float sc[2][4] = {};
+        // scores, transposed: S^T (16 rows of the cache x 8 query rows) = K Q^T
+        float sc[NT][4] = {};
 #pragma unroll
         for (int step = 0; step < kSteps; ++step) {
-          // matrices: keys 0-7 and 8-15, 16-byte chunks 2 step and 2 step + 1
           uint32_t kf[4];
-          const int key = (lane & 7) + (lane >> 4) * 8, ch = step * 2 + ((lane >> 3) & 1);
+          const int key = lane & 15, ch = step * 2 + (lane >> 4);
           ldmatrix4(k_tile + (ch / 8) * L::kPanelBytes + key * 128 + (((ch & 7) ^ (key & 7)) << 4), kf);
-          mma_16816(sc[0], qf[step], kf[0], kf[1]);
-          mma_16816(sc[1], qf[step], kf[2], kf[3]);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma_16816(sc[t], kf, qf[step][t][0], qf[step][t][1]);
         }
         if (there < kWarpRows) {
           // Rows that are not there: no score, and a V of zeros (what the page holds there could be anything).
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (h * 8 + (lane % 4) * 2 + (e & 1) >= there) sc[h][e] = -INFINITY;
+              if (lane / 4 + 8 * (e >> 1) >= there) sc[t][e] = -INFINITY;
           for (int i = lane; i < (kWarpRows - there) * D / 8; i += 32) {
             const int row = there + i / (D / 8), ch = i % (D / 8);
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_tile + (ch / 8) * L::kPanelBytes + row * 128 + ((ch & 7) << 4)),
@@ -317,53 +376,60 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           fence_proxy_async_smem();
           __syncwarp();
         }
-        float mx[2];
+        bool grown = false;
+        float mx[NT][2];
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-          mx[x] = __fmul_rn(fmaxf(fmaxf(sc[0][2 * x], sc[0][2 * x + 1]), fmaxf(sc[1][2 * x], sc[1][2 * x + 1])), scale_log2);
-        if (__any_sync(0xffffffffu, mx[0] > m[0] + kRescaleAt || mx[1] > m[1] + kRescaleAt || m[0] == -INFINITY || m[1] == -INFINITY)) {
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
-            mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
-            const float m_new = fmaxf(m[x], mx[x]);
-            const float corr = m[x] == -INFINITY ? 0.f : ex2(m[x] - m_new);
-            m[x] = m_new;
-            l[x] = __fmul_rn(l[x], corr);
-#pragma unroll
-            for (int i = 0; i < kSteps * 2; ++i) o[i][2 * x] *= corr, o[i][2 * x + 1] *= corr;
+            mx[t][x] = __fmul_rn(fmaxf(sc[t][x], sc[t][2 + x]), scale_log2);
+            grown |= mx[t][x] > m[t][x] + kRescaleAt || m[t][x] == -INFINITY;
           }
-        }
-        uint32_t pf[4];
+        if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const float neg = m[x] == -INFINITY ? 0.f : -m[x];
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) mx[t][x] = fmaxf(mx[t][x], __shfl_xor_sync(0xffffffffu, mx[t][x], d));
+              const float m_new = fmaxf(m[t][x], mx[t][x]);
+              const float corr = m[t][x] == -INFINITY ? 0.f : ex2(m[t][x] - m_new);
+              m[t][x] = m_new;
+              l[t][x] = __fmul_rn(l[t][x], corr);
+#pragma unroll
+              for (int i = 0; i < kSteps; ++i) o[i][t][x] *= corr, o[i][t][2 + x] *= corr;
+            }
+        }
+        uint32_t pf[NT][2];   // P^T as the second operand: the 8 x 8 blocks of the scores' layout, transposed
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
           float e[4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) e[2 * h + k] = ex2(fmaf(sc[h][2 * x + k], scale_log2, neg));
-          l[x] += (e[0] + e[1]) + (e[2] + e[3]);
-          pf[x] = pack_bf16(e[0], e[1]);
-          pf[2 + x] = pack_bf16(e[2], e[3]);
+          for (int i = 0; i < 4; ++i) e[i] = ex2(fmaf(sc[t][i], scale_log2, m[t][i & 1] == -INFINITY ? 0.f : -m[t][i & 1]));
+          l[t][0] += e[0] + e[2];
+          l[t][1] += e[1] + e[3];
+          pf[t][0] = transpose_8x8(pack_bf16(e[0], e[1]));
+          pf[t][1] = transpose_8x8(pack_bf16(e[2], e[3]));
         }
+        // O^T += V^T P^T, 16 columns of V at a time
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
           uint32_t vf[4];
-          const int key = lane & 15, ch = i * 2 + (lane >> 4);
+          const int key = (lane & 7) + (lane >> 4) * 8, ch = i * 2 + ((lane >> 3) & 1);
           ldmatrix4_trans(v_tile + (ch / 8) * L::kPanelBytes + key * 128 + (((ch & 7) ^ (key & 7)) << 4), vf);
-          mma_16816(o[2 * i], pf, vf[0], vf[1]);
-          mma_16816(o[2 * i + 1], pf, vf[2], vf[3]);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma_16816(o[i][t], vf, pf[t][0], pf[t][1]);
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.empty[s]);
     }
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
-      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-    }
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[t][x] += __shfl_xor_sync(0xffffffffu, l[t][x], d);
   }
 
   // ------------------------------ the warps', then the CTAs' results together ------------------------------
@@ -372,16 +438,18 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   float* sum = acc + kWarps * L::kWarpAcc;                   // [rows][kPitch]
   if (warp < kWarps) {
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int row = lane / 4 + 8 * x;
-      if (row < rows) {
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int i = 0; i < kSteps * 2; ++i)
-          *reinterpret_cast<float2*>(acc + warp * L::kWarpAcc + row * L::kPitch + i * 8 + (lane % 4) * 2) =
-              make_float2(o[i][2 * x], o[i][2 * x + 1]);
-        if (lane % 4 == 0) sh.m[warp][row] = m[x], sh.l[warp][row] = l[x];
+      for (int x = 0; x < 2; ++x) {
+        const int row = 8 * t + 2 * (lane % 4) + x;
+        if (row < rows) {
+#pragma unroll
+          for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) acc[warp * L::kWarpAcc + row * L::kPitch + i * 16 + lane / 4 + 8 * h] = o[i][t][2 * h + x];
+          if (lane < 4) sh.m[warp][row] = m[t][x], sh.l[warp][row] = l[t][x];
+        }
       }
-    }
   }
   __syncthreads();
   auto write_out = [&](int row, int col, float a, float b2, float l_tot) {
@@ -455,10 +523,13 @@ struct Maps {
   CUtensorMap k, v, k16, v16;
 };
 
-template <int D, int CLUSTER>
-int launch_decode(const Maps& maps, const DecodeParams& p, int items, cudaStream_t st) {
-  using L = Plan<D>;
-  auto kern = paged_decode_kernel<D, CLUSTER>;
+template <int D, int NT, int CLUSTER>
+int launch_decode(const Maps& maps, DecodeParams p, int items, cudaStream_t st) {
+  using L = Plan<D, NT>;
+  p.ranked = p.cache.B > 1 && p.cache.B <= 32 * kRanked &&
+             static_cast<long long>(items) * CLUSTER > static_cast<long long>(current_sm_count()) * L::kPerSm;
+
+  auto kern = paged_decode_kernel<D, NT, CLUSTER>;
   DAD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
   if (CLUSTER > 8) DAD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg = {};
@@ -478,22 +549,27 @@ int launch_decode(const Maps& maps, const DecodeParams& p, int items, cudaStream
   return DADATTN_OK;
 }
 
-// CTAs of a cluster: so many that they fill the GPU, and no more than there may be tiles for.
-int cluster_for(long long items, long long most_rows, int per_sm) {
+// CTAs of a cluster: as many as the GPU has room for, and no more than have two and a half tiles each of the longest sequence
+// that there may be. Of several sequences a quarter more: they are of different lengths, and the last to start are short. us,
+// clusters of 1 / 2 / 4 / 8 / 16 (head size 64 in the first, third and last row):
+//   1 x 12 heads, 699 rows    9.4 / 7.2 / 5.6 / 5.7 / 6.9     1 x 8, 60000          688 / 348 / 178 / 93 / 55
+//   64 x 12, up to 1023       21 / 30 / 48 / 88 / 230         8 x 8, up to 15999    187 / 98 / 60 / 46 / 67
+//   16 x 1, up to 1999        25 / 15 / 9.3 / 7.5 / 8.7       32 x 8, up to 3999    58 / 48 / 53 / 79 / 140
+int cluster_for(long long items, int sequences, long long most_rows, int per_sm) {
   const long long slots = static_cast<long long>(current_sm_count()) * per_sm;
   int c = 1;
-  while (c < kMaxCluster && items * c * 2 <= slots && static_cast<long long>(c) * 2 * kTile <= most_rows) c *= 2;
+  while (c < kMaxCluster && items * c * 2 * 4 <= slots * (sequences > 1 ? 5 : 4) && most_rows * 2 >= 5ll * c * 2 * kTile) c *= 2;
   return c;
 }
 
-template <int D>
+template <int D, int NT>
 int launch_decode_d(const Maps& maps, const DecodeParams& p, int items, long long most_rows, cudaStream_t st) {
-  switch (cluster_for(items, most_rows, Plan<D>::kPerSm)) {
-    case 1: return launch_decode<D, 1>(maps, p, items, st);
-    case 2: return launch_decode<D, 2>(maps, p, items, st);
-    case 4: return launch_decode<D, 4>(maps, p, items, st);
-    case 8: return launch_decode<D, 8>(maps, p, items, st);
-    default: return launch_decode<D, 16>(maps, p, items, st);
+  switch (cluster_for(items, p.cache.B, most_rows, Plan<D, NT>::kPerSm)) {
+    case 1: return launch_decode<D, NT, 1>(maps, p, items, st);
+    case 2: return launch_decode<D, NT, 2>(maps, p, items, st);
+    case 4: return launch_decode<D, NT, 4>(maps, p, items, st);
+    case 8: return launch_decode<D, NT, 8>(maps, p, items, st);
+    default: return launch_decode<D, NT, 16>(maps, p, items, st);
   }
 }
 
@@ -542,6 +618,9 @@ extern "C" int dadattn_decode_paged_bf16(uint16_t* out, float* lse, const uint16
   if (int rc = make_tensor_map_bf16(&maps.v16, v_pages, 1, rows, D, 16)) return rc;
   const long long most_rows = static_cast<long long>(max_pages) * page_size;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return D == 64 ? launch_decode_d<64>(maps, p, static_cast<int>(items), most_rows, st)
-                 : launch_decode_d<128>(maps, p, static_cast<int>(items), most_rows, st);
+  const bool few = group <= 8;   // rows of an item
+  if (D == 64) return few ? launch_decode_d<64, 1>(maps, p, static_cast<int>(items), most_rows, st)
+                          : launch_decode_d<64, 2>(maps, p, static_cast<int>(items), most_rows, st);
+  return few ? launch_decode_d<128, 1>(maps, p, static_cast<int>(items), most_rows, st)
+             : launch_decode_d<128, 2>(maps, p, static_cast<int>(items), most_rows, st);
 }
