@@ -58,6 +58,7 @@ SIGNATURES = {
     "dadattn_kv_cache_fill_fp8": (I, [P] * 10 + [I] * 6 + [P]),
     "dadattn_decode_fp8": (I, [P] * 11 + [I, I, I, I, F, I, I, P, SZ, P]),
     "dadattn_rotary_frequencies": (I, [P, I, F64, I, F64, F64, F64, F64]),
+    "dadattn_rotary_turns": (I, [P, P, I]),
     "dadattn_rotary": (I, [P] * 9 + [I64] + [I] * 5 + [P, F, I, I, I, I, P]),
     "dadattn_paged_append_bf16": (I, [P] * 13 + [I] * 8 + [P, F, I, I, I, P]),
     "dadattn_paged_attention_bf16": (I, [P] * 10 + [I] * 9 + [F, P]),

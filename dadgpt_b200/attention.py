@@ -248,7 +248,7 @@ class RotaryPositions:
     ``interleaved``, (2 i, 2 i + 1), pair i by ``position * freq[i]`` radians. ``scaling`` for contexts ``stretch`` times as
     long as those trained on: None, "linear", "base" or "parts" (by turns over ``trained_len``, from ``low`` to ``high``);
     include/dadattn.h has the formulas. ``factor`` multiplies the turned elements; None: 0.1 ln(stretch) + 1 with "parts",
-    else 1."""
+    else 1. ``freq``: radians per position (float64, on the host); ``turns``: as the kernels take them, on the device."""
 
     SCALINGS = {None: 0, "linear": 1, "base": 2, "parts": 3}   # DADATTN_ROTARY_*
 
@@ -263,14 +263,17 @@ class RotaryPositions:
         if factor is None:
             factor = 0.1 * math.log(stretch) + 1.0 if scaling == "parts" else 1.0
         self.factor = float(factor)
-        self.freq = host.to(device)
+        self.freq = host
+        turns = torch.empty(rot_dim // 2, dtype=torch.int64)
+        _lib.check(_lib.load().dadattn_rotary_turns(turns.data_ptr(), host.data_ptr(), rot_dim // 2))
+        self.turns = turns.to(device)
 
 
 def _turn(backward, q_out, k_out, q, k, rotary, positions, first):
     if q.dim() != 4 or (k is not None and k.dim() != 4):
         raise ValueError("q and k must be [B, S, heads, D]")
     B, S, H, D = q.shape
-    _native().rotary(backward, B, S, H, 0 if k is None else k.shape[2], D, first, rotary.freq, rotary.factor, rotary.rot_dim,
+    _native().rotary(backward, B, S, H, 0 if k is None else k.shape[2], D, first, rotary.turns, rotary.factor, rotary.rot_dim,
                      rotary.interleaved, q_out, k_out, q, k, positions)
 
 
@@ -305,7 +308,7 @@ class KVCachePagedBF16:
 
 
 def _rotary_args(rotary):
-    return (None, 1.0, 0, 0) if rotary is None else (rotary.freq, rotary.factor, rotary.rot_dim, rotary.interleaved)
+    return (None, 1.0, 0, 0) if rotary is None else (rotary.turns, rotary.factor, rotary.rot_dim, rotary.interleaved)
 
 
 def _packed(name, x):

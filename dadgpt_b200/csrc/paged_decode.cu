@@ -266,7 +266,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     const int half = p.r.rot / 2;
     // pieces of 16 elements: of the query rows, then of k and v
     const int pieces = (8 * NT + 2) * kUnits;
-    for (int e = t; e < half; e += kConsumers) sh.table[cos_sin_place(e)] = cos_sin<false>(ahead, turns_of(p.r.freq[e]), p.r.factor);
+    for (int e = t; e < half; e += kConsumers) sh.table[e] = cos_sin<false>(ahead, p.r.turns[e], p.r.factor);
     // (not the producer, who is at work)
     auto consumers_meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers) : "memory"); };
     consumers_meet();
@@ -292,7 +292,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       if (!is_v && u * kTurnUnit < p.r.rot) {
         float f[16];
         x.to_floats(f);
-        turn_unit(f, sh.table, u, p.r);
+        float2 cs[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) cs[k] = sh.table[u * 8 + k];
+        turn_unit(f, cs, p.r.interleaved);
         x.from_floats(f);
       }
       x.store(row < (8 * NT) ? sh.q[row] : is_v ? sh.v_new : sh.k_new, first, second);
@@ -583,13 +586,13 @@ extern "C" int dadattn_decode_paged_bf16(uint16_t* out, float* lse, const uint16
                                          const int64_t* k_strides, const int64_t* v_strides, uint16_t* k_pages,
                                          uint16_t* v_pages, const int32_t* page_table, const int32_t* lengths, int B, int Hq,
                                          int Hkv, int D, int pages, int page_size, int max_pages, float scale,
-                                         const double* freq, float factor, int rot_dim, int interleaved,
+                                         const uint64_t* turns, float factor, int rot_dim, int interleaved,
                                          dadattn_stream_t stream) {
   const char* name = "paged decode";
   if (int rc = check_paged(name, k_pages, v_pages, page_table, lengths, nullptr, B, Hkv, D, pages, page_size, max_pages)) return rc;
   if (Hq <= 0 || Hq % Hkv) return fail(DADATTN_E_ARG, "%s: Hq=%d must be a multiple of Hkv=%d", name, Hq, Hkv);
   if (!(scale > 0.0f && scale < INFINITY)) return fail(DADATTN_E_ARG, "%s: scale must be positive and finite", name);
-  if (int rc = check_rotary(name, freq, factor, rot_dim, D)) return rc;
+  if (int rc = check_rotary(name, turns, factor, rot_dim, D)) return rc;
   if (int rc = check_packed(name, out, out_strides, 8, true, B, Hq)) return rc;
   if (int rc = check_packed(name, q, q_strides, 8, false, B, Hq)) return rc;
   if (int rc = check_packed(name, k_new, k_strides, 8, false, B, Hkv)) return rc;
@@ -607,7 +610,7 @@ extern "C" int dadattn_decode_paged_bf16(uint16_t* out, float* lse, const uint16
   p.cache = PagedCache{page_table, lengths, nullptr, B, pages, log2_of(page_size), max_pages, Hkv};
   p.heads_q = Hq, p.group = group, p.parts = parts, p.chunk = page_size < kTile ? page_size : kTile;
   p.scale = scale;
-  p.r = RotaryParams{freq, factor, rot_dim, interleaved != 0, 0};
+  p.r = RotaryParams{turns, factor, rot_dim, interleaved != 0, 0};
   p.status = device_status_word();
   if (!p.status) return DADATTN_E_CUDA;
   const int rows = pages * Hkv * page_size;

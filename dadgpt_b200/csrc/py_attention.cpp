@@ -31,7 +31,7 @@ const char* type_name(at::ScalarType t) {
     case at::kBFloat16: return "torch.bfloat16";
     case at::kByte: return "torch.uint8";
     case at::kInt: return "torch.int32";
-    case at::kDouble: return "torch.float64";
+    case at::kLong: return "torch.int64";
     case at::kFloat8_e4m3fn: return "torch.float8_e4m3fn";
     default: return c10::toString(t);
   }
@@ -593,23 +593,23 @@ PyObject* evict_bf16(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// freq, factor, rot_dim, interleaved of a RotaryPositions; freq None: no rotation
+// turns, factor, rot_dim, interleaved of a RotaryPositions; turns None: no rotation
 struct Rotary {
-  const double* freq = nullptr;
+  const uint64_t* turns = nullptr;
   float factor = 1.f;
   int rot = 0, interleaved = 0;
   explicit Rotary(Args& p) {
     if (!p.none()) {
-      const at::Tensor& f = p.need("freq", at::kDouble);
-      Args::need_current("freq", f);
-      freq = static_cast<const double*>(f.data_ptr());
+      const at::Tensor& f = p.need("turns", at::kLong);
+      Args::need_current("turns", f);
+      turns = static_cast<const uint64_t*>(f.data_ptr());
       n = f.numel();
     }
     factor = p.real();
     rot = p.integer();
     interleaved = p.integer();
-    if (freq && n != rot / 2) {
-      PyErr_Format(PyExc_ValueError, "freq has %lld elements, expected %d", static_cast<long long>(n), rot / 2);
+    if (turns && n != rot / 2) {
+      PyErr_Format(PyExc_ValueError, "turns has %lld elements, expected %d", static_cast<long long>(n), rot / 2);
       throw Bad{};
     }
   }
@@ -617,7 +617,7 @@ struct Rotary {
 };
 const int32_t* ints(const at::Tensor& t) { return static_cast<const int32_t*>(t.data_ptr()); }
 
-// backward, B, S, Hq, Hk, D, first, freq, factor, rot_dim, interleaved, q_out, k_out or None, q, k or None, positions or None
+// backward, B, S, Hq, Hk, D, first, turns, factor, rot_dim, interleaved, q_out, k_out or None, q, k or None, positions or None
 PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Args p(a, n, 16, "rotary");
@@ -633,7 +633,7 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int32_t* const positions = p.none() ? nullptr : ints(p.here("positions", at::kInt, {B, S}));
     const dadattn_stream_t st = stream();
     return done(without_gil([&] {
-      return dadattn_rotary(qo, ko, q, k, s[0], s[1], s[2], s[3], positions, first, B, S, Hq, Hk, D, r.freq, r.factor, r.rot,
+      return dadattn_rotary(qo, ko, q, k, s[0], s[1], s[2], s[3], positions, first, B, S, Hq, Hk, D, r.turns, r.factor, r.rot,
                             r.interleaved, back, type == kB, st);
     }));
   });
@@ -671,7 +671,7 @@ PyObject* append_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const dadattn_stream_t st = stream();
     return done(without_gil([&] {
       return dadattn_paged_append_bf16(c.k, c.v, c.table, c.lengths, starts, qo, q, kn, vn, s[0], s[1], s[2], s[3], c.B, T, Hq, c.H,
-                                       c.D, c.pages, c.page_size, c.max_pages, r.freq, r.factor, r.rot, r.interleaved, type == kB, st);
+                                       c.D, c.pages, c.page_size, c.max_pages, r.turns, r.factor, r.rot, r.interleaved, type == kB, st);
     }));
   });
 }
@@ -712,7 +712,7 @@ PyObject* decode_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const dadattn_stream_t st = stream();
     return done(without_gil([&] {
       return dadattn_decode_paged_bf16(out, lse, q, kn, vn, s[0], s[1], s[2], s[3], c.k, c.v, c.table, c.lengths, c.B, Hq, c.H, c.D,
-                                       c.pages, c.page_size, c.max_pages, scale, r.freq, r.factor, r.rot, r.interleaved, st);
+                                       c.pages, c.page_size, c.max_pages, scale, r.turns, r.factor, r.rot, r.interleaved, st);
     }));
   });
 }

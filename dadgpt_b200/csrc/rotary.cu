@@ -1,20 +1,22 @@
 // Rotary positions for training: queries and keys turned by their positions ahead of the attention, their gradients turned
 // back behind it. The mathematics and the angles: rotary.cuh.
 //
-// Bound by HBM: every element is read and written once. A CTA takes a few tokens and all their heads: (cos, sin) of a token's
-// pairs are computed once, into shared memory, and serve every head of q and of k; the first elements are on their way
-// meanwhile. A thread turns 16 elements at a time, two 16-byte pieces (bf16) of a head's two halves or of one run.
+// Bound by HBM: every element is read and written once. A thread has one piece of 16 elements (two runs of 16 bytes in bf16) of a
+// token and goes through a group of its heads, with (cos, sin) of the piece's eight pairs in registers. (From a table in shared
+// memory, heads side by side in a warp, the table's reads alone were 16 wavefronts for every 8 of the tensors': 41 us instead of
+// 35.6 for forward and backward of 16 x 1024 x 24 heads of 64.)
+// Measured: 16 x 1024 x 24 heads of 64, bf16, heads split 17.8 us (5.7 TB/s), fp32 33.6 (6.0); 8192 tokens of 40 heads of 128 28.0 (6.0);
+// 140 tokens of 8 heads of 32, fp32, 2.3.
 #include "rotary.cuh"
 
+#include <algorithm>
 #include <cmath>
 #include <initializer_list>
 
 namespace dadattn {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kMaxTokens = 32;          // of a CTA
-constexpr int kTable = 2048;            // (cos, sin) pairs of a CTA
+constexpr int kThreads = 128;
 
 struct Strides {
   int64_t batch, token, head;
@@ -25,70 +27,31 @@ struct TurnParams {
   Strides from[2], to[2];
   const int32_t* positions;   // [B, S] or null: first + s
   int64_t first;
-  int S, heads_q, heads, units;       // heads of q; of q and k; pieces of a head that are worked on
-  int tokens, tiles, heads_first;     // of a CTA; tiles of a sequence; the order: 1 = a head's tokens next to each other
-  SmallDivisor by_units, by_inner;
+  int S, heads[2], units;      // units: pieces of a head that are worked on
+  int groups[2];               // of q's heads, and of k's behind them; a thread goes through one
+  int64_t tokens;              // B * S
   RotaryParams r;
 };
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const TurnParams p) {
   constexpr bool kExact = sizeof(T) == 4;
-  __shared__ __align__(16) float2 table[kTable];
   pdl_wait();
   pdl_launch_dependents();
-  const int b = blockIdx.x / p.tiles, s0 = (blockIdx.x - b * p.tiles) * p.tokens, n = min(p.tokens, p.S - s0);
-  const int half = p.r.rot / 2;
-  const uint32_t all = static_cast<uint32_t>(p.tokens) * p.heads * p.units;
-  struct At {
-    int token, u, which;
-    int64_t from, to;
-  };
-  auto locate = [&](uint32_t i) {
-    const uint32_t j = p.by_units.divide(i), u = i - j * p.units;
-    const uint32_t outer = p.by_inner.divide(j), inner = j - outer * p.by_inner.d;
-    At at;
-    at.token = p.heads_first ? inner : outer;
-    at.u = u;
-    int head = p.heads_first ? outer : inner;
-    at.which = head >= p.heads_q;
-    if (at.which) head -= p.heads_q;
-    const Strides &f = p.from[at.which], &t = p.to[at.which];
-    const int64_t x = unit_first(u, p.r);
-    at.from = b * f.batch + (s0 + at.token) * f.token + head * f.head + x;
-    at.to = b * t.batch + (s0 + at.token) * t.token + head * t.head + x;
-    return at;
-  };
-  uint32_t i = threadIdx.x;
-  At at = locate(i);
-  Sixteen<T> now;
-  if (i < all && at.token < n) now.load(p.in[at.which], at.from, unit_second(at.u, p.r));
-  for (int e = threadIdx.x; e < n * half; e += kThreads) {
-    const int token = e / half, pair = e - token * half;
-    const int64_t position = p.positions ? p.positions[static_cast<int64_t>(b) * p.S + s0 + token] : p.first + s0 + token;
-    table[token * half + cos_sin_place(pair)] = cos_sin<kExact>(position, turns_of(p.r.freq[pair]), p.r.factor);
-  }
-  __syncthreads();
-  while (i < all) {
-    const At here = at;
-    Sixteen<T> next;
-    const uint32_t j = i + kThreads;
-    if (j < all) {
-      at = locate(j);
-      if (at.token < n) next.load(p.in[at.which], at.from, unit_second(at.u, p.r));
-    }
-    if (here.token < n) {
-      if (here.u * kTurnUnit < p.r.rot) {
-        float x[16];
-        now.to_floats(x);
-        turn_unit(x, table + here.token * half, here.u, p.r);
-        now.from_floats(x);
-      }
-      now.store(p.out[here.which], here.to, unit_second(here.u, p.r));
-    }
-    now = next;
-    i = j;
-  }
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x, token = i / p.units;
+  if (token >= p.tokens) return;
+  const int u = static_cast<int>(i - token * p.units);
+  const int64_t b = token / p.S, s = token - b * p.S;
+  const int which = static_cast<int>(blockIdx.y) >= p.groups[0], g = blockIdx.y - (which ? p.groups[0] : 0);
+  const int head0 = g * p.heads[which] / p.groups[which], n = (g + 1) * p.heads[which] / p.groups[which] - head0;
+  const bool turned = u * kTurnUnit < p.r.rot;
+  float2 cs[8];
+  if (turned) cos_sin_of<kExact>(cs, u, p.positions ? p.positions[token] : p.first + s, p.r);
+  const Strides &f = p.from[which], &t = p.to[which];
+  const int x = unit_first(u, p.r);
+  const T* in = static_cast<const T*>(p.in[which]) + b * f.batch + s * f.token + head0 * f.head + x;
+  T* out = static_cast<T*>(p.out[which]) + b * t.batch + s * t.token + head0 * t.head + x;
+  turn_heads<sizeof(T) == 4 ? 2 : 4>(in, f.head, out, t.head, n, unit_second(u, p.r), turned, cs, p.r.interleaved);
 }
 
 }  // namespace
@@ -124,10 +87,23 @@ extern "C" int dadattn_rotary_frequencies(double* freq, int rot_dim, double base
   return DADATTN_OK;
 }
 
+extern "C" int dadattn_rotary_turns(uint64_t* turns, const double* freq, int count) {
+  if (!turns || !freq) return fail(DADATTN_E_ARG, "rotary turns: null pointer");
+  if (count <= 0) return fail(DADATTN_E_ARG, "rotary turns: count %d must be positive", count);
+  for (int i = 0; i < count; ++i) {
+    if (!(freq[i] > -1e15 && freq[i] < 1e15)) return fail(DADATTN_E_ARG, "rotary turns: frequency %d is not finite, or too large", i);
+    long double t = freq[i] * 0.159154943091895335768883763372514362L;   // 1 / (2 pi)
+    t = (t - std::floor(t)) * 18446744073709551616.0L;
+    const long double whole = std::floor(t + 0.5L);
+    turns[i] = whole >= 18446744073709551616.0L ? 0 : static_cast<uint64_t>(whole);
+  }
+  return DADATTN_OK;
+}
+
 extern "C" int dadattn_rotary(void* q_out, void* k_out, const void* q, const void* k, const int64_t* q_out_strides,
                               const int64_t* k_out_strides, const int64_t* q_strides, const int64_t* k_strides,
                               const int32_t* positions, int64_t first, int B, int S, int Hq, int Hk, int D,
-                              const double* freq, float factor, int rot_dim, int interleaved, int backward, int is_bf16,
+                              const uint64_t* turns, float factor, int rot_dim, int interleaved, int backward, int is_bf16,
                               dadattn_stream_t stream) {
   if (!q || !q_out || !q_strides || !q_out_strides) return fail(DADATTN_E_ARG, "rotary: null pointer");
   if (B <= 0 || S <= 0 || Hq <= 0 || Hk < 0 || D <= 0)
@@ -136,10 +112,9 @@ extern "C" int dadattn_rotary(void* q_out, void* k_out, const void* q, const voi
   if (D % kTurnUnit || D > kMaxRotaryHead)
     return fail(DADATTN_E_UNSUPPORTED, "rotary: unsupported D %d (a multiple of %d up to %d)", D, kTurnUnit, kMaxRotaryHead);
   if (rot_dim <= 0) return fail(DADATTN_E_ARG, "rotary: rot_dim %d must be positive", rot_dim);
-  if (int rc = check_rotary("rotary", freq, factor, rot_dim, D)) return rc;
+  if (int rc = check_rotary("rotary", turns, factor, rot_dim, D)) return rc;
   if (!aligned(positions, 4)) return fail(DADATTN_E_ARG, "rotary: positions must be 4-byte aligned");
-  if ((static_cast<long long>(Hq) + Hk) * (D / kTurnUnit) > 32768)
-    return fail(DADATTN_E_UNSUPPORTED, "rotary: %lld heads of %d are too many for a call", static_cast<long long>(Hq) + Hk, D);
+  if (Hq > 65535 - Hk) return fail(DADATTN_E_UNSUPPORTED, "rotary: Hq=%d and Hk=%d exceed 65535 together", Hq, Hk);
   const int64_t piece = is_bf16 ? 8 : 4;   // elements of 16 bytes
   TurnParams p = {};
   const int64_t* strides[4] = {q_strides, k_strides, q_out_strides, k_out_strides};
@@ -162,25 +137,21 @@ extern "C" int dadattn_rotary(void* q_out, void* k_out, const void* q, const voi
   p.in[0] = q, p.in[1] = k, p.out[0] = q_out, p.out[1] = k_out;
   p.positions = positions;
   p.first = first;
-  p.S = S, p.heads_q = Hq, p.heads = Hq + Hk;
+  p.S = S, p.heads[0] = Hq, p.heads[1] = Hk;
   // in place, what is not turned is where it belongs
   const bool same = q == q_out && (Hk == 0 || k == k_out);
   p.units = (same ? rot_dim : D) / kTurnUnit;
-  p.r = RotaryParams{freq, factor, rot_dim, interleaved != 0, backward != 0};
-  p.heads_first = p.from[0].head > p.from[0].token;
-  // Tokens of a CTA: about 1024 pieces, four a thread, but no fewer than two CTAs for each SM.
-  int tokens = 1;
-  const int sms = current_sm_count();
-  while (tokens * 2 <= kMaxTokens && tokens * p.heads * p.units < 1024 && tokens * 2 * (rot_dim / 2) <= kTable &&
-         static_cast<long long>(B) * ((S + tokens * 2 - 1) / (tokens * 2)) >= 2 * sms)
-    tokens *= 2;
-  p.tokens = tokens;
-  p.tiles = (S + tokens - 1) / tokens;
-  p.by_units = SmallDivisor(p.units);
-  p.by_inner = SmallDivisor(p.heads_first ? tokens : p.heads);
-  const long long blocks = static_cast<long long>(B) * p.tiles;
-  if (blocks > 0x7fffffffll) return fail(DADATTN_E_UNSUPPORTED, "rotary: B*S=%lld is too many tokens", static_cast<long long>(B) * S);
-  const dim3 grid(static_cast<unsigned>(blocks));
+  p.r = RotaryParams{turns, factor, rot_dim, interleaved != 0, backward != 0};
+  p.tokens = static_cast<int64_t>(B) * S;
+  const long long blocks = (p.tokens * p.units + kThreads - 1) / kThreads;
+  if (blocks > 0x7fffffffll) return fail(DADATTN_E_UNSUPPORTED, "rotary: B*S=%lld is too many tokens", static_cast<long long>(p.tokens));
+  // Four heads a thread, which are all on their way at once, or fewer where the call has less than four CTAs an SM. (us of
+  // forward and backward, 16 x 1024 x 24 heads of 64 and 8192 x 40 of 128: two or three heads 41 and -, four 35.6 and 56.5, five
+  // or six 37 and 59, eight - and 60.)
+  const auto groups = [&](int heads) { return heads ? std::max(head_groups(blocks, heads, Hq + Hk, 4), (heads + 3) / 4) : 0; };
+  p.groups[0] = groups(Hq);
+  p.groups[1] = groups(Hk);
+  const dim3 grid(static_cast<unsigned>(blocks), p.groups[0] + p.groups[1]);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (is_bf16) DAD_CUDA(launch_pdl(rotary_kernel<__nv_bfloat16>, grid, dim3(kThreads), 0, st, p));
   else DAD_CUDA(launch_pdl(rotary_kernel<float>, grid, dim3(kThreads), 0, st, p));

@@ -4,11 +4,11 @@
 //   y1 = f (cos(p w_i) x1 - sin(p w_i) x2),  y2 = f (cos(p w_i) x2 + sin(p w_i) x1)
 // with (x1, x2) elements (i, i + rot / 2), or (2 i, 2 i + 1) where pairs are interleaved. The gradient is turned by -p.
 //
-// Angles: p w in 32 bits loses 2^-24 of itself, 0.06 radians at a million positions, and in 64-bit arithmetic the reduction
-// of a large angle would cost more than the rotation. So a frequency becomes a 64-bit fraction of a turn, and p times it,
-// modulo 2^64, is the angle modulo a turn without any rounding: what is left is the fraction's own, 2^-53 of the frequency
-// and 2^-65 of a turn, times p. The nearest quarter turn is taken off in integers too, so that the sine and cosine are those
-// of at most an eighth of a turn, whose conversion to a float is off by 2^-28 of a turn at most (2.4e-8 radians).
+// Angles: p w in 32 bits loses 2^-24 of itself, 0.06 radians at a million positions, and in 64-bit floating point the reduction
+// of a large angle would cost more than the rotation. So a frequency comes as a 64-bit fraction of a turn (dadattn_rotary_turns),
+// and p times it, modulo 2^64, is the angle modulo a turn without any rounding: what is left is the fraction's own, half a unit,
+// times p. The nearest quarter turn is taken off in integers too, so that the sine and cosine are those of at most an eighth of
+// a turn, whose conversion to a float is off by 2^-28 of a turn at most (2.4e-8 radians).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -23,19 +23,19 @@ constexpr int kMaxRotaryHead = 256;      // largest head size
 
 // What a kernel needs to know of the rotation. rot = 0: none.
 struct RotaryParams {
-  const double* freq;   // [rot / 2], radians per position
-  float factor;         // of the turned elements
+  const uint64_t* turns;   // [rot / 2], 2^-64 turns per position
+  float factor;            // of the turned elements
   int rot;
   int interleaved;
-  int back;             // 1: by the negative angle (gradients)
+  int back;                // 1: by the negative angle (gradients)
 };
 
 // What every call with a rotation checks.
-inline int check_rotary(const char* name, const double* freq, float factor, int rot, int D) {
+inline int check_rotary(const char* name, const uint64_t* turns, float factor, int rot, int D) {
   if (rot == 0) return DADATTN_OK;
   if (rot < 0 || rot > D) return fail(DADATTN_E_ARG, "%s: rot_dim %d must be within the head's %d elements", name, rot, D);
   if (rot % kTurnUnit) return fail(DADATTN_E_UNSUPPORTED, "%s: rot_dim %d is not a multiple of %d", name, rot, kTurnUnit);
-  if (!freq || !aligned(freq, 8)) return fail(DADATTN_E_ARG, "%s: freq must be an 8-byte aligned device pointer", name);
+  if (!turns || !aligned(turns, 16)) return fail(DADATTN_E_ARG, "%s: turns must be a 16-byte aligned device pointer", name);
   if (!(factor > -INFINITY && factor < INFINITY)) return fail(DADATTN_E_ARG, "%s: factor must be finite", name);
   return DADATTN_OK;
 }
@@ -47,11 +47,23 @@ inline int current_sm_count() {
   return sms;
 }
 
+// Groups that `heads` heads are dealt out to, a thread going through one, where a head takes `blocks` CTAs and all heads of the
+// call are `all`: so many that the call has `per_sm` CTAs an SM.
+inline int head_groups(long long blocks, int heads, int all, int per_sm) {
+  const long long groups = (static_cast<long long>(per_sm) * current_sm_count() * heads + blocks * all - 1) / (blocks * all);
+  return static_cast<int>(groups < heads ? groups : heads);
+}
+
 #ifdef __CUDACC__
-// Turns per position, modulo 1, times 2^64.
-__device__ __forceinline__ uint64_t turns_of(double freq) {
-  const double t = freq * 0.15915494309189533577;   // 1 / (2 pi)
-  return __double2ull_rn((t - floor(t)) * 18446744073709551616.0);   // (a fraction that rounds to 1 saturates)
+// sin and cos of r half turns, |r| <= 1/4, by polynomials in r^2 that were fitted for the least error over that range: off by
+// 4.4e-8 and 5.8e-8 in fp32 (pi comes in two parts). 12 operations; sincospif, which takes any r, made a short fp32 call 1 us
+// longer, at eight pairs a thread.
+__device__ __forceinline__ void sin_cos_eighth(float r, float* s, float* c) {
+  const float z = r * r;
+  float p = fmaf(fmaf(-0.5894796f, z, 2.5498104f), z, -5.1677094f);
+  p = fmaf(r, p * z, r * -8.742278e-8f);
+  *s = fmaf(r, 3.14159274f, p);
+  *c = fmaf(fmaf(fmaf(fmaf(0.23142955f, z, -1.3350585f), z, 4.0587077f), z, -4.934802f), z, 1.0f);
 }
 
 // (cos, sin) of position * turns, times the factor. EXACT: to fp32 accuracy, else to 2^-21 (for results in bf16, whose
@@ -62,7 +74,7 @@ __device__ __forceinline__ float2 cos_sin(int64_t position, uint64_t turns, floa
   const uint64_t quarter = (a + (1ull << 61)) >> 62;          // to the nearest, 0..3 (wraps with the turn)
   const int32_t rest = static_cast<int32_t>(static_cast<int64_t>(a - (quarter << 62)) >> 32);   // [-1/8, 1/8] turns * 2^32
   float s, c;
-  if (EXACT) sincospif(static_cast<float>(rest) * 4.656612873077393e-10f, &s, &c);              // 2^-31: half turns
+  if (EXACT) sin_cos_eighth(static_cast<float>(rest) * 4.656612873077393e-10f, &s, &c);         // 2^-31: half turns
   else __sincosf(static_cast<float>(rest) * 1.4629180792671596e-9f, &s, &c);                    // 2 pi / 2^32
   const float cq = (quarter & 1) ? s : c, sq = (quarter & 1) ? c : s;
   return make_float2((quarter == 1 || quarter == 2 ? -cq : cq) * factor, (quarter >= 2 ? -sq : sq) * factor);
@@ -134,42 +146,75 @@ __device__ __forceinline__ int unit_second(int u, const RotaryParams& r) {
   return u * kTurnUnit < r.rot && !r.interleaved ? r.rot / 2 : 8;
 }
 
-// (cos, sin) of a token's pairs lie in shared memory, eight pairs (64 bytes) for a piece. The four 16-byte words of piece u
-// change places by u, so that the threads of eight neighbouring pieces, which read the same word at a time, find it in
-// different banks.
-__device__ __forceinline__ int cos_sin_place(int pair) {   // in float2
-  const int u = pair >> 3, word = (pair >> 1) & 3;
-  return u * 8 + ((word ^ (u >> 1 & 3)) << 1) + (pair & 1);
+// The eight (cos, sin) of piece u of a token at this position, for a thread that turns that piece of several heads.
+template <bool EXACT>
+__device__ __forceinline__ void cos_sin_of(float2 (&cs)[8], int u, int64_t position, const RotaryParams& r) {
+  const ulonglong2* turns = reinterpret_cast<const ulonglong2*>(r.turns + u * 8);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const ulonglong2 two = __ldg(turns + i);
+    cs[2 * i] = cos_sin<EXACT>(position, two.x, r.factor);
+    cs[2 * i + 1] = cos_sin<EXACT>(position, two.y, r.factor);
+  }
+  if (r.back) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) cs[i].y = -cs[i].y;
+  }
 }
-// Turns the 16 elements of piece u of a token, whose table is cs.
-__device__ __forceinline__ void turn_unit(float (&x)[16], const float2* cs, int u, const RotaryParams& r) {
-  const float4* table = reinterpret_cast<const float4*>(cs + u * 8);
-  const int move = u >> 1 & 3;
-  auto turn = [&](float& a, float& b, float c, float s) {
-    const float y = c * a - s * b;
-    b = c * b + s * a;
+// 16 elements by eight (cos, sin); both layouts of the pairs.
+__device__ __forceinline__ void turn_unit(float (&x)[16], const float2 (&cs)[8], bool interleaved) {
+  auto turn = [&](float& a, float& b, float2 c) {
+    const float y = c.x * a - c.y * b;
+    b = c.x * b + c.y * a;
     a = y;
   };
+  if (interleaved) {
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    float4 t = table[w ^ move];
-    if (r.back) t.y = -t.y, t.w = -t.w;
-    if (r.interleaved) {
-      turn(x[4 * w], x[4 * w + 1], t.x, t.y);
-      turn(x[4 * w + 2], x[4 * w + 3], t.z, t.w);
-    } else {
-      turn(x[2 * w], x[2 * w + 8], t.x, t.y);
-      turn(x[2 * w + 1], x[2 * w + 9], t.z, t.w);
-    }
+    for (int i = 0; i < 8; ++i) turn(x[2 * i], x[2 * i + 1], cs[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) turn(x[i], x[i + 8], cs[i]);
   }
 }
 
-// idx / d for idx and d below 2^16 and idx * d below 2^32.
-struct SmallDivisor {
-  uint32_t d, m;
-  SmallDivisor(int by = 1) : d(by), m(by == 1 ? 0 : static_cast<uint32_t>((0x100000000ull + by - 1) / by)) {}
-  __device__ __forceinline__ uint32_t divide(uint32_t i) const { return m ? __umulhi(i, m) : i; }
-};
+template <typename To, typename From>
+__device__ __forceinline__ Sixteen<To> converted(const Sixteen<From>& x) {
+  Sixteen<To> y;
+  float f[16];
+  x.to_floats(f);
+  y.from_floats(f);
+  return y;
+}
+template <>
+__device__ __forceinline__ Sixteen<__nv_bfloat16> converted(const Sixteen<__nv_bfloat16>& x) { return x; }   // (NaN as it is)
+template <>
+__device__ __forceinline__ Sixteen<float> converted(const Sixteen<float>& x) { return x; }
+
+// One piece of `n` heads, `in_step` and `out_step` elements apart, turned or passed on. AHEAD heads are on their way at a time.
+template <int AHEAD, typename From, typename To>
+__device__ __forceinline__ void turn_heads(const From* in, int64_t in_step, To* out, int64_t out_step, int n, int second,
+                                           bool turned, const float2 (&cs)[8], bool interleaved) {
+  for (int h = 0; h < n; h += AHEAD) {
+    Sixteen<From> x[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (h + k < n) x[k].load(in, (h + k) * in_step, second);
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      if (h + k >= n) break;
+      Sixteen<To> y;
+      if (turned) {
+        float f[16];
+        x[k].to_floats(f);
+        turn_unit(f, cs, interleaved);
+        y.from_floats(f);
+      } else {
+        y = converted<To>(x[k]);
+      }
+      y.store(out, (h + k) * out_step, second);
+    }
+  }
+}
 #endif
 
 }  // namespace dadattn

@@ -415,9 +415,9 @@ int dadattn_decode_fp8(uint16_t* out, const uint16_t* q, const uint16_t* k_new, 
  * the first rot_dim are rot_dim / 2 pairs, and pair i of the token at position p is turned by the angle p * freq[i]:
  *   y1 = factor (x1 cos - x2 sin),  y2 = factor (x2 cos + x1 sin),
  * (x1, x2) being elements (i, i + rot_dim / 2), or (2 i, 2 i + 1) when `interleaved`. Elements from rot_dim on pass unchanged.
- * Angles are formed without rounding (a 64-bit fraction of a turn), so that far positions lose nothing.
+ * Angles are formed without rounding, from 64-bit fractions of a turn, so that far positions lose nothing.
  *
- * Frequencies, radians per position, into a HOST array of rot_dim / 2 (which the caller copies to the device):
+ * Frequencies, radians per position, into a HOST array of rot_dim / 2:
  * w_i = base^(-2 i / rot_dim), and for contexts `stretch` times as long as the model was trained for
  *   DADATTN_ROTARY_LINEAR  w_i / stretch (positions interpolated)
  *   DADATTN_ROTARY_BASE    the base times stretch^(rot_dim / (rot_dim - 2)): the slowest pair is slowed by `stretch`, the
@@ -431,18 +431,21 @@ int dadattn_decode_fp8(uint16_t* out, const uint16_t* q, const uint16_t* k_new, 
 #define DADATTN_ROTARY_PARTS 3
 int dadattn_rotary_frequencies(double* freq, int rot_dim, double base, int scaling, double stretch, double trained_len,
                                double low, double high);
+/* Frequencies (host) to what the calls below take, 2^-64 turns per position (host; the caller copies them to the device). */
+int dadattn_rotary_turns(uint64_t* turns, const double* freq, int count);
 
 /* Queries and keys of a training step, or of any batch, turned; with `backward` by the negative angle, which takes the
  * gradients of the turned tensors to those of the tensors. q [B,S,Hq,D], k [B,S,Hk,D] in any order of the dimensions but the
  * last: element (b, s, h, d) lies at b strides[0] + s strides[1] + h strides[2] + d (host arrays of three, in elements). So
  * heads split, [B*H, S, D], and as the projections write them, [B*S, H*D], are both taken. bf16 when is_bf16, else fp32; the
  * arithmetic is fp32. The position of token (b, s) is positions[b S + s] (int32 on the device, may be negative), or first + s
- * with positions NULL. freq: device array. q_out may be q and k_out k (same strides); results do not overlap anything else.
+ * with positions NULL. turns: device array of
+ * rot_dim / 2, 16-byte aligned. q_out may be q and k_out k (same strides); results do not overlap anything else.
  * Hk = 0: no k. D and rot_dim are multiples of 16, D at most 256; every row begins at a multiple of 16 bytes; results'
- * strides are not zero. (Hq + Hk) D at most 524288. */
+ * strides are not zero. Hq + Hk at most 65535. */
 int dadattn_rotary(void* q_out, void* k_out, const void* q, const void* k, const int64_t* q_out_strides,
                    const int64_t* k_out_strides, const int64_t* q_strides, const int64_t* k_strides, const int32_t* positions,
-                   int64_t first, int B, int S, int Hq, int Hk, int D, const double* freq, float factor, int rot_dim,
+                   int64_t first, int B, int S, int Hq, int Hk, int D, const uint64_t* turns, float factor, int rot_dim,
                    int interleaved, int backward, int is_bf16, dadattn_stream_t stream);
 
 /* ---- KV cache in pages ----------------------------------------------------------------------------- */
@@ -464,15 +467,15 @@ int dadattn_rotary(void* q_out, void* k_out, const void* q, const void* k, const
  * No call needs a workspace; calls may overlap on the GPU unless one writes what the other reads or writes. */
 
 /* New rows to their pages: k_new, v_new [T,Hkv,D] (bf16 when new_is_bf16, else fp32, rounded to bf16 once), keys turned by
- * their rows in their sequences where rot_dim > 0 (as in dadattn_rotary; freq NULL and rot_dim 0: learned positions). Hq > 0:
+ * their rows in their sequences where rot_dim > 0 (as in dadattn_rotary; turns NULL and rot_dim 0: learned positions). Hq > 0:
  * q [T,Hq,D] of the same type is turned too, into q_out (bf16; may be q where that is bf16 with the same strides). A sequence's pages of
- * these rows belong to it alone. rot_dim a multiple of 16; (Hq + 2 Hkv) D at most 524288. A prefill's heads [H,n,D] are taken
+ * these rows belong to it alone. rot_dim a multiple of 16; Hq + 2 Hkv at most 65535. A prefill's heads [H,n,D] are taken
  * with the strides (D, n D) and B = 1. */
 int dadattn_paged_append_bf16(uint16_t* k_pages, uint16_t* v_pages, const int32_t* page_table, const int32_t* lengths,
                               const int32_t* starts, uint16_t* q_out, const void* q, const void* k_new, const void* v_new,
                               const int64_t* q_out_strides, const int64_t* q_strides, const int64_t* k_strides,
                               const int64_t* v_strides, int B, int T, int Hq, int Hkv, int D, int pages, int page_size,
-                              int max_pages, const double* freq, float factor, int rot_dim, int interleaved, int new_is_bf16,
+                              int max_pages, const uint64_t* turns, float factor, int rot_dim, int interleaved, int new_is_bf16,
                               dadattn_stream_t stream);
 
 /* Attention of the new tokens over all rows of their sequences, theirs among them, which are in their pages already: token i
@@ -497,7 +500,7 @@ int dadattn_decode_paged_bf16(uint16_t* out, float* lse, const uint16_t* q, cons
                               const int64_t* out_strides, const int64_t* q_strides, const int64_t* k_strides,
                               const int64_t* v_strides, uint16_t* k_pages, uint16_t* v_pages, const int32_t* page_table,
                               const int32_t* lengths, int B, int Hq, int Hkv, int D, int pages, int page_size, int max_pages,
-                              float scale, const double* freq, float factor, int rot_dim, int interleaved,
+                              float scale, const uint64_t* turns, float factor, int rot_dim, int interleaved,
                               dadattn_stream_t stream);
 
 /* The end of a step, behind its last layer: lengths[b] += the tokens that sequence b brought (starts as above). */

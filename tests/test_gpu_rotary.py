@@ -84,8 +84,8 @@ def test_far_positions(cuda, far):
         turns = far * Fraction(w) / (2 * pi)
         turns -= turns.numerator // turns.denominator
         angle = torch.tensor(float(turns * 2 * pi), dtype=torch.float64)
-        # the fraction of a turn per position: 2^-53 and 2^-65 of it, times the position
-        allowed = 2.0 ** -21 + 6.3 * abs(far) * (2.0 ** -53 * w + 2.0 ** -65)
+        # the fraction of a turn per position: half a unit of 2^-64, and its forming in 64 bits of mantissa, times the position
+        allowed = 2.0 ** -21 + 6.3 * abs(far) * (2.0 ** -62 * w + 2.0 ** -65)
         assert abs(y[0, 0, 0, i].item() - torch.cos(angle).item()) <= allowed
         assert abs(y[0, 0, 0, 64 + i].item() - torch.sin(angle).item()) <= allowed
 
@@ -132,9 +132,9 @@ def test_refusals(cuda):
         dad.rotary_forward(y, None, torch.zeros(2, 5, 4, 66, device=cuda)[..., 1:65], None, r)
     with pytest.raises(RuntimeError, match="over each other"):
         dad.rotary_forward(torch.empty(2, 5, 1, 64, device=cuda).expand(2, 5, 4, 64), None, x, None, r)
-    with pytest.raises(ValueError, match="freq"):
+    with pytest.raises(ValueError, match="turns"):
         bad = dad.RotaryPositions(32, device=cuda)
-        bad.freq = bad.freq[:3]
+        bad.turns = bad.turns[:3]
         dad.rotary_forward(y, None, x, None, bad)
     # a broadcast input is read as it is
     one = torch.randn(2, 5, 1, 64, device=cuda)

@@ -17,7 +17,7 @@ def _strides(*s):
 
 def _rotary(lib, **change):
     s = _strides(10 * 4 * 64, 4 * 64, 64)
-    a = dict(q_out=P, k_out=P, q=P, k=P, qo=s, ko=s, qs=s, ks=s, positions=None, first=0, B=2, S=10, Hq=4, Hk=4, D=64, freq=P,
+    a = dict(q_out=P, k_out=P, q=P, k=P, qo=s, ko=s, qs=s, ks=s, positions=None, first=0, B=2, S=10, Hq=4, Hk=4, D=64, turns=P,
              factor=1.0, rot=64, interleaved=0, backward=0, bf16=1, stream=None)
     a.update(change)
     return lib.dadattn_rotary(*a.values())
@@ -26,7 +26,7 @@ def _rotary(lib, **change):
 def _append(lib, **change):
     s = _strides(4 * 64, 64)
     a = dict(k=P, v=P, table=P, lengths=P, starts=P, q_out=P, q=P, k_new=P, v_new=P, qo=s, qs=s, ks=s, vs=s, B=2, T=10, Hq=4,
-             Hkv=4, D=64, pages=9, page=16, max_pages=4, freq=P, factor=1.0, rot=64, interleaved=0, bf16=1, stream=None)
+             Hkv=4, D=64, pages=9, page=16, max_pages=4, turns=P, factor=1.0, rot=64, interleaved=0, bf16=1, stream=None)
     a.update(change)
     return lib.dadattn_paged_append_bf16(*a.values())
 
@@ -42,7 +42,7 @@ def _attention(lib, **change):
 def _decode(lib, **change):
     s = _strides(8 * 64, 64)
     a = dict(out=P, lse=None, q=P, k_new=P, v_new=P, os=s, qs=s, ks=s, vs=s, k=P, v=P, table=P, lengths=P, B=2, Hq=8, Hkv=4,
-             D=64, pages=9, page=16, max_pages=4, scale=0.125, freq=P, factor=1.0, rot=64, interleaved=0, stream=None)
+             D=64, pages=9, page=16, max_pages=4, scale=0.125, turns=P, factor=1.0, rot=64, interleaved=0, stream=None)
     a.update(change)
     return lib.dadattn_decode_paged_bf16(*a.values())
 
@@ -56,8 +56,8 @@ def _advance(lib, **change):
 NAN, INF = float("nan"), float("inf")
 BAD = [(_rotary, c, rc) for c, rc in [
     (dict(q=None), -1), (dict(k_out=None), -1), (dict(qs=None), -1), (dict(B=0), -1), (dict(S=-1), -1), (dict(Hk=-1), -1),
-    (dict(D=72), -2), (dict(D=272), -2), (dict(rot=0), -1), (dict(rot=80), -1), (dict(rot=8), -2), (dict(freq=None), -1),
-    (dict(freq=P + 4), -1), (dict(factor=NAN), -1), (dict(factor=INF), -1), (dict(q=P + 8), -1), (dict(positions=P + 2), -1),
+    (dict(D=72), -2), (dict(D=272), -2), (dict(rot=0), -1), (dict(rot=80), -1), (dict(rot=8), -2), (dict(turns=None), -1),
+    (dict(turns=P + 8), -1), (dict(factor=NAN), -1), (dict(factor=INF), -1), (dict(q=P + 8), -1), (dict(positions=P + 2), -1),
     (dict(qs=_strides(640, 64, 4)), -1), (dict(qs=_strides(640, 64, -64)), -1), (dict(qo=_strides(640, 0, 64)), -1),
     (dict(q_out=2 * P, qo=_strides(0, 256, 64)), -1), (dict(qs=_strides(2560, 64, 640)), -1), (dict(Hq=1 << 20), -2)]]
 PAGED = [(dict(k=None), -1), (dict(table=None), -1), (dict(lengths=None), -1), (dict(B=0), -1), (dict(Hkv=0), -1), (dict(pages=0), -1),
@@ -66,7 +66,7 @@ PAGED = [(dict(k=None), -1), (dict(table=None), -1), (dict(lengths=None), -1), (
 BAD += [(call, c, rc) for call in (_append, _attention, _decode) for c, rc in PAGED]
 BAD += [(_append, c, rc) for c, rc in [
     (dict(T=0), -1), (dict(starts=None), -1), (dict(starts=P + 2), -1), (dict(rot=8), -2), (dict(rot=-16), -1), (dict(rot=128), -1),
-    (dict(freq=None), -1), (dict(q_out=None), -1), (dict(q=None), -1), (dict(k_new=None), -1), (dict(v_new=P + 8), -1),
+    (dict(turns=None), -1), (dict(q_out=None), -1), (dict(q=None), -1), (dict(k_new=None), -1), (dict(v_new=P + 8), -1),
     (dict(ks=None), -1), (dict(ks=_strides(256, 60)), -1), (dict(ks=_strides(-256, 64)), -1), (dict(qo=_strides(0, 64)), -1),
     (dict(bf16=0), -1), (dict(q_out=2 * P, Hq=1 << 20), -2), (dict(qs=_strides(512, 64)), -1)]]   # (bf16=0: fp32 queries in place)
 BAD += [(_attention, c, rc) for c, rc in [
@@ -76,7 +76,7 @@ BAD += [(_attention, c, rc) for c, rc in [
     (dict(qs=_strides(512, 0)), -1), (dict(qs=_strides(512, 4)), -1), (dict(T=1 << 30, B=1 << 29), -2), (dict(T=1 << 26, Hkv=1024, Hq=1024), -2)]]
 BAD += [(_decode, c, rc) for c, rc in [
     (dict(out=None), -1), (dict(v_new=None), -1), (dict(Hq=6), -1), (dict(scale=0.0), -1), (dict(scale=NAN), -1), (dict(rot=24), -2),
-    (dict(freq=None), -1), (dict(lse=P + 1), -1), (dict(q=P + 4), -1), (dict(os=_strides(512, 0)), -1), (dict(B=1 << 27), -2)]]
+    (dict(turns=None), -1), (dict(lse=P + 1), -1), (dict(q=P + 4), -1), (dict(os=_strides(512, 0)), -1), (dict(B=1 << 27), -2)]]
 BAD += [(_advance, c, rc) for c, rc in [
     (dict(lengths=None), -1), (dict(lengths=P + 2), -1), (dict(B=0), -1), (dict(T=0), -1), (dict(starts=None), -1), (dict(page=10), -2),
     (dict(max_pages=0), -1)]]
@@ -113,6 +113,24 @@ def test_frequencies_refused(lib, bad):
         dad.RotaryPositions(**bad, device="cpu")
     with pytest.raises(ValueError, match="unknown scaling"):
         dad.RotaryPositions(64, scaling="other", device="cpu")
+
+
+def test_turns(lib):
+    """Fractions of a turn, rounded to 2^-64: from fractions with 50 digits of pi."""
+    from fractions import Fraction
+    freq = dad.RotaryPositions(128, device="cpu").freq.tolist() + [-0.25, 0.0, 6.5, 1000.125]
+    a, got = (C.c_double * len(freq))(*freq), (C.c_uint64 * len(freq))()
+    assert lib.dadattn_rotary_turns(got, a, len(freq)) == 0
+    pi = Fraction(31415926535897932384626433832795028841971693993751, 10 ** 49)
+    for w, t in zip(freq, got):
+        want = Fraction(w) / (2 * pi)
+        off = (Fraction(t, 2 ** 64) - want) % 1
+        # half a unit, and the product's rounding in 64 bits of mantissa
+        assert min(off, 1 - off) <= Fraction(1, 2 ** 64) + abs(want) / 2 ** 62
+    assert lib.dadattn_rotary_turns(None, a, 1) == -1 and lib.dadattn_rotary_turns(got, None, 1) == -1
+    assert lib.dadattn_rotary_turns(got, a, 0) == -1
+    for bad in (NAN, INF, 1e30):
+        assert lib.dadattn_rotary_turns(got, (C.c_double * 1)(bad), 1) == -1
 
 
 def test_tensors_are_checked_in_python(lib):
