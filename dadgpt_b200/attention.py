@@ -269,25 +269,18 @@ class RotaryPositions:
         self.turns = turns.to(device)
 
 
-def _turn(backward, q_out, k_out, q, k, rotary, positions, first):
-    if q.dim() != 4 or (k is not None and k.dim() != 4):
-        raise ValueError("q and k must be [B, S, heads, D]")
-    B, S, H, D = q.shape
-    _native().rotary(backward, B, S, H, 0 if k is None else k.shape[2], D, first, rotary.turns, rotary.factor, rotary.rot_dim,
-                     rotary.interleaved, q_out, k_out, q, k, positions)
-
-
 def rotary_forward(q_out, k_out, q, k, rotary: RotaryPositions, *, positions=None, first=0):
     """Queries [B,S,H,D] and keys [B,S,Hk,D] (fp32 or bf16) turned by their positions: ``positions`` [B,S] int32 on the device,
     or first + s. Any order in memory with neighbouring elements in a row: heads-split tensors are passed as
     ``x.view(B, H, S, D).transpose(1, 2)``, activations [B*S, H*D] as ``x.view(B, S, H, D)``. The results may be the tensors
     themselves; k and k_out may be None."""
-    _turn(0, q_out, k_out, q, k, rotary, positions, first)
+    _native().rotary(0, first, rotary.turns, rotary.factor, rotary.rot_dim, rotary.interleaved, q_out, k_out, q, k, positions)
 
 
 def rotary_backward(dq, dk, dq_turned, dk_turned, rotary: RotaryPositions, *, positions=None, first=0):
     """Backward of the call above: gradients of the turned tensors to those of the tensors."""
-    _turn(1, dq, dk, dq_turned, dk_turned, rotary, positions, first)
+    _native().rotary(1, first, rotary.turns, rotary.factor, rotary.rot_dim, rotary.interleaved, dq, dk, dq_turned, dk_turned,
+                     positions)
 
 
 class KVCachePagedBF16:
@@ -311,35 +304,26 @@ def _rotary_args(rotary):
     return (None, 1.0, 0, 0) if rotary is None else (rotary.turns, rotary.factor, rotary.rot_dim, rotary.interleaved)
 
 
-def _packed(name, x):
-    if x.dim() != 3:
-        raise ValueError(f"{name} must be [tokens, heads, D], got {tuple(x.shape)}")
-    return x.shape
-
-
 def kv_cache_append_paged(cache: KVCachePagedBF16, k_new, v_new, starts=None, *, q=None, q_out=None, rotary=None):
     """The new rows of a packed batch, k_new and v_new [T,H,D] bf16 or fp32, to their pages: sequence b's are rows
     starts[b] .. starts[b+1]-1 (int32 [B+1]; None: one for each sequence) and become its rows lengths[b] and on, which stay the
     lengths until :func:`kv_cache_advance_paged`. With ``rotary``, keys are turned by their rows, and so are queries q
     [T,Hq,D], into q_out (bf16)."""
-    T = _packed("k_new", k_new)[0]
-    Hq = 0 if q is None else _packed("q", q)[1]
-    _native().append_paged(*cache._args(), *_rotary_args(rotary), T, Hq, starts, q_out, q, k_new, v_new)
+    _native().append_paged(*cache._args(), *_rotary_args(rotary), starts, q_out, q, k_new, v_new)
 
 
 def paged_attention_bf16(out, q, cache: KVCachePagedBF16, starts, max_new, scale, *, lse=None):
     """Causal attention of a packed batch's new tokens, q [T,Hq,D] bf16, over all rows of their sequences, whose pages hold
     theirs already (:func:`kv_cache_append_paged`): token i of sequence b sees rows j <= lengths[b] + i. ``max_new``: no sequence
     brings more tokens. Hq a multiple of the cache's heads. out [T,Hq,D]; lse [T,Hq] fp32 where it is wanted."""
-    T, Hq, _ = _packed("q", q)
-    _native().paged_attention(*cache._args(), T, max_new, Hq, scale, starts, out, lse, q)
+    _native().paged_attention(*cache._args(), max_new, scale, starts, out, lse, q)
 
 
 def decode_attention_paged_bf16(out, q, k_new, v_new, cache: KVCachePagedBF16, scale, *, rotary=None, lse=None):
     """One decode step for every sequence of a paged cache: the token is turned by its row (with ``rotary``), appended and
     attended for, q, out [B,Hq,D], k_new, v_new [B,H,D] bf16. The lengths stay what they are until
     :func:`kv_cache_advance_paged`: layers share them."""
-    _native().decode_paged(*cache._args(), *_rotary_args(rotary), _packed("q", q)[1], scale, out, lse, q, k_new, v_new)
+    _native().decode_paged(*cache._args(), *_rotary_args(rotary), scale, out, lse, q, k_new, v_new)
 
 
 def kv_cache_advance_paged(cache: KVCachePagedBF16, starts=None, tokens=None):

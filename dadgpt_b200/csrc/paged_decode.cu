@@ -17,6 +17,8 @@
 //   * four consumer warps, 16 rows of a tile each, with a running maximum and sum of their own. Scores and probabilities stay in
 //     registers: as a result they lie transposed to the next product's operand, which movmatrix puts right. Accumulators are
 //     rescaled only when the maximum has grown by 2^8.
+//   * turned queries are not rounded to bf16: what rounding leaves is a second operand, whose products are as good as free here
+//     (rounded, the result's error against 64 bits was 2.7e-3 and more of its norm; 2.1e-3 without, as without a rotation).
 //   * the new token needs no row of the cache: its scores, with k as rounded for the cache, are where one warp's running
 //     maximum begins, and v its accumulator.
 // Measured (us, rotating caches): 64 sequences of 9 .. 1023 rows, 12 heads of 64 21 (4.9 TB/s), all of 1000 38-39 (5.1); 8 of
@@ -71,7 +73,7 @@ struct DecodeShared {
   float m[kWarps][kRows], l[kWarps][kRows];
   float m_all[kRows], l_all[kRows];           // of the CTA, read by the cluster's others
   __align__(16) float2 table[kMaxRotaryHead / 4];   // (cos, sin): D / 2 at most
-  __align__(16) bf16 q[8 * NT][D + 8];
+  __align__(16) bf16 q[2][8 * NT][D + 8];           // turned queries in two parts, the second what rounding left of the first
   __align__(16) bf16 k_new[D], v_new[D];
 };
 
@@ -275,12 +277,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     if (!can_append) sh.bad = 1;
     const int64_t new_row = (((static_cast<int64_t>(new_page) * c.heads + kv_head) << c.page_shift) +
                              (ahead & ((1 << c.page_shift) - 1))) * D;
+    const bool turned = p.r.rot > 0;
     for (int i = t; i < pieces; i += kConsumers) {
       const int row = i / kUnits, u = i % kUnits;
       const bool is_v = row == (8 * NT) + 1;
       const int first = is_v ? u * kTurnUnit : unit_first(u, p.r), second = is_v ? 8 : unit_second(u, p.r);
       if (row >= (8 * NT) && !last_rank) continue;
-      Sixteen<bf16> x;
+      Sixteen<bf16> x, rest;
+      rest.a = rest.b = make_uint4(0, 0, 0, 0);
       if (row < (8 * NT)) {
         if (row < rows) x.load(p.q, b * p.q_token + (head0 + row) * p.q_head + first, second);
         else x.a = x.b = make_uint4(0, 0, 0, 0);
@@ -297,8 +301,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         for (int k = 0; k < 8; ++k) cs[k] = sh.table[u * 8 + k];
         turn_unit(f, cs, p.r.interleaved);
         x.from_floats(f);
+        float g[16];
+        x.to_floats(g);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) f[k] -= g[k];
+        rest.from_floats(f);
       }
-      x.store(row < (8 * NT) ? sh.q[row] : is_v ? sh.v_new : sh.k_new, first, second);
+      if (turned && row < (8 * NT)) rest.store(sh.q[1][row], first, second);
+      x.store(row < (8 * NT) ? sh.q[0][row] : is_v ? sh.v_new : sh.k_new, first, second);
       if (row >= (8 * NT) && part == 0 && can_append) x.store(is_v ? p.v_pages : p.k_pages, new_row + first, second);
     }
     consumers_meet();
@@ -310,7 +320,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          qf[s][t][h] = *reinterpret_cast<const uint32_t*>(&sh.q[8 * t + lane / 4][s * 16 + (lane % 4) * 2 + 8 * h]);
+          qf[s][t][h] = *reinterpret_cast<const uint32_t*>(&sh.q[0][8 * t + lane / 4][s * 16 + (lane % 4) * 2 + 8 * h]);
+    auto rest_of = [&](int s, int t, int h) {
+      return *reinterpret_cast<const uint32_t*>(&sh.q[1][8 * t + lane / 4][s * 16 + (lane % 4) * 2 + 8 * h]);
+    };
     const float scale_log2 = p.scale * kLog2e;
 #pragma unroll
     for (int i = 0; i < kSteps; ++i)
@@ -323,8 +336,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
         for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            fma_bf16(dot, qf[s][t][h], *reinterpret_cast<const uint32_t*>(&sh.k_new[s * 16 + (lane % 4) * 2 + 8 * h]));
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t k = *reinterpret_cast<const uint32_t*>(&sh.k_new[s * 16 + (lane % 4) * 2 + 8 * h]);
+            fma_bf16(dot, qf[s][t][h], k);
+            if (turned) fma_bf16(dot, rest_of(s, t, h), k);
+          }
         float d = dot.x + dot.y;
         d += __shfl_xor_sync(0xffffffffu, d, 1);
         d += __shfl_xor_sync(0xffffffffu, d, 2);
@@ -362,6 +378,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           ldmatrix4(k_tile + (ch / 8) * L::kPanelBytes + key * 128 + (((ch & 7) ^ (key & 7)) << 4), kf);
 #pragma unroll
           for (int t = 0; t < NT; ++t) mma_16816(sc[t], kf, qf[step][t][0], qf[step][t][1]);
+          if (turned) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) mma_16816(sc[t], kf, rest_of(step, t, 0), rest_of(step, t, 1));
+          }
         }
         if (there < kWarpRows) {
           // Rows that are not there: no score, and a V of zeros (what the page holds there could be anything).

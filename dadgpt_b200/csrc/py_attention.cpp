@@ -90,6 +90,23 @@ class Args {
     PyErr_Format(PyExc_ValueError, "%s is on cuda:%d, the current device is cuda:%d", name, static_cast<int>(t.get_device()), current);
     throw Bad{};
   }
+  // size `dim` of the `ahead`-th argument from the next, a tensor of `dims` dimensions (`layout` says which)
+  int size_of(int ahead, const char* name, int dims, int dim, const char* layout) {
+    i_ += ahead;
+    const at::Tensor& t = tensor(name);
+    i_ -= ahead + 1;
+    if (t.dim() != dims) {
+      PyErr_Format(PyExc_ValueError, "%s must be %s, got %d dimensions", name, layout, static_cast<int>(t.dim()));
+      throw Bad{};
+    }
+    const int64_t n = t.size(dim);
+    if (n != static_cast<int>(n)) {
+      PyErr_Format(PyExc_ValueError, "size %lld out of range", static_cast<long long>(n));
+      throw Bad{};
+    }
+    return static_cast<int>(n);
+  }
+  bool none_at(int ahead) const { return a_[i_ + ahead] == Py_None; }
   // the type of the next argument, a tensor
   at::ScalarType peek_type(const char* name) {
     const at::ScalarType type = tensor(name).scalar_type();
@@ -615,14 +632,18 @@ struct Rotary {
   }
   int64_t n = 0;
 };
+constexpr const char* kPacked = "[tokens, heads, D]";
 const int32_t* ints(const at::Tensor& t) { return static_cast<const int32_t*>(t.data_ptr()); }
 
-// backward, B, S, Hq, Hk, D, first, turns, factor, rot_dim, interleaved, q_out, k_out or None, q, k or None, positions or None
+// backward, first, turns, factor, rot_dim, interleaved, q_out, k_out or None, q, k or None, positions or None
 PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    Args p(a, n, 16, "rotary");
-    const int back = p.integer(), B = p.integer(), S = p.integer(), Hq = p.integer(), Hk = p.integer(), D = p.integer();
+    Args p(a, n, 11, "rotary");
+    const int back = p.integer();
     const int64_t first = p.integer64();
+    const char* const layout = "[B, S, heads, D]";   // (q and k are behind the rotation's four arguments, q_out and k_out)
+    const int B = p.size_of(6, "q", 4, 0, layout), S = p.size_of(6, "q", 4, 1, layout), Hq = p.size_of(6, "q", 4, 2, layout),
+              D = p.size_of(6, "q", 4, 3, layout), Hk = p.none_at(7) ? 0 : p.size_of(7, "k", 4, 2, layout);
     const Rotary r(p);
     const at::ScalarType type = p.peek_type("q_out") == kB ? kB : kF;
     int64_t s[4][3] = {};   // q_out, k_out, q, k
@@ -650,13 +671,13 @@ struct Paged {
         table(ints(p.here("page_table", at::kInt, {B, max_pages}))), lengths(ints(p.here("lengths", at::kInt, {B}))) {}
 };
 
-// paged cache, rotary, T, Hq, starts or None, q_out or None, q or None, k_new, v_new
+// paged cache, rotary, starts or None, q_out or None, q or None, k_new, v_new
 PyObject* append_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    Args p(a, n, 21, "append_paged");
+    Args p(a, n, 19, "append_paged");
+    const int T = p.size_of(17, "k_new", 3, 0, kPacked), Hq = p.none_at(16) ? 0 : p.size_of(16, "q", 3, 1, kPacked);
     const Paged c(p);
     const Rotary r(p);
-    const int T = p.integer(), Hq = p.integer();
     const int32_t* const starts = p.none() ? nullptr : ints(p.here("starts", at::kInt, {int64_t(c.B) + 1}));
     int64_t s[4][2] = {};
     uint16_t* const qo = p.none() ? nullptr : b16(p.strided("q_out", kB, {T, Hq, c.D}, s[0]));
@@ -676,12 +697,13 @@ PyObject* append_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// paged cache, T, max_new, Hq, scale, starts or None, out, lse or None, q
+// paged cache, max_new, scale, starts or None, out, lse or None, q
 PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    Args p(a, n, 18, "paged_attention");
+    Args p(a, n, 16, "paged_attention");
+    const int T = p.size_of(15, "q", 3, 0, kPacked), Hq = p.size_of(15, "q", 3, 1, kPacked);
     const Paged c(p);
-    const int T = p.integer(), max_new = p.integer(), Hq = p.integer();
+    const int max_new = p.integer();
     const float scale = p.real();
     const int32_t* const starts = p.none() ? nullptr : ints(p.here("starts", at::kInt, {int64_t(c.B) + 1}));
     int64_t s[2][2] = {};
@@ -696,13 +718,13 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// paged cache, rotary, Hq, scale, out, lse or None, q, k_new, v_new
+// paged cache, rotary, scale, out, lse or None, q, k_new, v_new
 PyObject* decode_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    Args p(a, n, 21, "decode_paged");
+    Args p(a, n, 20, "decode_paged");
+    const int Hq = p.size_of(17, "q", 3, 1, kPacked);
     const Paged c(p);
     const Rotary r(p);
-    const int Hq = p.integer();
     const float scale = p.real();
     int64_t s[4][2] = {};
     uint16_t* const out = b16(p.strided("out", kB, {c.B, Hq, c.D}, s[0]));

@@ -41,9 +41,12 @@ inline int check_rotary(const char* name, const uint64_t* turns, float factor, i
 }
 
 inline int current_sm_count() {
+  static std::atomic<int> seen[64];   // by device
   int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 148;   // (only rules of speed go by it; a call without a device fails at its launch)
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;   // (only rules of speed go by it; a call without a
+  if ((sms = seen[dev].load(std::memory_order_relaxed))) return sms;            // device fails at its launch)
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  seen[dev].store(sms, std::memory_order_relaxed);
   return sms;
 }
 
