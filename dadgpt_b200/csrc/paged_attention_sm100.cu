@@ -202,8 +202,7 @@ __device__ __forceinline__ Share share_of(const Item& it, const ChunkParams& p, 
 // that what starts last is short (one sequence after the other, each key head by itself: 16 prompts of up to 1024 tokens 46 us
 // instead of 36). An item's weight is twice its keys; one tile counts half, since both groups work on it. How many items of a
 // sequence reach a weight is an expression, so that the 64th of the range of weights in which the x-th falls is found by
-// halving, and the item in it by counting. (To the last bit of the weight the search took 1.6 us, 4-8 % of whole calls; this
-// one a third of that.) Where all items start at once (`sorted` false) the order does not matter.
+// halving, and the item in it by counting. (To the last bit of the weight the search took 1.6 us, 4-8 % of whole calls.) Where all items start at once (`sorted` false) the order does not matter.
 __device__ __forceinline__ Item find_item(const ChunkParams& p, unsigned block, bool sorted) {
   const PagedCache& c = p.cache;
   const int lane = threadIdx.x % 32, tokens = p.item_tokens;
@@ -235,34 +234,30 @@ __device__ __forceinline__ Item find_item(const ChunkParams& p, unsigned block, 
     } else {
       // (keys are 2^30 at most, DADATTN_MAX_CACHE_LEN: weights are unsigned)
       const bool one = count - (mine - 1) * tokens <= p.tile_tokens && tokens > p.tile_tokens;   // the last item is one tile
-      const unsigned keys = ahead + count, last = one ? keys : 2 * keys;
-      const unsigned most = __reduce_max_sync(0xffffffffu, mine ? 2 * keys : 0u);
-      const int unit = max(0, 26 - __clz(most));   // most < 64 << unit
+      const unsigned keys = ahead + count, most = __reduce_max_sync(0xffffffffu, mine ? 2 * keys : 0u);
+      const int unit = max(1, 26 - __clz(most));   // most < 64 << unit
+      const int whole = max(mine - 1, 0), last = mine > 0 ? static_cast<int>((one ? keys : 2 * keys) >> unit) : -1;
       // the first of the sequence's whole items that reaches so many units, behind which all do; the last one is its own
-      auto from = [&](unsigned units) -> int {
-        const int need = static_cast<int>((static_cast<uint64_t>(units) << unit) + 1 >> 1) - ahead;   // keys
-        const int i = need <= tokens ? 0 : (p.token_shift >= 0 ? (need + tokens - 1) >> p.token_shift : (need + tokens - 1) / tokens) - 1;
-        return min(i, max(mine - 1, 0));
+      auto from = [&](int units) -> int {
+        const int need = static_cast<int>(static_cast<unsigned>(units) << (unit - 1)) - ahead + tokens - 1;   // keys, to be divided
+        return min(max((p.token_shift >= 0 ? need >> p.token_shift : need / tokens) - 1, 0), whole);
       };
-      auto last_reaches = [&](unsigned units) -> bool { return mine > 0 && last >> unit >= units; };
-      auto reach = [&](unsigned units) -> int { return max(mine - 1, 0) - from(units) + last_reaches(units); };
-      unsigned low = 0;   // the most units that more than x items reach
-#pragma unroll 1
-      for (unsigned step = 32; step; step >>= 1)
-        if (__reduce_add_sync(0xffffffffu, reach(low + step)) > x) low += step;
-      const int above = __reduce_add_sync(0xffffffffu, reach(low + 1)), here = from(low + 1);
-      const bool with_last = last_reaches(low) && !last_reaches(low + 1);
-      const int with = here - from(low) + with_last;   // the sequence's items of so many units
+      auto reach = [&](int units) -> int { return whole - from(units) + (last >= units); };
+      int low = 0;   // the most units that more than x items reach
+#pragma unroll
+      for (int step = 32; step; step >>= 1)
+        if (__reduce_add_sync(0xffffffffu, reach(low + step)) > static_cast<int>(x)) low += step;
+      const int here = from(low + 1), with = here - from(low) + (last == low);   // the sequence's items of so many units
+      const int rest = static_cast<int>(x) - __reduce_add_sync(0xffffffffu, whole - here + (last > low));
       int upto = with;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int other = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += other;
       }
-      const int rest = static_cast<int>(x) - above;
       at = __ffs(__ballot_sync(0xffffffffu, upto > rest)) - 1;
       const int nth = rest - (upto - with);   // of them: the last one, then the others from behind
-      index = __shfl_sync(0xffffffffu, with_last && nth == 0 ? mine - 1 : here - 1 - nth + with_last, at);
+      index = __shfl_sync(0xffffffffu, last == low && nth == 0 ? mine - 1 : here - 1 - nth + (last == low), at);
     }
     it.b = base + at;
     it.token0 = index * tokens;

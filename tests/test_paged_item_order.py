@@ -7,32 +7,31 @@ def _find(x, ahead, count, tokens):
     """The x-th item of up to 32 sequences: (sequence, index), and its weight in units, by the kernel's arithmetic."""
     n = len(count)
     mine = [(c + tokens - 1) // tokens for c in count]
-    last = [(1 if c - (m - 1) * tokens <= tokens // 2 else 2) * (a + c) for a, c, m in zip(ahead, count, mine)]
-    most = max(2 * (a + c) if m else 0 for a, c, m in zip(ahead, count, mine))
+    keys = [a + c for a, c in zip(ahead, count)]
+    most = max(2 * k if m else 0 for k, m in zip(keys, mine))
     assert most < 2 ** 32
-    unit = max(0, most.bit_length() - 6)
+    unit = max(1, most.bit_length() - 6)
     assert most < 64 << unit
+    whole = [max(m - 1, 0) for m in mine]
+    last = [(k if c - (m - 1) * tokens <= tokens // 2 else 2 * k) >> unit if m else -1 for k, c, m in zip(keys, count, mine)]
 
     def start(i, units):
-        need = ((units << unit) + 1 >> 1) - ahead[i]
+        need = (units << (unit - 1)) - ahead[i] + tokens - 1
         assert abs(need) < 2 ** 31
-        return min(0 if need <= tokens else (need + tokens - 1) // tokens - 1, max(mine[i] - 1, 0))
-
-    def last_reaches(i, units):
-        return mine[i] > 0 and last[i] >> unit >= units
+        quotient = abs(need) // tokens * (1 if need >= 0 else -1)   # (as C divides; a shift would go below: both are clamped)
+        return min(max(quotient - 1, 0), whole[i])
 
     def reach(i, units):
-        return max(mine[i] - 1, 0) - start(i, units) + last_reaches(i, units)
+        return whole[i] - start(i, units) + (last[i] >= units)
 
     low, step = 0, 32
     while step:
         if sum(reach(i, low + step) for i in range(n)) > x:
             low += step
         step >>= 1
-    rest = x - sum(reach(i, low + 1) for i in range(n))
+    rest = x - sum(whole[i] - start(i, low + 1) + (last[i] > low) for i in range(n))
     for i in range(n):
-        with_last = last_reaches(i, low) and not last_reaches(i, low + 1)
-        here = start(i, low + 1)
+        here, with_last = start(i, low + 1), last[i] == low
         have = here - start(i, low) + with_last
         if rest < have:
             return (i, mine[i] - 1 if with_last and rest == 0 else here - 1 - rest + with_last), low, unit
