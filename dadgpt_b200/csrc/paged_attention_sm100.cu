@@ -429,16 +429,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         const Share s = share_of<CLUSTER>(it, p, rank);
         const int total = it.ahead + it.count;   // rows of the sequence
         const int32_t* table = c.table + static_cast<int64_t>(it.b) * c.max_pages;
-        // the page of this lane's box; -1: no row of it is there
-        auto look_up = [&](int tile) -> int {
-          const int row = tile * kT + box * p.chunk;
-          if (panel >= L::kPanels || row >= total) return -1;
-          const int page = table[row >> c.page_shift];
-          if (page >= 0 && page < c.pages) return page;
-          bars->item[e][6] = bars->any_bad = 1;
-          return -2;
-        };
-        int page = s.n_kv > 0 ? look_up(s.lo) : -1;
+        // Whether a row of this lane's box of a tile is there, and its page (looked at only when the box is fetched).
+        auto there = [&](int tile) { return panel < L::kPanels && tile * kT + box * p.chunk < total; };
+        auto look_up = [&](int tile) -> int { return there(tile) ? table[(tile * kT + box * p.chunk) >> c.page_shift] : 0; };
+        int page = s.n_kv > 0 ? look_up(s.lo) : 0;
         for (int j = 0; ok && j < s.n_kv; ++j) {
           const int tile = s.lo + j, mine = page;
           // The next block is asked for only now: what a CTA holds in advance no idle CTA can take.
@@ -447,13 +441,15 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
           const int boxes = min((total - tile * kT + p.chunk - 1) / p.chunk, per_tile);
           const int row = tile * kT + box * p.chunk;
           // (a row coordinate outside the pool reads zeros)
-          const int y = mine >= 0 ? ((mine * c.heads + it.kv_head) << c.page_shift) + (row & ((1 << c.page_shift) - 1)) : -kMaxPage;
+          const bool good = mine >= 0 && mine < c.pages, mine_there = there(tile);
+          if (!good) bars->item[e][6] = bars->any_bad = 1;
+          const int y = good ? ((mine * c.heads + it.kv_head) << c.page_shift) + (row & ((1 << c.page_shift) - 1)) : -kMaxPage;
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
             if (n_loaded >= kSlots && !(ok = warp_wait(&bars->slot_empty[slot], parity ^ 1u, abort_flag))) break;
             if (lane == 0) mbar_arrive_expect_tx(&bars->slot_full[slot], boxes * L::kPanels * p.chunk * 128);
             __syncwarp();
-            if (mine != -1)
+            if (mine_there)
               tma_load_3d(smem + L::kKV + slot * L::kTileBytes + panel * kPanel + box * p.chunk * 128, m ? &map_v : &map_k,
                           &bars->slot_full[slot], panel * 64, y, 0);
             __syncwarp();
