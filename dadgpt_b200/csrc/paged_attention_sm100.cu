@@ -546,7 +546,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             const SmemDescBase v_desc{kv_desc0.lo + v.at * (L::kTileBytes >> 4) + h * (kN * 128 >> 4), kv_desc0.hi};
 #pragma unroll
             for (int part = 0; part < kN / 64; ++part) {
-              if (!(ok = mbar_wait(&bars->p_full[x][part], g & 1, abort_flag))) break;
+              // (polled for a while before the wait that suspends: 1.5 % at head size 128. Polls by the softmax threads: -2 %.)
+              if (!(ok = mbar_wait_at<24>(&bars->p_full[x][part], g & 1, abort_flag, __LINE__))) break;
               tc_fence_after_sync();
 #pragma unroll
               for (int kk = 4 * part; kk < 4 * part + 4; ++kk)
