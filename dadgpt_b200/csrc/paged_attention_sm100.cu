@@ -108,7 +108,10 @@ struct ChunkParams {
 
 __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
   float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 __device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
@@ -202,7 +205,8 @@ __device__ __forceinline__ Share share_of(const Item& it, const ChunkParams& p, 
 // that what starts last is short (one sequence after the other, each key head by itself: 16 prompts of up to 1024 tokens 46 us
 // instead of 36). An item's weight is twice its keys; one tile counts half, since both groups work on it. How many items of a
 // sequence reach a weight is an expression, so that the 64th of the range of weights in which the x-th falls is found by
-// halving, and the item in it by counting. (To the last bit of the weight the search took 1.6 us, 4-8 % of whole calls.) Where all items start at once (`sorted` false) the order does not matter.
+// halving, and the item in it by counting. (To the last bit of the weight the search took 1.6 us, 4-8 % of whole calls.) Where
+// all items start at once (`sorted` false) the order does not matter.
 __device__ __forceinline__ Item find_item(const ChunkParams& p, unsigned block, bool sorted) {
   const PagedCache& c = p.cache;
   const int lane = threadIdx.x % 32, tokens = p.item_tokens;
@@ -362,7 +366,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       for (int w = 0; w < 4; ++w) bars->exps[x][w] = 0;
     }
     mbar_init(&bars->joined, 8);
-    mbar_init(&bars->parted, 8);
+    // softmax warps and, where another item may follow, the issuers: one whose group has no keys of a tile would not be missed
+    // otherwise, and could find the barrier two items on
+    mbar_init(&bars->parted, CLUSTER == 1 ? 8 + 2 : 8);
     bars->abort_flag = 0;
     bars->any_bad = 0;
     fence_mbar_init();
@@ -563,7 +569,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
           if (!s.single)
             for (int j = s.n(x); ok && j < s.n_kv; ++j) ok = skip(gone + j);
           // (the groups' maxima and sums change hands where the next item's scores go)
-          if (s.single && CLUSTER == 1) ok = ok && mbar_wait(&bars->parted, joins++ & 1, abort_flag);
+          if (s.single && CLUSTER == 1 && ok) {
+            mbar_arrive(&bars->parted);
+            ok = mbar_wait(&bars->parted, joins++ & 1, abort_flag);
+          }
           gone += s.n_kv;
           feed.give_back();
         }
@@ -587,7 +596,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       const Tile t = it.tile(p, s.single ? 0 : x);
       const int steps = s.steps(x, kSteps), total = it.ahead + it.count;
       const bool active = quad * 32 < t.rows;          // whether the warp has a row
-      const int token = t.token0 + min(row, t.rows - 1) / p.group, limit = it.ahead + token;   // (rows that are not there: the last one's mask)
+      const int token = t.token0 + min(row, t.rows - 1) / p.group;   // (rows that are not there: the last one's mask)
+      const int limit = it.ahead + token;
       float m = -INFINITY, l = 0.f;   // running max (log2 units, scaled) and sum
       for (int k = 0; k < steps; ++k, ++g) {
         if (!(ok = mbar_wait(&bars->s_full[x], g & 1, abort_flag))) break;
