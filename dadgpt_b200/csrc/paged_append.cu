@@ -3,10 +3,10 @@
 //
 // Bound by HBM: every element is read and written once. As in rotary.cu a thread has one piece of 16 elements of a token and goes
 // through a group of its heads, of q, k or v. A CTA's tokens are next to each other; which sequences they belong to is counted
-// from `starts` by the whole CTA. A page holds the rows of a head one after the other, so a token's row of a head is a run of 128 or
-// 256 bytes.
-// Measured: 16 prompts, 14700 tokens, 32 query and 8 key heads of 128, turned, bf16 59.5 us (6.1 TB/s); 301 tokens of 12 heads of 64,
-// fp32, 3.0.
+// from `starts` by the whole CTA. A page holds the rows of a head one after the other, so a token's row of a head is a run of 128
+// or 256 bytes.
+// Measured: 16 prompts, 14700 tokens, 32 query and 8 key heads of 128, turned, bf16 59.5 us (6.1 TB/s); 301 tokens of 12 heads of
+// 64, fp32, 3.0.
 #include <initializer_list>
 
 #include "paged.cuh"
@@ -59,7 +59,8 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const AppendPara
     b = before;
     for (int j = 1; j <= at && j < n; ++j) b += later[j];
   }
-  if (at >= n || b >= c.B) return;   // (tokens behind the last sequence belong to nobody)
+  // (tokens behind the last sequence and ahead of the first belong to nobody)
+  if (at >= n || b >= c.B || (c.starts && t0 + at < c.starts[0])) return;
   int ahead, first, count;
   const int in = sequence_rows(c, b, p.T, ahead, first, count) ? t0 + at - first : -1;
   int page = -1;

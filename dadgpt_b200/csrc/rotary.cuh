@@ -70,7 +70,7 @@ __device__ __forceinline__ void sin_cos_eighth(float r, float* s, float* c) {
 }
 
 // (cos, sin) of position * turns, times the factor. EXACT: to fp32 accuracy, else to 2^-21 (for results in bf16, whose
-// rounding is 2^-9).
+// rounding is 2^-8).
 template <bool EXACT>
 __device__ __forceinline__ float2 cos_sin(int64_t position, uint64_t turns, float factor) {
   const uint64_t a = static_cast<uint64_t>(position) * turns;

@@ -153,3 +153,25 @@ def test_one_token_each(cuda):
         dad.kv_cache_append_paged(c, k, v.bfloat16())
     with pytest.raises(ValueError, match="q_out"):
         dad.kv_cache_append_paged(c, k, v, q=k, q_out=k)
+
+
+@pytest.mark.parametrize("rotate", [False, True])
+def test_rows_ahead_of_the_first_sequence_belong_to_nobody(cuda, rotate):
+    """starts[0] above 0: the packed rows ahead of it are another batch's, as those behind the last are."""
+    Hq, Hkv, D, ahead, counts, lead = 4, 2, 64, [3, 40], [17, 1], 37
+    c, starts, g = made(cuda, Hkv, D, 16, ahead, counts, 11)
+    n = sum(counts)
+    r = dad.RotaryPositions(D, device=cuda) if rotate else None
+    q, k, v = (torch.randn(lead + n + 5, h, D, generator=g, device=cuda).to(torch.bfloat16) for h in (Hq, Hkv, Hkv))
+    part = slice(lead, lead + n)
+    want = torch.full_like(q, 9.0)
+    dad.kv_cache_append_paged(c, k[part], v[part], starts, q=q[part], q_out=want[part], rotary=r)
+    want_pages = c.k.clone(), c.v.clone()
+    where = _places(c, ahead, counts)
+    for x in (c.k, c.v):
+        x[where[0], :, where[1]] = 0
+    q_out = torch.full_like(q, 9.0)
+    dad.kv_cache_append_paged(c, k, v, starts + lead, q=q, q_out=q_out, rotary=r)
+    assert torch.equal(c.k, want_pages[0]) and torch.equal(c.v, want_pages[1]) and torch.equal(q_out, want)
+    dad.kv_cache_advance_paged(c, starts + lead, lead + n + 5)
+    assert c.lengths.tolist() == [20, 41] and device_status() == 0

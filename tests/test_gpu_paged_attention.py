@@ -223,3 +223,16 @@ def test_rows_beyond_31_bits_of_bytes(cuda):
     o, _, ob, _ = attend(q[:1].double(), rows_of(c, c.k, 0, n + 1), rows_of(c, c.v, 0, n + 1), n, 0.09)
     check(out[:1], o, ob)
     assert device_status() == 0
+
+
+@pytest.mark.parametrize("many", [False, True], ids=["few", "many"])
+def test_rows_ahead_of_the_first_sequence_belong_to_nobody(cuda, many):
+    ahead, counts, lead = ([30, 200], [50, 1], 19) if not many else ([30, 200] * 40, [150, 1] * 40, 301)
+    c, starts, g = made(cuda, 2, 64, 16, ahead, counts, 41)
+    n = sum(counts)
+    q = torch.randn(lead + n + 3, 4, 64, generator=g, device=cuda).to(torch.bfloat16)
+    part = slice(lead, lead + n)
+    want, out = torch.full_like(q, 9.0), torch.full_like(q, 9.0)
+    dad.paged_attention_bf16(want[part], q[part], c, starts, max(counts), 0.125)
+    dad.paged_attention_bf16(out, q, c, starts + lead, max(counts), 0.125)
+    assert torch.equal(out, want) and bool((want[part] != 9.0).any(-1).all()) and device_status() == 0
