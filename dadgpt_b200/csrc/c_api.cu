@@ -79,7 +79,7 @@ extern "C" int dadattn_device_status(dadattn_stream_t stream) {
   if (host[0] == DADATTN_E_TIMEOUT)
     fail(host[0], "a bounded device-side wait ran out (wait at source line %d of its kernel)", host[1]);
   else if (host[0] == DADATTN_E_ARG)
-    fail(host[0], "a kernel skipped work: sequence length outside [0, max_len)");
+    fail(host[0], "a kernel skipped work: sequence length outside [0, max_len), or a page outside its pool");
   else if (host[0] != 0)
     fail(host[0], "device status %d", host[0]);
   return host[0];

@@ -460,16 +460,18 @@ int dadattn_rotary(void* q_out, void* k_out, const void* q, const void* k, const
  * not falling, starts[B] <= T), none, one or many, and are its rows lengths[b] and on. starts NULL: one token for each sequence,
  * T = B. Packed tensors have strides (host arrays of two: token, head, in elements), every row beginning at a multiple of 16
  * bytes; those of results and of the attention's queries are not zero. Rows of the packed results that belong to no sequence
- * (behind starts[B]) are left as they were. Hq query heads share Hkv key heads, Hq / Hkv neighbours each.
+ * (ahead of starts[0], behind starts[B]) are left as they were. Hq query heads share Hkv key heads, Hq / Hkv neighbours each.
  * A sequence whose numbers do not fit (lengths[b] below 0, rows beyond max_pages * page_size, starts[b + 1] below starts[b]) is
  * left untouched, and so is a row whose page is outside [0, pages); both are reported through DADATTN_E_ARG at the next
- * dadattn_device_status(). (Where starts fall, whose the rows are that two sequences claim is not said.) Nothing outside the pages is read or written for any contents of the device arrays.
- * No call needs a workspace; calls may overlap on the GPU unless one writes what the other reads or writes. */
+ * dadattn_device_status(). (Where starts fall, whose the rows are that two sequences claim is not said.) Nothing outside the
+ * pages is read or written for any contents of the device arrays.
+ * No call needs a workspace; results overlap nothing that a call reads, but where that is said; calls may overlap on the GPU
+ * unless one writes what the other reads or writes. */
 
 /* New rows to their pages: k_new, v_new [T,Hkv,D] (bf16 when new_is_bf16, else fp32, rounded to bf16 once), keys turned by
  * their rows in their sequences where rot_dim > 0 (as in dadattn_rotary; turns NULL and rot_dim 0: learned positions). Hq > 0:
- * q [T,Hq,D] of the same type is turned too, into q_out (bf16; may be q where that is bf16 with the same strides). A sequence's pages of
- * these rows belong to it alone. rot_dim a multiple of 16; Hq + 2 Hkv at most 65535. A prefill's heads [H,n,D] are taken
+ * q [T,Hq,D] of the same type is turned too, into q_out (bf16; may be q where that is bf16 with the same strides). A
+ * sequence's pages of these rows belong to it alone. rot_dim a multiple of 16; Hq + 2 Hkv at most 65535. A prefill's heads [H,n,D] are taken
  * with the strides (D, n D) and B = 1. */
 int dadattn_paged_append_bf16(uint16_t* k_pages, uint16_t* v_pages, const int32_t* page_table, const int32_t* lengths,
                               const int32_t* starts, uint16_t* q_out, const void* q, const void* k_new, const void* v_new,
@@ -493,9 +495,9 @@ int dadattn_paged_attention_bf16(uint16_t* out, float* lse, const uint16_t* q, c
 
 /* One decode step in one launch: the token of every sequence (q [B,Hq,D], k_new, v_new [B,Hkv,D] bf16, strides as above) is
  * turned by its row where rot_dim > 0, appended at row lengths[b] and attended for over rows 0 .. lengths[b]; out [B,Hq,D],
- * lse [B,Hq] or NULL. What dadattn_paged_append_bf16 and dadattn_paged_attention_bf16 do with starts NULL, in one launch and without
- * the rounding of turned queries to bf16 between them. Where a page that holds a row of the sequence is outside the pool, out of that sequence and key head is left
- * untouched. */
+ * lse [B,Hq] or NULL. What dadattn_paged_append_bf16 and dadattn_paged_attention_bf16 do with starts NULL, without the rounding
+ * of turned queries to bf16 between them. Where a page that holds a row of the sequence is outside the pool, out of that
+ * sequence and key head is left untouched. */
 int dadattn_decode_paged_bf16(uint16_t* out, float* lse, const uint16_t* q, const uint16_t* k_new, const uint16_t* v_new,
                               const int64_t* out_strides, const int64_t* q_strides, const int64_t* k_strides,
                               const int64_t* v_strides, uint16_t* k_pages, uint16_t* v_pages, const int32_t* page_table,
