@@ -23,6 +23,15 @@
 //   warp 0       scheduler + K / V producer        warp 1     issuer of group A, tensor memory
 //   warp 2       issuer of group B                 warp 3     Q
 //   warps 4-7    softmax group A                   warps 8-11 softmax group B
+// Bound by the steps of a group, which wait for each other: scores, maximum, exponentials, probabilities, product. At head size
+// 128 one CTA has an SM, a step of both groups takes 3500 clk (2048 of the exp2 unit, 2048 of the tensor pipe, which is what is
+// busy 60 % of the time); at head size 64 two CTAs do, and 64 keys of their four groups take 3300 (2048 of the exp2 unit).
+// Measured (us): 2048 tokens behind 14336 rows, 32 heads on 8 of 128 453 (1137 TFLOP/s; 516 at the power cap); 24 sequences with
+// up to 3690 rows ahead and 1 to 512 new ones, the same heads, 112-130; 16 prompts of up to 1024 tokens, 12 heads of 64 38; 301
+// tokens behind 700 rows, 12 heads of 64 12.5.
+// Not kept: exponentials as polynomials, in any share (slower at both head sizes: the threads, not the exp2 unit, are short of
+// time); 64-key steps with two score buffers at head size 128 (514 for the first); probabilities handed over in quarters (481),
+// the turn passed on earlier (482-501).
 // Every wait is bounded (sm100_ptx.cuh).
 #include <cuda_bf16.h>
 

@@ -22,10 +22,10 @@
 //   * the new token needs no row of the cache: its scores, with k as rounded for the cache, are where one warp's running
 //     maximum begins, and v its accumulator.
 // Measured (us, rotating caches): 64 sequences of 9 .. 1023 rows, 12 heads of 64 21 (4.9 TB/s), all of 1000 38-39 (5.1); 8 of
-// 1000 .. 15999, 8 key heads of 128 for 32 46 (5.8), one of 60000 55 (4.5); 12 heads of 64, 699 rows 5.6. Two warps a CTA,
-// seven CTAs an SM: 31 for the first; eight warps, two CTAs: 23, and 5.2 for the last, but 53 for 128 sequences of up to 999
-// (45); persistent CTAs that take a long and a short item each 24. A CTA by itself draws 44 GB/s, what its ring of 64 KB gives
-// at 1.4 us from request to use.
+// 999 .. 15999, 8 key heads of 128 for 32 46 (5.6; 47.5 turned), one of 60000 55 (4.5); 12 heads of 64, 699 rows 5.6 (6.1 turned).
+// Two warps a CTA, seven CTAs an SM: 31 for the first; eight warps, two CTAs: 23, and 5.2 for the last, but 53 for 128 sequences
+// of up to 999 (45); persistent CTAs that take a long and a short item each 24. A CTA by itself draws 44 GB/s, what its ring of
+// 64 KB gives at 1.4 us from request to use.
 // Rows behind the last one are not trusted: their scores are masked and their V set to zero in shared memory.
 // Every wait is bounded (sm100_ptx.cuh).
 #include <cuda_bf16.h>

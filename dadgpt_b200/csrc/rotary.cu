@@ -5,8 +5,8 @@
 // token and goes through a group of its heads, with (cos, sin) of the piece's eight pairs in registers. (From a table in shared
 // memory, heads side by side in a warp, the table's reads alone were 16 wavefronts for every 8 of the tensors': 41 us instead of
 // 35.6 for forward and backward of 16 x 1024 x 24 heads of 64.)
-// Measured: 16 x 1024 x 24 heads of 64, bf16, heads split 17.8 us (5.7 TB/s), fp32 33.6 (6.0); 8192 tokens of 40 heads of 128 28.0 (6.0);
-// 140 tokens of 8 heads of 32, fp32, 2.3.
+// Measured: 16 x 1024 x 24 heads of 64, bf16, heads split 17.8 us (5.7 TB/s), fp32 33.6 (6.0); 8192 tokens of 40 heads of 128
+// 28.0 (6.0); 140 tokens of 8 heads of 32, fp32, 2.3.
 #include "rotary.cuh"
 
 #include <algorithm>
