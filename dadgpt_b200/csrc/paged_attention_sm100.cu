@@ -10,8 +10,9 @@
 // item is
 //   * a pair of adjacent query tiles, A and B, of a sequence and key head. Both use every K / V tile of the ring; while the
 //     threads of one compute exponentials the tensor pipe runs the products of the other;
-//   * or one tile, where a sequence has no second one: the groups share its keys, A the even tiles of the ring, B the odd ones,
-//     and join their maxima, sums and accumulators, which each finds in tensor memory, at the end.
+//   * or one tile, where a sequence has no second one: the groups share its keys, A takes the even steps (of 128 keys, or of 64
+//     at head size 64), B the odd ones, and they join their maxima, sums and accumulators, which each finds in tensor memory, at
+//     the end.
 // CTAs are persistent and take items from the grid's own queue (clusterlaunchcontrol): keys of the next item are on their way
 // while the current one ends. Where the tiles do not fill the GPU (CLUSTER > 1), every CTA of a cluster takes a run of one tile's
 // keys, both groups as above, and the results are joined through distributed shared memory: no workspace.
@@ -27,7 +28,7 @@
 // 128 one CTA has an SM, a step of both groups takes 3500 clk (2048 of the exp2 unit, 2048 of the tensor pipe, which is what is
 // busy 60 % of the time); at head size 64 two CTAs do, and 64 keys of their four groups take 3300 (2048 of the exp2 unit).
 // Measured (us): 2048 tokens behind 14336 rows, 32 heads on 8 of 128 453 (1137 TFLOP/s; 516 at the power cap); 24 sequences with
-// up to 3690 rows ahead and 1 to 512 new ones, the same heads, 112-130; 16 prompts of up to 1024 tokens, 12 heads of 64 38; 301
+// up to 3690 rows ahead and 1 to 512 new ones, the same heads, 112-130; 16 prompts of up to 1024 tokens, 12 heads of 64 36; 301
 // tokens behind 700 rows, 12 heads of 64 12.5.
 // Not kept: exponentials as polynomials, in any share (slower at both head sizes: the threads, not the exp2 unit, are short of
 // time); 64-key steps with two score buffers at head size 128 (514 for the first); probabilities handed over in quarters (481),
@@ -92,7 +93,7 @@ struct Bars {
   uint64_t item_ready[kItems], item_free[kItems];
   uint64_t q_full[2], q_empty[2], slot_full[kSlots], slot_empty[kSlots];
   uint64_t s_full[2], p_full[2][2], o_done[2], settled[2];   // [group]; p_full: [group][64 keys of a step]
-  uint64_t joined, parted;                // groups that share a tile: results are there; have been read
+  uint64_t joined, parted, freed;         // groups that share a tile: results are there; numbers, accumulators have been read
   uint32_t tmem_base;
   int abort_flag;
   int any_bad;                            // a page outside the pool, in any item
@@ -177,23 +178,30 @@ struct Item {
     return t;
   }
 };
-// What a CTA does of an item: key tiles lo .. lo + n_kv - 1, of which group x takes n(x), its i-th being the CTA's at(x, i)-th.
+// What a CTA does of an item: key tiles lo .. lo + n_kv - 1, of STEPS steps each. Of a pair group A sees the first n_first. Of a
+// single tile the groups take the steps in turn, or, with CTAs of a cluster, the tiles: those have no second CTA on their SM, and
+// groups that begin with the same keys hinder each other (301 tokens, 12 heads of 64 13.3 us instead of 12.6).
+template <int STEPS, int CLUSTER>
 struct Share {
+  static constexpr int kTurn = CLUSTER > 1 ? STEPS : 1;   // steps of a turn
   bool single;
   int lo, n_kv, n_first;
-  int half;   // the CTA's tile (of group x: bit x) of which only the first half is seen is its last one
-  __device__ __forceinline__ int n(int x) const { return single ? (n_kv - x + 1) / 2 : x ? n_kv : n_first; }
-  __device__ __forceinline__ int at(int x, int i) const { return single ? 2 * i + x : i; }
-  // steps of group x, `per_tile` to a tile but for a last half that nothing is seen of
-  __device__ __forceinline__ int steps(int x, int per_tile) const {
-    const int tiles = n(x);
-    const bool has_last = single ? tiles > 0 && at(x, tiles - 1) == n_kv - 1 : true;
-    return per_tile * tiles - (per_tile == 2 && has_last && (half >> x & 1) ? 1 : 0);
+  int half;   // of the last of these tiles (of group x: bit x) only the first half is seen
+  // steps of group x: all but a last half that nothing is seen of
+  __device__ __forceinline__ int steps(int x) const {
+    const int tiles = single || x ? n_kv : n_first;
+    const int all = STEPS * tiles - (STEPS == 2 && tiles > 0 && (half >> x & 1) ? 1 : 0);
+    return single ? all / (2 * kTurn) * kTurn + min(max(all % (2 * kTurn) - x * kTurn, 0), kTurn) : all;
   }
+  // the k-th of them, among the steps of the CTA's tiles
+  __device__ __forceinline__ int at(int x, int k) const { return single ? k / kTurn * 2 * kTurn + x * kTurn + k % kTurn : k; }
+  // whether it is the group's first of a tile; its last, but for the very last
+  __device__ __forceinline__ bool first_of(int k) const { return (single && kTurn < STEPS) || k % STEPS == 0; }
+  __device__ __forceinline__ bool last_of(int k) const { return (single && kTurn < STEPS) || k % STEPS == STEPS - 1; }
 };
-template <int CLUSTER>
-__device__ __forceinline__ Share share_of(const Item& it, const ChunkParams& p, int rank) {
-  Share s;
+template <int STEPS, int CLUSTER>
+__device__ __forceinline__ Share<STEPS, CLUSTER> share_of(const Item& it, const ChunkParams& p, int rank) {
+  Share<STEPS, CLUSTER> s;
   s.single = CLUSTER > 1 || it.single(p);
   const Tile last = it.tile(p, s.single ? 0 : 1);
   const int n = last.n;
@@ -375,9 +383,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       for (int w = 0; w < 4; ++w) bars->exps[x][w] = 0;
     }
     mbar_init(&bars->joined, 8);
-    // softmax warps and, where another item may follow, the issuers: one whose group has no keys of a tile would not be missed
-    // otherwise, and could find the barrier two items on
-    mbar_init(&bars->parted, CLUSTER == 1 ? 8 + 2 : 8);
+    // (softmax warps and the issuers: one whose group has no keys of a tile would not be missed otherwise, and could find the
+    // barrier two items on)
+    mbar_init(&bars->parted, 8 + 2);
+    mbar_init(&bars->freed, 8);
     bars->abort_flag = 0;
     bars->any_bad = 0;
     fence_mbar_init();
@@ -441,7 +450,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         __syncwarp();
         ++n_pub;
         if (it.b < 0) break;
-        const Share s = share_of<CLUSTER>(it, p, rank);
+        const auto s = share_of<kSteps, CLUSTER>(it, p, rank);
         const int total = it.ahead + it.count;   // rows of the sequence
         const int32_t* table = c.table + static_cast<int64_t>(it.b) * c.max_pages;
         // Whether a row of this lane's box of a tile is there, and its page (looked at only when the box is fetched).
@@ -486,10 +495,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         int n[2] = {0, 0};
         bool ok = true;
         while (ok && feed.next(it)) {
-          const Share s = share_of<CLUSTER>(it, p, rank);
+          const auto s = share_of<kSteps, CLUSTER>(it, p, rank);
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            if (s.n(x) == 0) continue;
+            if (s.steps(x) == 0) continue;
             if (n[x] > 0 && !(ok = mbar_wait(&bars->q_empty[x], (n[x] - 1) & 1, abort_flag))) break;
             mbar_arrive_expect_tx(&bars->q_full[x], L::kPanels * p.tile_tokens * p.group * 128);
             for (int h = 0; h < L::kPanels; ++h)
@@ -528,13 +537,14 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
           return true;
         };
         while (ok && feed.next(it)) {
-          const Share s = share_of<CLUSTER>(it, p, rank);
-          const int steps = s.steps(x, kSteps);
-          // Scores of the k-th step: part k % kSteps of the group's k / kSteps-th tile
+          const auto s = share_of<kSteps, CLUSTER>(it, p, rank);
+          const int steps = s.steps(x);
+          auto tile_of = [&](int k) -> int { return s.at(x, k) / kSteps; };
+          // Scores of the k-th step
           auto issue_s = [&](int k) -> bool {
-            const int at = s.at(x, k / kSteps), h = k % kSteps;
+            const int at = tile_of(k), h = s.at(x, k) % kSteps;
             const Slot<D> slot(gone + at, 0);
-            if (h == 0 && !wait_slot(slot)) return false;
+            if (s.first_of(k) && !wait_slot(slot)) return false;
             tc_fence_after_sync();
             const SmemDescBase k_desc{kv_desc0.lo + slot.at * (L::kTileBytes >> 4) + h * (kN * 128 >> 4), kv_desc0.hi};
 #pragma unroll
@@ -542,20 +552,20 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
               const uint32_t off = (kk / 4) * kPanel + (kk % 4) * 32;
               mma_ss(tS, desc_at(q_desc, off), desc_at(k_desc, off), idesc_s, kk > 0 ? 1u : 0u);
             }
-            const bool last = k + 1 == steps, through = h == kSteps - 1 || last;
-            if (through) mma_commit(&bars->slot_empty[slot.at]);
+            const bool last = k + 1 == steps;
+            if (s.last_of(k) || last) mma_commit(&bars->slot_empty[slot.at]);
             if (last) mma_commit(&bars->q_empty[x]);
             mma_commit(&bars->s_full[x]);
             // (the other's next tile, ahead of the wait for these probabilities: its slots are not to wait for those)
-            if (s.single && through && at + 1 < s.n_kv) return skip(gone + at + 1);
+            if (s.single && (s.last_of(k) || last) && at + 1 < (last ? s.n_kv : tile_of(k + 1))) return skip(gone + at + 1);
             return true;
           };
-          if (s.single && x == 1 && s.n_kv > 0) ok = skip(gone);
+          if (s.single && (steps > 0 ? tile_of(0) : s.n_kv) > 0) ok = skip(gone);
           if (ok && steps > 0) ok = mbar_wait(&bars->q_full[x], u++ & 1, abort_flag) && issue_s(0);
           for (int k = 0; ok && k < steps; ++k, ++g) {
-            const int h = k % kSteps;
-            const Slot<D> v(gone + s.at(x, k / kSteps), 1);
-            if (h == 0 && !(ok = wait_slot(v))) break;
+            const int h = s.at(x, k) % kSteps;
+            const Slot<D> v(gone + tile_of(k), 1);
+            if (s.first_of(k) && !(ok = wait_slot(v))) break;
             // O (+)= P V, 64 keys at a time. (A new item's first may overwrite O: its probabilities come after the last results
             // have been read.)
             const SmemDescBase v_desc{kv_desc0.lo + v.at * (L::kTileBytes >> 4) + h * (kN * 128 >> 4), kv_desc0.hi};
@@ -570,13 +580,13 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             }
             if (!ok) break;
             const bool last = k + 1 == steps;
-            if (h == kSteps - 1 || last) mma_commit(&bars->slot_empty[v.at]);
+            if (s.last_of(k) || last) mma_commit(&bars->slot_empty[v.at]);
             if (last) mma_commit(&bars->o_done[x]);
             else ok = issue_s(k + 1);   // over the probabilities, whose product is ahead in the pipe
           }
           // tiles that only the pair's other group sees
           if (!s.single)
-            for (int j = s.n(x); ok && j < s.n_kv; ++j) ok = skip(gone + j);
+            for (int j = x ? s.n_kv : s.n_first; ok && j < s.n_kv; ++j) ok = skip(gone + j);
           // (the groups' maxima and sums change hands where the next item's scores go)
           if (s.single && CLUSTER == 1 && ok) {
             mbar_arrive(&bars->parted);
@@ -599,11 +609,14 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const float scale_log2 = p.scale * kLog2e;
     uint32_t g = 0, u = 0, joins = 0;     // steps, items with any and shared tiles of this group so far
     int gone = 0, others = 0;             // key tiles of the CTA and steps of the other group so far
-    bool ok = true;
+    bool ok = true, shared = false;       // shared: the item before was, and its accumulators may still be read
     while (ok && feed.next(it)) {
-      const Share s = share_of<CLUSTER>(it, p, rank);
+      // (its first probabilities let a product overwrite them, its numbers others)
+      if (shared && !(ok = mbar_wait(&bars->freed, (joins - 1) & 1, abort_flag))) break;
+      shared = false;
+      const auto s = share_of<kSteps, CLUSTER>(it, p, rank);
       const Tile t = it.tile(p, s.single ? 0 : x);
-      const int steps = s.steps(x, kSteps), total = it.ahead + it.count;
+      const int steps = s.steps(x), total = it.ahead + it.count;
       const bool active = quad * 32 < t.rows;          // whether the warp has a row
       const int token = t.token0 + min(row, t.rows - 1) / p.group;   // (rows that are not there: the last one's mask)
       const int limit = it.ahead + token;
@@ -611,8 +624,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       for (int k = 0; k < steps; ++k, ++g) {
         if (!(ok = mbar_wait(&bars->s_full[x], g & 1, abort_flag))) break;
         tc_fence_after_sync();
-        const int tile = s.at(x, k / kSteps), key0 = (s.lo + tile) * kT;
-        const int seen = limit - key0 - (k % kSteps) * kN;   // the last column that the row sees
+        const int tile = s.at(x, k) / kSteps, h = s.at(x, k) % kSteps, key0 = (s.lo + tile) * kT;
+        const int seen = limit - key0 - h * kN;   // the last column that the row sees
         const bool masked = __any_sync(0xffffffffu, seen < kN - 1);
         // 32 of the thread's scores
         auto load = [&](uint32_t (&sc)[32], int q) { tmem_ld32(tS + q * 32, sc); };
@@ -673,13 +686,13 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars->p_full[x][part]);
         };
-        if (k % kSteps == 0 && total - key0 < kT) {
-          // The sequence ends in this tile: V of the rows behind it.
+        if (s.first_of(k) && total - key0 < kT) {
+          // The sequence ends in this tile: V of the rows behind it, as far as the group goes.
           const Slot<D> v(gone + tile, 1);
-          const int there = total - key0;
+          const int there = max(total - key0, h * kN), end = s.last_of(k) ? (h + 1) * kN : kT;
           if (!(ok = mbar_wait(&bars->slot_full[v.at], v.parity, abort_flag))) break;
           uint8_t* rows = smem + L::kKV + v.at * L::kTileBytes;
-          for (int e = threadIdx.x % kGroup; e < (kT - there) * (D / 8); e += kGroup) {
+          for (int e = threadIdx.x % kGroup; e < (end - there) * (D / 8); e += kGroup) {
             const int r = there + e / (D / 8), ch = e % (D / 8);
             *reinterpret_cast<uint4*>(rows + (ch / 8) * kPanel + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
@@ -699,7 +712,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
           }
           // A's turn is behind B's step before, B's behind A's of the same place.
           {
-            const int due = x == 0 ? min(k, s.steps(1, kSteps)) : min(k + 1, s.steps(0, kSteps));
+            const int due = x == 0 ? min(k, s.steps(1)) : min(k + 1, s.steps(0));
             const volatile int* done = &bars->exps[1 - x][quad];
             for (int i = 0; i < 256 && *done < others + due; ++i) {}
           }
@@ -780,6 +793,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         float m1, l1;
         tmem_ld2(tlane + kColS + (1 - x) * kN, m1, l1);
         tmem_wait_ld();
+        if (CLUSTER == 1) {   // (the next item's scores may go there)
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->parted);
+        }
         const float m_all = fmaxf(m, m1);
         // (a part that has seen nothing has nothing but garbage)
         const float f0 = m == -INFINITY ? 0.f : ex2(m - m_all), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - m_all);
@@ -810,14 +828,16 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         }
         if (CLUSTER == 1 && x == 0 && write && p.lse) p.lse[to_token * p.heads_q + to_head] = (m_all + log2f(l_all)) * kLn2;
         if (CLUSTER > 1 && x == 0) reinterpret_cast<float2*>(smem + L::kStats)[row] = make_float2(m_all, l_all);
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->parted);
-        if (!(ok = mbar_wait(&bars->parted, joins++ & 1, abort_flag))) break;
-        tc_fence_after_sync();
+        if (CLUSTER == 1) {
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->freed);
+          ++joins;
+          shared = true;
+        }
       }
       gone += s.n_kv;
-      others += s.steps(1 - x, kSteps);
+      others += s.steps(1 - x);
       __syncwarp();
       feed.give_back(lane == 0);
     }

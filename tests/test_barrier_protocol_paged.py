@@ -1,7 +1,7 @@
 """CPU: barrier model (tests/barrier_model.py) of attention over a paged cache, dadgpt_b200/csrc/paged_attention_sm100.cu.
 An item is a pair of query tiles with the key tiles that each of them sees, ("pair", a, b), or one tile whose keys the groups
-share, ("one", n). The key tiles are of one step and two parts (head size 128) or of two steps, the last of which may be left out
-(head size 64). A softmax group is two agents, each with its rows. The request for another block is a load whose answer names
+share, ("one", n), taking its steps in turn. The key tiles are of one step and two parts (head size 128) or of two steps, the last
+of which may be left out (head size 64; there a turn may be a tile's two steps, which is what CTAs of a cluster do). A softmax group is two agents, each with its rows. The request for another block is a load whose answer names
 the item. The turns that the groups' exponentials take bound nobody's progress and are not part of it."""
 import random
 
@@ -12,15 +12,18 @@ from tests.barrier_model import Aborted, Model, survives
 HALVES = (0, 1)
 
 
+KINDS = {"d128": (1, 2, 1), "d64": (2, 1, 1), "d64_tiles": (2, 1, 2)}   # steps of a key tile, parts of a step, steps of a turn
+
+
 class Paged(Model):
     SLOTS, RING = 5, 4
-    need = {"slot_empty": 2, "item_free": 7, "p_full": 2, "joined": 4, "parted": 6}
+    need = {"slot_empty": 2, "item_free": 7, "p_full": 2, "joined": 4, "parted": 6, "freed": 4}
 
-    def __init__(self, items, two_steps, rng, abort=False):
+    def __init__(self, items, kind, rng, abort=False):
         super().__init__(rng, abort)
         self.items = items
-        self.per_tile, self.parts = (2, 1) if two_steps else (1, 2)
-        self.half = [[two_steps and rng.random() < 0.5 for _ in HALVES] for _ in items]   # of the last tile only a half is seen
+        self.per_tile, self.parts, self.turn = KINDS[kind]
+        self.half = [[self.per_tile == 2 and rng.random() < 0.5 for _ in HALVES] for _ in items]   # of the last tile only a half is seen
 
     # what Share says
     def single(self, i):
@@ -30,15 +33,17 @@ class Paged(Model):
         return self.items[i][-1]
 
     def n(self, i, x):
-        return (self.items[i][1] - x + 1) // 2 if self.single(i) else self.items[i][1 + x]
+        return self.items[i][1] if self.single(i) else self.items[i][1 + x]
 
-    def at(self, i, x, j):
-        return 2 * j + x if self.single(i) else j
+    def at(self, i, x, k):
+        return (k // self.turn * 2 + x) * self.turn + k % self.turn if self.single(i) else k
 
     def steps(self, i, x):
-        tiles = self.n(i, x)
-        last = tiles > 0 and self.at(i, x, tiles - 1) == self.n_kv(i) - 1 if self.single(i) else True
-        return self.per_tile * tiles - (last and self.half[i][0 if self.single(i) else x])
+        every = self.per_tile * self.n(i, x) - self.half[i][0 if self.single(i) else x]
+        return sum(u // self.turn % 2 == x for u in range(every)) if self.single(i) else every
+
+    def every(self, i):   # whether each step is its group's only one of the tile
+        return self.single(i) and self.turn < self.per_tile
 
     def slot(self, tile, m):
         return (2 * tile + m) % self.SLOTS, (2 * tile + m) // self.SLOTS
@@ -78,7 +83,7 @@ class Paged(Model):
 
         def own(i):
             for x in HALVES:
-                if self.n(i, x):
+                if self.steps(i, x):
                     if n[x] > 0:
                         yield ("wait", f"q_empty[{x}]", n[x] - 1)
                     yield ("tma", f"q_full[{x}]", [(("q", x), i)])
@@ -103,29 +108,37 @@ class Paged(Model):
             nonlocal g, u, joins, gone
             steps = self.steps(i, x)
 
+            def tile_of(k):
+                return self.at(i, x, k) // self.per_tile
+
+            def first_of(k):
+                return self.every(i) or k % self.per_tile == 0
+
+            def last_of(k):
+                return self.every(i) or k % self.per_tile == self.per_tile - 1 or k + 1 == steps
+
             def scores(k):
-                at, h = self.at(i, x, k // self.per_tile), k % self.per_tile
-                if h == 0:
+                at = tile_of(k)
+                if first_of(k):
                     yield wait_slot(gone + at, 0)
                 yield ("mma", [(("q", x), i), held(gone + at, 0)], [(("s", x, c, a), ("s", i, k)) for c in range(self.parts) for a in HALVES])
-                through = h == self.per_tile - 1 or k + 1 == steps
-                if through:
+                if last_of(k):
                     yield ("commit", "slot_empty[%d]" % self.slot(gone + at, 0)[0])
                 if k + 1 == steps:
                     yield ("commit", f"q_empty[{x}]")
                 yield ("commit", f"s_full[{x}]")
-                if self.single(i) and through and at + 1 < self.n_kv(i):
+                if self.single(i) and last_of(k) and at + 1 < (self.n_kv(i) if k + 1 == steps else tile_of(k + 1)):
                     yield from skip(gone + at + 1)
 
-            if self.single(i) and x == 1:
+            if self.single(i) and (tile_of(0) if steps else self.n_kv(i)) > 0:
                 yield from skip(gone)
             if steps:
                 yield ("wait", f"q_full[{x}]", u)
                 u += 1
                 yield from scores(0)
             for k in range(steps):
-                tile, h = gone + self.at(i, x, k // self.per_tile), k % self.per_tile
-                if h == 0:
+                tile = gone + tile_of(k)
+                if first_of(k):
                     yield wait_slot(tile, 1)
                 for c in range(self.parts):
                     yield ("wait", f"p_full[{x}{c}]", g)
@@ -133,7 +146,7 @@ class Paged(Model):
                     so_far = [(("o", x), (i, k, c))] if k or c else []
                     yield ("mma", [(("s", x, c, a), ("p", i, k)) for a in HALVES] + [held(tile, 1)] + zeroed + so_far,
                            [(("o", x), (i, k, c + 1) if c + 1 < self.parts else (i, k + 1, 0))])
-                if h == self.per_tile - 1 or k + 1 == steps:
+                if last_of(k):
                     yield ("commit", "slot_empty[%d]" % self.slot(tile, 1)[0])
                 if k + 1 == steps:
                     yield ("commit", f"o_done[{x}]")
@@ -152,10 +165,15 @@ class Paged(Model):
 
     def softmax(self, x, a):
         g = u = joins = gone = 0
+        shared = False
 
         def own(i):
-            nonlocal g, u, joins, gone
+            nonlocal g, u, joins, gone, shared
             steps = self.steps(i, x)
+
+            if shared:
+                yield ("wait", "freed", joins - 1)
+                shared = False
             for k in range(steps):
                 yield ("wait", f"s_full[{x}]", g)
                 for c in range(self.parts):
@@ -163,8 +181,8 @@ class Paged(Model):
                 if k > 0 and self.rng.random() < 0.3:   # the rescale
                     yield ("read", ("o", x), (i, k, 0))
                     yield ("write", ("o", x), (i, k, 0))
-                tile = gone + self.at(i, x, k // self.per_tile)
-                if k % self.per_tile == 0 and tile == gone + self.n_kv(i) - 1:   # V behind the sequence's end
+                tile = gone + self.at(i, x, k) // self.per_tile
+                if (self.every(i) or k % self.per_tile == 0) and tile == gone + self.n_kv(i) - 1:   # V behind the sequence's end
                     s, use = self.slot(tile, 1)
                     yield ("wait", f"slot_full[{s}]", use)
                     yield ("read", ("kv", s), 2 * tile + 1)
@@ -181,13 +199,14 @@ class Paged(Model):
                 yield ("arrive", "joined")
                 yield ("wait", "joined", joins)
                 yield ("read", ("s", 1 - x, 0, a), ("stats", i))
+                yield ("arrive", "parted")
             for y in HALVES if self.single(i) else (x,):
                 if self.steps(i, y):
                     yield ("read", ("o", y), (i, self.steps(i, y), 0))
             if self.single(i):
-                yield ("arrive", "parted")
-                yield ("wait", "parted", joins)
+                yield ("arrive", "freed")
                 joins += 1
+                shared = True
             gone += self.n_kv(i)
         yield from self.items_of(own)
 
@@ -215,16 +234,16 @@ WORK = ([("pair", 1, 1)], [("pair", 5, 6), ("pair", 3, 3), ("pair", 1, 3)], [("o
 
 
 @pytest.mark.parametrize("abort", [False, True], ids=["runs", "gives_up"])
-@pytest.mark.parametrize("two_steps", [False, True], ids=["d128", "d64"])
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("items", WORK)
-def test_every_schedule(items, two_steps, abort):
-    assert survives(lambda s: Paged(items, two_steps, random.Random(s), abort), range(60)) is None
+def test_every_schedule(items, kind, abort):
+    assert survives(lambda s: Paged(items, kind, random.Random(s), abort), range(60)) is None
 
 
 @pytest.mark.parametrize("role,gone", [("scheduler", "slot_empty"), ("scheduler", "stolen"),
                                        ("q_producer", "q_empty"), ("issuer", "q_full"), ("issuer", "p_full"), ("issuer", "slot_full"),
                                        ("issuer", "parted"), ("softmax", "s_full"), ("softmax", "o_done"), ("softmax", "joined"),
-                                       ("softmax", "parted"), ("softmax", "slot_full")])
+                                       ("softmax", "freed"), ("softmax", "slot_full")])
 def test_the_model_misses_no_wait_that_is_left_out(role, gone):
     class Faulty(Paged):
         pass
@@ -234,4 +253,4 @@ def test_the_model_misses_no_wait_that_is_left_out(role, gone):
             if not (op[0] == "wait" and op[1].split("[")[0] == gone):
                 yield op
     setattr(Faulty, role, faulty)
-    assert any(survives(lambda s: Faulty(items, two, random.Random(s)), range(200)) for two in (False, True) for items in WORK)
+    assert any(survives(lambda s: Faulty(items, kind, random.Random(s)), range(200)) for kind in KINDS for items in WORK)
