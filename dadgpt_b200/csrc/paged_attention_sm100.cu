@@ -26,7 +26,7 @@
 //   warps 4-7    softmax group A                   warps 8-11 softmax group B
 // Bound by the steps of a group, which wait for each other: scores, maximum, exponentials, probabilities, product. At head size
 // 128 one CTA has an SM, a step of both groups takes 3500 clk (2048 of the exp2 unit, 2048 of the tensor pipe, which is what is
-// busy 60 % of the time); at head size 64 two CTAs do, and 64 keys of their four groups take 3300 (2048 of the exp2 unit).
+// busy 60 % of the time); at head size 64 two CTAs do, and 64 keys of their four groups take 3300 to 3600 (2048 of the exp2 unit).
 // Measured (us): 2048 tokens behind 14336 rows, 32 heads on 8 of 128 453 (1137 TFLOP/s; 516 at the power cap); 24 sequences with
 // up to 3690 rows ahead and 1 to 512 new ones, the same heads, 112-130; 16 prompts of up to 1024 tokens, 12 heads of 64 36; 301
 // tokens behind 700 rows, 12 heads of 64 12.5.
@@ -98,7 +98,7 @@ struct Bars {
   int abort_flag;
   int any_bad;                            // a page outside the pool, in any item
   int exps[2][4];                         // tiles whose exponentials a warp of a group is through with
-  int item[kItems][8];                    // sequence (-1: the end), first token, rows ahead, first packed row, tokens, key head, bad
+  int item[kItems][8];   // sequence (-1: the end), first token, rows ahead, first packed row, tokens, key head, bad
 };
 static_assert(sizeof(Bars) <= 1024, "barrier block");
 
@@ -932,8 +932,9 @@ int launch_chunk(const Maps& maps, ChunkParams p, long long items, cudaStream_t 
 // How a call's tiles (of every key head) are shared out: pairs of them to a CTA, or each to a CTA or to a cluster of 2, 4 or 8.
 // Pairs read a key tile once for two, and win where there are many (us, pairs / single tiles): 512 tiles of 2048 tokens behind
 // 14336 of head size 128 466 / 539, 1024 tiles of 4096 128 / 147; at head size 64, where two CTAs are on an SM, 1536 of 16 x
-// 1024 56 / 65, 768 of 8 x 1024 36 / 37, 384 of 4 x 1024 33 / 22. Of fewer tiles the cheapest in key tiles, 2 us each, that a
-// group goes through: its items' own, and something for joining, by how often an SM is filled. One tile a CTA / 2 / 4 / 8:
+// 1024 57 / 64, 1152 of 12 x 1024 45 / 50, 768 of 8 x 1024 36 / 36, of 16 x 512 22 / 26, of 8192 222 / 158. Of fewer tiles the
+// cheapest in key tiles, 2 us each, that a group goes through: its items' own, and something for joining, by how often an SM is
+// filled. One tile a CTA / 2 / 4 / 8:
 //   head size 128   16 tiles, 8033 rows 70 / 40 / 27 / 38    64, 8256 72 / 43 / 57 / 109     128, 16512 142 / 147 / 175 / 274
 //                   8, 60001 485 / 245 / 128 / 70            64, 256 8.8 / 11 / 25 / 71      160, 4001 87 / 83 / 90 / 150
 //   head size 64    12, 1024 13.6 / 10.2 / 8.6 / 9.0         36, 1001 17 / 13 / 14 / 24      192, 4096 65 / 61 / 72 / 115

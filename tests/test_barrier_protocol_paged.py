@@ -1,8 +1,9 @@
 """CPU: barrier model (tests/barrier_model.py) of attention over a paged cache, dadgpt_b200/csrc/paged_attention_sm100.cu.
 An item is a pair of query tiles with the key tiles that each of them sees, ("pair", a, b), or one tile whose keys the groups
 share, ("one", n), taking its steps in turn. The key tiles are of one step and two parts (head size 128) or of two steps, the last
-of which may be left out (head size 64; there a turn may be a tile's two steps, which is what CTAs of a cluster do). A softmax group is two agents, each with its rows. The request for another block is a load whose answer names
-the item. The turns that the groups' exponentials take bound nobody's progress and are not part of it."""
+of which may be left out (head size 64; there a turn may be a tile's two steps, which is what CTAs of a cluster do). A softmax
+group is two agents, each with its rows. The request for another block is a load whose answer names the item. The turns that the
+groups' exponentials take bound nobody's progress and are not part of it."""
 import random
 
 import pytest
@@ -23,7 +24,8 @@ class Paged(Model):
         super().__init__(rng, abort)
         self.items = items
         self.per_tile, self.parts, self.turn = KINDS[kind]
-        self.half = [[self.per_tile == 2 and rng.random() < 0.5 for _ in HALVES] for _ in items]   # of the last tile only a half is seen
+        # of the last tile only a half is seen
+        self.half = [[self.per_tile == 2 and rng.random() < 0.5 for _ in HALVES] for _ in items]
 
     # what Share says
     def single(self, i):
@@ -121,7 +123,8 @@ class Paged(Model):
                 at = tile_of(k)
                 if first_of(k):
                     yield wait_slot(gone + at, 0)
-                yield ("mma", [(("q", x), i), held(gone + at, 0)], [(("s", x, c, a), ("s", i, k)) for c in range(self.parts) for a in HALVES])
+                yield ("mma", [(("q", x), i), held(gone + at, 0)],
+                       [(("s", x, c, a), ("s", i, k)) for c in range(self.parts) for a in HALVES])
                 if last_of(k):
                     yield ("commit", "slot_empty[%d]" % self.slot(gone + at, 0)[0])
                 if k + 1 == steps:
