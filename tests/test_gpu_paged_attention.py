@@ -236,3 +236,26 @@ def test_rows_ahead_of_the_first_sequence_belong_to_nobody(cuda, many):
     dad.paged_attention_bf16(want[part], q[part], c, starts, max(counts), 0.125)
     dad.paged_attention_bf16(out, q, c, starts + lead, max(counts), 0.125)
     assert torch.equal(out, want) and bool((want[part] != 9.0).any(-1).all()) and device_status() == 0
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_sequences(cuda, D):
+    """Every CTA goes through items of many sequences, some without new tokens, one that does not fit."""
+    B, g = 500, torch.Generator().manual_seed(70)
+    ahead = torch.randint(0, 200, (B,), generator=g).tolist()
+    counts = [0 if b % 7 == 3 else 150 if b % 40 == 0 else 1 + b % 20 for b in range(B)]
+    c, starts, gen = made(cuda, 4, D, 16, ahead, counts, 71)
+    q = torch.randn(sum(counts), 8, D, generator=gen, device=cuda).to(torch.bfloat16)
+    out = torch.full_like(q, 9.0)
+    dad.paged_attention_bf16(out, q, c, starts, 150, 0.125)
+    assert device_status() == 0 and bool((out != 9.0).any(-1).all())
+    _check(c, out, None, q, ahead, counts, 0.125, set(range(0, B, 23)) | {1, B - 1})
+    refused = 321
+    c.lengths[refused] = -1
+    again = torch.full_like(q, 9.0)
+    dad.paged_attention_bf16(again, q, c, starts, 150, 0.125)
+    assert device_status() != 0
+    rows = slice(int(starts[refused]), int(starts[refused + 1]))
+    assert bool((again[rows] == 9.0).all())
+    again[rows] = out[rows]
+    assert torch.equal(again, out)
