@@ -10,26 +10,26 @@
 // byte; what counts is that enough of them are on their way, and that a call is over soon after its longest sequence. tcgen05
 // would need its scores back from tensor memory, and 128 rows for each product.
 //   * a CTA (a cluster, where few items share the GPU) per sequence, key head and 16 query heads. Of a cluster each CTA takes
-//     a run of the 64-row tiles, and they join their maxima, sums and accumulators through distributed shared memory: no
+//     a run of the tiles (64 or 128 rows), and they join their maxima, sums and accumulators through distributed shared memory: no
 //     workspace, and nothing that two calls could share.
 //   * one producer warp: lane i fetches the i-th box of a tile (TMA, 128-byte swizzle, boxes as high as a page, up to the
 //     tile; 16 rows in a sequence's last tile, of which only those with a row are fetched), and looks its page up a tile ahead.
-//   * four consumer warps, 16 rows of a tile each, with a running maximum and sum of their own. Scores and probabilities stay in
-//     registers: as a result they lie transposed to the next product's operand, which movmatrix puts right. Accumulators are
-//     rescaled only when the maximum has grown by 2^8.
+//   * four consumer warps, or eight where a CTA has its SM to itself, 16 rows of a tile each, with a running maximum and sum of
+//     their own. Scores and probabilities stay in registers: as a result they lie transposed to the next product's operand, which
+//     movmatrix puts right. Accumulators are rescaled only when the maximum has grown by 2^8.
 //   * turned queries are not rounded to bf16: what rounding leaves is a second operand, whose products are as good as free here
 //     (rounded, the result's error against 64 bits was 2.7e-3 and more of its norm; 2.1e-3 without, as without a rotation).
 //   * the new token needs no row of the cache: its scores, with k as rounded for the cache, are where one warp's running
 //     maximum begins, and v its accumulator.
-// Measured (us, rotating caches): 64 sequences of 9 .. 1023 rows, 12 heads of 64 21 (4.9 TB/s), all of 1000 38-39 (5.1); 8 of
-// 999 .. 15999, 8 key heads of 128 for 32 46 (5.6; 47.5 turned), one of 60000 55 (4.5); 12 heads of 64, 699 rows 5.6 (6.1 turned).
-// Two warps a CTA, seven CTAs an SM: 31 for the first; eight warps, two CTAs: 23, and 5.2 for the last, but 53 for 128 sequences
-// of up to 999 (45); persistent CTAs that take a long and a short item each 24. A CTA by itself draws 44 GB/s, what its ring of
-// 64 KB gives at 1.4 us from request to use.
+// Measured (us, rotating caches): 64 sequences of 3 .. 1023 rows, 12 heads of 64 21 (4.9 TB/s), all of 1000 38-39 (5.1); 8 of
+// 999 .. 15999, 8 key heads of 128 for 32 46 (5.6; 47 turned), one of 60000 59 (4.2); 12 heads of 64, 699 rows 5.2 (6.0 turned).
+// Two warps a CTA, seven CTAs an SM: 31 for the first; eight warps, two CTAs: 23, and 53 for 128 sequences of up to 999 (45);
+// persistent CTAs that take a long and a short item each 24. More figures at share_out.
 // Rows behind the last one are not trusted: their scores are masked and their V set to zero in shared memory.
 // Every wait is bounded (sm100_ptx.cuh).
 #include <cuda_bf16.h>
 
+#include <algorithm>
 #include <climits>
 
 #include "decode_common.cuh"
@@ -42,35 +42,36 @@ namespace {
 using namespace ptx;
 using bf16 = __nv_bfloat16;
 
-constexpr int kWarps = 4;                     // consumer warps
-constexpr int kThreads = (kWarps + 1) * 32;   // and one producer warp
-constexpr int kWarpRows = 16;                 // cache rows of a warp in a stage
-constexpr int kTile = kWarps * kWarpRows;
+constexpr int kWarpRows = 16;                 // cache rows of a consumer warp in a stage
 constexpr int kRows = 16;                     // query rows of an item, at most
 constexpr int kMaxCluster = 16;
 constexpr int kRanked = 4;                    // sequences of a lane that are ranked: 128 of a call
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kRescaleAt = 8.0f;
 
-template <int D, int NT>
+// WARPS: consumer warps, 4, or 8 where a CTA has its SM to itself.
+template <int D, int NT, int WARPS>
 struct Plan {
-  static constexpr int kStages = D == 64 ? 3 : 2;            // with kPerSm: 192 KB on their way into an SM
-  static constexpr int kPerSm = D == 64 ? 4 : 3;
+  static constexpr int kThreads = (WARPS + 1) * 32;          // and one producer warp
+  static constexpr int kTile = WARPS * kWarpRows;
+  static constexpr int kPerSm = WARPS == 8 ? 1 : D == 64 ? 4 : 3;
+  static constexpr int kStages = 192 * 1024 / (kPerSm * kTile * D * 4);   // 192 KB on their way into an SM
   static constexpr int kPanels = D / 64;
-  static constexpr int kPanelBytes = kTile * 128;            // [64 rows][64 bf16], swizzled
+  static constexpr int kPanelBytes = kTile * 128;            // [kTile rows][64 bf16], swizzled
   static constexpr int kSide = kPanels * kPanelBytes;        // K or V of a tile
   static constexpr int kStageBytes = 2 * kSide;
   // Behind the ring, or in its place once it has been read: accumulators of the warps and the CTA's.
   static constexpr int kPitch = D + 4;                       // floats of a row (banks)
   static constexpr int kWarpAcc = 8 * NT * kPitch;
-  static constexpr int kBytes = kStages * kStageBytes > (kWarps + 1) * kWarpAcc * 4 ? kStages * kStageBytes : (kWarps + 1) * kWarpAcc * 4;
+  static constexpr int kAccBytes = (WARPS + 1) * kWarpAcc * 4;
+  static constexpr int kBytes = kStages * kStageBytes > kAccBytes ? kStages * kStageBytes : kAccBytes;
 };
 
-template <int D, int NT>
+template <int D, int NT, int WARPS>
 struct DecodeShared {
-  uint64_t full[Plan<D, NT>::kStages], empty[Plan<D, NT>::kStages];
+  uint64_t full[Plan<D, NT, WARPS>::kStages], empty[Plan<D, NT, WARPS>::kStages];
   int abort_flag, bad;
-  float m[kWarps][kRows], l[kWarps][kRows];
+  float m[WARPS][kRows], l[WARPS][kRows];
   float m_all[kRows], l_all[kRows];           // of the CTA, read by the cluster's others
   __align__(16) float2 table[kMaxRotaryHead / 4];   // (cos, sin): D / 2 at most
   __align__(16) bf16 q[2][8 * NT][D + 8];           // turned queries in two parts, the second what rounding left of the first
@@ -166,15 +167,15 @@ __device__ __forceinline__ void by_length(const PagedCache& c, int place, int& b
   }
 }
 
-template <int D, int NT, int CLUSTER>
-__global__ void __launch_bounds__(kThreads, Plan<D, NT>::kPerSm)
+template <int D, int NT, int CLUSTER, int WARPS>
+__global__ void __launch_bounds__(Plan<D, NT, WARPS>::kThreads, Plan<D, NT, WARPS>::kPerSm)
 paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                     const __grid_constant__ CUtensorMap map_k16, const __grid_constant__ CUtensorMap map_v16,
                     const DecodeParams p) {
-  using L = Plan<D, NT>;
-  constexpr int kStages = L::kStages, kSteps = D / 16;
+  using L = Plan<D, NT, WARPS>;
+  constexpr int kStages = L::kStages, kSteps = D / 16, kTile = L::kTile, kThreads = L::kThreads;
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ DecodeShared<D, NT> sh;
+  __shared__ DecodeShared<D, NT, WARPS> sh;
   volatile int* abort_flag = &sh.abort_flag;
   const PagedCache& c = p.cache;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -191,7 +192,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&sh.full[s], 1);
-      mbar_init(&sh.empty[s], kWarps);
+      mbar_init(&sh.empty[s], WARPS);
     }
     sh.abort_flag = 0;
     sh.bad = 0;
@@ -220,7 +221,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   float o[kSteps][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
   for (int t = 0; t < NT; ++t) m[t][0] = m[t][1] = -INFINITY, l[t][0] = l[t][1] = 0.f;
-  if (warp == kWarps) {
+  if (warp == WARPS) {
     // ------------------------------ producer ------------------------------
     const int32_t* table = c.table + static_cast<int64_t>(b) * c.max_pages;
     int issued = 0;
@@ -264,7 +265,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   } else {
     // ------------------------------ set-up of the consumers ------------------------------
     const int t = threadIdx.x;
-    constexpr int kConsumers = kWarps * 32, kUnits = D / kTurnUnit;
+    constexpr int kConsumers = WARPS * 32, kUnits = D / kTurnUnit;
     const int half = p.r.rot / 2;
     // pieces of 16 elements: of the query rows, then of k and v
     const int pieces = (8 * NT + 2) * kUnits;
@@ -392,9 +393,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
               if (lane / 4 + 8 * (e >> 1) >= there) sc[t][e] = -INFINITY;
           for (int i = lane; i < (kWarpRows - there) * D / 8; i += 32) {
             const int row = there + i / (D / 8), ch = i % (D / 8);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_tile + (ch / 8) * L::kPanelBytes + row * 128 + ((ch & 7) << 4)),
-                         "r"(0)
-                         : "memory");
+            const uint32_t at = v_tile + (ch / 8) * L::kPanelBytes + row * 128 + ((ch & 7) << 4);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -458,8 +458,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   // ------------------------------ the warps', then the CTAs' results together ------------------------------
   __syncthreads();   // (nobody reads the ring any more; the producer has seen its copies land)
   float* acc = reinterpret_cast<float*>(smem);               // [warps][rows][kPitch]
-  float* sum = acc + kWarps * L::kWarpAcc;                   // [rows][kPitch]
-  if (warp < kWarps) {
+  float* sum = acc + WARPS * L::kWarpAcc;                   // [rows][kPitch]
+  if (warp < WARPS) {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -483,10 +483,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     const int row = i / (D / 2), col = i % (D / 2) * 2;
     float m_tot = sh.m[0][row];
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) m_tot = fmaxf(m_tot, sh.m[w][row]);
+    for (int w = 1; w < WARPS; ++w) m_tot = fmaxf(m_tot, sh.m[w][row]);
     float l_tot = 0.f, a = 0.f, b2 = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
       const float mw = sh.m[w][row], f = mw == -INFINITY ? 0.f : ex2(mw - m_tot);
       const float2 v = *reinterpret_cast<const float2*>(acc + w * L::kWarpAcc + row * L::kPitch + col);
       l_tot = fmaf(sh.l[w][row], f, l_tot);
@@ -546,54 +546,124 @@ struct Maps {
   CUtensorMap k, v, k16, v16;
 };
 
-template <int D, int NT, int CLUSTER>
-int launch_decode(const Maps& maps, DecodeParams p, int items, cudaStream_t st) {
-  using L = Plan<D, NT>;
-  p.ranked = p.cache.B > 1 && p.cache.B <= 32 * kRanked &&
-             static_cast<long long>(items) * CLUSTER > static_cast<long long>(current_sm_count()) * L::kPerSm;
+template <int D, int NT, int CLUSTER, int WARPS>
+struct Launch {
+  using L = Plan<D, NT, WARPS>;
+  static int prepare() {
+    auto kern = paged_decode_kernel<D, NT, CLUSTER, WARPS>;
+    DAD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
+    if (CLUSTER > 8) DAD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    return DADATTN_OK;
+  }
+  static void configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], int items, cudaStream_t st) {
+    cfg.gridDim = dim3(static_cast<unsigned>(items) * CLUSTER);
+    cfg.blockDim = dim3(L::kThreads);
+    cfg.dynamicSmemBytes = L::kBytes;
+    cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = CLUSTER;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = CLUSTER > 1 ? 2 : 1;
+  }
+  // Items that the GPU works on at once. (Clusters stay within a part of the GPU, and not all of these are of one size.)
+  static int places(int dev) {
+    if (CLUSTER == 1) return current_sm_count() * L::kPerSm;
+    static std::atomic<int> seen[64];   // by device; 1 more, 0: not asked yet
+    if (dev < 0 || dev >= 64) return 0;
+    int n = seen[dev].load(std::memory_order_relaxed) - 1;
+    if (n >= 0) return n;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    configure(cfg, attr, 1, nullptr);
+    cfg.attrs = attr + 1, cfg.numAttrs = 1;
+    if (prepare() != DADATTN_OK ||
+        cudaOccupancyMaxActiveClusters(&n, paged_decode_kernel<D, NT, CLUSTER, WARPS>, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      return 0;   // (no cluster of this size: not taken)
+    }
+    seen[dev].store(n + 1, std::memory_order_relaxed);
+    return n;
+  }
+  static int run(const Maps& maps, DecodeParams p, int items, cudaStream_t st) {
+    p.ranked = p.cache.B > 1 && p.cache.B <= 32 * kRanked &&
+               static_cast<long long>(items) * CLUSTER > static_cast<long long>(current_sm_count()) * L::kPerSm;
+    if (int rc = prepare()) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    configure(cfg, attr, items, st);
+    DAD_CUDA(cudaLaunchKernelEx(&cfg, paged_decode_kernel<D, NT, CLUSTER, WARPS>, maps.k, maps.v, maps.k16, maps.v16, p));
+    return DADATTN_OK;
+  }
+};
 
-  auto kern = paged_decode_kernel<D, NT, CLUSTER>;
-  DAD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
-  if (CLUSTER > 8) DAD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(items) * CLUSTER);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = L::kBytes;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = CLUSTER;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = CLUSTER > 1 ? 2 : 1;
-  DAD_CUDA(cudaLaunchKernelEx(&cfg, kern, maps.k, maps.v, maps.k16, maps.v16, p));
-  return DADATTN_OK;
+// The instance for `cluster` CTAs of an item: f(Launch<...>()).
+template <int D, int NT, int WARPS, typename F>
+int with_cluster(int cluster, F f) {
+  switch (cluster) {
+    case 1: return f(Launch<D, NT, 1, WARPS>());
+    case 2: return f(Launch<D, NT, 2, WARPS>());
+    case 4: return f(Launch<D, NT, 4, WARPS>());
+    case 8: return f(Launch<D, NT, 8, WARPS>());
+    default: return f(Launch<D, NT, 16, WARPS>());
+  }
 }
 
-// CTAs of a cluster: as many as the GPU has room for, and no more than have two and a half tiles each of the longest sequence
-// that there may be. Of several sequences a quarter more: they are of different lengths, and the last to start are short. us,
-// clusters of 1 / 2 / 4 / 8 / 16 (head size 64 in the first, third and last row):
-//   1 x 12 heads, 699 rows    9.4 / 7.2 / 5.6 / 5.7 / 6.9     1 x 8, 60000          688 / 348 / 178 / 93 / 55
-//   64 x 12, up to 1023       21 / 30 / 48 / 88 / 230         8 x 8, up to 15999    187 / 98 / 60 / 46 / 67
-//   16 x 1, up to 1999        25 / 15 / 9.3 / 7.5 / 8.7       32 x 8, up to 3999    58 / 48 / 53 / 79 / 140
-int cluster_for(long long items, int sequences, long long most_rows, int per_sm) {
-  const long long slots = static_cast<long long>(current_sm_count()) * per_sm;
-  int c = 1;
-  while (c < kMaxCluster && items * c * 2 * 4 <= slots * (sequences > 1 ? 5 : 4) && most_rows * 2 >= 5ll * c * 2 * kTile) c *= 2;
-  return c;
+// How items are shared out: to clusters of so many CTAs, each by itself on its SM with eight consumer warps (`alone`), or with
+// others and four. A CTA is bound by its warps' waits for their own steps: 16 rows of a tile take a warp 1450 clk at head size 64,
+// whatever the ring holds (three times as deep a ring: nothing), so that eight warps are as good as twice the cluster, which has
+// more to join. us, clusters of 1 / 2 / 4 / 8 / 16 with four warps, and with eight (-: they do not all fit):
+//   1 x 12 heads of 64, 699 rows    9.4 / 7.2 / 5.6 / 5.7 / 6.9      - / - / 5.2 / 5.6 / -
+//   1 x 13 of 64, 2000              23 / 14 / 8.7 / 6.9 / 7.7        14 / 9.4 / 6.7 / 6.2 / -
+//   1 x 7 of 128, 16000             190 / 98 / 52 / 30 / 20          115 / 61 / 33 / 20 / 16
+//   1 x 18 of 128, 16000            191 / 98 / 53 / 33 / 28          116 / 61 / 34 / - / -
+//   1 x 24 of 128, 16000            191 / 98 / 53 / 35 / -           116 / 61 / 34 / - / -
+//   8 x 4 of 128, up to 3750        47 / 27 / 17 / 13 / -            30 / 18 / 12 / - / -
+//   64 x 2 of 128, up to 694        11.3 / 9.1 / - / - / -           8.2 / - / - / - / -
+//   64 x 12 of 64, up to 1023       21 / 30 / 48 / 88 / 230          -
+//   8 x 8 of 128, up to 15999       187 / 98 / 60 / 46 / 67          -
+//   32 x 8 of 128, up to 3999       58 / 48 / 53 / 79 / 140          -
+// So as many CTAs to an item as all items have room for at once (half as many items again where there are several sequences, of
+// different lengths, and long ones), and no more than have two and a half tiles each of the longest sequence that there may be (of
+// eight warps' tiles, which are 128 rows, one and a quarter, but in clusters of 16).
+struct Sharing {
+  int cluster;
+  bool alone;
+};
+template <int D, int NT>
+Sharing share_out(int items, int sequences, long long most_rows) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return {1, false};
+  auto places = [&](int cluster, bool alone) {
+    auto ask = [&](auto launch) { return decltype(launch)::places(dev); };
+    return alone ? with_cluster<D, NT, 8>(cluster, ask) : with_cluster<D, NT, 4>(cluster, ask);
+  };
+  auto holds = [&](int cluster) {
+    const long long n = places(cluster, false);
+    return items <= n || (sequences > 1 && 2ll * items <= 3 * n && most_rows >= 512ll * cluster);
+  };
+  int c = 1, a = 0;
+  while (c < kMaxCluster && most_rows >= 320ll * c && holds(2 * c)) c *= 2;
+  for (int k = 1; k <= kMaxCluster && most_rows >= (k == 1 ? 0 : k == kMaxCluster ? 320ll * k : 160ll * k); k *= 2)
+    if (items <= places(k, true)) a = k;
+  return 2 * a >= c ? Sharing{a, true} : Sharing{c, false};
 }
 
 template <int D, int NT>
-int launch_decode_d(const Maps& maps, const DecodeParams& p, int items, long long most_rows, cudaStream_t st) {
-  switch (cluster_for(items, p.cache.B, most_rows, Plan<D, NT>::kPerSm)) {
-    case 1: return launch_decode<D, NT, 1>(maps, p, items, st);
-    case 2: return launch_decode<D, NT, 2>(maps, p, items, st);
-    case 4: return launch_decode<D, NT, 4>(maps, p, items, st);
-    case 8: return launch_decode<D, NT, 8>(maps, p, items, st);
-    default: return launch_decode<D, NT, 16>(maps, p, items, st);
-  }
+int launch_decode(DecodeParams& p, int items, int page_size, cudaStream_t st) {
+  const PagedCache& c = p.cache;
+  const Sharing how = share_out<D, NT>(items, c.B, static_cast<long long>(c.max_pages) * page_size);
+  const int tile = how.alone ? Plan<D, NT, 8>::kTile : Plan<D, NT, 4>::kTile, rows = c.pages * c.heads * page_size;
+  p.chunk = std::min(page_size, tile);
+  Maps maps;
+  if (int rc = make_tensor_map_bf16(&maps.k, p.k_pages, 1, rows, D, p.chunk)) return rc;
+  if (int rc = make_tensor_map_bf16(&maps.v, p.v_pages, 1, rows, D, p.chunk)) return rc;
+  if (int rc = make_tensor_map_bf16(&maps.k16, p.k_pages, 1, rows, D, 16)) return rc;
+  if (int rc = make_tensor_map_bf16(&maps.v16, p.v_pages, 1, rows, D, 16)) return rc;
+  auto run = [&](auto launch) { return decltype(launch)::run(maps, p, items, st); };
+  return how.alone ? with_cluster<D, NT, 8>(how.cluster, run) : with_cluster<D, NT, 4>(how.cluster, run);
 }
 
 }  // namespace
@@ -623,27 +693,20 @@ extern "C" int dadattn_decode_paged_bf16(uint16_t* out, float* lse, const uint16
   if (items * kMaxCluster > 0x7fffffffll) return fail(DADATTN_E_UNSUPPORTED, "%s: B=%d and Hkv=%d are too many", name, B, Hkv);
   DecodeParams p = {};
   p.out = reinterpret_cast<bf16*>(out), p.lse = lse;
-  p.q = reinterpret_cast<const bf16*>(q), p.k_new = reinterpret_cast<const bf16*>(k_new), p.v_new = reinterpret_cast<const bf16*>(v_new);
+  p.q = reinterpret_cast<const bf16*>(q);
+  p.k_new = reinterpret_cast<const bf16*>(k_new), p.v_new = reinterpret_cast<const bf16*>(v_new);
   p.k_pages = reinterpret_cast<bf16*>(k_pages), p.v_pages = reinterpret_cast<bf16*>(v_pages);
   p.out_token = out_strides[0], p.out_head = out_strides[1], p.q_token = q_strides[0], p.q_head = q_strides[1];
   p.k_token = k_strides[0], p.k_head = k_strides[1], p.v_token = v_strides[0], p.v_head = v_strides[1];
   p.cache = PagedCache{page_table, lengths, nullptr, B, pages, log2_of(page_size), max_pages, Hkv};
-  p.heads_q = Hq, p.group = group, p.parts = parts, p.chunk = page_size < kTile ? page_size : kTile;
+  p.heads_q = Hq, p.group = group, p.parts = parts;
   p.scale = scale;
   p.r = RotaryParams{turns, factor, rot_dim, interleaved != 0, 0};
   p.status = device_status_word();
   if (!p.status) return DADATTN_E_CUDA;
-  const int rows = pages * Hkv * page_size;
-  Maps maps;
-  if (int rc = make_tensor_map_bf16(&maps.k, k_pages, 1, rows, D, p.chunk)) return rc;
-  if (int rc = make_tensor_map_bf16(&maps.v, v_pages, 1, rows, D, p.chunk)) return rc;
-  if (int rc = make_tensor_map_bf16(&maps.k16, k_pages, 1, rows, D, 16)) return rc;
-  if (int rc = make_tensor_map_bf16(&maps.v16, v_pages, 1, rows, D, 16)) return rc;
-  const long long most_rows = static_cast<long long>(max_pages) * page_size;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool few = group <= 8;   // rows of an item
-  if (D == 64) return few ? launch_decode_d<64, 1>(maps, p, static_cast<int>(items), most_rows, st)
-                          : launch_decode_d<64, 2>(maps, p, static_cast<int>(items), most_rows, st);
-  return few ? launch_decode_d<128, 1>(maps, p, static_cast<int>(items), most_rows, st)
-             : launch_decode_d<128, 2>(maps, p, static_cast<int>(items), most_rows, st);
+  const int n = static_cast<int>(items);
+  if (D == 64) return few ? launch_decode<64, 1>(p, n, page_size, st) : launch_decode<64, 2>(p, n, page_size, st);
+  return few ? launch_decode<128, 1>(p, n, page_size, st) : launch_decode<128, 2>(p, n, page_size, st);
 }

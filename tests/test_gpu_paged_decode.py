@@ -63,6 +63,27 @@ def test_decode(cuda, case, rotate, garbage):
     assert torch.equal(again, out)
 
 
+@pytest.mark.parametrize("group", [1, 12])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("page", [16, 256])
+@pytest.mark.parametrize("Hkv,lengths", [(1, [6001]), (3, [5500, 127]), (10, [3000]), (13, [128]), (7, [900, 641, 0, 1]),
+                                         (2, [255, 257] * 17), (1, [700, 30] * 50)])
+def test_ctas_with_an_sm_to_themselves(cuda, Hkv, lengths, page, D, group):
+    """Eight consumer warps, tiles of 128 rows: clusters of 16, 8, 4, 2 and single CTAs."""
+    B, scale = len(lengths), D ** -0.5
+    c, _, g = made(cuda, Hkv, D, page, lengths, [1] * B, 21, garbage=NAN)
+    q, k, v = _inputs(g, cuda, B, group * Hkv, Hkv, D)
+    r = dad.RotaryPositions(D, device=cuda)
+    out, lse = torch.full_like(q, 9.0), torch.empty(B, group * Hkv, device=cuda)
+    dad.decode_attention_paged_bf16(out, q, k, v, c, scale, rotary=r, lse=lse)
+    qs = turn(q, torch.tensor(lengths, device=cuda), r)[0]
+    _check(c, out, lse, qs, HALF_BF16 + 2.0 ** -20 * 2, lengths, scale, None if B <= 10 else [0, 1, B // 2, B - 1])
+    assert device_status() == 0
+    again = torch.empty_like(out)
+    dad.decode_attention_paged_bf16(again, q, k, v, c, scale, rotary=r)
+    assert torch.equal(again, out)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_extreme_values(cuda, D):
     """Scores far apart, infinite keys and NaN: what the formula gives."""
