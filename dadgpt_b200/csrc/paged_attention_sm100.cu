@@ -950,24 +950,26 @@ int launch_chunk(const Maps& maps, ChunkParams p, long long items, cudaStream_t 
 //   head size 128   16 tiles, 8033 rows 70 / 40 / 27 / 38    64, 8256 72 / 43 / 57 / 109     128, 16512 142 / 147 / 175 / 274
 //                   8, 60001 485 / 245 / 128 / 70            64, 256 8.8 / 11 / 25 / 71      160, 4001 87 / 83 / 90 / 150
 //   head size 64    12, 1024 13.6 / 10.2 / 8.6 / 9.0         36, 1001 17 / 13 / 14 / 24      192, 4096 65 / 61 / 72 / 115
+//                   15, 6322 76 / 37 / 23 / 19               128, 1512 24 / 20 / 32 / 64     32, 30128 341 / 162 / 88 / 67
 // The sequences' counts and lengths are on the device, so tiles and rows are the most that there may be.
 struct Sharing {
   bool pairs;
   int cluster;
 };
 Sharing share_out(long long tiles, long long pairs, long long most_rows, bool alike, int per_sm, int sms) {
-  if (tiles >= (per_sm == 1 ? 2 : 8) * sms) return {true, 1};
+  if (2 * tiles >= (per_sm == 1 ? 4 : 15) * sms) return {true, 1};
   const long long n = (most_rows + kT - 1) / kT;
-  // how often `ctas` fill the GPU, or the part of it that clusters of their size can have (of eight: 14 clusters on 148 SMs)
+  // how often `ctas` fill the GPU, or the part of it that clusters of their size can have (of 4 and 8: 33 and 15 on 148 SMs)
   auto fills = [&](double ctas, double slots) {
     const double x = ctas / slots;
     if (x <= 1.0) return 1.0;
-    if (per_sm == 2) return std::max(1.5, 0.75 * x + 0.35);   // (two CTAs on an SM take half as long again as one)
+    if (per_sm == 2) return std::max(1.3, 0.75 * x - 0.2);   // (two CTAs on an SM take a third as long again as one)
     return alike ? std::ceil(x) : x + 0.5;
   };
   Sharing best = {true, 1};
-  double least = fills(pairs, sms) * n;
-  const struct { int cluster; double slots, join; } ways[] = {{1, 1.0, 0.5}, {2, 1.0, 1.5}, {4, 0.97, 1.75}, {8, 0.76, 2.5}};
+  // (two pairs on an SM take half as long again as one)
+  double least = n * (per_sm == 2 && pairs > sms ? std::max(1.5, 0.75 * pairs / sms + 0.35) : fills(pairs, sms));
+  const struct { int cluster; double slots, join; } ways[] = {{1, 1.0, 0.5}, {2, 1.0, 1.5}, {4, 0.892, 1.75}, {8, 0.811, 2.5}};
   for (const auto& w : ways) {
     const double each = static_cast<double>((n + 2 * w.cluster - 1) / (2 * w.cluster)) + w.join;
     const double cost = fills(static_cast<double>(tiles * w.cluster), w.slots * sms) * each;
