@@ -740,7 +740,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
           hand_over(1);
         } else {
           if (active) {
-            // (the probabilities go over the scores; 88 registers hold half of these, so the first half is read twice)
+            // (the probabilities go over the scores; 88 registers hold half of these, so the first half is read twice. All at once,
+            // with 96 and the other warps at 48: 38 us for 16 prompts' 36.)
             uint32_t sc[32], first[16], second[16];
             load(sc, 0);
             tmem_wait_ld();

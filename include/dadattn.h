@@ -496,7 +496,8 @@ int dadattn_paged_attention_bf16(uint16_t* out, float* lse, const uint16_t* q, c
 /* One decode step in one launch: the token of every sequence (q [B,Hq,D], k_new, v_new [B,Hkv,D] bf16, strides as above) is
  * turned by its row where rot_dim > 0, appended at row lengths[b] and attended for over rows 0 .. lengths[b]; out [B,Hq,D],
  * lse [B,Hq] or NULL. What dadattn_paged_append_bf16 and dadattn_paged_attention_bf16 do with starts NULL, without the rounding
- * of turned queries to bf16 between them. Where a page that holds a row of the sequence is outside the pool, out of that
+ * of turned queries to bf16 between them. (From some 64 query heads to a key head on, and with several sequences, those two
+ * are faster.) Where a page that holds a row of the sequence is outside the pool, out of that
  * sequence and key head is left untouched. */
 int dadattn_decode_paged_bf16(uint16_t* out, float* lse, const uint16_t* q, const uint16_t* k_new, const uint16_t* v_new,
                               const int64_t* out_strides, const int64_t* q_strides, const int64_t* k_strides,
