@@ -98,7 +98,9 @@ struct Bars {
   int abort_flag;
   int any_bad;                            // a page outside the pool, in any item
   int exps[2][4];                         // tiles whose exponentials a warp of a group is through with
-  int item[kItems][8];   // sequence (-1: the end), first token, rows ahead, first packed row, tokens, key head, bad
+  // sequence (-1: the end), first token, rows ahead, first packed row, tokens, key head, and whether a page is outside the pool:
+  // of the key tiles that both groups see, of those that only a pair's second one sees
+  int item[kItems][8];
 };
 static_assert(sizeof(Bars) <= 1024, "barrier block");
 
@@ -456,7 +458,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         if (n_pub >= kItems && !(ok = warp_wait(&bars->item_free[e], (n_pub / kItems - 1) & 1, abort_flag))) break;
         if (lane == 0) {
           volatile int* to = bars->item[e];
-          to[0] = it.b, to[1] = it.token0, to[2] = it.ahead, to[3] = it.first, to[4] = it.count, to[5] = it.kv_head, to[6] = 0;
+          to[0] = it.b, to[1] = it.token0, to[2] = it.ahead, to[3] = it.first, to[4] = it.count, to[5] = it.kv_head, to[6] = to[7] = 0;
           mbar_arrive(&bars->item_ready[e]);
         }
         __syncwarp();
@@ -478,7 +480,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
           const int row = tile * kT + box * p.chunk;
           // (a row coordinate outside the pool reads zeros)
           const bool good = mine >= 0 && mine < c.pages, mine_there = there(tile);
-          if (!good) bars->item[e][6] = bars->any_bad = 1;
+          if (!good) bars->item[e][s.single || j < s.n_first ? 6 : 7] = bars->any_bad = 1;
           const int y = good ? ((mine * c.heads + it.kv_head) << c.page_shift) + (row & ((1 << c.page_shift) - 1)) : -kMaxPage;
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
@@ -770,18 +772,22 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       const int64_t to_token = it.first + token;
       const int to_head = it.kv_head * p.group + min(row, t.rows - 1) % p.group;
       bf16* to = p.out + to_token * p.out_token + to_head * p.out_head;
-      const bool write = row < t.rows && !feed.entry()[6];
+      // Whether the row is written: not where a key tile that its query tile sees has a page outside the pool. Asked behind the
+      // last product on these tiles, of a tile that the groups share behind the other's too: a group may have no steps of it, and
+      // would find the flag as it was before the pages were looked at.
+      auto write = [&] { return row < t.rows && !feed.entry()[6] && !(x == 1 && feed.entry()[7]); };
       l *= ex2(m == -INFINITY ? 0.f : m - m);   // (NaN where the max is not finite)
       if (!s.single) {
         // out = O / l, lse in natural-log units of the scaled scores
         const float f = 1.0f / l;
+        const bool mine = write();
         if (active) {
 #pragma unroll
           for (int q = 0; q < D / 32; ++q) {
             uint32_t o[32];
             tmem_ld32(tO + q * 32, o);
             tmem_wait_ld();
-            if (write) {
+            if (mine) {
 #pragma unroll
               for (int e = 0; e < 32; e += 16) {
                 float y[16];
@@ -792,7 +798,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             }
           }
         }
-        if (write && p.lse) p.lse[to_token * p.heads_q + to_head] = (m + log2f(l)) * kLn2;
+        if (mine && p.lse) p.lse[to_token * p.heads_q + to_head] = (m + log2f(l)) * kLn2;
       } else {
         // The other group has the rest of the row's keys: each group joins one half of the columns. The rows' maxima and sums
         // change hands in the first columns of the scores.
@@ -803,6 +809,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         if (lane == 0) mbar_arrive(&bars->joined);
         if (!(ok = mbar_wait(&bars->joined, joins & 1, abort_flag))) break;
         tc_fence_after_sync();
+        const bool mine = write();
         float m1, l1;
         tmem_ld2(tlane + kColS + (1 - x) * kN, m1, l1);
         tmem_wait_ld();
@@ -834,12 +841,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 #pragma unroll
               for (int i = 0; i < 16; i += 4)
                 *reinterpret_cast<float4*>(acc + q * 16 + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
-            } else if (write) {
+            } else if (mine) {
               store_16(to + q * 16, y, p.wide);
             }
           }
         }
-        if (CLUSTER == 1 && x == 0 && write && p.lse) p.lse[to_token * p.heads_q + to_head] = (m_all + log2f(l_all)) * kLn2;
+        if (CLUSTER == 1 && x == 0 && mine && p.lse) p.lse[to_token * p.heads_q + to_head] = (m_all + log2f(l_all)) * kLn2;
         if (CLUSTER > 1 && x == 0) reinterpret_cast<float2*>(smem + L::kStats)[row] = make_float2(m_all, l_all);
         if (CLUSTER == 1) {
           tc_fence_before_sync();

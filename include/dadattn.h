@@ -483,10 +483,10 @@ int dadattn_paged_append_bf16(uint16_t* k_pages, uint16_t* v_pages, const int32_
 /* Attention of the new tokens over all rows of their sequences, theirs among them, which are in their pages already: token i
  * of sequence b sees rows j <= lengths[b] + i. out, q [T,Hq,D] bf16; lse [T,Hq] fp32 (natural log of the sum of exp of the
  * scaled scores; may be NULL). scale > 0. max_new: no sequence brings more tokens than this (one that does is left untouched
- * and reported); it bounds the launch. Hq / Hkv at most 128. Where a page is outside the pool, the rows of the 128-row query
- * tiles that would read it (256 rows where two tiles share their keys) are left untouched. What pages hold behind a sequence's
- * last row has no influence; an infinite or NaN row of a sequence makes NaN of the rows of a 128-row query tile that reads its
- * tile of 128 keys, as in dadattn_flash_fwd_bf16. */
+ * and reported); it bounds the launch. Hq / Hkv at most 128. Where a page is outside the pool, the rows of out and lse of the
+ * 128-row query tiles that read a tile of 128 keys with rows of it are left untouched, and no others. What pages hold behind a
+ * sequence's last row has no influence; an infinite or NaN row of a sequence makes NaN of the rows of a 128-row query tile that
+ * reads its tile of 128 keys, as in dadattn_flash_fwd_bf16. */
 int dadattn_paged_attention_bf16(uint16_t* out, float* lse, const uint16_t* q, const int64_t* out_strides,
                                  const int64_t* q_strides, const uint16_t* k_pages, const uint16_t* v_pages,
                                  const int32_t* page_table, const int32_t* lengths, const int32_t* starts, int B, int T,
