@@ -55,6 +55,13 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const AppendPara
     }
     count = __reduce_add_sync(0xffffffffu, count);
     if (t % 32 == 0 && count) atomicAdd(&before, count);
+    // A sequence without new rows is reported here: the CTAs of V's last heads, which form no angles, look at some each. (us
+    // without / by all these CTAs / by one: 2000 sequences 10.2 / 10.5 / 12.8, 300 6.75 / 6.95 / 6.95, 16 3.4 / 3.45 / 3.45.)
+    if (blockIdx.y == gridDim.y - 1) {
+      int ahead, first, many;
+      for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + t; i < c.B; i += static_cast<int64_t>(gridDim.x) * kThreads)
+        if (!sequence_rows(c, static_cast<int>(i), p.T, ahead, first, many)) atomicExch(p.status, DADATTN_E_ARG);
+    }
     __syncthreads();
     b = before;
     for (int j = 1; j <= at && j < n; ++j) b += later[j];
