@@ -286,7 +286,8 @@ def rotary_backward(dq, dk, dq_turned, dk_turned, rotary: RotaryPositions, *, po
 class KVCachePagedBF16:
     """A cache of one layer in pages: k, v [pages,H,page_size,D] bf16. Row j of sequence b is row j % page_size of page
     ``page_table[b, j // page_size]`` (int32 [B,max_pages], filled by the caller); ``lengths`` [B] int32 rows are there ahead
-    of a call. Layers of a model share table and lengths: pass those of the first. H: key heads."""
+    of a call. Layers of a model share table and lengths: pass those of the first. H: key heads. Small calls are faster with a
+    table no wider than the longest sequence needs."""
 
     def __init__(self, B, H, pages, page_size, max_pages, D, device="cuda", page_table=None, lengths=None):
         self.B, self.H, self.pages, self.page_size, self.max_pages, self.D = B, H, pages, page_size, max_pages, D
@@ -308,7 +309,8 @@ def kv_cache_append_paged(cache: KVCachePagedBF16, k_new, v_new, starts=None, *,
     """The new rows of a packed batch, k_new and v_new [T,H,D] bf16 or fp32, to their pages: sequence b's are rows
     starts[b] .. starts[b+1]-1 (int32 [B+1]; None: one for each sequence) and become its rows lengths[b] and on, which stay the
     lengths until :func:`kv_cache_advance_paged`. With ``rotary``, keys are turned by their rows, and so are queries q
-    [T,Hq,D], into q_out (bf16)."""
+    [T,Hq,D], into q_out (bf16: they are rounded, which :func:`decode_attention_paged_bf16` does not do, so that the two ways
+    differ in their last bits)."""
     _native().append_paged(*cache._args(), *_rotary_args(rotary), starts, q_out, q, k_new, v_new)
 
 

@@ -30,6 +30,7 @@
 // Measured (us): 2048 tokens behind 14336 rows, 32 heads on 8 of 128 453 (1137 TFLOP/s; 516 at the power cap); 24 sequences with
 // up to 3690 rows ahead and 1 to 512 new ones, the same heads, 112-130; 16 prompts of up to 1024 tokens, 12 heads of 64 36; 301
 // tokens behind 700 rows, 12 heads of 64 12.5.
+// At head size 128 an instance has all 168 registers of a thread and spills 40 (single CTAs) or 52 bytes.
 // Not kept: exponentials as polynomials, in any share (slower at both head sizes: the threads, not the exp2 unit, are short of
 // time); 64-key steps with two score buffers at head size 128 (514 for the first); probabilities handed over in quarters (481),
 // the turn passed on earlier (482-501).
@@ -959,7 +960,9 @@ int launch_chunk(const Maps& maps, ChunkParams p, long long items, cudaStream_t 
 //                   8, 60001 485 / 245 / 128 / 70            64, 256 8.8 / 11 / 25 / 71      160, 4001 87 / 83 / 90 / 150
 //   head size 64    12, 1024 13.6 / 10.2 / 8.6 / 9.0         36, 1001 17 / 13 / 14 / 24      192, 4096 65 / 61 / 72 / 115
 //                   15, 6322 76 / 37 / 23 / 19               128, 1512 24 / 20 / 32 / 64     32, 30128 341 / 162 / 88 / 67
-// The sequences' counts and lengths are on the device, so tiles and rows are the most that there may be.
+// The sequences' counts and lengths are on the device, so tiles and rows are the most that there may be: rows those that the table
+// has room for. Behind a wider table few tiles go to larger clusters than their rows are worth (us, tight / 8192 rows and more: 301
+// tokens behind 700 rows, 12 heads of 64 12.5 / 24; one prompt of 2000, 12 of 128 26.6 / 47).
 struct Sharing {
   bool pairs;
   int cluster;

@@ -45,7 +45,9 @@ using bf16 = __nv_bfloat16;
 constexpr int kWarpRows = 16;                 // cache rows of a consumer warp in a stage
 constexpr int kRows = 16;                     // query rows of an item, at most
 constexpr int kMaxCluster = 16;
-constexpr int kRanked = 4;                    // sequences of a lane that are ranked: 128 of a call
+// Sequences of a lane that are ranked: 128 of a call. (More come in the caller's order. us, mixed / longest first: 256 of up to 1000
+// rows, 12 heads of 64 66 / 71; 256 of up to 2000, 8 of 128 156 / 153; 130 of up to 4000 163 / 151.)
+constexpr int kRanked = 4;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kRescaleAt = 8.0f;
 
@@ -625,9 +627,24 @@ int with_cluster(int cluster, F f) {
 //   64 x 12 of 64, up to 1023       21 / 30 / 48 / 88 / 230          -
 //   8 x 8 of 128, up to 15999       187 / 98 / 60 / 46 / 67          -
 //   32 x 8 of 128, up to 3999       58 / 48 / 53 / 79 / 140          -
+// Eight key heads are where the two ways meet, clusters of 16 with four warps and of 8 with eight, and the tie goes to the second,
+// which is faster up to some 30000 rows and slower behind that:
+//   1 x 8 of 128: 4000 rows 9.6 and 8.4, 8000 13.8 and 12.8, 16000 20.9 and 20.0, 30000 32.3 and 32.5, 60000 56.5 and 58.8,
+//   120000 104.6 and 111.0; 1 x 12 of 64: 16000 17.6 and 17.0, 60000 46.9 and 48.7; 1 x 10 of 128: 60000 59.6 and 59.0
+// More than 8 query heads to a key head (NT = 2; five of its instances at head size 128 spill 8 to 16 bytes):
+//   1 x 8 x 16 of 64, 4000 rows     45 / 26 / 15 / 10.9 / 10.1       28 / 16 / 10.6 / 8.2 / 16
+//   1 x 1 x 12 of 128, 16000        256 / 130 / 69 / 38 / 24         120 / 63 / 35 / 21 / 14.7
+//   16 x 1 x 16 of 64, up to 3875   43 / 25 / 15 / 10.8 / 10.5       27 / 16 / 10.5 / 14 / 26
+//   16 x 8 x 12 of 128, up to 3875  68 / 44 / 31.6 / 47 / -          35 / 32 / 49 / 94 / -
+//   64 x 1 x 12 of 128, up to 992   20 / 14.5 / 11.7 / 19 / 42       11.5 / 9.4 / 16 / 41 / 94
+//   64 x 8 x 16 of 64, up to 992    18 / 24 / - / - / -              29 / 53 / - / - / -
+//   16 x 8 x 32 of 128, up to 3875  74 / 47 / 54 / - / -             37.8 / 56 / 90 / - / -   (the rule: 47)
 // So as many CTAs to an item as all items have room for at once (half as many items again where there are several sequences, of
 // different lengths, and long ones), and no more than have two and a half tiles each of the longest sequence that there may be (of
-// eight warps' tiles, which are 128 rows, one and a quarter, but in clusters of 16).
+// eight warps' tiles, which are 128 rows, one and a quarter, but in clusters of 16). The longest sequence that there may be is what
+// the table has room for: behind a wider one clusters are larger than the rows are worth. (us, tight / 8192 rows and more: 8
+// sequences of 300 rows, 8 key heads of 128 6.0 / 15.1, of 1000 9.3 / 18.8; 16 of 300, 12 of 64 6.3 / 12.5; one of 100, 12 of 64
+// 3.6 / 6.0, of 700 5.5 / 5.9.)
 struct Sharing {
   int cluster;
   bool alone;

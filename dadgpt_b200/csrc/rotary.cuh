@@ -59,7 +59,7 @@ inline int head_groups(long long blocks, int heads, int all, int per_sm) {
 
 #ifdef __CUDACC__
 // sin and cos of r half turns, |r| <= 1/4, by polynomials in r^2 that were fitted for the least error over that range: off by
-// 4.4e-8 and 5.8e-8 in fp32 (pi comes in two parts). 12 operations; sincospif, which takes any r, made a short fp32 call 1 us
+// 4.6e-8 and 5.9e-8 in fp32 over all their arguments (pi comes in two parts). 12 operations; sincospif, which takes any r, made a short fp32 call 1 us
 // longer, at eight pairs a thread.
 __device__ __forceinline__ void sin_cos_eighth(float r, float* s, float* c) {
   const float z = r * r;

@@ -465,6 +465,10 @@ int dadattn_rotary(void* q_out, void* k_out, const void* q, const void* k, const
  * left untouched, and so is a row whose page is outside [0, pages); both are reported through DADATTN_E_ARG at the next
  * dadattn_device_status(). (Where starts fall, whose the rows are that two sequences claim is not said.) Nothing outside the
  * pages is read or written for any contents of the device arrays.
+ * How attention and decode share a small call out over the GPU goes by max_pages * page_size as the most rows that a sequence may
+ * have: behind a table that is far wider than the longest sequence they are right, but take up to two and a half times as long
+ * (8 sequences of 300 rows, a decode step: 6 us, 15 with room for 8192). A table of the step's own, as wide as its longest sequence
+ * needs, costs nothing of that.
  * No call needs a workspace; results overlap nothing that a call reads, but where that is said; calls may overlap on the GPU
  * unless one writes what the other reads or writes. */
 
